@@ -27,7 +27,7 @@
 extern "C" {
 #endif
 
-#define PNGPD_ABI_VERSION 7
+#define PNGPD_ABI_VERSION 8
 
 enum {
     PNGPD_OK = 0,
@@ -49,6 +49,21 @@ enum {
     PNGPD_EPI_RELU = 1,          /* F.relu(bn(fc(x))) with BN folded   pointnet.py:35-36,191-192 */
     PNGPD_EPI_ADD_IDEN3 = 2,     /* fc3(x) + eye(3).view(1,9)          pointnet.py:37-43         */
     PNGPD_EPI_LOG_SOFTMAX = 3    /* F.log_softmax(fc3(x), dim=-1)      pointnet.py:193-194       */
+};
+
+/* Element types of the training operators. */
+enum {
+    PNGPD_F32 = 0,
+    PNGPD_BF16 = 1,
+    PNGPD_F16 = 2
+};
+
+/* Activations of pngpd_group_norm_*. */
+enum {
+    PNGPD_ACT_NONE = 0,
+    PNGPD_ACT_RELU = 1,
+    PNGPD_ACT_SILU = 2,          /* z / (1 + exp(-z))                                   */
+    PNGPD_ACT_GELU = 3           /* z * Phi(z), Phi the normal distribution (not tanh)   */
 };
 
 int pngpd_abi_version(void);
@@ -449,6 +464,39 @@ int pngpd_adam_flat(float *p, const float *g, float *m, float *v, long long n, f
                     float beta1, float beta2, float eps, float step, const float *step_dev, float gscale,
                     const float *gdiv_dev, void *stream);
 int pngpd_adam_step_inc(float *step_dev, void *stream);
+
+/* Global norm of n gradients and their clipping in place: *total_norm = the 2-norm (norm_kind 2), the 1-norm (1) or the
+ * largest magnitude (0) over every element of every tensor; then g *= min(1, max_norm / (*total_norm + 1e-6)).
+ * g, numel, dtype: HOST arrays (dtype NULL: all float32); tensors dense, each aligned to its element, none overlapping
+ * another; an empty one may be NULL.  Sums in fp64, in a fixed order.  A NaN or infinite gradient gives a norm of NaN or
+ * infinity and reaches the gradients through the factor.  max_norm infinite: the norm alone.  Two launches a 128 tensors. */
+size_t pngpd_grad_clip_workspace_bytes(int n);
+int pngpd_grad_clip(void *const *g, const long long *numel, const int *dtype, int n, int norm_kind, float max_norm,
+                    float *total_norm, void *workspace, size_t workspace_bytes, void *stream);
+/* pngpd_adam_flat over `runs` ranges [offset, offset + length) of the flat buffers (HOST arrays; offsets multiples of 4)
+ * with the gradients clipped by their 2-norm over all the ranges.  norm and factor are of the gradients AS USED (times
+ * gscale, divided by *gdiv_dev); *total_norm receives that norm; the gradient buffer is not written.  Workspace:
+ * pngpd_grad_clip_workspace_bytes(runs).  The betas are fp64: 1 - beta and the bias corrections keep float32's digits,
+ * which pngpd_adam_flat's do not (1 - 0.999f is 1.3e-5 off), so an update here differs from its by about that much. */
+int pngpd_adam_flat_clip(float *p, const float *g, float *m, float *v, const long long *offset, const long long *length,
+                         int runs, float lr, const float *lr_dev, double beta1, double beta2, float eps, float step,
+                         const float *step_dev, float gscale, const float *gdiv_dev, float max_norm, float *total_norm,
+                         void *workspace, size_t workspace_bytes, void *stream);
+
+/* Group norm + activation over channels-last features, y = act((x - mean) / sqrt(var + eps) * w + b) with mean and
+ * (biased) variance over the N rows and C / G channels of each of the G groups of a sample.
+ *   x (B,N,C) of `dtype`, element strides stride_b, stride_n, channels adjacent; y, dy, dx (B,N,C) contiguous, of `dtype`
+ *   w, b (C) of wdtype (= dtype or PNGPD_F32), each NULL: 1 / 0;  dw, db likewise, each NULL: not wanted; dx NULL: same
+ *   stats (B,G,2) fp64 = mean, 1/sqrt(var + eps): written by the forward call, read by the backward one
+ * The backward call takes the forward's x, w, b, act.  Deterministic; no row or channel count is special.           */
+size_t pngpd_group_norm_workspace_bytes(int B, int N, int C, int G, int dtype, int backward);
+int pngpd_group_norm_fwd(const void *x, int dtype, int B, int N, int C, long long stride_b, long long stride_n, int G,
+                         const void *w, const void *b, int wdtype, float eps, int act, void *y, double *stats,
+                         void *workspace, size_t workspace_bytes, void *stream);
+int pngpd_group_norm_bwd(const void *x, int dtype, int B, int N, int C, long long stride_b, long long stride_n, int G,
+                         const void *w, const void *b, int wdtype, float eps, int act, const double *stats,
+                         const void *dy, void *dx, void *dw, void *db, void *workspace, size_t workspace_bytes,
+                         void *stream);
 
 /* =======================================================================================
  * Batched in-gripper crop + resample (upstream of the scorer).

@@ -9,7 +9,7 @@ import os
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("PNGPD_LIB") or os.path.join(_HERE, "libpngpd.so")   # PNGPD_LIB: A/B builds only
-ABI_VERSION = 7
+ABI_VERSION = 8
 
 _lib = None
 _load_error = None
@@ -151,6 +151,21 @@ SIGNATURES = {
                                                       ctypes.c_float, ctypes.c_float, ctypes.c_float, c_void,
                                                       ctypes.c_float, c_void, c_void]),
     "pngpd_adam_step_inc": (ctypes.c_int, [c_void, c_void]),
+    # ---- gradient clipping, group norm + activation
+    "pngpd_grad_clip_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int]),
+    "pngpd_grad_clip": (ctypes.c_int, [c_void, c_void, c_void, ctypes.c_int, ctypes.c_int, ctypes.c_float, c_void, c_void,
+                                       ctypes.c_size_t, c_void]),
+    "pngpd_adam_flat_clip": (ctypes.c_int, [c_void] * 6 + [ctypes.c_int, ctypes.c_float, c_void, ctypes.c_double,
+                                                           ctypes.c_double, ctypes.c_float, ctypes.c_float, c_void,
+                                                           ctypes.c_float, c_void, ctypes.c_float, c_void, c_void,
+                                                           ctypes.c_size_t, c_void]),
+    "pngpd_group_norm_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int] * 6),
+    "pngpd_group_norm_fwd": (ctypes.c_int, [c_void] + [ctypes.c_int] * 4 + [ctypes.c_longlong] * 2 +
+                             [ctypes.c_int, c_void, c_void, ctypes.c_int, ctypes.c_float, ctypes.c_int, c_void, c_void,
+                              c_void, ctypes.c_size_t, c_void]),
+    "pngpd_group_norm_bwd": (ctypes.c_int, [c_void] + [ctypes.c_int] * 4 + [ctypes.c_longlong] * 2 +
+                             [ctypes.c_int, c_void, c_void, ctypes.c_int, ctypes.c_float, ctypes.c_int] + [c_void] * 6 +
+                             [ctypes.c_size_t, c_void]),
     # ---- crop / resample
     "pngpd_crop_count_compact": (ctypes.c_int, [c_void, ctypes.c_int, ctypes.c_int, c_void, ctypes.c_int,
                                                 ctypes.c_int, c_void, c_void, c_void]),

@@ -1,0 +1,804 @@
+// Group norm with an activation over channels-last features, forward and backward.
+//
+//   x (B,N,C), group g of sample b = the channels [g Cg, (g+1) Cg) of all N rows, m = N Cg values:
+//     mean = sum x / m      var = sum x^2 / m - mean^2      rstd = 1/sqrt(var + eps)      (sums in fp64)
+//     xh = (x - mean) rstd      z = xh w_c + b_c      y = act(z)
+//   dz = dy act'(z)      A_c = sum_n dz      B_c = sum_n dz xh      db_c = sum_b A_c      dw_c = sum_b B_c
+//     S1 = sum_c w_c A_c / m      S2 = sum_c w_c B_c / m      dx = rstd (w_c dz - S1 - xh S2)
+//
+// Memory-bound: x is read and y written once forward, x and dy read and dx written once backward.  Two forms:
+//   * slab: one workgroup owns the N rows of a few whole groups of one sample (64 to 512 bytes of a row) and holds
+//     them in REGISTERS between the sums and the output: each byte moves once, one launch;
+//   * split: groups too large for that (a 50,000-point scene) are cut along N over workgroups: partial sums, a tiny
+//     launch that joins them, a second walk over the data.
+// A thread owns a fixed 16-byte column of channels, so w, b and the group's statistics sit in its registers, and the
+// per-channel sums of the backward pass need no transposition.  Columns may start anywhere (Cg is any number): gfx950
+// loads 16 bytes from any element's address; the ragged last column of a range goes element by element.
+// The sums of x and x^2 are fp64: a cloud's coordinates-like features have means many times their spread, where a
+// float32 E[x^2] - mean^2 loses the variance; memory hides the fp64 rate.  relu's slope is taken from a z in fp64 (its
+// statistics are kept in fp64 for that): it jumps at 0, and a value next to it would otherwise take either side.
+#include "pngpd_common.h"
+#include "pngpd_types.h"
+
+struct GnArgs {
+    const void *x, *dy, *w, *b;
+    void *y, *dx;
+    double *stats;                 // (B,G,2): mean, rstd
+    float *ab;                     // (B,C,2): A, B of the sample
+    double *part;                  // split form: (B,S,units,2) sums;  backward: (B,S,C,2) as float
+    float *gsum;                   // split form, backward: (B,G,2): S1, S2
+    long long sB, sN;              // strides of x (elements)
+    int B, N, C, G, Cg, act, wf32; // wf32: w, b are float32 (else of x's type)
+    float eps;
+    int lx;                        // log2 of the columns of a workgroup
+    int gpr, ranges;               // slab: groups of a workgroup, workgroups of a sample
+    int cols, S, rows;             // split: column blocks, cuts of N, rows of one
+};
+
+// ---------------------------------------------------------------- columns of VEC elements, 16 bytes (or one element)
+template <int DT, int VEC> struct Col {
+    static constexpr int WORDS = VEC == 1 ? 1 : 4;
+    unsigned q[WORDS];
+    __device__ __forceinline__ float get(int e) const {
+        if constexpr (DT == PNGPD_F32) return __uint_as_float(q[e]);
+        else return half_to_f(DT, (u16)(q[e >> 1] >> (16 * (e & 1))));
+    }
+    // n of the VEC elements exist; the others read as 0
+    __device__ __forceinline__ void load(const typename elem<DT>::t *p, int n) {
+        if (VEC > 1 && n == VEC) { __builtin_memcpy(q, p, 16); return; }
+        load_tail(p, n);
+    }
+    __device__ __forceinline__ void load_tail(const typename elem<DT>::t *p, int n) {
+#pragma unroll
+        for (int i = 0; i < WORDS; ++i) q[i] = 0u;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            if (e < n) {
+                if constexpr (DT == PNGPD_F32) q[e] = __float_as_uint(p[e]);
+                else q[e >> 1] |= (unsigned)p[e] << (16 * (e & 1));
+            }
+        }
+    }
+    static __device__ __forceinline__ void store(typename elem<DT>::t *p, const float (&v)[VEC], int n) {
+        if (VEC > 1 && n == VEC) {
+            unsigned o[WORDS];
+#pragma unroll
+            for (int i = 0; i < WORDS; ++i) {
+                if constexpr (DT == PNGPD_F32) o[i] = __float_as_uint(v[i]);
+                else o[i] = (unsigned)f_to_half(DT, v[(2 * i) % VEC]) | ((unsigned)f_to_half(DT, v[(2 * i + 1) % VEC]) << 16);
+            }
+            __builtin_memcpy(p, o, 16);
+            return;
+        }
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) if (e < n) st_elem<DT>(p + e, v[e]);
+    }
+};
+
+// K rows row, row + step, ... of a column; a row at or past `end` reads row `row0` (which exists) in its place
+template <int K, int DT, int VEC>
+__device__ __forceinline__ void load_rows(Col<DT, VEC> (&q)[K], const typename elem<DT>::t *p, long long stride, int row,
+                                          int step, int end, int n, int row0 = 0) {
+    if (VEC > 1 && n == VEC) {
+#pragma unroll
+        for (int i = 0; i < K; ++i) {
+            const int at = row + i * step;
+            __builtin_memcpy(q[i].q, p + (long long)(at < end ? at : row0) * stride, 16);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < K; ++i) {
+            const int at = row + i * step;
+            q[i].load_tail(p + (long long)(at < end ? at : row0) * stride, n);
+        }
+    }
+}
+
+// ---------------------------------------------------------------- activations
+// Phi(z), the normal distribution, and e = exp(-z^2/2): erf by Abramowitz & Stegun 7.1.26 (|error| < 1.5e-7), whose
+// exponential is the density's too; ~16 instructions where erff takes both its branches in a divergent wave.
+__device__ __forceinline__ float phi_cdf(float z, float &e) {
+    const float a = fabsf(z) * 0.70710678118654752f;
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, a, 1.f));
+    e = __expf(-0.5f * z * z);
+    const float p = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
+    const float tail = 0.5f * p * e;
+    return z < 0.f ? tail : 1.f - tail;
+}
+__device__ __forceinline__ float act_value(int act, float z) {
+    float e;
+    switch (act) {
+    case PNGPD_ACT_RELU: return z < 0.f ? 0.f : z;                    // NaN passes
+    case PNGPD_ACT_SILU: return z * __builtin_amdgcn_rcpf(1.f + __expf(-z));
+    case PNGPD_ACT_GELU: return z * phi_cdf(z, e);
+    default: return z;
+    }
+}
+// act'(z) for relu takes its own z (see gn_slope)
+__device__ __forceinline__ float act_slope(int act, float z) {
+    float e, s;
+    switch (act) {
+    case PNGPD_ACT_SILU: s = __builtin_amdgcn_rcpf(1.f + __expf(-z)); return s * fmaf(z, 1.f - s, 1.f);
+    case PNGPD_ACT_GELU: s = phi_cdf(z, e); return fmaf(z * 0.39894228040143268f, e, s);
+    default: return 1.f;
+    }
+}
+
+// What a thread keeps of its column: w, b and, for each of SUB groups it touches, the statistics.  SUB = 1: the column
+// lies inside one group (Cg a multiple of VEC); SUB = VEC: every element may belong to another one.
+template <int VEC, int SUB> struct ColPar {
+    float w[VEC], b[VEC];
+    double mean[SUB], rstd[SUB];
+};
+template <int DT, int VEC, int SUB>
+__device__ __forceinline__ void load_wb(const GnArgs &a, int c, int n, ColPar<VEC, SUB> &p) {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+        p.w[e] = 1.f; p.b[e] = 0.f;
+        if (e < n) {
+            if (a.w) p.w[e] = a.wf32 ? ((const float *)a.w)[c + e] : ld_elem<DT>((const typename elem<DT>::t *)a.w + c + e);
+            if (a.b) p.b[e] = a.wf32 ? ((const float *)a.b)[c + e] : ld_elem<DT>((const typename elem<DT>::t *)a.b + c + e);
+        }
+    }
+}
+// statistics of the column's groups out of st (mean, rstd pairs), whose first entry is group g0
+template <int VEC, int SUB>
+__device__ __forceinline__ void load_stats(const GnArgs &a, const double *st, int c, int n, int g0, ColPar<VEC, SUB> &p) {
+#pragma unroll
+    for (int e = 0; e < SUB; ++e) {
+        p.mean[e] = 0.0; p.rstd[e] = 0.0;
+        if (e < n) {
+            const int g = (c + e) / a.Cg - g0;
+            p.mean[e] = st[2 * g]; p.rstd[e] = st[2 * g + 1];
+        }
+    }
+}
+template <int VEC, int SUB>
+__device__ __forceinline__ void gn_apply(const GnArgs &a, const ColPar<VEC, SUB> &p, const float (&x)[VEC], float (&y)[VEC]) {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+        const int s = SUB == 1 ? 0 : e;
+        y[e] = act_value(a.act, fmaf((x[e] - (float)p.mean[s]) * (float)p.rstd[s], p.w[e], p.b[e]));
+    }
+}
+// dz and xh of one element
+template <int VEC, int SUB>
+__device__ __forceinline__ float gn_dz(const GnArgs &a, const ColPar<VEC, SUB> &p, int e, float x, float dy, float &xh) {
+    const int s = SUB == 1 ? 0 : e;
+    xh = (x - (float)p.mean[s]) * (float)p.rstd[s];
+    if (a.act == PNGPD_ACT_NONE) return dy;
+    if (a.act == PNGPD_ACT_RELU)
+        return fma(((double)x - p.mean[s]) * p.rstd[s], (double)p.w[e], (double)p.b[e]) <= 0.0 ? 0.f : dy;
+    return dy * act_slope(a.act, fmaf(xh, p.w[e], p.b[e]));
+}
+
+// sum over the lanes of a wave that hold the same column (lane ^ (1 << lx), ... )
+template <class T> __device__ __forceinline__ T lanes_sum(T v, int lx) {
+    for (int k = 1 << lx; k < 64; k <<= 1) v += __shfl_xor(v, k);
+    return v;
+}
+__device__ __forceinline__ double wave_sum(double v) {
+#pragma unroll
+    for (int k = 32; k >= 1; k >>= 1) v += __shfl_xor(v, k);
+    return v;
+}
+
+// ranges of one sample stay on one XCD (workgroup i runs on XCD i % 8): neighbouring ranges share cache lines
+__device__ __forceinline__ int slab_item(int i, int ranges, int total) {
+    const int whole = total / (8 * ranges) * (8 * ranges);
+    if (i >= whole) return i;
+    const int k = i >> 3;
+    return (k / ranges) * 8 * ranges + (i & 7) * ranges + k % ranges;
+}
+
+// ---------------------------------------------------------------------------------------------- slab form
+template <int DT, int VEC, int SUB, int RPT>
+__global__ __launch_bounds__(1024) void gn_fwd_slab_kernel(const GnArgs a) {
+    typedef typename elem<DT>::t T;
+    extern __shared__ double sh[];
+    const int tid = threadIdx.x, X = 1 << a.lx, tx = tid & (X - 1), ty = tid >> a.lx, TY = blockDim.x >> a.lx;
+    const int waves = blockDim.x >> 6, wave = tid >> 6, lane = tid & 63;
+    const int item = slab_item(blockIdx.x, a.ranges, a.B * a.ranges), b = item / a.ranges, r = item - b * a.ranges;
+    const int g0 = r * a.gpr, gn = min(a.gpr, a.G - g0), c0 = g0 * a.Cg, c1 = c0 + gn * a.Cg;
+    const int c = c0 + tx * VEC, n = max(0, min(VEC, c1 - c));
+    const T *x = (const T *)a.x + (long long)b * a.sB + c;
+    Col<DT, VEC> q[RPT];                                  // rows past the last one: row 0 again, never used
+    load_rows<RPT>(q, x, a.sN, ty, TY, a.N, n);
+    ColPar<VEC, SUB> p;
+    load_wb<DT>(a, c, n, p);
+    double s[SUB], s2[SUB];
+#pragma unroll
+    for (int e = 0; e < SUB; ++e) { s[e] = 0.0; s2[e] = 0.0; }
+#pragma unroll
+    for (int i = 0; i < RPT; ++i) {
+        if (ty + i * TY < a.N) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const double v = (double)q[i].get(e);
+                const int k = SUB == 1 ? 0 : e;
+                s[k] += v; s2[k] = fma(v, v, s2[k]);
+            }
+        }
+    }
+    // per wave: (X * SUB) units of (sum, sum of squares)
+    const int units = X * SUB;
+#pragma unroll
+    for (int e = 0; e < SUB; ++e) {
+        const double u = lanes_sum(s[e], a.lx), v = lanes_sum(s2[e], a.lx);
+        if (lane < X) {
+            double *o = sh + 2 * ((size_t)wave * units + tx * SUB + e);
+            o[0] = u; o[1] = v;
+        }
+    }
+    double *st = sh + 2 * (size_t)waves * units;
+    __syncthreads();
+    const int upg = SUB == 1 ? a.Cg / VEC : a.Cg;       // units of a group
+    const double m = (double)a.N * a.Cg;
+    for (int g = wave; g < gn; g += waves) {
+        double u = 0.0, v = 0.0;
+        for (int k = lane; k < waves * upg; k += 64) {
+            const int w = k / upg, j = k - w * upg;
+            const double *o = sh + 2 * ((size_t)w * units + g * upg + j);
+            u += o[0]; v += o[1];
+        }
+        u = wave_sum(u); v = wave_sum(v);
+        if (lane == 0) {
+            const double mean = u / m;
+            double var = v / m - mean * mean;
+            var = var < 0.0 ? 0.0 : var;                  // NaN passes
+            const double rstd = 1.0 / sqrt(var + (double)a.eps);
+            st[2 * g] = mean; st[2 * g + 1] = rstd;
+            double *o = a.stats + 2 * ((size_t)b * a.G + g0 + g);
+            o[0] = mean; o[1] = rstd;
+        }
+    }
+    __syncthreads();
+    load_stats(a, st, c, n, g0, p);
+    T *y = (T *)a.y + (size_t)b * a.N * a.C + c;
+#pragma unroll
+    for (int i = 0; i < RPT; ++i) {
+        const int row = ty + i * TY;
+        if (row < a.N && n > 0) {
+            float v[VEC], o[VEC];
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) v[e] = q[i].get(e);
+            gn_apply(a, p, v, o);
+            Col<DT, VEC>::store(y + (size_t)row * a.C, o, n);
+        }
+    }
+}
+
+template <int DT, int VEC, int SUB, int RPT>
+__global__ __launch_bounds__(1024) void gn_bwd_slab_kernel(const GnArgs a) {
+    typedef typename elem<DT>::t T;
+    extern __shared__ double sh[];
+    const int tid = threadIdx.x, X = 1 << a.lx, tx = tid & (X - 1), ty = tid >> a.lx, TY = blockDim.x >> a.lx;
+    const int waves = blockDim.x >> 6, wave = tid >> 6, lane = tid & 63;
+    const int item = slab_item(blockIdx.x, a.ranges, a.B * a.ranges), b = item / a.ranges, r = item - b * a.ranges;
+    const int g0 = r * a.gpr, gn = min(a.gpr, a.G - g0), c0 = g0 * a.Cg, c1 = c0 + gn * a.Cg;
+    const int c = c0 + tx * VEC, n = max(0, min(VEC, c1 - c));
+    const T *x = (const T *)a.x + (long long)b * a.sB + c;
+    const T *dy = (const T *)a.dy + (size_t)b * a.N * a.C + c;
+    Col<DT, VEC> q[RPT], d[RPT];
+    load_rows<RPT>(q, x, a.sN, ty, TY, a.N, n);
+    load_rows<RPT>(d, dy, a.C, ty, TY, a.N, n);
+    ColPar<VEC, SUB> p;
+    load_wb<DT>(a, c, n, p);
+    load_stats(a, a.stats + 2 * ((size_t)b * a.G + g0), c, n, g0, p);
+    float A[VEC], Bs[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) { A[e] = 0.f; Bs[e] = 0.f; }
+#pragma unroll
+    for (int i = 0; i < RPT; ++i) {
+        if (ty + i * TY < a.N) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                float xh;
+                const float dz = gn_dz(a, p, e, q[i].get(e), d[i].get(e), xh);
+                A[e] += dz; Bs[e] = fmaf(dz, xh, Bs[e]);
+            }
+        }
+    }
+    const int chans = X * VEC;
+    float *shf = (float *)sh;                            // [wave][chans][2]
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+        const float u = lanes_sum(A[e], a.lx), v = lanes_sum(Bs[e], a.lx);
+        if (lane < X) {
+            float *o = shf + 2 * ((size_t)wave * chans + tx * VEC + e);
+            o[0] = u; o[1] = v;
+        }
+    }
+    double *ch = sh + (size_t)waves * chans;             // [chans][2]: w A, w B
+    double *st = ch + 2 * (size_t)chans;                 // [gn][2]: S1, S2
+    __syncthreads();
+    for (int k = tid; k < c1 - c0; k += blockDim.x) {
+        double u = 0.0, v = 0.0;
+        for (int w = 0; w < waves; ++w) {
+            const float *o = shf + 2 * ((size_t)w * chans + k);
+            u += (double)o[0]; v += (double)o[1];
+        }
+        if (a.ab) {
+            float *o = a.ab + 2 * ((size_t)b * a.C + c0 + k);
+            o[0] = (float)u; o[1] = (float)v;
+        }
+        const float w = !a.w ? 1.f : a.wf32 ? ((const float *)a.w)[c0 + k] : ld_elem<DT>((const T *)a.w + c0 + k);
+        ch[2 * k] = u * w; ch[2 * k + 1] = v * w;
+    }
+    __syncthreads();
+    const double m = (double)a.N * a.Cg;
+    for (int g = wave; g < gn; g += waves) {
+        double u = 0.0, v = 0.0;
+        for (int k = lane; k < a.Cg; k += 64) { u += ch[2 * (g * a.Cg + k)]; v += ch[2 * (g * a.Cg + k) + 1]; }
+        u = wave_sum(u); v = wave_sum(v);
+        if (lane == 0) { st[2 * g] = u / m; st[2 * g + 1] = v / m; }
+    }
+    __syncthreads();
+    if (n == 0 || !a.dx) return;
+    float S1[SUB], S2[SUB];
+#pragma unroll
+    for (int e = 0; e < SUB; ++e) {
+        const int g = (c + min(e, n - 1)) / a.Cg - g0;
+        S1[e] = (float)st[2 * g]; S2[e] = (float)st[2 * g + 1];
+    }
+    T *dx = (T *)a.dx + (size_t)b * a.N * a.C + c;
+#pragma unroll
+    for (int i = 0; i < RPT; ++i) {
+        const int row = ty + i * TY;
+        if (row < a.N) {
+            float o[VEC];
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const int s = SUB == 1 ? 0 : e;
+                float xh;
+                const float dz = gn_dz(a, p, e, q[i].get(e), d[i].get(e), xh);
+                o[e] = (float)p.rstd[s] * (fmaf(dz, p.w[e], -S1[s]) - xh * S2[s]);
+            }
+            Col<DT, VEC>::store(dx + (size_t)row * a.C, o, n);
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------- split form
+// Workgroups of 256 threads: column block, cut and sample out of one index (a batch may pass a grid's 65535).
+__device__ __forceinline__ void split_item(const GnArgs &a, int &col, int &sp, int &b) {
+    const int i = blockIdx.x / a.cols;
+    col = blockIdx.x - i * a.cols;
+    b = i / a.S; sp = i - b * a.S;
+}
+
+template <int DT, int VEC, int SUB>
+__global__ __launch_bounds__(256) void gn_fwd_part_kernel(const GnArgs a) {
+    typedef typename elem<DT>::t T;
+    extern __shared__ double sh[];
+    const int tid = threadIdx.x, X = 1 << a.lx, tx = tid & (X - 1), ty = tid >> a.lx, TY = 256 >> a.lx;
+    const int wave = tid >> 6, lane = tid & 63;
+    int col, sp, b;
+    split_item(a, col, sp, b);
+    const int c = (col * X + tx) * VEC, n = max(0, min(VEC, a.C - c));
+    const int r0 = sp * a.rows, r1 = min(a.N, r0 + a.rows);
+    const T *x = (const T *)a.x + (long long)b * a.sB + c;
+    double s[SUB], s2[SUB];
+#pragma unroll
+    for (int e = 0; e < SUB; ++e) { s[e] = 0.0; s2[e] = 0.0; }
+    for (int row = r0 + ty; row < r1; row += 4 * TY) {
+        Col<DT, VEC> q[4];
+        load_rows<4>(q, x, a.sN, row, TY, r1, n, row);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (row + i * TY < r1) {
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    const double v = (double)q[i].get(e);
+                    const int k = SUB == 1 ? 0 : e;
+                    s[k] += v; s2[k] = fma(v, v, s2[k]);
+                }
+            }
+        }
+    }
+    // X <= 64: the rows of a wave by shuffles, the four waves through LDS
+    const int units = X * SUB;
+#pragma unroll
+    for (int e = 0; e < SUB; ++e) {
+        const double u = lanes_sum(s[e], a.lx), v = lanes_sum(s2[e], a.lx);
+        if (lane < X) {
+            double *o = sh + 2 * (wave * units + tx * SUB + e);
+            o[0] = u; o[1] = v;
+        }
+    }
+    __syncthreads();
+    const int per = SUB == 1 ? VEC : 1, total = a.C / per;          // channels of a unit, units of a row
+    double *out = a.part + 2 * ((size_t)b * a.S + sp) * total;
+    for (int k = tid; k < units; k += 256) {
+        const int u = col * units + k;
+        if (u < total) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+                out[2 * (size_t)u + j] = (sh[2 * k + j] + sh[2 * (units + k) + j]) + (sh[2 * (2 * units + k) + j] + sh[2 * (3 * units + k) + j]);
+        }
+    }
+}
+
+// one workgroup a (sample, group): statistics from the partial sums; per: channels of a unit
+__global__ __launch_bounds__(256) void gn_stats_kernel(const GnArgs a, int per) {
+    __shared__ double sh[4][2];
+    const int b = blockIdx.x / a.G, g = blockIdx.x - b * a.G, total = a.C / per, upg = a.Cg / per;
+    const double *in = a.part + 2 * ((size_t)b * a.S * total + (size_t)g * upg);
+    double u = 0.0, v = 0.0;
+    for (long long k = threadIdx.x; k < (long long)a.S * upg; k += 256) {
+        const long long s = k / upg, j = k - s * upg;
+        const double *o = in + 2 * (s * total + j);
+        u += o[0]; v += o[1];
+    }
+    u = wave_sum(u); v = wave_sum(v);
+    if ((threadIdx.x & 63) == 0) { sh[threadIdx.x >> 6][0] = u; sh[threadIdx.x >> 6][1] = v; }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        const double m = (double)a.N * a.Cg;
+        const double mean = ((sh[0][0] + sh[1][0]) + (sh[2][0] + sh[3][0])) / m;
+        double var = ((sh[0][1] + sh[1][1]) + (sh[2][1] + sh[3][1])) / m - mean * mean;
+        var = var < 0.0 ? 0.0 : var;
+        a.stats[2 * (size_t)blockIdx.x] = mean;
+        a.stats[2 * (size_t)blockIdx.x + 1] = 1.0 / sqrt(var + (double)a.eps);
+    }
+}
+
+template <int DT, int VEC, int SUB>
+__global__ __launch_bounds__(256) void gn_fwd_apply_kernel(const GnArgs a) {
+    typedef typename elem<DT>::t T;
+    const int tid = threadIdx.x, X = 1 << a.lx, tx = tid & (X - 1), ty = tid >> a.lx, TY = 256 >> a.lx;
+    int col, sp, b;
+    split_item(a, col, sp, b);
+    const int c = (col * X + tx) * VEC, n = max(0, min(VEC, a.C - c));
+    if (n == 0) return;
+    const int r0 = sp * a.rows, r1 = min(a.N, r0 + a.rows);
+    ColPar<VEC, SUB> p;
+    load_wb<DT>(a, c, n, p);
+    load_stats(a, a.stats + 2 * (size_t)b * a.G, c, n, 0, p);
+    const T *x = (const T *)a.x + (long long)b * a.sB + c;
+    T *y = (T *)a.y + (size_t)b * a.N * a.C + c;
+    for (int row = r0 + ty; row < r1; row += 4 * TY) {
+        Col<DT, VEC> q[4];
+        load_rows<4>(q, x, a.sN, row, TY, r1, n, row);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (row + i * TY < r1) {
+                float v[VEC], o[VEC];
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) v[e] = q[i].get(e);
+                gn_apply(a, p, v, o);
+                Col<DT, VEC>::store(y + (size_t)(row + i * TY) * a.C, o, n);
+            }
+        }
+    }
+}
+
+template <int DT, int VEC, int SUB>
+__global__ __launch_bounds__(256) void gn_bwd_part_kernel(const GnArgs a) {
+    typedef typename elem<DT>::t T;
+    extern __shared__ double sh[];
+    float *shf = (float *)sh;
+    const int tid = threadIdx.x, X = 1 << a.lx, tx = tid & (X - 1), ty = tid >> a.lx, TY = 256 >> a.lx;
+    const int wave = tid >> 6, lane = tid & 63;
+    int col, sp, b;
+    split_item(a, col, sp, b);
+    const int c = (col * X + tx) * VEC, n = max(0, min(VEC, a.C - c));
+    const int r0 = sp * a.rows, r1 = min(a.N, r0 + a.rows);
+    ColPar<VEC, SUB> p;
+    load_wb<DT>(a, c, n, p);
+    load_stats(a, a.stats + 2 * (size_t)b * a.G, c, n, 0, p);
+    const T *x = (const T *)a.x + (long long)b * a.sB + c;
+    const T *dy = (const T *)a.dy + (size_t)b * a.N * a.C + c;
+    float A[VEC], Bs[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) { A[e] = 0.f; Bs[e] = 0.f; }
+    if (n > 0) {
+        for (int row = r0 + ty; row < r1; row += 2 * TY) {
+            Col<DT, VEC> q[2], d[2];
+            load_rows<2>(q, x, a.sN, row, TY, r1, n, row);
+            load_rows<2>(d, dy, a.C, row, TY, r1, n, row);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                if (row + i * TY < r1) {
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) {
+                        float xh;
+                        const float dz = gn_dz(a, p, e, q[i].get(e), d[i].get(e), xh);
+                        A[e] += dz; Bs[e] = fmaf(dz, xh, Bs[e]);
+                    }
+                }
+            }
+        }
+    }
+    const int chans = X * VEC;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+        const float u = lanes_sum(A[e], a.lx), v = lanes_sum(Bs[e], a.lx);
+        if (lane < X) {
+            float *o = shf + 2 * (wave * chans + tx * VEC + e);
+            o[0] = u; o[1] = v;
+        }
+    }
+    __syncthreads();
+    float *out = (float *)a.part + 2 * ((size_t)b * a.S + sp) * a.C;
+    for (int k = tid; k < chans; k += 256) {
+        const int ch = col * chans + k;
+        if (ch < a.C) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+                out[2 * (size_t)ch + j] = (shf[2 * k + j] + shf[2 * (chans + k) + j]) + (shf[2 * (2 * chans + k) + j] + shf[2 * (3 * chans + k) + j]);
+        }
+    }
+}
+
+// one workgroup a (sample, group): the channels' A, B over the cuts, then the group's S1, S2.  A wave takes 16 channels x
+// 4 cuts at a time.
+template <int DT>
+__global__ __launch_bounds__(256) void gn_bwd_join_kernel(const GnArgs a) {
+    __shared__ double sh[4][2];
+    const int b = blockIdx.x / a.G, g = blockIdx.x - b * a.G, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const float *in = (const float *)a.part + 2 * ((size_t)b * a.S * a.C + (size_t)g * a.Cg);
+    double gu = 0.0, gv = 0.0;
+    for (int k0 = wave * 16; k0 < a.Cg; k0 += 64) {
+        const int k = k0 + (lane & 15);
+        double u = 0.0, v = 0.0;
+        if (k < a.Cg) {
+            for (int s = lane >> 4; s < a.S; s += 4) {
+                const float *o = in + 2 * ((size_t)s * a.C + k);
+                u += (double)o[0]; v += (double)o[1];
+            }
+        }
+        u += __shfl_xor(u, 16); v += __shfl_xor(v, 16);
+        u += __shfl_xor(u, 32); v += __shfl_xor(v, 32);
+        if (k < a.Cg && lane < 16) {
+            const int c = g * a.Cg + k;
+            if (a.ab) {
+                float *o = a.ab + 2 * ((size_t)b * a.C + c);
+                o[0] = (float)u; o[1] = (float)v;
+            }
+            const float w = !a.w ? 1.f : a.wf32 ? ((const float *)a.w)[c] : ld_elem<DT>((const typename elem<DT>::t *)a.w + c);
+            gu += u * w; gv += v * w;
+        }
+    }
+    gu = wave_sum(gu); gv = wave_sum(gv);
+    if (lane == 0) { sh[wave][0] = gu; sh[wave][1] = gv; }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        const double m = (double)a.N * a.Cg;
+        a.gsum[2 * (size_t)blockIdx.x] = (float)(((sh[0][0] + sh[1][0]) + (sh[2][0] + sh[3][0])) / m);
+        a.gsum[2 * (size_t)blockIdx.x + 1] = (float)(((sh[0][1] + sh[1][1]) + (sh[2][1] + sh[3][1])) / m);
+    }
+}
+
+template <int DT, int VEC, int SUB>
+__global__ __launch_bounds__(256) void gn_bwd_apply_kernel(const GnArgs a) {
+    typedef typename elem<DT>::t T;
+    const int tid = threadIdx.x, X = 1 << a.lx, tx = tid & (X - 1), ty = tid >> a.lx, TY = 256 >> a.lx;
+    int col, sp, b;
+    split_item(a, col, sp, b);
+    const int c = (col * X + tx) * VEC, n = max(0, min(VEC, a.C - c));
+    if (n == 0) return;
+    const int r0 = sp * a.rows, r1 = min(a.N, r0 + a.rows);
+    ColPar<VEC, SUB> p;
+    load_wb<DT>(a, c, n, p);
+    load_stats(a, a.stats + 2 * (size_t)b * a.G, c, n, 0, p);
+    float S1[SUB], S2[SUB];
+#pragma unroll
+    for (int e = 0; e < SUB; ++e) {
+        const float *o = a.gsum + 2 * ((size_t)b * a.G + (c + min(e, n - 1)) / a.Cg);
+        S1[e] = o[0]; S2[e] = o[1];
+    }
+    const T *x = (const T *)a.x + (long long)b * a.sB + c;
+    const T *dy = (const T *)a.dy + (size_t)b * a.N * a.C + c;
+    T *dx = (T *)a.dx + (size_t)b * a.N * a.C + c;
+    for (int row = r0 + ty; row < r1; row += 2 * TY) {
+        Col<DT, VEC> q[2], d[2];
+        load_rows<2>(q, x, a.sN, row, TY, r1, n, row);
+        load_rows<2>(d, dy, a.C, row, TY, r1, n, row);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            if (row + i * TY < r1) {
+                float o[VEC];
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    const int s = SUB == 1 ? 0 : e;
+                    float xh;
+                    const float dz = gn_dz(a, p, e, q[i].get(e), d[i].get(e), xh);
+                    o[e] = (float)p.rstd[s] * (fmaf(dz, p.w[e], -S1[s]) - xh * S2[s]);
+                }
+                Col<DT, VEC>::store(dx + (size_t)(row + i * TY) * a.C, o, n);
+            }
+        }
+    }
+}
+
+// db_c, dw_c = the samples' A_c, B_c summed in fp64: 16 channels x 64 sample lanes a workgroup
+template <int DT>
+__global__ __launch_bounds__(1024) void gn_dwdb_kernel(const GnArgs a, void *dw, void *db) {
+    __shared__ double sh[64][16][2];
+    const int cx = threadIdx.x & 15, ry = threadIdx.x >> 4, c = blockIdx.x * 16 + cx;
+    double u = 0.0, v = 0.0;
+    if (c < a.C) {
+        for (int b = ry; b < a.B; b += 64) {
+            const float *o = a.ab + 2 * ((size_t)b * a.C + c);
+            u += (double)o[0]; v += (double)o[1];
+        }
+    }
+    sh[ry][cx][0] = u; sh[ry][cx][1] = v;
+    __syncthreads();
+    for (int k = 32; k >= 1; k >>= 1) {
+        if (ry < k) { sh[ry][cx][0] += sh[ry + k][cx][0]; sh[ry][cx][1] += sh[ry + k][cx][1]; }
+        __syncthreads();
+    }
+    if (ry == 0 && c < a.C) {
+        const float A = (float)sh[0][cx][0], B = (float)sh[0][cx][1];
+        if (db) { if (a.wf32) ((float *)db)[c] = A; else st_elem<DT>((typename elem<DT>::t *)db + c, A); }
+        if (dw) { if (a.wf32) ((float *)dw)[c] = B; else st_elem<DT>((typename elem<DT>::t *)dw + c, B); }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------- plan
+// rpt rows a thread can hold: forward 16 (64 registers of data), backward 8 of x and of dy.
+struct GnPlan { int vec, sub, slab, lx, gpr, ranges, threads, rpt, cols, S, rows; };
+
+static inline int log2_up(int n) { int k = 0; while ((1 << k) < n) ++k; return k; }
+
+static GnPlan gn_plan(int B, int N, int C, int G, int dt, int bwd) {
+    GnPlan p;
+    const int Cg = C / G, e = dt == PNGPD_F32 ? 4 : 2, wide = 16 / e;
+    p.vec = C >= wide ? wide : 1;
+    p.sub = Cg % p.vec == 0 ? 1 : p.vec;
+    // slab: columns of a range = 128 bytes of a row (whole cache lines), or one group where that is more (up to 512
+    // bytes); halved, down to 32 bytes, while the rows do not fit or the card (256 CUs) is not filled
+    p.slab = 0; p.gpr = p.ranges = p.threads = p.rpt = 0;
+    const int most = bwd ? 8 : 16;
+    for (int bytes = 128; bytes >= 32; bytes >>= 1) {
+        int gpr = bytes / e / Cg;
+        if (gpr < 1) gpr = 1;
+        if (gpr > G) gpr = G;
+        const int cols = (gpr * Cg + p.vec - 1) / p.vec;
+        const int lx = log2_up(cols);
+        if (lx > 5) break;
+        const int ranges = (G + gpr - 1) / gpr;
+        const long long need = ((long long)N + most - 1) / most << lx;
+        if (need <= 1024) {
+            p.slab = 1; p.gpr = gpr; p.ranges = ranges; p.lx = lx;
+            if ((long long)B * ranges >= 256) break;
+        }
+        if (gpr == 1) break;
+    }
+    if (p.slab) {
+        // as many threads as there are rows for, up to 1024; then the rows a thread holds
+        long long t = (long long)N << p.lx;
+        int th = 64;
+        while (th < t && th < 1024) th <<= 1;
+        p.threads = th;
+        int r = (int)(((long long)N + (th >> p.lx) - 1) / (th >> p.lx));
+        p.rpt = r <= 2 ? 2 : r <= 4 ? 4 : r <= 8 ? 8 : 16;
+        p.cols = p.S = p.rows = 0;
+    }
+    if (!p.slab) {
+        const int cols = (C + p.vec - 1) / p.vec;
+        p.lx = log2_up(cols);
+        if (p.lx > 6) p.lx = 6;
+        p.cols = (cols + (1 << p.lx) - 1) >> p.lx;
+        // cuts: 2048 workgroups (8 a CU), of at least 4 rows a thread
+        const int TY = 256 >> p.lx;
+        long long S = 2048 / ((long long)B * p.cols);
+        const long long top = ((long long)N + 4 * TY - 1) / (4 * TY);
+        if (S > top) S = top;
+        if (S < 1) S = 1;
+        p.rows = (int)(((long long)N + S - 1) / S);
+        p.S = (N + p.rows - 1) / p.rows;
+    }
+    return p;
+}
+
+static size_t gn_part_bytes(const GnPlan &p, int B, int C, int bwd) {
+    if (p.slab) return 0;
+    return (size_t)B * p.S * (bwd ? (size_t)C * 8 : (size_t)(p.sub == 1 ? C / p.vec : C) * 16);
+}
+
+// workgroups of one launch past the grid's (and the kernels' int) range
+static bool gn_too_many(const GnPlan &p, int B, int G) {
+    const long long most = 0x7fffffffll;
+    return p.slab ? (long long)B * p.ranges > most : (long long)p.cols * p.S * B > most || (long long)B * G > most;
+}
+
+static bool gn_bad(const void *x, int dt, int B, int N, int C, int G, int act, const void *w, int wdt, float eps) {
+    return !x || dt < PNGPD_F32 || dt > PNGPD_F16 || B <= 0 || N <= 0 || C <= 0 || G <= 0 || C % G ||
+           act < PNGPD_ACT_NONE || act > PNGPD_ACT_GELU || !(eps >= 0.f) || (wdt != PNGPD_F32 && wdt != dt);
+}
+
+template <int DT, int VEC, int SUB>
+static int gn_fwd_launch(GnArgs &a, const GnPlan &p, hipStream_t st) {
+    if (p.slab) {
+        const size_t lds = (size_t)(p.threads / 64) * (1 << p.lx) * SUB * 16 + (size_t)p.gpr * 16;
+#define GN_SLAB(R) { const int rc = pngpd_allow_lds((const void *)gn_fwd_slab_kernel<DT, VEC, SUB, R>, lds); if (rc) return rc; \
+        hipLaunchKernelGGL((gn_fwd_slab_kernel<DT, VEC, SUB, R>), dim3((unsigned)(a.B * p.ranges)), dim3(p.threads), lds, st, a); }
+        if (p.rpt == 2) GN_SLAB(2) else if (p.rpt == 4) GN_SLAB(4) else if (p.rpt == 8) GN_SLAB(8) else GN_SLAB(16)
+#undef GN_SLAB
+        return pngpd_launch_status();
+    }
+    const dim3 grid((unsigned)(p.cols * p.S * a.B));
+    hipLaunchKernelGGL((gn_fwd_part_kernel<DT, VEC, SUB>), grid, dim3(256), (size_t)4 * (1 << p.lx) * SUB * 16, st, a);
+    hipLaunchKernelGGL(gn_stats_kernel, dim3((unsigned)(a.B * a.G)), dim3(256), 0, st, a, SUB == 1 ? VEC : 1);
+    hipLaunchKernelGGL((gn_fwd_apply_kernel<DT, VEC, SUB>), grid, dim3(256), 0, st, a);
+    return pngpd_launch_status();
+}
+
+template <int DT, int VEC, int SUB>
+static int gn_bwd_launch(GnArgs &a, const GnPlan &p, void *dw, void *db, hipStream_t st) {
+    if (p.slab) {
+        const size_t chans = (size_t)(1 << p.lx) * VEC;
+        const size_t lds = (size_t)(p.threads / 64) * chans * 8 + chans * 16 + (size_t)p.gpr * 16;
+#define GN_SLAB(R) { const int rc = pngpd_allow_lds((const void *)gn_bwd_slab_kernel<DT, VEC, SUB, R>, lds); if (rc) return rc; \
+        hipLaunchKernelGGL((gn_bwd_slab_kernel<DT, VEC, SUB, R>), dim3((unsigned)(a.B * p.ranges)), dim3(p.threads), lds, st, a); }
+        if (p.rpt == 2) GN_SLAB(2) else if (p.rpt == 4) GN_SLAB(4) else GN_SLAB(8)
+#undef GN_SLAB
+    } else {
+        const dim3 grid((unsigned)(p.cols * p.S * a.B));
+        hipLaunchKernelGGL((gn_bwd_part_kernel<DT, VEC, SUB>), grid, dim3(256), (size_t)4 * (1 << p.lx) * VEC * 8, st, a);
+        hipLaunchKernelGGL(gn_bwd_join_kernel<DT>, dim3((unsigned)(a.B * a.G)), dim3(256), 0, st, a);
+        if (a.dx) hipLaunchKernelGGL((gn_bwd_apply_kernel<DT, VEC, SUB>), grid, dim3(256), 0, st, a);
+    }
+    if (a.ab) hipLaunchKernelGGL(gn_dwdb_kernel<DT>, dim3((unsigned)((a.C + 15) / 16)), dim3(1024), 0, st, a, dw, db);
+    return pngpd_launch_status();
+}
+
+#define GN_DISPATCH(call) \
+    if (dtype == PNGPD_F32) return p.vec == 1 ? call(PNGPD_F32, 1, 1) : p.sub == 1 ? call(PNGPD_F32, 4, 1) : call(PNGPD_F32, 4, 4); \
+    if (dtype == PNGPD_BF16) return p.vec == 1 ? call(PNGPD_BF16, 1, 1) : p.sub == 1 ? call(PNGPD_BF16, 8, 1) : call(PNGPD_BF16, 8, 8); \
+    return p.vec == 1 ? call(PNGPD_F16, 1, 1) : p.sub == 1 ? call(PNGPD_F16, 8, 1) : call(PNGPD_F16, 8, 8);
+
+extern "C" {
+
+size_t pngpd_group_norm_workspace_bytes(int B, int N, int C, int G, int dtype, int backward) {
+    if (B <= 0 || N <= 0 || C <= 0 || G <= 0 || C % G || dtype < PNGPD_F32 || dtype > PNGPD_F16) return 0;
+    const GnPlan p = gn_plan(B, N, C, G, dtype, backward != 0);
+    size_t n = (gn_part_bytes(p, B, C, backward != 0) + 255) & ~(size_t)255;
+    if (backward) n += (((size_t)B * C * 8 + 255) & ~(size_t)255) + (p.slab ? 0 : (size_t)B * G * 8);
+    return n;
+}
+
+int pngpd_group_norm_fwd(const void *x, int dtype, int B, int N, int C, long long stride_b, long long stride_n, int G,
+                         const void *w, const void *b, int wdtype, float eps, int act, void *y, double *stats,
+                         void *workspace, size_t workspace_bytes, void *stream) {
+    if (gn_bad(x, dtype, B, N, C, G, act, w, wdtype, eps) || !y || !stats) return PNGPD_ERR_INVALID_ARG;
+    const GnPlan p = gn_plan(B, N, C, G, dtype, 0);
+    if (gn_too_many(p, B, G)) return PNGPD_ERR_UNSUPPORTED;
+    if (workspace_bytes < pngpd_group_norm_workspace_bytes(B, N, C, G, dtype, 0) || (!p.slab && !workspace)) return PNGPD_ERR_WORKSPACE;
+    GnArgs a = {};
+    a.x = x; a.w = w; a.b = b; a.y = y; a.stats = stats; a.part = (double *)workspace;
+    a.sB = stride_b; a.sN = stride_n; a.B = B; a.N = N; a.C = C; a.G = G; a.Cg = C / G; a.act = act;
+    a.wf32 = wdtype == PNGPD_F32; a.eps = eps; a.lx = p.lx; a.gpr = p.gpr; a.ranges = p.ranges; a.cols = p.cols; a.S = p.S; a.rows = p.rows;
+    hipStream_t st = (hipStream_t)stream;
+#define GN_CALL(D, V, U) gn_fwd_launch<D, V, U>(a, p, st)
+    GN_DISPATCH(GN_CALL)
+#undef GN_CALL
+}
+
+int pngpd_group_norm_bwd(const void *x, int dtype, int B, int N, int C, long long stride_b, long long stride_n, int G,
+                         const void *w, const void *b, int wdtype, float eps, int act, const double *stats,
+                         const void *dy, void *dx, void *dw, void *db, void *workspace, size_t workspace_bytes,
+                         void *stream) {
+    if (gn_bad(x, dtype, B, N, C, G, act, w, wdtype, eps) || !stats || !dy) return PNGPD_ERR_INVALID_ARG;
+    if (!dx && !dw && !db) return PNGPD_OK;
+    const GnPlan p = gn_plan(B, N, C, G, dtype, 1);
+    if (gn_too_many(p, B, G)) return PNGPD_ERR_UNSUPPORTED;
+    if (workspace_bytes < pngpd_group_norm_workspace_bytes(B, N, C, G, dtype, 1) || !workspace) return PNGPD_ERR_WORKSPACE;
+    GnArgs a = {};
+    char *ws = (char *)workspace;
+    const size_t part = (gn_part_bytes(p, B, C, 1) + 255) & ~(size_t)255;
+    a.x = x; a.dy = dy; a.w = w; a.b = b; a.dx = dx; a.stats = (double *)stats; a.part = (double *)ws;
+    a.ab = dw || db ? (float *)(ws + part) : nullptr;
+    a.gsum = (float *)(ws + part + (((size_t)B * C * 8 + 255) & ~(size_t)255));
+    a.sB = stride_b; a.sN = stride_n; a.B = B; a.N = N; a.C = C; a.G = G; a.Cg = C / G; a.act = act;
+    a.wf32 = wdtype == PNGPD_F32; a.eps = eps; a.lx = p.lx; a.gpr = p.gpr; a.ranges = p.ranges; a.cols = p.cols; a.S = p.S; a.rows = p.rows;
+    hipStream_t st = (hipStream_t)stream;
+#define GN_CALL(D, V, U) gn_bwd_launch<D, V, U>(a, p, dw, db, st)
+    GN_DISPATCH(GN_CALL)
+#undef GN_CALL
+}
+
+}  // extern "C"

@@ -20,7 +20,7 @@ On ``--cuda`` the optimizer is ``optim.FlatAdam`` — the same Adam (main_1v.py:
 launch per step, gradients written in place by the fused backward.  Running accuracy is accumulated on the device
 and read at ``--log-interval`` / epoch end instead of the reference's per-batch ``.cpu()`` (main_1v.py:78).
 Additive flags: ``--seed --num-workers --synthetic --max-batches --persistent-optimizer --precision --hip-graph
---device-data``.
+--device-data --clip-grad``.
 """
 import argparse
 import json
@@ -37,6 +37,7 @@ from torch.optim.lr_scheduler import StepLR
 
 from . import ddp
 from .model.pointnet import PointNetCls
+from .optim import clip_grad_norm_
 
 VARIANTS = {
     "1v": dict(dataset="PointGraspOneViewDataset", fullview=False, k=2, num_points=750, good=0.6, bad=0.6,
@@ -85,6 +86,8 @@ def build_parser():
                    help="--cuda: arithmetic of the trunk contractions. fp32 = exact (default); bf16x3 = 3-term split "
                         "bf16 products on the bf16 matrix cores (meets the fp32 parity bars); bf16 = plain bf16 "
                         "operands and bf16 z2/g2 tiles (BASELINE configs[2]; does NOT meet 1e-3 in training)")
+    p.add_argument("--clip-grad", type=float, default=0.0, metavar="NORM",
+                   help="clip the gradients of every step to this global 2-norm (0: no clipping, as the reference)")
     p.add_argument("--log-dir", type=str, default="./assets/log/")
     return p
 
@@ -243,6 +246,8 @@ def save_model(model, path, world=1):
 def run(variant, argv=None):
     cfg = VARIANTS[variant]
     args = build_parser().parse_args(argv)
+    if not args.clip_grad >= 0.0:
+        raise SystemExit(f"--clip-grad must not be negative, got {args.clip_grad}")
     args.cuda = args.cuda if torch.cuda.is_available else False      # sic: main_1v.py:35 never calls it
     os.makedirs(args.model_path, exist_ok=True)
     # Debug switch shared with bench.py (never set by a launcher): every rank on cuda:0 over gloo, so that the
@@ -314,13 +319,19 @@ def run(variant, argv=None):
             # the fused backward; for a captured graph the lr lives in a device tensor (StepLR fills it in place)
             from .optim import FlatAdam
             lr = torch.tensor(float(args.lr), device=device) if use_graph else args.lr
-            state["optimizer"] = FlatAdam(model.parameters(), lr=lr, capturable=use_graph)
+            state["optimizer"] = FlatAdam(model.parameters(), lr=lr, capturable=use_graph,
+                                          max_grad_norm=args.clip_grad or None)
             if averager is not None:
                 averager.attach(state["optimizer"])
         else:
             state["optimizer"] = optim.Adam(model.parameters(), lr=args.lr)
         state["scheduler"] = StepLR(state["optimizer"], step_size=30, gamma=0.5)
         state["graph"] = None
+
+    def clip():
+        """--clip-grad for the CPU's torch.optim.Adam; FlatAdam clips inside its update."""
+        if args.clip_grad and not args.cuda:
+            clip_grad_norm_(model.parameters(), args.clip_grad)
 
     recreate = cfg["recreate_optimizer"] and not args.persistent_optimizer
     if not recreate:
@@ -378,6 +389,7 @@ def run(variant, argv=None):
                 if total is not None:
                     optimizer.step(grad_div=total)
                 else:
+                    clip()
                     optimizer.step()
             elif not runnable:
                 if n_local == 1:
@@ -393,6 +405,7 @@ def run(variant, argv=None):
                 optimizer.zero_grad()
                 loss, output, _ = forward_loss(data, target, "mean")      # main_1v.py:73-74
                 loss_backward(loss)                                       # :75
+                clip()
                 optimizer.step()
             if output is not None:
                 pred = output.data.max(1, keepdim=True)[1]

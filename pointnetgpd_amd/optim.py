@@ -16,6 +16,8 @@ The update is torch's single-tensor Adam in fp32 (torch/optim/adam.py ``_single_
 ``state`` entries (``step``, ``exp_avg``, ``exp_avg_sq``) are views of the flat moments, so ``state_dict()`` has the
 layout of ``torch.optim.Adam``'s and checkpoints move between the two.
 """
+import ctypes
+import math
 import weakref
 
 import torch
@@ -117,14 +119,99 @@ def ungroup(params):
     _GROUPS.pop(id(params[0]), None)
 
 
+_NORM_KINDS = {2.0: 2, 1.0: 1, math.inf: 0}
+_GRAD_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # PNGPD_F32, PNGPD_BF16, PNGPD_F16
+
+
+def _dense(t):
+    """Whether t's elements fill one range of memory, each once (a permutation of a contiguous tensor)."""
+    if t.is_contiguous():
+        return True
+    want = 1
+    for stride, size in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n > 1):
+        if stride != want:
+            return False
+        want *= size
+    return True
+
+
+@torch.no_grad()
+def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
+    """Clip the gradients of ``parameters`` (a tensor or an iterable of tensors; those without ``.grad`` are passed over)
+    in place by their global norm, as ``torch.nn.utils.clip_grad_norm_`` does: the norm over every element of all of
+    them as if one vector, then ``grad *= min(1, max_norm / (norm + 1e-6))``.  Returns the norm before clipping, a
+    float32 scalar on the gradients' device that no host wait has touched.
+
+    Gradients: float32, bfloat16 and float16, in any mix, on one device.  ``norm_type`` 2, 1 or ``math.inf``.  Two
+    launches for up to 128 tensors (sums in float64, in a fixed order: the same gradients give the same bits).  A
+    gradient reached twice (one parameter listed twice, views of one storage) is refused.  A NaN or infinite norm
+    reaches the gradients through the factor, or raises with ``error_if_nonfinite`` (which waits for the device).
+    ``max_norm=math.inf`` returns the norm and leaves the gradients alone.
+    CPU gradients go to ``torch.nn.utils.clip_grad_norm_``.  With ``FlatAdam(max_grad_norm=...)`` no call is needed:
+    the update clips."""
+    params = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
+    max_norm, norm_type = float(max_norm), float(norm_type)
+    if not max_norm >= 0.0:
+        raise ValueError(f"clip_grad_norm_: max_norm must not be negative, got {max_norm}")
+    if norm_type not in _NORM_KINDS:
+        raise ValueError(f"clip_grad_norm_: norm_type must be 2, 1 or inf, got {norm_type}")
+    grads = [p.grad for p in params if p.grad is not None]
+    if not grads:
+        return torch.tensor(0.0)
+    dev = grads[0].device
+    if any(g.device != dev for g in grads):
+        raise RuntimeError("clip_grad_norm_: the gradients are on more than one device")
+    if dev.type != "cuda":
+        return torch.nn.utils.clip_grad_norm_(params, max_norm, norm_type, error_if_nonfinite)
+    for g in grads:
+        if g.layout != torch.strided or g.dtype not in _GRAD_TYPES:
+            raise RuntimeError("clip_grad_norm_: expected dense float32, bfloat16 or float16 gradients, got "
+                               f"{g.dtype}, {g.layout}")
+        if 0 in g.stride() and any(st == 0 and k > 1 for st, k in zip(g.stride(), g.shape)):
+            raise RuntimeError("clip_grad_norm_: a gradient's elements share memory (an expanded tensor)")
+    # a gradient with gaps (a column of a wider buffer) is clipped in a copy and written back
+    work = [g if _dense(g) else g.contiguous() for g in grads]
+    spans = sorted((g.data_ptr(), g.numel() * g.element_size()) for g in work if g.numel())
+    if any(a + n > b for (a, n), (b, _) in zip(spans, spans[1:])) or len(set(map(id, grads))) != len(grads):
+        raise RuntimeError("clip_grad_norm_: two of the gradients share memory (a parameter listed twice?)")
+    n = len(work)
+    lib = _lib.load()
+    total = torch.empty((), device=dev, dtype=torch.float32)
+    nbytes = lib.pngpd_grad_clip_workspace_bytes(n)
+    ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
+    ptr = (ctypes.c_void_p * n)(*[g.data_ptr() for g in work])
+    num = (ctypes.c_longlong * n)(*[g.numel() for g in work])
+    typ = (ctypes.c_int * n)(*[_GRAD_TYPES[g.dtype] for g in work])
+    stream = torch.cuda.current_stream(dev).cuda_stream
+    with _lib.device_guard(dev):
+        for bound in (math.inf, max_norm) if error_if_nonfinite else (max_norm,):       # inf: the norm alone
+            _lib.check(lib.pngpd_grad_clip(ptr, num, typ, n, _NORM_KINDS[norm_type], bound, total.data_ptr(), ws.data_ptr(),
+                                           nbytes, stream), "grad_clip")
+            if error_if_nonfinite and not math.isfinite(float(total)):
+                raise RuntimeError(f"clip_grad_norm_: the norm of the gradients is {float(total)}; nothing was clipped")
+    for g, c in zip(grads, work):
+        if c is not g:
+            g.copy_(c)
+    torch.autograd.graph.increment_version(grads)
+    return total
+
+
 class FlatAdam(torch.optim.Optimizer):
     """Bias correction uses ONE step count for the whole buffer (``_step``; torch.optim.Adam keeps one per parameter).
     They agree whenever every parameter takes part in every step — the case for a PointNetCls.  A fused piece that sat
     out k steps (its slices are skipped, as torch skips ``grad is None``) resumes with the GLOBAL count in its bias
     correction where torch would use its own smaller count: after the first few hundred steps the two corrections are
-    both within 1e-3 of 1, before that the resumed piece takes slightly smaller steps than torch's would."""
+    both within 1e-3 of 1, before that the resumed piece takes slightly smaller steps than torch's would.
 
-    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, capturable=False):
+    ``max_grad_norm``: every step first clips the gradients it uses (after ``grad_scale`` / ``grad_div``) by their global
+    2-norm, as ``clip_grad_norm_`` before the step would; the factor is applied inside the update, the gradient buffer
+    keeps the unclipped values (bias corrections from float64: updates differ from the plain step's by up to 1e-4 of
+    themselves in the first steps), and ``grad_norm`` holds the norm (a device scalar that no host wait has
+    touched).  The parameters a step leaves alone do not count."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, capturable=False, max_grad_norm=None):
+        if max_grad_norm is not None and not float(max_grad_norm) >= 0.0:
+            raise ValueError(f"FlatAdam: max_grad_norm must not be negative, got {max_grad_norm}")
         params = [p for p in params]
         if not params:
             raise ValueError("optimizer got an empty parameter list")
@@ -146,6 +233,8 @@ class FlatAdam(torch.optim.Optimizer):
         z = lambda: torch.zeros(off, device=dev, dtype=torch.float32)
         self.flat_p, self.flat_g, self.flat_m, self.flat_v = z(), z(), z(), z()
         self.capturable = bool(capturable)
+        self.max_grad_norm = None if max_grad_norm is None else float(max_grad_norm)
+        self.grad_norm = torch.zeros((), device=dev, dtype=torch.float32) if max_grad_norm is not None else None
         # device-resident step count / learning rate for captured graphs (StepLR rewrites group["lr"] in place)
         self.step_dev = torch.zeros((), device=dev, dtype=torch.float32) if capturable else None
         self._step = 0
@@ -248,6 +337,19 @@ class FlatAdam(torch.optim.Optimizer):
         with _lib.device_guard(self.device):
             if self.step_dev is not None:
                 _lib.check(lib.pngpd_adam_step_inc(self.step_dev.data_ptr(), stream), "adam_step_inc")
+            if self.max_grad_norm is not None and runs:
+                k = len(runs)
+                nbytes = lib.pngpd_grad_clip_workspace_bytes(k)
+                ws = torch.empty(nbytes, device=self.device, dtype=torch.uint8)
+                _lib.check(lib.pngpd_adam_flat_clip(self.flat_p.data_ptr(), self.flat_g.data_ptr(), self.flat_m.data_ptr(),
+                                                    self.flat_v.data_ptr(), (ctypes.c_longlong * k)(*[lo for lo, _ in runs]),
+                                                    (ctypes.c_longlong * k)(*[n for _, n in runs]), k, lr_host, lr_dev,
+                                                    float(b1), float(b2), float(eps), float(self._step),
+                                                    self.step_dev.data_ptr() if self.step_dev is not None else None,
+                                                    float(grad_scale), grad_div.data_ptr() if grad_div is not None else None,
+                                                    self.max_grad_norm, self.grad_norm.data_ptr(), ws.data_ptr(), nbytes,
+                                                    stream), "adam_flat_clip")
+                runs = []
             for lo, n in runs:
                 h = lo * 4
                 _lib.check(lib.pngpd_adam_flat(self.flat_p.data_ptr() + h, self.flat_g.data_ptr() + h,
