@@ -58,6 +58,13 @@ enum {
     PNGPD_F16 = 2
 };
 
+/* Reductions of pngpd_lce_*. */
+enum {
+    PNGPD_REDUCE_NONE = 0,
+    PNGPD_REDUCE_MEAN = 1,       /* over the rows whose target is not ignore_index      */
+    PNGPD_REDUCE_SUM = 2
+};
+
 /* Activations of pngpd_group_norm_*. */
 enum {
     PNGPD_ACT_NONE = 0,
@@ -447,7 +454,7 @@ typedef struct pngpd_head_train {
  * sink: >= 512 x CU-count floats of scratch (never written).                                                          */
 int pngpd_probe_mfma_rate(int dtype, int waves_per_simd, int iters, float *sink, long long *flops_out, void *stream);
 
-size_t pngpd_struct_bytes(int which);   /* sizeof of pngpd_trunk_train_t (0) / pngpd_head_train_t (1) / pngpd_fold_model_t (2): FFI self-check */
+size_t pngpd_struct_bytes(int which);   /* sizeof of pngpd_trunk_train_t (0) / pngpd_head_train_t (1) / pngpd_fold_model_t (2) / pngpd_lce_t (3): FFI self-check */
 size_t pngpd_head_train_save_bytes(const pngpd_head_train_t *a);        /* reads B, H1, H2 */
 size_t pngpd_head_train_scratch_bytes(const pngpd_head_train_t *a);     /* reads B, H1, H2, k */
 int pngpd_head_train_fwd(const pngpd_head_train_t *a, void *stream);
@@ -482,6 +489,31 @@ int pngpd_adam_flat_clip(float *p, const float *g, float *m, float *v, const lon
                          int runs, float lr, const float *lr_dev, double beta1, double beta2, float eps, float step,
                          const float *step_dev, float gscale, const float *gdiv_dev, float max_norm, float *total_norm,
                          void *workspace, size_t workspace_bytes, void *stream);
+
+/* Softmax cross entropy of a linear classifier, z = x W^T + bias, whose logits are never kept:
+ *   loss_t = log sum_v exp(z[t,v]) - (1 - smoothing) z[t,target_t] - smoothing mean_v z[t,v],  0 where target_t is ignore_index
+ * (F.nll_loss(F.log_softmax(F.linear(x, W, bias))), main_1v.py:73-74 with pointnet.py:193-194, for a head of any width).
+ * Rows' channels adjacent; ldx, ldw in elements, any (rows at 16-byte addresses of whole 16 bytes are read in place,
+ * others are copied into the workspace first).  A target outside [0,V) that is not ignore_index gives a NaN loss and NaN
+ * gradients.  Deterministic.  The workspace is bounded in V (a piece's gradient of the logits, 256 MB at most unless 256
+ * classes of all rows take more).
+ *   forward   writes stat (T,2) and kept (1), which the backward call reads, and loss: (T), or one value
+ *   backward  reads dloss (T, or one value); dx (T,D), dw (V,D), db (V) contiguous, each NULL: not wanted             */
+typedef struct pngpd_lce {
+    const void *x, *w, *bias;      /* (T,D), (V,D) of dtype; (V) of bias_dtype (= dtype or PNGPD_F32), NULL: none  */
+    const int64_t *target;         /* (T)                                                                          */
+    int64_t ldx, ldw, ignore_index;
+    int T, D, V, dtype, bias_dtype, reduction;
+    float smoothing;
+    float *stat, *kept, *loss;
+    const float *dloss;
+    void *dx, *dw, *db;
+    void *workspace;               /* 256-byte aligned; pngpd_lce_workspace_bytes of the same descriptor           */
+    size_t workspace_bytes;
+} pngpd_lce_t;
+size_t pngpd_lce_workspace_bytes(const pngpd_lce_t *a, int backward);
+int pngpd_lce_fwd(const pngpd_lce_t *a, void *stream);
+int pngpd_lce_bwd(const pngpd_lce_t *a, void *stream);
 
 /* Group norm + activation over channels-last features, y = act((x - mean) / sqrt(var + eps) * w + b) with mean and
  * (biased) variance over the N rows and C / G channels of each of the G groups of a sample.

@@ -3,10 +3,15 @@
 * ``group_norm_act``       — group norm with an activation over channels-last point features.  The trunks' BatchNorm
                              (PointNetGPD/model/pointnet.py:29-31,144-147) needs two samples a rank and keeps statistics of
                              its replica; this one's are of each sample alone.
+* ``linear_cross_entropy`` — the loss of a linear classifier of any width, F.nll_loss(F.log_softmax(F.linear(...)))
+                             (main_1v.py:73-74, pointnet.py:193-194), without its logits ever being kept: codebooks of
+                             grasps, one class for each point of a scene.
 
 CUDA tensors run the HIP kernels of libpngpd (a missing library raises), CPU tensors the same formulas in ATen operations.
 The gradients are those of the formulas; they are not differentiable again.
 """
+import ctypes
+
 import torch
 from torch.autograd.function import once_differentiable
 
@@ -128,3 +133,113 @@ def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, act="none"):
     if v.stride(2) != 1 and C > 1:
         v = v.contiguous()
     return GroupNormActFn.apply(v, weight, bias, groups, eps, ACTIVATIONS[act]).view(x.shape)
+
+
+# ------------------------------------------------------------------------------------------------ linear cross entropy
+REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
+
+
+def _lce_call(entry, a, ref, backward):
+    """One C call on ``ref``'s device and current stream with a workspace of its own."""
+    lib, dev = _lib.load(), ref.device
+    ws = _bytes(dev, lib.pngpd_lce_workspace_bytes(ctypes.addressof(a), backward))
+    a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+    with _lib.device_guard(dev):
+        _lib.check(getattr(lib, entry)(ctypes.addressof(a), torch.cuda.current_stream(dev).cuda_stream), entry)
+
+
+class LinearCrossEntropyFn(torch.autograd.Function):
+    """x (T,D), w (V,D), target (T) -> loss (T) or (); T, V, D > 0, channels adjacent."""
+
+    @staticmethod
+    def forward(ctx, x, w, bias, target, reduction, ignore_index, smoothing):
+        dev, f32 = x.device, torch.float32
+        T, D = x.shape
+        bias = bias.detach().contiguous() if bias is not None else None
+        stat, kept = torch.empty(T, 2, device=dev, dtype=f32), torch.empty((), device=dev, dtype=f32)
+        loss = torch.empty((T,) if reduction == 0 else (), device=dev, dtype=f32)
+        ctx.scalars = (reduction, ignore_index, smoothing)
+        ctx.save_for_backward(x, w, target, stat, kept, *(() if bias is None else (bias,)))
+        a = LinearCrossEntropyFn._args(ctx.scalars, x, w, bias, target, stat, kept)
+        a.loss = loss.data_ptr()
+        _lce_call("pngpd_lce_fwd", a, x, 0)
+        return loss
+
+    @staticmethod
+    def _args(scalars, x, w, bias, target, stat, kept):
+        a = _lib.LceArgs()
+        a.x, a.w, a.target, a.stat, a.kept = (t.data_ptr() for t in (x, w, target, stat, kept))
+        a.bias = None if bias is None else bias.data_ptr()
+        (a.T, a.D), a.V = x.shape, w.shape[0]
+        a.ldx, a.ldw = (t.stride(0) if t.shape[0] > 1 else t.shape[1] for t in (x, w))
+        a.dtype = DTYPES[x.dtype]
+        a.bias_dtype = a.dtype if bias is None else DTYPES[bias.dtype]
+        a.reduction, a.ignore_index, a.smoothing = scalars
+        return a
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dloss):
+        x, w, target, stat, kept, *bias = ctx.saved_tensors
+        bias = bias[0] if bias else None
+        need = ctx.needs_input_grad
+        dloss = dloss.float().contiguous()
+        dx = torch.empty(x.shape, device=x.device, dtype=x.dtype) if need[0] else None
+        dw = torch.empty(w.shape, device=x.device, dtype=w.dtype) if need[1] else None
+        db = torch.empty_like(bias) if bias is not None and need[2] else None
+        a = LinearCrossEntropyFn._args(ctx.scalars, x, w, bias, target, stat, kept)
+        a.dloss = dloss.data_ptr()
+        a.dx, a.dw, a.db = (None if t is None else t.data_ptr() for t in (dx, dw, db))
+        _lce_call("pngpd_lce_bwd", a, x, 1)
+        return dx, dw, db, None, None, None, None
+
+
+def linear_cross_entropy(x, weight, target, bias=None, reduction="mean", ignore_index=-100, label_smoothing=0.0):
+    """``F.cross_entropy(F.linear(x, weight, bias), target, ...)`` without the logits: x (..., D), weight (V, D), target
+    (...) int64, bias (V) or None.  The forward pass reduces the logits tile by tile, the backward pass computes them again
+    a piece of the classes at a time, so memory grows with the rows and not with rows x classes.
+
+    Returns float32: a scalar for ``reduction`` "mean" (over the rows whose target is not ``ignore_index``; NaN if there is
+    none, with zero gradients) or "sum", target's shape for "none".  Ignored rows have loss 0 and no gradient, whatever
+    their x holds.  ``label_smoothing`` in [0, 1] as in ``F.cross_entropy``.  A target outside [0, V) gives a NaN loss
+    and NaN gradients (there is no host check: it would wait for the device).  x and weight of one type, float32 (exact
+    fp32 products), bfloat16 or float16 (fp32 accumulation; the logits' gradient is rounded once to that type before its
+    two products); bias of the same type or float32.  A bias of -inf takes a class out.  Rows with adjacent channels are
+    read in place where they start at 16-byte addresses, others through a copy."""
+    if not (isinstance(x, torch.Tensor) and isinstance(weight, torch.Tensor)) or x.dim() < 1 or weight.dim() != 2:
+        raise RuntimeError("linear_cross_entropy: x must have shape (..., D) and weight (V, D)")
+    V, D = weight.shape
+    if x.shape[-1] != D or tuple(target.shape) != tuple(x.shape[:-1]):
+        raise RuntimeError(f"linear_cross_entropy: x {tuple(x.shape)}, weight {tuple(weight.shape)} and target "
+                           f"{tuple(target.shape)} do not fit: expected (..., D), (V, D), (...)")
+    if target.dtype != torch.int64:
+        raise RuntimeError(f"linear_cross_entropy: target must be int64, got {target.dtype}")
+    if bias is not None and tuple(bias.shape) != (V,):
+        raise RuntimeError(f"linear_cross_entropy: bias must have shape ({V},), got {tuple(bias.shape)}")
+    if reduction not in REDUCTIONS:
+        raise ValueError(f"linear_cross_entropy: reduction must be 'none', 'mean' or 'sum', got {reduction!r}")
+    label_smoothing, ignore_index = float(label_smoothing), int(ignore_index)
+    if not 0.0 <= label_smoothing <= 1.0:
+        raise ValueError(f"linear_cross_entropy: label_smoothing must be in [0, 1], got {label_smoothing}")
+    if V < 1 or D < 1:
+        raise RuntimeError("linear_cross_entropy: no classes or no channels")
+    _same_device(x, "linear_cross_entropy", ("weight", weight), ("target", target), ("bias", bias))
+    if x.dtype != weight.dtype:
+        raise RuntimeError(f"linear_cross_entropy: x is {x.dtype}, weight {weight.dtype}")
+    if not x.is_cuda or not target.numel():
+        F = torch.nn.functional
+        f32 = x.dtype in (torch.bfloat16, torch.float16)
+        z = F.linear(*((t.float() if t is not None and f32 else t) for t in (x, weight, bias)))
+        loss = F.cross_entropy(z.reshape(-1, V), target.reshape(-1), ignore_index=ignore_index, reduction=reduction,
+                               label_smoothing=label_smoothing)
+        return loss.reshape(target.shape) if reduction == "none" else loss
+    _dtype(x, "linear_cross_entropy: x")
+    if bias is not None and bias.dtype not in (x.dtype, torch.float32):
+        raise RuntimeError(f"linear_cross_entropy: bias must be of x's type ({x.dtype}) or float32, got {bias.dtype}")
+    if max(V, D, target.numel()) >= 2 ** 31 - 256:
+        raise RuntimeError("linear_cross_entropy: more than 2^31 - 257 rows, classes or channels")
+    rows = [v if (v.shape[1] == 1 or v.stride(1) == 1) and (v.shape[0] == 1 or v.stride(0) >= v.shape[1]) else v.contiguous()
+            for v in (x.reshape(-1, D), weight)]
+    loss = LinearCrossEntropyFn.apply(rows[0], rows[1], bias, target.reshape(-1).contiguous(), REDUCTIONS[reduction],
+                                      ignore_index, label_smoothing)
+    return loss.reshape(target.shape) if reduction == "none" else loss

@@ -1,0 +1,316 @@
+"""Linear cross entropy (train_ops.linear_cross_entropy) against its formulas in 64 bits.
+
+Bounds, with u = 2^-24, U = finfo(type).eps / 2 (a rounding to the inputs' type), a_tv = sum_d |x w| + |b| + 1:
+  z    products of 16-bit inputs are exact in float32, float32's are fused: D + 1 additions, each rounding a partial sum
+       below a_tv; the matrix unit adds in blocks, so (D / 2 + 8) u a_tv bounds it with the accumulator's rounding to nearest
+       or towards zero alike (2 u each, D / 4 of them at least)                                          -> ez
+  p    exp(z - m): ez and m's (the same size), the exponential's own 2^-22 (1 + |z - m|); the sum s the same, relatively:
+       ep = p (2 max_v ez + 2^-21 (1 + |z - m|) + mean of those over the row)
+  loss max_v ez + 2^-20, rounded to float32
+  g    rounded to the inputs' type: |g| U + |c| ep (+ the step below the type's normal range)
+  dx   sum_v |W| eg + n u sum_v |g W|, n = V / 2 + 8 as above, then U |dx|;  dW, db likewise over the rows
+"""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+U32 = 2.0 ** -24
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+
+
+def data(T, D, V, dtype, seed, bias=True, ignored=0.2, spread=2.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    x = torch.randn(T, D, generator=g, device="cuda").to(dtype)
+    w = (torch.randn(V, D, generator=g, device="cuda") * spread / math.sqrt(D)).to(dtype)
+    b = torch.randn(V, generator=g, device="cuda").to(dtype) if bias else None
+    y = torch.randint(0, V, (T,), generator=g, device="cuda")
+    y[torch.rand(T, generator=g, device="cuda") < ignored] = -100
+    c = torch.randn(T, generator=g, device="cuda")
+    return x, w, b, y, c
+
+
+def reference(x, w, b, y, c, reduction, smooth, ignore=-100):
+    """Outputs and the elementwise bounds of their errors but for the output's own rounding."""
+    U = torch.finfo(x.dtype).eps / 2
+    x, w = x.double(), w.double()
+    T, D = x.shape
+    V = w.shape[0]
+    bd = torch.zeros(V, device=x.device, dtype=torch.double) if b is None else b.double()
+    kept = y != ignore
+    x = torch.where(kept.unsqueeze(1), x, torch.zeros_like(x))           # an ignored row holds nothing
+    z = x @ w.t() + bd
+    ez = (D / 2 + 8) * U32 * (x.abs() @ w.abs().t() + bd.abs().nan_to_num(posinf=0.0) + 1)
+    m = z.max(1, keepdim=True).values
+    p = torch.softmax(z, 1)
+    gap = (z - m).abs().nan_to_num(posinf=0.0)
+    rel = 2 * ez.max(1, keepdim=True).values + 2.0 ** -21 * (1 + gap)
+    ep = p * (rel + (p * rel).sum(1, keepdim=True))
+    at = y.clamp_min(0).unsqueeze(1)
+    lse = torch.logsumexp(z, 1)
+    row = lse - (1 - smooth) * z.gather(1, at).squeeze(1) - (smooth * z.mean(1) if smooth else 0)
+    row = torch.where(kept, row, torch.zeros_like(row))
+    erow = torch.where(kept, 2 * ez.max(1).values + 2.0 ** -20, torch.zeros_like(row))
+    n = kept.sum()
+    loss, eloss = ((row, erow) if reduction == "none" else (row.sum(), erow.sum()) if reduction == "sum"
+                   else (row.sum() / n, erow.sum() / n))
+    c = c.double() if reduction == "none" else c[0].double() * torch.ones_like(row) / (n if reduction == "mean" else 1)
+    c = torch.where(kept, c, torch.zeros_like(c)).unsqueeze(1)
+    hot = torch.zeros_like(p).scatter_(1, at, 1 - smooth)
+    g = c * (p - hot - smooth / V)
+    # under the normal range: float32's exponential, and bfloat16 or float32 holding g, may give 0 below 2^-126 (of the
+    # largest coefficient: g is held over it); float16 holds it times 2^15 in steps of 2^-24, so half of 2^-39 is lost
+    low = c.abs().max() * (2.0 ** -39 if U == 2.0 ** -11 else 2.0 ** -125)
+    eg = c.abs() * ep + (U + 4 * U32) * g.abs() + 4 * U32 * c.abs() * hot + low
+    sums = lambda k, q, r, eq: eq @ r.abs() + (k / 2 + 8) * U32 * (q.abs() @ r.abs())
+    out = dict(loss=(loss, eloss), dx=(g @ w, sums(V, g, w, eg)), dw=(g.t() @ x, sums(T, g.t(), x, eg.t())),
+               db=(g.sum(0), eg.sum(0) + 8 * U32 * g.abs().sum(0)))
+    return out
+
+
+def run(x, w, b, y, c, reduction, smooth, ignore=-100, need=(True, True, True)):
+    from pointnetgpd_amd.train_ops import linear_cross_entropy
+    leaves = [None if t is None else t.detach().requires_grad_(r) for t, r in zip((x, w, b), need)]
+    loss = linear_cross_entropy(leaves[0], leaves[1], y, bias=leaves[2], reduction=reduction, ignore_index=ignore,
+                                label_smoothing=smooth)
+    assert loss.dtype == F32 and loss.shape == (y.shape if reduction == "none" else ())
+    have = [(k, t) for k, t in zip(("dx", "dw", "db"), leaves) if t is not None and t.requires_grad]
+    grads = torch.autograd.grad(loss, [t for _, t in have], c.view(y.shape) if reduction == "none" else c[0])
+    return dict(loss=loss.detach(), **{k: v for (k, _), v in zip(have, grads)})
+
+
+def check(got, want, bound, what):
+    t = torch.finfo(got.dtype)
+    assert got.shape == want.shape, what
+    limit = bound + t.eps / 2 * (want.abs() + bound) + t.smallest_normal * t.eps
+    off = (got.double() - want).abs()
+    bad = ~(off <= limit)
+    assert not bad.any(), f"{what}: {int(bad.sum())} of {bad.numel()} off, worst {(off / limit).nan_to_num(9e9).max().item():.3g} of the bound"
+
+
+def compare(x, w, b, y, c, reduction="mean", smooth=0.0, ignore=-100):
+    got = run(x, w, b, y, c, reduction, smooth, ignore)
+    want = reference(x, w, b, y, c, reduction, smooth, ignore)
+    for k, v in got.items():
+        check(v, *want[k], k)
+    return got
+
+
+# (T, D, V): single rows, classes and channels; odd channels (copied rows); tiles' edges; the large tiles; cut sums
+SHAPES = [(1, 1, 2), (1, 256, 6500), (2, 8, 1), (3, 17, 5), (33, 40, 65), (64, 256, 6500), (31, 250, 999), (130, 129, 777),
+          (257, 64, 1000), (1000, 96, 9000), (2500, 264, 4097), (5, 1024, 30001), (4097, 48, 2050), (300, 520, 20000)]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("i", range(len(SHAPES)), ids=[str(s) for s in SHAPES])
+def test_shapes(i, dtype):
+    T, D, V = SHAPES[i]
+    args = data(T, D, V, dtype, i, bias=i % 3 != 1, ignored=0.2 if T > 4 else 0.0)
+    compare(*args, reduction=("mean", "sum", "none")[i % 3], smooth=0.1 if i % 2 else 0.0)
+
+
+@pytest.mark.parametrize("reduction", ["none", "mean", "sum"])
+@pytest.mark.parametrize("smooth", [0.0, 0.3, 1.0])
+def test_reductions_and_smoothing(reduction, smooth):
+    for dtype in (F32, F16):
+        compare(*data(70, 72, 300, dtype, 1), reduction=reduction, smooth=smooth)
+
+
+def test_pieces():
+    """Rows so many that the classes are cut into pieces."""
+    args = data(300_000, 16, 1500, BF16, 2)
+    compare(*args, reduction="none", smooth=0.1)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_strides_shapes_and_bias_types(dtype):
+    g = torch.Generator(device="cuda").manual_seed(3)
+    wide = torch.randn(60, 200, generator=g, device="cuda").to(dtype)
+    wv = (torch.randn(150, 320, generator=g, device="cuda") / 8).to(dtype)
+    b = torch.randn(150, generator=g, device="cuda")
+    y = torch.randint(0, 150, (60,), generator=g, device="cuda")
+    c = torch.randn(60, generator=g, device="cuda")
+    for x, w in ((wide[:, :64], wv[:, 8:72]), (wide[:, 3:67], wv[:, 1:65]), (wide[:, :64], wv.t()[:64, :].t()),
+                 (wide[:, 136:], wv[:, 256:]), (wide[0, :64].expand(60, 64), wv[:, :64])):
+        for bias in (b, b.to(dtype), None):
+            compare(x, w, bias, y, c, "none", 0.1)
+    x3 = wide[:, :64].reshape(3, 4, 5, 64)                                     # more than one dimension of rows
+    a = run(x3, wv[:, :64], None, y.view(3, 4, 5), c, "none", 0.0)
+    f = run(wide[:, :64], wv[:, :64], None, y, c, "none", 0.0)
+    assert torch.equal(a["loss"].view(60), f["loss"]) and torch.equal(a["dx"].view(60, 64), f["dx"]) and torch.equal(a["dw"], f["dw"])
+    one = run(wide[7, :64], wv[:, :64], None, y[7], c[7:8], "mean", 0.0)        # a single row without a dimension for it
+    assert one["dx"].shape == (64,)
+
+
+def test_partial_gradients():
+    args = data(90, 64, 500, BF16, 4)
+    full = run(*args, "mean", 0.0)
+    for need in ((True, False, False), (False, True, False), (False, False, True), (False, True, True)):
+        part = run(*args, "mean", 0.0, need=need)
+        assert all(torch.equal(full[k], v) for k, v in part.items())
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_ignored_rows_hold_nothing(dtype):
+    """NaN and infinity in ignored rows reach neither the loss nor any gradient; an index within the classes can be ignored."""
+    x, w, b, y, c = data(200, 64, 700, dtype, 5, ignored=0.4)
+    clean = run(x, w, b, y, c, "mean", 0.1)
+    bad = x.clone()
+    rows = (y == -100).nonzero().squeeze(1)
+    bad[rows[::2]] = float("nan")
+    bad[rows[1::2]] = float("inf")
+    got = run(bad, w, b, y, c, "mean", 0.1)
+    assert all(torch.equal(got[k], clean[k]) for k in got)
+    assert not got["dx"][rows].any()
+    y = torch.where(y == -100, torch.full_like(y, 3), y)
+    compare(x, w, b, y, c, "mean", 0.0, ignore=3)
+
+
+def test_all_rows_ignored():
+    x, w, b, y, c = data(40, 32, 100, F32, 6)
+    y.fill_(-100)
+    for reduction, want in (("mean", math.nan), ("sum", 0.0)):
+        got = run(x, w, b, y, c, reduction, 0.1)
+        assert got["loss"].item() == want or (math.isnan(want) and got["loss"].isnan())
+        assert not any(got[k].any() or got[k].isnan().any() for k in ("dx", "dw", "db"))
+    assert not run(x, w, b, y, c, "none", 0.0)["loss"].any()
+
+
+def test_classes_taken_out():
+    """A bias of -inf takes a class out: no probability, no gradient, whole tiles of them included; float32's lowest value too."""
+    for low in (-math.inf, torch.finfo(F32).min):
+        x, w, _, y, c = data(50, 64, 900, BF16, 7, bias=False, ignored=0.1)
+        b = torch.zeros(900, device="cuda")
+        out = torch.zeros(900, dtype=torch.bool, device="cuda")
+        out[128:640] = True
+        out[::7] = True
+        b[out] = low
+        keep = (~out).nonzero().squeeze(1)
+        y = torch.where(y >= 0, keep[y.clamp_min(0) % len(keep)], y)
+        got = run(x, w, b, y, c, "sum", 0.0)
+        place = torch.zeros(900, dtype=torch.long, device="cuda")
+        place[keep] = torch.arange(len(keep), device="cuda")
+        want = reference(x, w[keep], None, torch.where(y >= 0, place[y.clamp_min(0)], y), c, "sum", 0.0)
+        check(got["loss"], *want["loss"], "loss")
+        check(got["dx"], *want["dx"], "dx")
+        check(got["dw"][keep], *want["dw"], "dw")
+        assert not got["dw"][out].any() and not got["db"][out].any()
+
+
+def test_large_logits():
+    """Logits far past where exponentials overflow."""
+    for dtype in (F32, BF16, F16):
+        compare(*data(80, 64, 300, dtype, 8, spread=300.0), reduction="mean")
+
+
+def test_targets_that_do_not_exist():
+    x, w, b, y, c = data(20, 32, 50, F32, 9, ignored=0.0)
+    for wrong in (50, -1, 2 ** 40):
+        y2 = y.clone()
+        y2[4] = wrong
+        got = run(x, w, b, y2, c, "none", 0.0)
+        assert got["loss"][4].isnan() and not got["loss"][[0, 1, 2, 3, 5]].isnan().any()
+        assert got["dx"][4].isnan().all() and not got["dx"][5].isnan().any()
+        assert run(x, w, b, y2, c, "mean", 0.0)["loss"].isnan()
+
+
+def test_upstream_of_any_size():
+    """Row weights across the float range, zeros among them; a scalar upstream of 2^15 (a loss scaler's) and of 2^-20."""
+    x, w, b, y, c = data(60, 48, 200, F16, 10, ignored=0.1)
+    for s in (1e-30, 1e25):
+        want = reference(x.float(), w.float(), b.float(), y, c * s, "none", 0.0)
+        got = run(x.float(), w.float(), b.float(), y, c * s, "none", 0.0)
+        for k in ("dx", "dw", "db"):
+            check(got[k], *want[k], k)
+    z = c.clone()
+    z[::3] = 0
+    compare(x, w, b, y, z, "none", 0.0)
+    compare(x, w, b, y, 0 * c, "none", 0.0)
+    compare(x, w, b, y, torch.full_like(c, 2.0 ** 9), "mean", 0.0)
+    compare(x, w, b, y, torch.full_like(c, 2.0 ** -12), "sum", 0.0)
+
+
+def test_no_rows():
+    from pointnetgpd_amd.train_ops import linear_cross_entropy
+    x, w = torch.empty(0, 8, device="cuda", requires_grad=True), torch.randn(5, 8, device="cuda", requires_grad=True)
+    y = torch.empty(0, dtype=torch.int64, device="cuda")
+    assert linear_cross_entropy(x, w, y, reduction="none").shape == (0,)
+    loss = linear_cross_entropy(x, w, y, reduction="sum")
+    dx, dw = torch.autograd.grad(loss, (x, w))
+    assert loss.item() == 0 and dx.shape == (0, 8) and not dw.any()
+    assert linear_cross_entropy(x, w, y).isnan()
+
+
+def test_gradient_against_differences():
+    x, w, b, y, c = data(30, 24, 90, F32, 11)
+    g = torch.Generator(device="cuda").manual_seed(12)
+    v = [torch.randn(t.shape, generator=g, device="cuda") for t in (x, w, b)]
+    for reduction, smooth in (("none", 0.2), ("mean", 0.0)):
+        got = run(x, w, b, y, c, reduction, smooth)
+
+        def f(h):
+            row = reference(*(t.double() + h * d for t, d in zip((x, w, b), v)), y, c, reduction, smooth)["loss"][0]
+            return ((row * c.double()).sum() if reduction == "none" else row * c[0].double()).item()
+        h = 1e-5                                  # truncation h^2, rounding 1e-16 / h: both below 1e-8 of sums of ~1e2
+        want = (f(h) - f(-h)) / (2 * h)
+        parts = [(got[k].double() * d) for k, d in zip(("dx", "dw", "db"), v)]
+        size = sum(p.abs().sum() for p in parts).item()
+        assert abs(sum(p.sum() for p in parts).item() - want) <= 2.0 ** -17 * size
+
+
+@pytest.mark.parametrize("shape", [(100, 64, 3000), (1100, 256, 7000)])
+def test_same_bits_streams_and_graph(shape):
+    x, w, b, y, c = data(*shape, BF16, 13)
+    first = run(x, w, b, y, c, "none", 0.1)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = run(x, w, b, y, c, "none", 0.1)
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(first[k], other[k]) for k in first)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = run(x, w, b, y, c, "mean", 0.1)
+    for k in range(4):
+        x.copy_(data(*shape, BF16, 20 + k)[0])
+        y.copy_(data(*shape, BF16, 30 + k)[3])
+        graph.replay()
+        eager = run(x, w, b, y, c, "mean", 0.1)
+        torch.cuda.synchronize()
+        assert all(torch.equal(held[n], eager[n]) for n in eager), k
+
+
+def test_run_together():
+    """A step of a network of the operators: features -> group norm + activation -> pooled -> linear cross entropy ->
+    backward -> clipped flat Adam, against the same step in 64-bit torch operations; three steps, each from our weights."""
+    from pointnetgpd_amd.optim import FlatAdam
+    from pointnetgpd_amd.train_ops import group_norm_act, linear_cross_entropy
+    g = torch.Generator(device="cuda").manual_seed(14)
+    B, N, C, G, V = 24, 90, 64, 8, 700
+    ps = [torch.nn.Parameter(t) for t in (torch.randn(C, 3, generator=g, device="cuda"), torch.ones(C, device="cuda"),
+                                          torch.zeros(C, device="cuda"), torch.randn(V, C, generator=g, device="cuda") / 8,
+                                          torch.zeros(V, device="cuda"))]
+    opt = FlatAdam(ps, lr=0.01, max_grad_norm=0.05)
+    F = torch.nn.functional
+    for k in range(3):
+        pts = torch.randn(B, N, 3, generator=g, device="cuda")
+        y = torch.randint(0, V, (B,), generator=g, device="cuda")
+        opt.zero_grad()
+        h = group_norm_act(pts @ ps[0].t(), G, ps[1], ps[2], act="gelu")
+        loss = linear_cross_entropy(h.mean(1), ps[3], y, bias=ps[4], label_smoothing=0.1)
+        loss.backward()
+        q = [p.detach().double().requires_grad_() for p in ps]
+        f = (pts.double() @ q[0].t()).unflatten(2, (G, C // G))
+        var, mean = torch.var_mean(f, (1, 3), correction=0, keepdim=True)
+        h64 = F.gelu(((f - mean) * torch.rsqrt(var + 1e-5)).flatten(2) * q[1] + q[2]).mean(1)
+        l64 = F.cross_entropy(F.linear(h64, q[3], q[4]), y, label_smoothing=0.1)
+        grads = torch.autograd.grad(l64, q)
+        assert abs(loss.item() - l64.item()) <= 2.0 ** -18 * l64.item()
+        for p, r in zip(ps, grads):            # chains of ~2^6 float32 roundings
+            assert (p.grad.double() - r).norm() <= 2.0 ** -16 * r.norm()
+        before = [p.detach().clone() for p in ps]
+        opt.step()
+        norm = torch.sqrt(sum((r ** 2).sum() for r in grads)).item()
+        assert abs(opt.grad_norm.item() - norm) <= 2.0 ** -16 * norm and norm > 0.05
+        assert all(0 < (p.detach() - o).abs().max() <= 0.011 for p, o in zip(ps, before))
