@@ -497,7 +497,8 @@ int pngpd_adam_flat_clip(float *p, const float *g, float *m, float *v, const lon
  * others are copied into the workspace first).  A target outside [0,V) that is not ignore_index gives a NaN loss and NaN
  * gradients.  Deterministic.  The workspace is bounded in V (a piece's gradient of the logits, 256 MB at most unless 256
  * classes of all rows take more).
- *   forward   writes stat (T,2) and kept (1), which the backward call reads, and loss: (T), or one value
+ *   forward   writes stat (T,2), kept (1) and rows (pngpd_lce_rows_ints(T) values, NULL where that is 0: the list of the
+ *             rows that are not ignored), which the backward call reads, and loss: (T), or one value
  *   backward  reads dloss (T, or one value); dx (T,D), dw (V,D), db (V) contiguous, each NULL: not wanted             */
 typedef struct pngpd_lce {
     const void *x, *w, *bias;      /* (T,D), (V,D) of dtype; (V) of bias_dtype (= dtype or PNGPD_F32), NULL: none  */
@@ -506,11 +507,13 @@ typedef struct pngpd_lce {
     int T, D, V, dtype, bias_dtype, reduction;
     float smoothing;
     float *stat, *kept, *loss;
+    int *rows;
     const float *dloss;
     void *dx, *dw, *db;
     void *workspace;               /* 256-byte aligned; pngpd_lce_workspace_bytes of the same descriptor           */
     size_t workspace_bytes;
 } pngpd_lce_t;
+size_t pngpd_lce_rows_ints(int T);
 size_t pngpd_lce_workspace_bytes(const pngpd_lce_t *a, int backward);
 int pngpd_lce_fwd(const pngpd_lce_t *a, void *stream);
 int pngpd_lce_bwd(const pngpd_lce_t *a, void *stream);

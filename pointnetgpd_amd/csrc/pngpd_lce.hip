@@ -10,32 +10,116 @@
 // inputs' type, as the operand of the matrix instructions has to be) lives in a workspace of bounded size, and two products
 // turn it into the piece's dW and its share of dx.  8 T D V operations for both directions where keeping T V logits takes
 // 6: the price of not keeping them.  Bound by the matrix cores for T in the hundreds and above, by reading W below.
+// Rows whose target is ignored are left out of the products (from LCE_ROWS rows on): a list of the kept ones is made on
+// the device, and the workgroups past them leave.
 // float16 holds g times 2^15 (|g| <= 1: below 65504, and its normal range then reaches down to 2e-9, under 1/V); the
 // coefficients c_t are scaled to at most 1 the same way; both factors come back in float32 on the way out.
 #include "pngpd_lce_gemm.h"
 
 #define LCE_PIECE_BYTES (256ll << 20)      // a piece's g
 
+#define LCE_ROWS 512                       // below, dropping rows does not drop enough tiles to pay for the list's launch
+#define LOG2E 1.44269504088896340736f
+
+// Where the kept rows lie: [0] how many, [1 ..] their row, [1 + T ..] a row's place among them or -1.  NULL: all, in order.
+struct LceRows {
+    const int *p;
+    int T;
+    __device__ __forceinline__ int count() const { return p ? p[0] : T; }
+    __device__ __forceinline__ const int *list() const { return p ? p + 1 : nullptr; }
+    __device__ __forceinline__ int row(int k) const { return p ? p[1 + k] : k; }
+    __device__ __forceinline__ int place(int t) const { return p ? p[1 + T + t] : t; }
+};
+
 struct LceArgs {
     LceOperand x, w;                       // rows of 16-byte multiples
+    LceRows rows;
+    int packed;                            // x holds the kept rows only
     const void *bias;
     int bf32;
     const long long *target;
     long long ignore;
-    int T, D, V, mt, nt;
+    int T, D, V, mt;
     float smooth;
     float *pm, *ps, *zt;                   // forward: (mt,T,2) max / sum, (mt,T) sum of z, (T) z at the target
     const float *stat, *coef;              // backward: (T,2) max / sum, (T)
     void *g;
     int v0, vc, ldg;                       // the piece
-};
+};                                         // (T above, but for target: by place among the kept rows)
 
-template <int DT> __device__ __forceinline__ void lce_bias4(const LceArgs &a, int v, float (&b)[4]) {
+// The kept rows in order: 8 targets a thread and round, the places by a scan over the workgroup.
+__global__ __launch_bounds__(1024) void lce_rows_kernel(const long long *__restrict__ target, long long ignore, int T,
+                                                        int *__restrict__ rows) {
+    __shared__ int sh[16];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int base = 0;
+    for (int t0 = 0; t0 < T; t0 += 8192) {
+        const int t = t0 + threadIdx.x * 8;
+        unsigned keep = 0;
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-        b[e] = !a.bias || v + e >= a.V ? 0.f
-             : a.bf32 ? ((const float *)a.bias)[v + e] : ld_elem<DT>((const typename elem<DT>::t *)a.bias + v + e);
+        for (int e = 0; e < 8; ++e) if (t + e < T && target[t + e] != ignore) keep |= 1u << e;
+        const int n = __popc(keep);
+        int at = n;
+#pragma unroll
+        for (int k = 1; k < 64; k <<= 1) { const int u = __shfl_up(at, k); if (lane >= k) at += u; }
+        __syncthreads();
+        if (lane == 63) sh[wave] = at;
+        __syncthreads();
+        int before = base, all = 0;
+        for (int w = 0; w < 16; ++w) { if (w < wave) before += sh[w]; all += sh[w]; }
+        int k = before + at - n;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            if (t + e < T) {
+                const bool on = keep >> e & 1;
+                rows[1 + T + t + e] = on ? k : -1;
+                if (on) rows[1 + k++] = t + e;
+            }
+        }
+        base += all;
+    }
+    if (threadIdx.x == 0) rows[0] = base;
 }
+
+// bias of classes v .. v + 3; whole: all of them exist (classes past V read the last one's, for values nobody uses)
+template <int DT> __device__ __forceinline__ void lce_bias4(const LceArgs &a, int v, bool whole, float (&b)[4]) {
+    typedef typename elem<DT>::t E;
+    if (a.bf32) {
+        const float *p = (const float *)a.bias;
+        if (whole) __builtin_memcpy(b, p + v, 16);
+        else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) b[e] = p[min(v + e, a.V - 1)];
+        }
+    } else {
+        const E *p = (const E *)a.bias;
+        E q[4];
+        if (whole) __builtin_memcpy(q, p + v, sizeof(q));
+        else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) q[e] = p[min(v + e, a.V - 1)];
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) b[e] = ld_elem<DT>(q + e);
+    }
+}
+
+// four values of column pairs q, q + 1 of a lane and of its partner in the other half: the lane of half h is given the
+// eight consecutive ones of q + h
+__device__ __forceinline__ uint4 lce_pair(uint2 x, uint2 y) {
+    const auto a = __builtin_amdgcn_permlane32_swap(x.x, y.x, false, false);
+    const auto b = __builtin_amdgcn_permlane32_swap(x.y, y.y, false, false);
+    return make_uint4(a[0], b[0], a[1], b[1]);
+}
+template <int DT> __device__ __forceinline__ uint2 lce_half4(float a, float b, float c, float d) {
+    return make_uint2((unsigned)f_to_half(DT, a) | ((unsigned)f_to_half(DT, b) << 16),
+                      (unsigned)f_to_half(DT, c) | ((unsigned)f_to_half(DT, d) << 16));
+}
+
+// 2^((z - m) log2 e) is one FMA, z log2 e - (m log2 e), where the rounding of the product in brackets is small: an error of
+// 2^-24 |m| in the exponent, so for maxima up to 64 (2^-18) and 16-bit inputs; otherwise the difference is taken first
+// (a row of classes masked by the type's lowest value, large logits, float32).
+template <int DT> __device__ __forceinline__ bool lce_far(float m) { return DT == PNGPD_F32 || fabsf(m) > 64.f; }
 
 // (max, sum) of two parts of a row; a part without values is (-inf, 0)
 __device__ __forceinline__ void lce_join(float &m, float &s, float m2, float s2) {
@@ -44,64 +128,103 @@ __device__ __forceinline__ void lce_join(float &m, float &s, float m2, float s2)
     m = M;
 }
 
-template <int DT, int BM, int BN, int WGM, int WGN>
+// The epilogues cost vector instructions that the matrix pipe waits for (128 values a lane): what only some tiles need
+// (the target's logit, classes past V, smoothing) is asked once a wave, and an exponential is one FMA and one v_exp_f32.
+template <int DT, int BM, int BN, int WGM, int WGN, int PIPE>
 __global__ __launch_bounds__(WGM * WGN * 64, 2) void lce_stats_kernel(const LceArgs a) {
-    typedef LceCore<DT, false, false, BM, BN, WGM, WGN> Core;
+    typedef LceCore<DT, false, false, BM, BN, WGM, WGN, PIPE> Core;
     extern __shared__ __align__(16) char smem[];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
     const int wm = (wave % WGM) * Core::WM, wn = (wave / WGM) * Core::WN;
+    const int T = a.rows.count(), nt = (T + BN - 1) / BN;
+    if ((int)blockIdx.x >= a.mt * nt) return;
     int tm, tn;
-    lce_tile_of(blockIdx.x, a.mt * a.nt, a.mt, a.nt, tm, tn);
+    lce_tile_of(blockIdx.x, a.mt, nt, tm, tn);
     const int m0 = tm * BM, n0 = tn * BN;
     Core c;
-    c.run(smem, a.w, a.x, m0, a.V, n0, a.T, 0, a.D);
+    c.run(smem, a.w, a.x, a.packed ? nullptr : a.rows.list(), m0, a.V, n0, T, 0, a.D);
     float *sh = (float *)smem;                                    // [WGM][BN][3]
-    const bool ragged = m0 + BM > a.V;
+    const int vb = m0 + wm + 4 * half;                            // class of the lane's row 0
+    const bool whole = m0 + BM <= a.V;
+    if (a.bias) {
 #pragma unroll
-    for (int i = 0; i < Core::FM; ++i) {
+        for (int i = 0; i < Core::FM; ++i) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const int v = m0 + wm + 32 * i + 8 * q + 4 * half;
-            float b[4];
-            lce_bias4<DT>(a, v, b);
+            for (int q = 0; q < 4; ++q) {
+                float b[4];
+                lce_bias4<DT>(a, vb + 32 * i + 8 * q, whole, b);
 #pragma unroll
-            for (int j = 0; j < Core::FN; ++j) {
+                for (int j = 0; j < Core::FN; ++j) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) c.acc[i][j][4 * q + e] += b[e];
+                    for (int e = 0; e < 4; ++e) c.acc[i][j][4 * q + e] += b[e];
+                }
             }
         }
     }
 #pragma unroll
     for (int j = 0; j < Core::FN; ++j) {
-        const int col = wn + 32 * j + (lane & 31), t = n0 + col;
-        float m = -INFINITY, s = 0.f, sz = 0.f;
-        const long long y = t < a.T ? a.target[t] : -1;
-        const long long rel = y - (m0 + wm + 4 * half);
-        const bool here = rel >= 0 && rel < Core::WM && y < a.V;
+        const int col = wn + 32 * j + (lane & 31), k = n0 + col;
+        const long long y = k < T ? a.target[a.rows.row(k)] : -1;
+        const int rel = y >= vb && y < a.V && y < vb + Core::WM ? (int)(y - vb) : -1;
+        if (__any(rel >= 0)) {
+            float z = 0.f;
+            bool mine = false;                                    // (the other half has the other rows of four)
+#pragma unroll
+            for (int i = 0; i < Core::FM; ++i) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const bool it = rel == 32 * i + (r & 3) + 8 * (r >> 2);
+                    z = it ? c.acc[i][j][r] : z;
+                    mine |= it;
+                }
+            }
+            if (mine) a.zt[k] = z;
+        }
+        float sz = 0.f;
+        if (whole) {
+            if (a.smooth != 0.f) {
+#pragma unroll
+                for (int i = 0; i < Core::FM; ++i) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) sz += c.acc[i][j][r];
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < Core::FM; ++i) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const bool past = vb + 32 * i + (r & 3) + 8 * (r >> 2) >= a.V;
+                    sz += past ? 0.f : c.acc[i][j][r];
+                    c.acc[i][j][r] = past ? -INFINITY : c.acc[i][j][r];
+                }
+            }
+        }
+        sz = half_sum(sz);
+        float m = -INFINITY, s = 0.f;
 #pragma unroll
         for (int i = 0; i < Core::FM; ++i) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int off = 32 * i + (r & 3) + 8 * (r >> 2);
-                float z = c.acc[i][j][r];
-                if (here && rel == off) a.zt[t] = z;
-                if (ragged && m0 + wm + 4 * half + off >= a.V) z = -INFINITY;
-                else if (a.smooth != 0.f) sz += z;
-                c.acc[i][j][r] = z;
-                m = fmaxf(m, z);
-            }
+            for (int r = 0; r < 16; r += 2) m = max3f(m, c.acc[i][j][r], c.acc[i][j][r + 1]);
         }
         float lo, hi;
         half_pair(m, lo, hi);
         m = fmaxf(lo, hi);
-        const float ref = m == -INFINITY ? 0.f : m;
+        const float mf = m == -INFINITY ? 0.f : m, ref = mf * LOG2E;
+        if (__any(lce_far<DT>(m) && y != a.ignore)) {            // (not for what an ignored row holds: the others' bits stay)
 #pragma unroll
-        for (int i = 0; i < Core::FM; ++i) {
+            for (int i = 0; i < Core::FM; ++i) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s += __expf(c.acc[i][j][r] - ref);
+                for (int r = 0; r < 16; ++r) s += __builtin_amdgcn_exp2f((c.acc[i][j][r] - mf) * LOG2E);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < Core::FM; ++i) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s += __builtin_amdgcn_exp2f(fmaf(c.acc[i][j][r], LOG2E, -ref));
+            }
         }
         s = half_sum(s);
-        if (a.smooth != 0.f) sz = half_sum(sz);
         if (half == 0) {
             float *o = sh + ((wave % WGM) * BN + col) * 3;
             o[0] = m; o[1] = s; o[2] = sz;
@@ -109,31 +232,32 @@ __global__ __launch_bounds__(WGM * WGN * 64, 2) void lce_stats_kernel(const LceA
     }
     __syncthreads();
     for (int col = threadIdx.x; col < BN; col += Core::THREADS) {
-        const int t = n0 + col;
-        if (t >= a.T) continue;
+        const int k = n0 + col;
+        if (k >= T) continue;
         float m = sh[col * 3], s = sh[col * 3 + 1], sz = sh[col * 3 + 2];
 #pragma unroll
-        for (int k = 1; k < WGM; ++k) {
-            const float *o = sh + (k * BN + col) * 3;
+        for (int w = 1; w < WGM; ++w) {
+            const float *o = sh + (w * BN + col) * 3;
             lce_join(m, s, o[0], o[1]);
             sz += o[2];
         }
-        const size_t at = (size_t)tm * a.T + t;
+        const size_t at = (size_t)tm * a.T + k;
         *(f32x2 *)(a.pm + 2 * at) = f32x2{m, s};
         if (a.smooth != 0.f) a.ps[at] = sz;
     }
 }
 
-// One row a group of 8 lanes: joins its tiles, in fp64; stat (T,2) = max, sum; row (T) = the row's loss.
+// One kept row a group of 8 lanes: joins its tiles, in fp64; stat (T,2) = max, sum; row (T) = every row's loss.
 __global__ __launch_bounds__(256) void lce_join_kernel(const LceArgs a, float *__restrict__ stat, float *__restrict__ row) {
     __shared__ double sh[8][32][2];
     __shared__ float shm[8][32];
     const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5, t = blockIdx.x * 32 + tx;
+    const int place = t < a.T ? a.rows.place(t) : -1;
     float m = -INFINITY;
     double s = 0.0, sz = 0.0;
-    if (t < a.T) {
+    if (place >= 0) {
         for (int k = ty; k < a.mt; k += 8) {
-            const size_t at = (size_t)k * a.T + t;
+            const size_t at = (size_t)k * a.T + place;
             const f32x2 p = *(const f32x2 *)(a.pm + 2 * at);
             const float M = fmaxf(m, p[0]), ref = M == -INFINITY ? 0.f : M;
             s = s * (double)expf(m - ref) + (double)p[1] * (double)expf(p[0] - ref);
@@ -144,19 +268,21 @@ __global__ __launch_bounds__(256) void lce_join_kernel(const LceArgs a, float *_
     shm[ty][tx] = m; sh[ty][tx][0] = s; sh[ty][tx][1] = sz;
     __syncthreads();
     if (ty || t >= a.T) return;
+    if (place < 0) { row[t] = 0.f; return; }
     float M = m;
     for (int k = 1; k < 8; ++k) M = fmaxf(M, shm[k][tx]);
     const float ref = M == -INFINITY ? 0.f : M;
     s = sz = 0.0;
     for (int k = 0; k < 8; ++k) { s += sh[k][tx][0] * (double)expf(shm[k][tx] - ref); sz += sh[k][tx][1]; }
-    stat[2 * (size_t)t] = M; stat[2 * (size_t)t + 1] = (float)s;
+    stat[2 * (size_t)place] = M; stat[2 * (size_t)place + 1] = (float)s;
     const long long y = a.target[t];
     double l = 0.0;
     if (y != a.ignore) {
         if (y < 0 || y >= a.V) l = NAN;                            // a class that does not exist: as loud as a value can be
         else {
-            l = (double)M + log(s) - (1.0 - (double)a.smooth) * (double)a.zt[t];
-            if (a.smooth != 0.f) l -= (double)a.smooth * sz / a.V;
+            // differences from the maximum first: beside a maximum of 1e30 the logarithm would be lost
+            l = log(s) + (1.0 - (double)a.smooth) * ((double)M - (double)a.zt[place]);
+            if (a.smooth != 0.f) l += (double)a.smooth * ((double)M - sz / a.V);
         }
     }
     row[t] = (float)l;
@@ -193,9 +319,10 @@ __global__ __launch_bounds__(1024) void lce_loss_kernel(const float *__restrict_
 
 // coef (T) = c_t over the largest finite |c_t| (times up, the factor of the type's range), scale = what gives c_t back
 __global__ __launch_bounds__(1024) void lce_coef_kernel(const float *__restrict__ dloss, const float *__restrict__ kept,
-                                                        const long long *__restrict__ target, long long ignore, int T, int V,
-                                                        int reduction, float up, float *__restrict__ coef,
+                                                        const long long *__restrict__ target, long long ignore, LceRows rows,
+                                                        int V, int reduction, float up, float *__restrict__ coef,
                                                         float *__restrict__ scale) {
+    const int T = rows.T;
     __shared__ float sh[16];
     float top = 1.f;
     if (reduction == PNGPD_REDUCE_NONE) {
@@ -215,7 +342,8 @@ __global__ __launch_bounds__(1024) void lce_coef_kernel(const float *__restrict_
         float c = reduction == PNGPD_REDUCE_NONE ? dloss[t] / top * up : up;
         if (y == ignore) c = 0.f;
         else if (y < 0 || y >= V) c = NAN;
-        coef[t] = c;
+        const int k = rows.place(t);
+        if (k >= 0) coef[k] = c;
     }
     if (threadIdx.x == 0) {
         float s = top / up;
@@ -225,62 +353,153 @@ __global__ __launch_bounds__(1024) void lce_coef_kernel(const float *__restrict_
     }
 }
 
-template <int DT, int BM, int BN, int WGM, int WGN>
+template <int DT, int BM, int BN, int WGM, int WGN, int PIPE>
 __global__ __launch_bounds__(WGM * WGN * 64, 2) void lce_grad_kernel(const LceArgs a) {
-    typedef LceCore<DT, false, false, BM, BN, WGM, WGN> Core;
+    typedef LceCore<DT, false, false, BM, BN, WGM, WGN, PIPE> Core;
     typedef typename elem<DT>::t E;
     extern __shared__ __align__(16) char smem[];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
     const int wm = (wave % WGM) * Core::WM, wn = (wave / WGM) * Core::WN;
+    const int T = a.rows.count(), nt = (T + BN - 1) / BN;
+    if ((int)blockIdx.x >= a.mt * nt) return;
     int tm, tn;
-    lce_tile_of(blockIdx.x, a.mt * a.nt, a.mt, a.nt, tm, tn);
+    lce_tile_of(blockIdx.x, a.mt, nt, tm, tn);
     const int m0 = tm * BM, n0 = tn * BN;
     LceOperand w = a.w;
     w.p = (const E *)a.w.p + (long long)a.v0 * a.w.ld;
     Core c;
-    c.run(smem, w, a.x, m0, a.vc, n0, a.T, 0, a.D);
-    const float flat = a.smooth / (float)a.V, hit = 1.f - a.smooth;
+    c.run(smem, w, a.x, nullptr, m0, a.vc, n0, T, 0, a.D);
+    const int vb = m0 + wm + 4 * half;                            // the piece's class of the lane's row 0
+    const bool whole = m0 + BM <= a.vc;
+    float m[Core::FN], ks[Core::FN], kf[Core::FN], co[Core::FN];
+    bool far = false;
 #pragma unroll
     for (int j = 0; j < Core::FN; ++j) {
-        const int t = n0 + wn + 32 * j + (lane & 31);
-        if (t >= a.T) continue;
-        const float m = a.stat[2 * (size_t)t], is = 1.f / a.stat[2 * (size_t)t + 1], co = a.coef[t];
-        const long long rel = a.target[t] - (a.v0 + m0 + wm + 4 * half);
-        E *g = (E *)a.g + (size_t)t * a.ldg + m0 + wm + 4 * half;
+        const int k = min(n0 + wn + 32 * j + (lane & 31), T - 1);
+        co[j] = a.coef[k];
+        m[j] = a.stat[2 * (size_t)k];
+        ks[j] = co[j] / a.stat[2 * (size_t)k + 1];
+        kf[j] = co[j] * (a.smooth / (float)a.V);
+        far |= lce_far<DT>(m[j]) && co[j] != 0.f;
+    }
+    far = __any(far);
+#pragma unroll
+    for (int i = 0; i < Core::FM; ++i) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            float b[4] = {0.f, 0.f, 0.f, 0.f};
+            if (a.bias) lce_bias4<DT>(a, a.v0 + vb + 32 * i + 8 * q, whole, b);
+#pragma unroll
+            for (int j = 0; j < Core::FN; ++j) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) c.acc[i][j][4 * q + e] += b[e];
+            }
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < Core::FN; ++j) {
+        const float ref = m[j] * LOG2E;
+        if (far) {
+#pragma unroll
+            for (int i = 0; i < Core::FM; ++i) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    c.acc[i][j][r] = fmaf(__builtin_amdgcn_exp2f((c.acc[i][j][r] - m[j]) * LOG2E), ks[j], -kf[j]);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < Core::FM; ++i) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    c.acc[i][j][r] = fmaf(__builtin_amdgcn_exp2f(fmaf(c.acc[i][j][r], LOG2E, -ref)), ks[j], -kf[j]);
+            }
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < Core::FN; ++j) {
+        const int k = n0 + wn + 32 * j + (lane & 31);
+        const long long y = k < T ? a.target[a.rows.row(k)] - a.v0 : -1;
+        const int rel = y >= vb && y < vb + Core::WM ? (int)(y - vb) : -1;
+        const float hit = co[j] * (1.f - a.smooth);
+        if (__any(rel >= 0)) {
+#pragma unroll
+            for (int i = 0; i < Core::FM; ++i) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) if (rel == 32 * i + (r & 3) + 8 * (r >> 2)) c.acc[i][j][r] -= hit;
+            }
+        }
+        // rows without a weight (ignored ones that are still here among them) have no gradient, whatever they hold
+        const bool none = co[j] == 0.f;
+        if (__any(none) || !whole) {
+#pragma unroll
+            for (int i = 0; i < Core::FM; ++i) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (none || vb + 32 * i + (r & 3) + 8 * (r >> 2) >= a.vc) c.acc[i][j][r] = 0.f;
+            }
+        }
+        if (k >= T) continue;                                     // (T - 1's partner lane leaves with it: both hold row k)
+        E *g = (E *)a.g + (size_t)k * a.ldg + m0 + wm;
 #pragma unroll
         for (int i = 0; i < Core::FM; ++i) {
+            const f32x16 &v = c.acc[i][j];
+            if constexpr (DT == PNGPD_F32) {
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int off = 32 * i + 8 * q;
-                float b[4], o[4];
-                lce_bias4<DT>(a, a.v0 + m0 + wm + 4 * half + off, b);
+                for (int q = 0; q < 4; ++q)
+                    *(f32x4 *)(g + 32 * i + 8 * q + 4 * half) = f32x4{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
+            } else {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float p = __expf(c.acc[i][j][4 * q + e] + b[e] - m) * is;
-                    const float d = p - flat - (rel == off + e ? hit : 0.f);
-                    o[e] = co == 0.f || m0 + wm + 4 * half + off + e >= a.vc ? 0.f : co * d;
-                }
-                if constexpr (DT == PNGPD_F32) *(f32x4 *)(g + off) = f32x4{o[0], o[1], o[2], o[3]};
-                else *(uint2 *)(g + off) = make_uint2((unsigned)f_to_half(DT, o[0]) | ((unsigned)f_to_half(DT, o[1]) << 16),
-                                                      (unsigned)f_to_half(DT, o[2]) | ((unsigned)f_to_half(DT, o[3]) << 16));
+                for (int q = 0; q < 4; q += 2)
+                    *(uint4 *)(g + 32 * i + 8 * (q + half)) =
+                        lce_pair(lce_half4<DT>(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]),
+                                 lce_half4<DT>(v[4 * q + 4], v[4 * q + 5], v[4 * q + 6], v[4 * q + 7]));
             }
         }
     }
 }
 
-// db of a piece: column sums of g (fp32, rounded g), 64 columns x 16 row lanes a workgroup
+// db of a piece: column sums of g (as rounded), in two steps.  A thread takes 16 bytes of a row and every 32nd row of the
+// workgroup's share; the shares' sums (S, ldg) in float32, then one thread a class.
 template <int DT>
-__global__ __launch_bounds__(1024) void lce_db_kernel(const void *__restrict__ gp, int T, int vc, int ldg,
-                                                      const float *__restrict__ scale, void *__restrict__ db, int f32) {
-    __shared__ double sh[16][64];
-    const int cx = threadIdx.x & 63, ry = threadIdx.x >> 6, v = blockIdx.x * 64 + cx;
+__global__ __launch_bounds__(256) void lce_db_kernel(const void *__restrict__ gp, LceRows rows, int ldg, int share, int cols,
+                                                     float *__restrict__ out) {
+    constexpr int EPC = DT == PNGPD_F32 ? 4 : 8, X = 8;           // 8 chunks by 32 rows
+    __shared__ float sh[32][X * EPC + 1];
+    const int T = rows.count(), cx = threadIdx.x % X, ry = threadIdx.x / X, v = (blockIdx.x * X + cx) * EPC;
+    const int t0 = blockIdx.y * share, t1 = min(T, t0 + share);
     const typename elem<DT>::t *g = (const typename elem<DT>::t *)gp + v;
-    double s = 0.0;
-    for (int t = ry; t < T; t += 16) s += (double)ld_elem<DT>(g + (size_t)t * ldg);      // (columns are padded to 64)
-    sh[ry][cx] = s;
+    float s[EPC];
+#pragma unroll
+    for (int e = 0; e < EPC; ++e) s[e] = 0.f;
+    if (v < cols) {
+#pragma unroll 4
+        for (int t = t0 + ry; t < t1; t += 32) {
+            const uint4 q = *(const uint4 *)(g + (size_t)t * ldg);
+            const unsigned w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+            for (int e = 0; e < EPC; ++e) {
+                if constexpr (DT == PNGPD_F32) s[e] += __uint_as_float(w[e]);
+                else s[e] += half_to_f(DT, (u16)(w[e >> 1] >> (16 * (e & 1))));
+            }
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < EPC; ++e) sh[ry][cx * EPC + e] = s[e];
     __syncthreads();
-    if (ry || v >= vc) return;
-    for (int k = 1; k < 16; ++k) s += sh[k][cx];
+    if (threadIdx.x < X * EPC) {
+        float u = 0.f;
+        for (int k = 0; k < 32; ++k) u += sh[k][threadIdx.x];
+        const int col = blockIdx.x * X * EPC + threadIdx.x;
+        if (col < cols) out[(size_t)blockIdx.y * ldg + col] = u;
+    }
+}
+template <int DT>
+__global__ __launch_bounds__(256) void lce_db_join_kernel(const float *__restrict__ part, int S, int ldg, int vc,
+                                                          const float *__restrict__ scale, void *__restrict__ db, int f32) {
+    const int v = blockIdx.x * 256 + threadIdx.x;
+    if (v >= vc) return;
+    double s = 0.0;
+    for (int k = 0; k < S; ++k) s += (double)part[(size_t)k * ldg + v];
     const float o = (float)s * *scale;
     if (f32) ((float *)db)[v] = o;
     else st_elem<DT>((typename elem<DT>::t *)db + v, o);
@@ -288,107 +507,130 @@ __global__ __launch_bounds__(1024) void lce_db_kernel(const void *__restrict__ g
 
 struct LceOut {
     LceOperand a, b;
-    int M, N, mt, nt;                      // M: m that exist in a's rows (padded); N likewise
-    int mo, no;                            // outputs stored
-    long long K, kper;                     // k of a split
+    LceRows rows;                          // counts N (dx) or K (dW)
+    int M, N, mt, nt;                      // M: m that exist in a's rows (padded); N likewise, -1: the kept rows
+    int mo, no;                            // outputs stored (no: N = -1's are the kept rows)
+    long long K, kper;                     // k (-1: the kept rows), k of a split
+    int splits;
     void *out;                             // typed: out[n * ldo + m] = scale * sum
     long long ldo;
-    float *part;                           // or fp32 partial sums (splits, no, M), added to what is there
+    float *part;                           // or fp32 partial sums (splits, T, M), added to what is there
     int add;
     const float *scale;
-    int vec;                               // out rows take 4 values at once
+    int vec;                               // out's rows are whole 16-byte chunks
 };
 
-template <int DT, bool BMC, int BM, int BN, int WGM, int WGN>
+template <int DT, bool BMC, int BM, int BN, int WGM, int WGN, int PIPE>
 __global__ __launch_bounds__(WGM * WGN * 64, 2) void lce_out_kernel(const LceOut a) {
-    typedef LceCore<DT, true, BMC, BM, BN, WGM, WGN> Core;
+    typedef LceCore<DT, true, BMC, BM, BN, WGM, WGN, PIPE> Core;
     typedef typename elem<DT>::t E;
     extern __shared__ __align__(16) char smem[];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
     const int wm = (wave % WGM) * Core::WM, wn = (wave / WGM) * Core::WN;
-    const int tiles = a.mt * a.nt, split = blockIdx.x / tiles;
+    const int N = a.N < 0 ? a.rows.count() : a.N, no = a.N < 0 ? N : a.no, nt = a.N < 0 ? (N + BN - 1) / BN : a.nt;
+    const long long K = a.K < 0 ? a.rows.count() : a.K;
+    const int tiles = a.mt * nt;
+    if ((int)blockIdx.x >= tiles * a.splits) return;
+    const int split = blockIdx.x / tiles;
     int tm, tn;
-    lce_tile_of(blockIdx.x - split * tiles, tiles, a.mt, a.nt, tm, tn);
+    lce_tile_of(blockIdx.x - split * tiles, a.mt, nt, tm, tn);
     const int m0 = tm * BM, n0 = tn * BN;
-    const long long k0 = split * a.kper, k1 = k0 + a.kper < a.K ? k0 + a.kper : a.K;
+    const long long k0 = split * a.kper, k1 = k0 + a.kper < K ? k0 + a.kper : K;
     Core c;
-    c.run(smem, a.a, a.b, m0, a.M, n0, a.N, k0, k1);
+    c.run(smem, a.a, a.b, nullptr, m0, a.M, n0, N, k0, k1);
     const float sc = a.part ? 1.f : *a.scale;
 #pragma unroll
     for (int j = 0; j < Core::FN; ++j) {
         const int n = n0 + wn + 32 * j + (lane & 31);
-        if (n >= a.no) continue;
+        if (n >= no) continue;
 #pragma unroll
         for (int i = 0; i < Core::FM; ++i) {
+            f32x16 v = c.acc[i][j];
+            const int mb = m0 + wm + 32 * i;
+            if (a.part) {
+                float *o = a.part + ((size_t)split * a.rows.T + n) * a.M + mb + 4 * half;
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int m = m0 + wm + 32 * i + 8 * q + 4 * half;
-                f32x4 v = {c.acc[i][j][4 * q], c.acc[i][j][4 * q + 1], c.acc[i][j][4 * q + 2], c.acc[i][j][4 * q + 3]};
-                if (a.part) {
-                    if (m < a.M) {
-                        f32x4 *o = (f32x4 *)(a.part + ((size_t)split * a.no + n) * a.M + m);
-                        *o = a.add ? *o + v : v;
+                for (int q = 0; q < 4; ++q) {
+                    if (mb + 8 * q + 4 * half < a.M) {
+                        const f32x4 u = {v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
+                        f32x4 *at = (f32x4 *)(o + 8 * q);
+                        *at = a.add ? *at + u : u;
                     }
+                }
+                continue;
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) v[r] *= sc;
+            E *o = (E *)a.out + n * a.ldo + mb;
+            if (a.vec && mb + 32 <= a.mo) {
+                if constexpr (DT == PNGPD_F32) {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        *(f32x4 *)(o + 8 * q + 4 * half) = f32x4{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
                 } else {
-                    v *= sc;
-                    E *o = (E *)a.out + n * a.ldo + m;
-                    if (a.vec && m + 4 <= a.mo) {
-                        if constexpr (DT == PNGPD_F32) *(f32x4 *)o = v;
-                        else *(uint2 *)o = make_uint2((unsigned)f_to_half(DT, v[0]) | ((unsigned)f_to_half(DT, v[1]) << 16),
-                                                      (unsigned)f_to_half(DT, v[2]) | ((unsigned)f_to_half(DT, v[3]) << 16));
-                    } else {
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) if (m + e < a.mo) st_elem<DT>(o + e, v[e]);
-                    }
+                    for (int q = 0; q < 4; q += 2)
+                        *(uint4 *)(o + 8 * (q + half)) = lce_pair(lce_half4<DT>(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]),
+                                                                  lce_half4<DT>(v[4 * q + 4], v[4 * q + 5], v[4 * q + 6], v[4 * q + 7]));
+                }
+            } else {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int m = (r & 3) + 8 * (r >> 2) + 4 * half;
+                    if (mb + m < a.mo) st_elem<DT>(o + m, v[r]);
                 }
             }
         }
     }
 }
 
-// dx = scale * sum of the splits' partial sums (rows of Dp, a multiple of 4)
+// dx = scale * sum of the splits' partial sums (rows of Dp, a multiple of 4); 0 where a row is not among the kept
 template <int DT>
-__global__ __launch_bounds__(256) void lce_dx_kernel(const float *__restrict__ part, int splits, int T, int D, int Dp,
+__global__ __launch_bounds__(256) void lce_dx_kernel(const float *__restrict__ part, int splits, LceRows rows, int D, int Dp,
                                                      const float *__restrict__ scale, void *__restrict__ dx) {
     typedef typename elem<DT>::t E;
     const int per = Dp / 4;
     const long long q = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (q >= (long long)T * per) return;
+    if (q >= (long long)rows.T * per) return;
     const long long t = q / per;
-    const int d = (int)(q - t * per) * 4;
+    const int d = (int)(q - t * per) * 4, k = rows.place((int)t);
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < splits; ++s) v += *(const f32x4 *)(part + ((size_t)s * T + t) * Dp + d);
+    if (k >= 0)
+        for (int s = 0; s < splits; ++s) v += *(const f32x4 *)(part + ((size_t)s * rows.T + k) * Dp + d);
     const float sc = *scale;
     E *o = (E *)dx + t * D + d;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) if (d + e < D) st_elem<DT>(o + e, v[e] * sc);
+    for (int e = 0; e < 4; ++e) if (d + e < D) st_elem<DT>(o + e, k < 0 ? 0.f : v[e] * sc);
 }
 
-// dst (R,Dp) = src (R,D) with zeros behind, and a row of zeros where the target is ignored (what such a row holds is
-// nobody's: a NaN there must not meet g's zeros in a product).  One 16-byte chunk of dst a thread.
+// dst (R,Dp) = src (R,D) with zeros behind; with `mask` the kept rows only, in their places (all of them, in order: a row
+// of zeros where the target is ignored — what such a row holds is nobody's, a NaN there must not meet g's zeros in a
+// product).  One 16-byte chunk of dst a thread.
 template <int DT>
 __global__ __launch_bounds__(256) void lce_copy_kernel(const void *__restrict__ src, long long ld, int D, int Dp, long long R,
-                                                       const long long *__restrict__ target, long long ignore,
-                                                       void *__restrict__ dst) {
+                                                       int mask, LceRows rows, const long long *__restrict__ target,
+                                                       long long ignore, void *__restrict__ dst) {
     typedef typename elem<DT>::t E;
     constexpr int EPC = 16 / (int)sizeof(E);
     const int per = Dp / EPC;
     const long long q = (long long)blockIdx.x * 256 + threadIdx.x;
     if (q >= R * per) return;
-    const long long r = q / per;
-    const int d = (int)(q - r * per) * EPC;
+    const long long k = q / per;
+    const int d = (int)(q - k * per) * EPC;
+    if (mask && k >= rows.count()) return;
+    const long long r = mask ? rows.row((int)k) : k;
     const E *s = (const E *)src + r * ld + d;
     __align__(16) E v[EPC];
 #pragma unroll
     for (int e = 0; e < EPC; ++e) v[e] = (E)0;
-    if (!target || target[r] != ignore) {
+    if (!mask || rows.p || target[r] != ignore) {
         if (d + EPC <= D) __builtin_memcpy(v, s, 16);
         else {
 #pragma unroll
             for (int e = 0; e < EPC; ++e) if (d + e < D) v[e] = s[e];
         }
     }
-    *(uint4 *)((E *)dst + r * Dp + d) = *(const uint4 *)v;
+    *(uint4 *)((E *)dst + k * Dp + d) = *(const uint4 *)v;
 }
 
 // ---------------------------------------------------------------------------------------------------- host
@@ -396,13 +638,18 @@ typedef pngpd_lce_t Lce;
 static inline size_t lce_up(size_t n) { return (n + 255) & ~(size_t)255; }
 static inline int lce_esize(int dt) { return dt == PNGPD_F32 ? 4 : 2; }
 static inline int lce_dp(const Lce *a) { const int c = 16 / lce_esize(a->dtype); return (a->D + c - 1) / c * c; }
-// rows that the loads can take as they are: 16-byte aligned, D a whole number of chunks
-static inline bool lce_plain(const Lce *a, const void *p, long long ld) {
-    return lce_dp(a) == a->D && !((uintptr_t)p & 15) && (ld * lce_esize(a->dtype)) % 16 == 0;
+// rows that the loads can take as they are: 16-byte aligned, D a whole number of chunks, and `reach` of them within the
+// 4 GiB of a lane's offset
+static inline bool lce_plain(const Lce *a, const void *p, long long ld, long long reach) {
+    const int es = lce_esize(a->dtype);
+    return lce_dp(a) == a->D && !((uintptr_t)p & 15) && (ld * es) % 16 == 0 && (double)ld * es * (double)reach < 4e9;
 }
 
 // tile shapes: 0 = 256 x 128, 1 = 64 x 64, 2 = 64 x 32
 static const int LCE_BM[3] = {256, 64, 64}, LCE_BN[3] = {128, 64, 32};
+#define LCE_SHAPE0 256, 128, 2, 2, 3
+#define LCE_SHAPE1 64, 64, 2, 2, 4
+#define LCE_SHAPE2 64, 32, 2, 1, 4
 static inline int lce_cdiv(long long a, int b) { return (int)((a + b - 1) / b); }
 // The large tile needs a workgroup for every CU; the narrow one is for rows that would leave half of 64 unused.
 static int lce_shape(long long M, long long N) {
@@ -413,20 +660,21 @@ static int lce_shape(long long M, long long N) {
 struct LcePlan {
     int Dp, fshape, fmt, padx, padw;
     int piece, ldg, gshape, xshape, splits, wshape;
+    int share, shares;                     // db: rows of a share, shares
     long long kper;
-    size_t o_part, o_ps, o_zt, o_row, o_x, o_w, o_coef, o_scale, o_g, o_dx, bytes;
+    size_t o_part, o_ps, o_zt, o_row, o_x, o_w, o_coef, o_scale, o_g, o_dx, o_db, bytes;
 };
 
 static LcePlan lce_plan(const Lce *a, bool bwd) {
     LcePlan p = {};
     const int es = lce_esize(a->dtype);
     p.Dp = lce_dp(a);
-    p.padw = !lce_plain(a, a->w, a->ldw);
+    p.padw = !lce_plain(a, a->w, a->ldw, 256);
     size_t at = 0;
     auto take = [&](size_t n) { const size_t o = at; at += lce_up(n); return o; };
     if (p.padw) p.o_w = take((size_t)a->V * p.Dp * es);
     if (!bwd) {
-        p.padx = !lce_plain(a, a->x, a->ldx);
+        p.padx = !lce_plain(a, a->x, a->ldx, a->rows ? a->T : 256);
         if (p.padx) p.o_x = take((size_t)a->T * p.Dp * es);
         p.fshape = lce_shape(a->V, a->T);
         p.fmt = lce_cdiv(a->V, LCE_BM[p.fshape]);
@@ -457,6 +705,13 @@ static LcePlan lce_plan(const Lce *a, bool bwd) {
         p.kper = (((long long)p.piece + s - 1) / s + 63) / 64 * 64;
         p.splits = (int)(((long long)p.piece + p.kper - 1) / p.kper);
         p.o_dx = take((size_t)p.splits * a->T * p.Dp * 4);
+        // db: about 1024 workgroups
+        const long long across = lce_cdiv(p.piece, es == 4 ? 32 : 64);
+        long long n2 = 1024 / across;
+        if (n2 > a->T / 64) n2 = a->T / 64;
+        if (n2 < 1) n2 = 1;
+        p.share = lce_cdiv(a->T, (int)n2); p.shares = lce_cdiv(a->T, p.share);
+        p.o_db = take((size_t)p.shares * p.ldg * 4);
     }
     p.bytes = at;
     return p;
@@ -466,59 +721,49 @@ static bool lce_bad(const Lce *a) {
     return !a || !a->x || !a->w || !a->target || a->T <= 0 || a->D <= 0 || a->V <= 0 || a->dtype < PNGPD_F32 || a->dtype > PNGPD_F16 ||
            a->ldx < (a->T > 1 ? a->D : 0) || a->ldw < (a->V > 1 ? a->D : 0) || (a->bias_dtype != PNGPD_F32 && a->bias_dtype != a->dtype) ||
            a->reduction < PNGPD_REDUCE_NONE || a->reduction > PNGPD_REDUCE_SUM || !(a->smoothing >= 0.f && a->smoothing <= 1.f) ||
-           !a->stat || !a->kept;
+           !a->stat || !a->kept || !a->rows != !pngpd_lce_rows_ints(a->T);
 }
 
-template <int DT, int KIND, int BM, int BN, int WGM, int WGN>          // KIND 0: stats, 1: grad
-static int lce_launch_z(const LceArgs &a, hipStream_t st) {
-    constexpr int lds = LceCore<DT, false, false, BM, BN, WGM, WGN>::LDS;
-    if constexpr (KIND == 0) {
-        const int rc = pngpd_allow_lds((const void *)lce_stats_kernel<DT, BM, BN, WGM, WGN>, lds);
-        if (rc) return rc;
-        hipLaunchKernelGGL((lce_stats_kernel<DT, BM, BN, WGM, WGN>), dim3((unsigned)(a.mt * a.nt)), dim3(WGM * WGN * 64), lds, st, a);
-    } else {
-        const int rc = pngpd_allow_lds((const void *)lce_grad_kernel<DT, BM, BN, WGM, WGN>, lds);
-        if (rc) return rc;
-        hipLaunchKernelGGL((lce_grad_kernel<DT, BM, BN, WGM, WGN>), dim3((unsigned)(a.mt * a.nt)), dim3(WGM * WGN * 64), lds, st, a);
-    }
-    return pngpd_launch_status();
-}
-template <int DT, int KIND> static int lce_z(LceArgs &a, int shape, int M, hipStream_t st) {
-    a.mt = lce_cdiv(M, LCE_BM[shape]); a.nt = lce_cdiv(a.T, LCE_BN[shape]);
-    if ((long long)a.mt * a.nt > 0x7fffffffll) return PNGPD_ERR_UNSUPPORTED;
-    if (shape == 0) return lce_launch_z<DT, KIND, 256, 128, 2, 2>(a, st);
-    if (shape == 1) return lce_launch_z<DT, KIND, 64, 64, 2, 2>(a, st);
-    return lce_launch_z<DT, KIND, 64, 32, 2, 1>(a, st);
-}
-
-template <int DT, bool BMC, int BM, int BN, int WGM, int WGN>
-static int lce_launch_out(const LceOut &a, int splits, hipStream_t st) {
-    constexpr int lds = LceCore<DT, true, BMC, BM, BN, WGM, WGN>::LDS;
-    const int rc = pngpd_allow_lds((const void *)lce_out_kernel<DT, BMC, BM, BN, WGM, WGN>, lds);
+template <class K, class A> static int lce_launch(K kernel, int lds, long long grid, int threads, const A &a, hipStream_t st) {
+    if (grid > 0x7fffffffll) return PNGPD_ERR_UNSUPPORTED;
+    const int rc = pngpd_allow_lds((const void *)kernel, lds);
     if (rc) return rc;
-    hipLaunchKernelGGL((lce_out_kernel<DT, BMC, BM, BN, WGM, WGN>), dim3((unsigned)(a.mt * a.nt * splits)), dim3(WGM * WGN * 64), lds, st, a);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(threads), lds, st, a);
     return pngpd_launch_status();
 }
-template <int DT, bool BMC> static int lce_out(LceOut &a, int shape, int splits, hipStream_t st) {
-    a.mt = lce_cdiv(a.M, LCE_BM[shape]); a.nt = lce_cdiv(a.no, LCE_BN[shape]);
-    if ((long long)a.mt * a.nt * splits > 0x7fffffffll) return PNGPD_ERR_UNSUPPORTED;
-    if (shape == 0) return lce_launch_out<DT, BMC, 256, 128, 2, 2>(a, splits, st);
-    if (shape == 1) return lce_launch_out<DT, BMC, 64, 64, 2, 2>(a, splits, st);
-    if constexpr (!BMC) return lce_launch_out<DT, BMC, 64, 32, 2, 1>(a, splits, st);
-    return PNGPD_ERR_UNSUPPORTED;
+template <int DT, bool GRAD, int BM, int BN, int WGM, int WGN, int PIPE> static int lce_z_shape(LceArgs &a, int M, hipStream_t st) {
+    constexpr int lds = LceCore<DT, false, false, BM, BN, WGM, WGN, PIPE>::LDS;
+    a.mt = lce_cdiv(M, BM);
+    const long long grid = (long long)a.mt * lce_cdiv(a.T, BN);
+    if constexpr (GRAD) return lce_launch(lce_grad_kernel<DT, BM, BN, WGM, WGN, PIPE>, lds, grid, WGM * WGN * 64, a, st);
+    else return lce_launch(lce_stats_kernel<DT, BM, BN, WGM, WGN, PIPE>, lds, grid, WGM * WGN * 64, a, st);
+}
+template <int DT, bool GRAD> static int lce_z(LceArgs &a, int shape, int M, hipStream_t st) {
+    return shape == 0 ? lce_z_shape<DT, GRAD, LCE_SHAPE0>(a, M, st) : shape == 1 ? lce_z_shape<DT, GRAD, LCE_SHAPE1>(a, M, st)
+                                                                                : lce_z_shape<DT, GRAD, LCE_SHAPE2>(a, M, st);
+}
+template <int DT, bool BMC, int BM, int BN, int WGM, int WGN, int PIPE> static int lce_out_shape(LceOut &a, hipStream_t st) {
+    a.mt = lce_cdiv(a.M, BM); a.nt = lce_cdiv(a.no, BN);
+    return lce_launch(lce_out_kernel<DT, BMC, BM, BN, WGM, WGN, PIPE>, LceCore<DT, true, BMC, BM, BN, WGM, WGN, PIPE>::LDS,
+                      (long long)a.mt * a.nt * a.splits, WGM * WGN * 64, a, st);
+}
+template <int DT, bool BMC> static int lce_out(LceOut &a, int shape, hipStream_t st) {
+    if (shape == 0) return lce_out_shape<DT, BMC, LCE_SHAPE0>(a, st);
+    if constexpr (!BMC) if (shape == 2) return lce_out_shape<DT, BMC, LCE_SHAPE2>(a, st);
+    return lce_out_shape<DT, BMC, LCE_SHAPE1>(a, st);
 }
 
 template <int DT>
-static void lce_copy(const Lce *a, const void *src, long long ld, long long R, const long long *target, void *dst, hipStream_t st) {
+static void lce_copy(const Lce *a, const void *src, long long ld, long long R, int mask, LceRows rows, void *dst, hipStream_t st) {
     const int Dp = lce_dp(a);
     const long long n = R * (Dp * lce_esize(DT) / 16);
-    hipLaunchKernelGGL(lce_copy_kernel<DT>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, src, ld, a->D, Dp, R, target,
-                       a->ignore_index, dst);
+    hipLaunchKernelGGL(lce_copy_kernel<DT>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, src, ld, a->D, Dp, R, mask, rows,
+                       (const long long *)a->target, (long long)a->ignore_index, dst);
 }
 
 static LceArgs lce_args(const Lce *a) {
     LceArgs k = {};
-    k.x = LceOperand{a->x, a->ldx}; k.w = LceOperand{a->w, a->ldw};
+    k.x = LceOperand{a->x, a->ldx}; k.w = LceOperand{a->w, a->ldw}; k.rows = LceRows{a->rows, a->T};
     k.bias = a->bias; k.bf32 = a->bias_dtype == PNGPD_F32; k.target = (const long long *)a->target; k.ignore = a->ignore_index;
     k.T = a->T; k.D = a->D; k.V = a->V; k.smooth = a->smoothing;
     return k;
@@ -527,11 +772,12 @@ static LceArgs lce_args(const Lce *a) {
 template <int DT> static int lce_forward(const Lce *a, const LcePlan &p, hipStream_t st) {
     char *ws = (char *)a->workspace;
     LceArgs k = lce_args(a);
-    if (p.padx) { lce_copy<DT>(a, a->x, a->ldx, a->T, nullptr, ws + p.o_x, st); k.x = LceOperand{ws + p.o_x, p.Dp}; }
-    if (p.padw) { lce_copy<DT>(a, a->w, a->ldw, a->V, nullptr, ws + p.o_w, st); k.w = LceOperand{ws + p.o_w, p.Dp}; }
+    if (a->rows) hipLaunchKernelGGL(lce_rows_kernel, dim3(1), dim3(1024), 0, st, k.target, k.ignore, a->T, a->rows);
+    if (p.padx) { lce_copy<DT>(a, a->x, a->ldx, a->T, 0, k.rows, ws + p.o_x, st); k.x = LceOperand{ws + p.o_x, p.Dp}; }
+    if (p.padw) { lce_copy<DT>(a, a->w, a->ldw, a->V, 0, k.rows, ws + p.o_w, st); k.w = LceOperand{ws + p.o_w, p.Dp}; }
     k.D = p.Dp;
     k.pm = (float *)(ws + p.o_part); k.ps = (float *)(ws + p.o_ps); k.zt = (float *)(ws + p.o_zt);
-    int rc = lce_z<DT, 0>(k, p.fshape, a->V, st);
+    int rc = lce_z<DT, false>(k, p.fshape, a->V, st);
     if (rc) return rc;
     float *row = a->reduction == PNGPD_REDUCE_NONE ? a->loss : (float *)(ws + p.o_row);
     hipLaunchKernelGGL(lce_join_kernel, dim3((unsigned)((a->T + 31) / 32)), dim3(256), 0, st, k, a->stat, row);
@@ -544,50 +790,56 @@ template <int DT> static int lce_backward(const Lce *a, const LcePlan &p, hipStr
     typedef typename elem<DT>::t E;
     char *ws = (char *)a->workspace;
     LceArgs k = lce_args(a);
-    lce_copy<DT>(a, a->x, a->ldx, a->T, k.target, ws + p.o_x, st);
+    lce_copy<DT>(a, a->x, a->ldx, a->T, 1, k.rows, ws + p.o_x, st);
     k.x = LceOperand{ws + p.o_x, p.Dp};
-    if (p.padw) { lce_copy<DT>(a, a->w, a->ldw, a->V, nullptr, ws + p.o_w, st); k.w = LceOperand{ws + p.o_w, p.Dp}; }
+    k.packed = 1;
+    if (p.padw) { lce_copy<DT>(a, a->w, a->ldw, a->V, 0, k.rows, ws + p.o_w, st); k.w = LceOperand{ws + p.o_w, p.Dp}; }
     k.D = p.Dp;
     float *coef = (float *)(ws + p.o_coef), *scale = (float *)(ws + p.o_scale), *part = (float *)(ws + p.o_dx);
-    hipLaunchKernelGGL(lce_coef_kernel, dim3(1), dim3(1024), 0, st, a->dloss, a->kept, k.target, k.ignore, a->T, a->V, a->reduction,
+    hipLaunchKernelGGL(lce_coef_kernel, dim3(1), dim3(1024), 0, st, a->dloss, a->kept, k.target, k.ignore, k.rows, a->V, a->reduction,
                        DT == PNGPD_F16 ? 32768.f : 1.f, coef, scale);
     k.stat = a->stat; k.coef = coef; k.g = ws + p.o_g; k.ldg = p.ldg;
     for (int v0 = 0; v0 < a->V; v0 += p.piece) {
         k.v0 = v0; k.vc = a->V - v0 < p.piece ? a->V - v0 : p.piece;
         const int cols = (k.vc + 63) / 64 * 64;                    // columns of g that are written (zeros past vc)
-        int rc = lce_z<DT, 1>(k, p.gshape, k.vc, st);
+        int rc = lce_z<DT, true>(k, p.gshape, k.vc, st);
         if (rc) return rc;
         const E *w = (const E *)k.w.p + (long long)v0 * k.w.ld;
         if (a->db) {
+            float *sums = (float *)(ws + p.o_db);
             void *db = a->bias_dtype == PNGPD_F32 ? (void *)((float *)a->db + v0) : (void *)((E *)a->db + v0);
-            hipLaunchKernelGGL(lce_db_kernel<DT>, dim3((unsigned)(cols / 64)), dim3(1024), 0, st, k.g, a->T, k.vc, p.ldg, scale, db,
-                               a->bias_dtype == PNGPD_F32);
+            hipLaunchKernelGGL(lce_db_kernel<DT>, dim3((unsigned)lce_cdiv(cols, DT == PNGPD_F32 ? 32 : 64), p.shares), dim3(256), 0, st,
+                               k.g, k.rows, p.ldg, p.share, cols, sums);
+            hipLaunchKernelGGL(lce_db_join_kernel<DT>, dim3((unsigned)lce_cdiv(k.vc, 256)), dim3(256), 0, st, sums, p.shares, p.ldg,
+                               k.vc, scale, db, a->bias_dtype == PNGPD_F32);
         }
         if (a->dx) {
             LceOut o = {};
-            o.a = LceOperand{w, k.w.ld}; o.b = LceOperand{k.g, p.ldg};
-            o.M = p.Dp; o.N = a->T; o.mo = a->D; o.no = a->T; o.K = k.vc; o.kper = p.kper;
+            o.a = LceOperand{w, k.w.ld}; o.b = LceOperand{k.g, p.ldg}; o.rows = k.rows;
+            o.M = p.Dp; o.N = -1; o.mo = a->D; o.no = a->T; o.K = k.vc; o.kper = p.kper; o.splits = p.splits;
             o.part = part; o.add = v0 > 0; o.scale = scale;
-            if ((rc = lce_out<DT, false>(o, p.xshape, p.splits, st))) return rc;
+            if ((rc = lce_out<DT, false>(o, p.xshape, st))) return rc;
         }
         if (a->dw) {
             LceOut o = {};
-            o.a = LceOperand{k.x.p, p.Dp}; o.b = LceOperand{k.g, p.ldg};
-            o.M = p.Dp; o.N = cols; o.mo = a->D; o.no = k.vc; o.K = a->T; o.kper = a->T;
+            o.a = LceOperand{k.x.p, p.Dp}; o.b = LceOperand{k.g, p.ldg}; o.rows = k.rows;
+            o.M = p.Dp; o.N = cols; o.mo = a->D; o.no = k.vc; o.K = -1; o.kper = a->T; o.splits = 1;
             o.out = (E *)a->dw + (long long)v0 * a->D; o.ldo = a->D; o.scale = scale;
-            o.vec = a->D % 4 == 0 && !((uintptr_t)a->dw & 15);
-            if ((rc = lce_out<DT, true>(o, p.wshape, 1, st))) return rc;
+            o.vec = (a->D * (long long)sizeof(E)) % 16 == 0 && !((uintptr_t)a->dw & 15);
+            if ((rc = lce_out<DT, true>(o, p.wshape, st))) return rc;
         }
     }
     if (a->dx) {
         const long long n = (long long)a->T * (p.Dp / 4);
-        hipLaunchKernelGGL(lce_dx_kernel<DT>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, part, p.splits, a->T, a->D, p.Dp,
+        hipLaunchKernelGGL(lce_dx_kernel<DT>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, part, p.splits, k.rows, a->D, p.Dp,
                            scale, a->dx);
     }
     return pngpd_launch_status();
 }
 
 extern "C" {
+
+size_t pngpd_lce_rows_ints(int T) { return T < LCE_ROWS ? 0 : 2 * (size_t)T + 1; }
 
 size_t pngpd_lce_workspace_bytes(const pngpd_lce_t *a, int backward) {
     return lce_bad(a) ? 0 : lce_plan(a, backward != 0).bytes;

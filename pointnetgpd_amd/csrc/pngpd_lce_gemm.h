@@ -11,11 +11,13 @@
 // inside a lane, and stores are 8 or 16 bytes.
 //
 // A K tile (64 bytes of k: 32 of 16 bits, 16 of 32) of both operands goes from global memory straight into LDS
-// (global_load_lds_dwordx4, no registers), one tile ahead of the matrix instructions, one barrier a tile; two workgroups
-// share a CU, so one's barrier and epilogue hide behind the other's products.  The LDS destination of that load is lane
-// after lane, so the XOR swizzle against bank conflicts is put on the SOURCE: slot p of LDS row r holds chunk p ^ f(r).
+// (global_load_lds_dwordx4, no registers, the address a scalar base that walks along k plus a 32-bit lane offset that
+// stays), PIPE - 1 tiles ahead of the matrix instructions, one barrier a tile; two workgroups of the large tile share a
+// CU, so one's barrier and epilogue hide behind the other's products.  The LDS destination of that load is lane after
+// lane, so the XOR swizzle against bank conflicts is put on the SOURCE: slot p of LDS row r holds chunk p ^ f(r).
 //   KC: fragments are ds_read_b128 (8 or 4 consecutive k of a row);
 //   MC, 16 bits: ds_read_b64_tr_b16, which transposes a [4 k][16 m] block over 16 lanes; 32 bits: ds_read_b32 per k.
+// (Measured: no bank conflict in any of the three products.)
 // float32 runs on v_mfma_f32_32x32x2_f32 (exact products, fp32 accumulation); chunk j of the two lane halves are k and
 // k + 4 of the same 8, for A and B alike.
 #pragma once
@@ -29,8 +31,6 @@ typedef __attribute__((address_space(3))) lce_bf16x4 lds_lce_bf16x4;
 typedef __attribute__((address_space(3))) char lds_char;
 
 #define LCE_KB 64                          // bytes of k in a tile
-#define LCE_PIPE 2                         // tiles in LDS
-
 struct LceOperand {
     const void *p;
     long long ld;                          // elements from row to row
@@ -47,6 +47,13 @@ template <int N> __device__ __forceinline__ void lce_wait_barrier() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(N) : "memory");
 }
 
+// for a pipeline of DEPTH tiles of LOADS loads each: the oldest tile has landed, `younger` of the others are on their way
+template <int LOADS, int DEPTH> __device__ __forceinline__ void lce_wait_tile(int younger) {
+    if (DEPTH >= 3 && younger >= 2) lce_wait_barrier<2 * LOADS>();
+    else if (DEPTH >= 2 && younger >= 1) lce_wait_barrier<LOADS>();
+    else lce_wait_barrier<0>();
+}
+
 __device__ __align__(16) unsigned lce_zero[4];       // what a chunk past the end of k reads
 
 // One operand's tile: ROWS values of m (or n) by LCE_KB bytes of k.
@@ -55,41 +62,46 @@ template <int DT, bool MC, int ROWS, int THREADS> struct LceTile {
     static constexpr int BYTES = ROWS * LCE_KB, LOADS = BYTES / (THREADS * 16);
     static constexpr int RB = MC ? ROWS * E : LCE_KB, CPR = RB / 16;      // bytes, chunks of an LDS row
     static_assert(BYTES % (THREADS * 16) == 0, "a tile is whole loads of the workgroup");
-    const char *p[LOADS];
-    int k[LOADS];                          // k of the chunk (KC) or of the row (MC), from the tile's start
+    const char *base;                      // uniform: the tile's start
+    unsigned off[LOADS];                   // bytes from there to the lane's chunks (below 4 GiB: the host sees to it)
 
     static __device__ __forceinline__ int swz(int row) {
         if constexpr (!MC) return (row >> 2) & 3;
         else if constexpr (DT == PNGPD_F32) return RB >= 256 ? ((row >> 2) & 1) << 3 : 0;
         else return RB >= 256 ? (row & 3) << 2 : RB == 128 ? ((row >> 1) & 1) << 2 : 0;
     }
-    // m0: first m of the tile, M: how many exist; k0: first k
-    __device__ __forceinline__ void init(const LceOperand &o, int m0, int M, long long k0) {
+    static __device__ __forceinline__ int row_of(int i) { return (i * THREADS + (int)threadIdx.x) / CPR; }
+    static __device__ __forceinline__ int chunk_of(int i) { return ((i * THREADS + (int)threadIdx.x) % CPR) ^ swz(row_of(i)); }
+    // m0: first m of the tile, M: how many exist; k0: first k; rows (KC): where row m of the operand lies, NULL: at m
+    __device__ __forceinline__ void init(const LceOperand &o, const int *rows, int m0, int M, long long k0) {
+        if constexpr (MC) base = (const char *)o.p + (k0 * o.ld + m0) * E;
+        else base = (const char *)o.p + ((rows ? 0 : m0 * o.ld) + k0) * E;
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
-            const int q = i * THREADS + (int)threadIdx.x, row = q / CPR, c = (q % CPR) ^ swz(row);
+            const int row = row_of(i), c = chunk_of(i) * EPC;
             if constexpr (MC) {
-                int m = m0 + c * EPC;
-                if (m >= M) m = M - EPC;                       // outputs past M are not stored
-                k[i] = row;
-                p[i] = (const char *)o.p + ((k0 + row) * o.ld + m) * E;
+                // (a column past M: the last one there is; outputs past M are not stored)
+                off[i] = (unsigned)(row * o.ld + (m0 + c < M ? c : M - EPC - m0)) * E;
             } else {
                 const int m = m0 + row < M ? m0 + row : M - 1;
-                k[i] = c * EPC;
-                p[i] = (const char *)o.p + ((long long)m * o.ld + k0 + k[i]) * E;
+                off[i] = (unsigned)((rows ? rows[m] : m - m0) * o.ld + c) * E;
             }
         }
     }
     // left: k that exist from the tile's start (a whole tile where left >= BK)
     __device__ __forceinline__ void load(unsigned lds, int left, long long ld) {
-        const unsigned base = lds + (threadIdx.x & ~63u) * 16;
+        const unsigned to = __builtin_amdgcn_readfirstlane(lds + (threadIdx.x & ~63u) * 16);
+        if (left >= BK) {
 #pragma unroll
-        for (int i = 0; i < LOADS; ++i) {
-            const char *g = p[i];
-            if (left < BK) g = k[i] < left ? g : (const char *)lce_zero;
-            lce_load16(g, __builtin_amdgcn_readfirstlane(base + i * THREADS * 16));
-            p[i] += MC ? ld * BK * E : (long long)LCE_KB;
+            for (int i = 0; i < LOADS; ++i) lce_load16(base + (unsigned long long)off[i], to + i * THREADS * 16);
+        } else {
+#pragma unroll
+            for (int i = 0; i < LOADS; ++i) {
+                const char *g = (MC ? row_of(i) : chunk_of(i) * EPC) < left ? base + (unsigned long long)off[i] : (const char *)lce_zero;
+                lce_load16(g, to + i * THREADS * 16);
+            }
         }
+        base += MC ? ld * BK * E : (long long)LCE_KB;
     }
     // the fragment of rows [row0, row0 + 32) at step s (16 or 8 values of k)
     static __device__ __forceinline__ f32x4 frag(const char *lds, int row0, int s, int lane) {
@@ -130,16 +142,17 @@ template <int DT> __device__ __forceinline__ f32x16 lce_mma(const f32x4 &a, cons
     }
 }
 
-// The accumulators of one workgroup's tile: BM x BN, WGM x WGN waves.  k in [k0, k1).
-template <int DT, bool AMC, bool BMC, int BM, int BN, int WGM, int WGN> struct LceCore {
+// The accumulators of one workgroup's tile: BM x BN, WGM x WGN waves, PIPE tiles of k in LDS.  k in [k0, k1).
+template <int DT, bool AMC, bool BMC, int BM, int BN, int WGM, int WGN, int PIPE> struct LceCore {
     static constexpr int THREADS = WGM * WGN * 64, WM = BM / WGM, WN = BN / WGN, FM = WM / 32, FN = WN / 32;
     typedef LceTile<DT, AMC, BM, THREADS> TA;
     typedef LceTile<DT, BMC, BN, THREADS> TB;
-    static constexpr int STAGE = TA::BYTES + TB::BYTES, LDS = LCE_PIPE * STAGE, BK = TA::BK;
+    static constexpr int STAGE = TA::BYTES + TB::BYTES, LDS = PIPE * STAGE, BK = TA::BK;
+    static_assert(PIPE >= 2 && PIPE <= 4, "lce_wait_tile counts up to three tiles");
     f32x16 acc[FM][FN];
 
-    __device__ __forceinline__ void run(char *smem, const LceOperand &a, const LceOperand &b, int m0, int M, int n0, int N,
-                                        long long k0, long long k1) {
+    __device__ __forceinline__ void run(char *smem, const LceOperand &a, const LceOperand &b, const int *rows, int m0, int M,
+                                        int n0, int N, long long k0, long long k1) {
         const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
         const int wm = (wave % WGM) * WM, wn = (wave / WGM) * WN;
         const unsigned lds0 = (unsigned)(uintptr_t)(lds_char *)smem;
@@ -153,22 +166,24 @@ template <int DT, bool AMC, bool BMC, int BM, int BN, int WGM, int WGN> struct L
         }
         TA ta;
         TB tb;
-        ta.init(a, m0, M, k0);
-        tb.init(b, n0, N, k0);
-        const long long K = k1 - k0;
-        const int tiles = (int)((K + BK - 1) / BK);
-        ta.load(lds0, K < BK ? (int)K : BK, a.ld);
-        tb.load(lds0 + TA::BYTES, K < BK ? (int)K : BK, b.ld);
+        ta.init(a, nullptr, m0, M, k0);
+        tb.init(b, rows, n0, N, k0);
+        long long left = k1 - k0;                                  // k that the next tile to load has
+        const int tiles = left > 0 ? (int)((left + BK - 1) / BK) : 0;
+        auto load = [&](int stage) {
+            const int l = left < BK ? (int)left : BK;
+            ta.load(lds0 + stage * STAGE, l, a.ld);
+            tb.load(lds0 + stage * STAGE + TA::BYTES, l, b.ld);
+            left -= BK;
+        };
+#pragma unroll
+        for (int t = 0; t < PIPE - 1; ++t) if (t < tiles) load(t);
+        int cur = 0;
         for (int t = 0; t < tiles; ++t) {
-            lce_wait_barrier<0>();
-            const int cur = t % LCE_PIPE, nxt = (t + 1) % LCE_PIPE;
-            if (t + 1 < tiles) {
-                const long long left = K - (long long)(t + 1) * BK;
-                const int l = left < BK ? (int)left : BK;
-                ta.load(lds0 + nxt * STAGE, l, a.ld);
-                tb.load(lds0 + nxt * STAGE + TA::BYTES, l, b.ld);
-            }
+            lce_wait_tile<TA::LOADS + TB::LOADS, PIPE - 1>(tiles - 1 - t);      // tile t is there, t - 1's LDS is free
+            if (t + PIPE - 1 < tiles) load(cur ? cur - 1 : PIPE - 1);
             const char *sa = smem + cur * STAGE, *sb = sa + TA::BYTES;
+            cur = cur == PIPE - 1 ? 0 : cur + 1;
 #pragma unroll
             for (int s = 0; s < LCE_KB / 32; ++s) {
                 f32x4 fa[FM], fb[FN];
@@ -188,9 +203,9 @@ template <int DT, bool AMC, bool BMC, int BM, int BN, int WGM, int WGN> struct L
 };
 
 // Workgroup -> tile.  Workgroup i runs on XCD i % 8: each XCD takes a contiguous stretch of a walk over the tiles that
-// goes down bands of 8 n tiles, so the operands of its running workgroups overlap in its own L2.
-__device__ __forceinline__ void lce_tile_of(int i, int total, int mt, int nt, int &m, int &n) {
-    const int per = total >> 3;
+// goes down bands of 8 n tiles, so the operands of its running workgroups overlap in its own L2.  (i < mt * nt)
+__device__ __forceinline__ void lce_tile_of(int i, int mt, int nt, int &m, int &n) {
+    const int per = (mt * nt) >> 3;
     int w = i;
     if (i < per * 8) w = (i & 7) * per + (i >> 3);
     const int band = w / (8 * mt), r = w - band * 8 * mt;

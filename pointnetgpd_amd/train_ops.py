@@ -158,16 +158,20 @@ class LinearCrossEntropyFn(torch.autograd.Function):
         bias = bias.detach().contiguous() if bias is not None else None
         stat, kept = torch.empty(T, 2, device=dev, dtype=f32), torch.empty((), device=dev, dtype=f32)
         loss = torch.empty((T,) if reduction == 0 else (), device=dev, dtype=f32)
+        n = _lib.load().pngpd_lce_rows_ints(T)
+        rows = torch.empty(n, device=dev, dtype=torch.int32) if n else None
         ctx.scalars = (reduction, ignore_index, smoothing)
-        ctx.save_for_backward(x, w, target, stat, kept, *(() if bias is None else (bias,)))
-        a = LinearCrossEntropyFn._args(ctx.scalars, x, w, bias, target, stat, kept)
+        ctx.has = (bias is not None, rows is not None)
+        ctx.save_for_backward(x, w, target, stat, kept, *(t for t in (bias, rows) if t is not None))
+        a = LinearCrossEntropyFn._args(ctx.scalars, x, w, bias, target, stat, kept, rows)
         a.loss = loss.data_ptr()
         _lce_call("pngpd_lce_fwd", a, x, 0)
         return loss
 
     @staticmethod
-    def _args(scalars, x, w, bias, target, stat, kept):
+    def _args(scalars, x, w, bias, target, stat, kept, rows):
         a = _lib.LceArgs()
+        a.rows = None if rows is None else rows.data_ptr()
         a.x, a.w, a.target, a.stat, a.kept = (t.data_ptr() for t in (x, w, target, stat, kept))
         a.bias = None if bias is None else bias.data_ptr()
         (a.T, a.D), a.V = x.shape, w.shape[0]
@@ -180,14 +184,15 @@ class LinearCrossEntropyFn(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dloss):
-        x, w, target, stat, kept, *bias = ctx.saved_tensors
-        bias = bias[0] if bias else None
+        x, w, target, stat, kept, *more = ctx.saved_tensors
+        bias = more.pop(0) if ctx.has[0] else None
+        rows = more.pop(0) if ctx.has[1] else None
         need = ctx.needs_input_grad
         dloss = dloss.float().contiguous()
         dx = torch.empty(x.shape, device=x.device, dtype=x.dtype) if need[0] else None
         dw = torch.empty(w.shape, device=x.device, dtype=w.dtype) if need[1] else None
         db = torch.empty_like(bias) if bias is not None and need[2] else None
-        a = LinearCrossEntropyFn._args(ctx.scalars, x, w, bias, target, stat, kept)
+        a = LinearCrossEntropyFn._args(ctx.scalars, x, w, bias, target, stat, kept, rows)
         a.dloss = dloss.data_ptr()
         a.dx, a.dw, a.db = (None if t is None else t.data_ptr() for t in (dx, dw, db))
         _lce_call("pngpd_lce_bwd", a, x, 1)

@@ -198,6 +198,18 @@ def test_classes_taken_out():
         assert not got["dw"][out].any() and not got["db"][out].any()
 
 
+@pytest.mark.parametrize("low", [torch.finfo(F32).min, -1e30])
+def test_every_class_at_the_lowest_value(low):
+    """All classes masked alike: as if none were (the logits' own differences vanish beside it)."""
+    x, w, _, y, c = data(20, 32, 400, F32, 15, bias=False)
+    b = torch.full((400,), low, device="cuda")
+    got = run(x, w, b, y, c, "none", 0.0)
+    kept = (y >= 0)
+    assert (got["loss"][kept] - math.log(400)).abs().max() <= 2.0 ** -20 * math.log(400)
+    flat = torch.where(kept, c, torch.zeros_like(c)).double().unsqueeze(1) * (1 / 400 - torch.nn.functional.one_hot(y.clamp_min(0), 400))
+    assert (got["db"].double() - flat.sum(0)).abs().max() <= 2.0 ** -18 * c.abs().sum()
+
+
 def test_large_logits():
     """Logits far past where exponentials overflow."""
     for dtype in (F32, BF16, F16):
