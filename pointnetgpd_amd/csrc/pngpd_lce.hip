@@ -39,12 +39,12 @@ struct LceArgs {
     int bf32;
     const long long *target;
     long long ignore;
-    int T, D, V, mt;
+    int T, D, V, mt, mt0;                  // mt: tiles of classes of a launch (lce_join_kernel: of all), mt0: those before
     float smooth;
     float *pm, *ps, *zt;                   // forward: (mt,T,2) max / sum, (mt,T) sum of z, (T) z at the target
     const float *stat, *coef;              // backward: (T,2) max / sum, (T)
     void *g;
-    int v0, vc, ldg;                       // the piece
+    int v0, vc, ldg;                       // the launch's classes (g starts at the first one)
 };                                         // (T above, but for target: by place among the kept rows)
 
 // The kept rows in order: 8 targets a thread and round, the places by a scan over the workgroup.
@@ -81,29 +81,6 @@ __global__ __launch_bounds__(1024) void lce_rows_kernel(const long long *__restr
     if (threadIdx.x == 0) rows[0] = base;
 }
 
-// bias of classes v .. v + 3; whole: all of them exist (classes past V read the last one's, for values nobody uses)
-template <int DT> __device__ __forceinline__ void lce_bias4(const LceArgs &a, int v, bool whole, float (&b)[4]) {
-    typedef typename elem<DT>::t E;
-    if (a.bf32) {
-        const float *p = (const float *)a.bias;
-        if (whole) __builtin_memcpy(b, p + v, 16);
-        else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) b[e] = p[min(v + e, a.V - 1)];
-        }
-    } else {
-        const E *p = (const E *)a.bias;
-        E q[4];
-        if (whole) __builtin_memcpy(q, p + v, sizeof(q));
-        else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) q[e] = p[min(v + e, a.V - 1)];
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) b[e] = ld_elem<DT>(q + e);
-    }
-}
-
 // four values of column pairs q, q + 1 of a lane and of its partner in the other half: the lane of half h is given the
 // eight consecutive ones of q + h
 __device__ __forceinline__ uint4 lce_pair(uint2 x, uint2 y) {
@@ -128,135 +105,181 @@ __device__ __forceinline__ void lce_join(float &m, float &s, float m2, float s2)
     m = M;
 }
 
-// The epilogues cost vector instructions that the matrix pipe waits for (128 values a lane): what only some tiles need
-// (the target's logit, classes past V, smoothing) is asked once a wave, and an exponential is one FMA and one v_exp_f32.
-template <int DT, int BM, int BN, int WGM, int WGN, int PIPE>
-__global__ __launch_bounds__(WGM * WGN * 64, 2) void lce_stats_kernel(const LceArgs a) {
-    typedef LceCore<DT, false, false, BM, BN, WGM, WGN, PIPE> Core;
-    extern __shared__ __align__(16) char smem[];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
-    const int wm = (wave % WGM) * Core::WM, wn = (wave / WGM) * Core::WN;
-    const int T = a.rows.count(), nt = (T + BN - 1) / BN;
-    if ((int)blockIdx.x >= a.mt * nt) return;
-    int tm, tn;
-    lce_tile_of(blockIdx.x, a.mt, nt, tm, tn);
-    const int m0 = tm * BM, n0 = tn * BN;
-    Core c;
-    c.run(smem, a.w, a.x, a.packed ? nullptr : a.rows.list(), m0, a.V, n0, T, 0, a.D);
-    float *sh = (float *)smem;                                    // [WGM][BN][3]
-    const int vb = m0 + wm + 4 * half;                            // class of the lane's row 0
-    const bool whole = m0 + BM <= a.V;
-    if (a.bias) {
-#pragma unroll
-        for (int i = 0; i < Core::FM; ++i) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                float b[4];
-                lce_bias4<DT>(a, vb + 32 * i + 8 * q, whole, b);
-#pragma unroll
-                for (int j = 0; j < Core::FN; ++j) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) c.acc[i][j][4 * q + e] += b[e];
-                }
-            }
-        }
+// What the epilogue of a tile needs beside the accumulators, fetched ahead of its loads and kept in LDS: a load issued
+// behind the next tile's would wait for those.  v: bias (both); n: target's place among the tile's classes or -1, and
+// for the gradient m log2 e, c/s, c e/V, c (or -m, where the difference is taken first: lce_far).
+template <int BM, int BN> struct LceSide {
+    float bias[BM];
+    int rel[BN];
+    float m[BN], ks[BN], kf[BN], co[BN];
+};
+
+template <int DT, int BM, int BN, int THREADS>
+__device__ __forceinline__ void lce_side(const LceArgs &a, LceSide<BM, BN> *s, int v0, int m0, int n0, int T, bool grad) {
+    typedef typename elem<DT>::t E;
+    for (int i = threadIdx.x; i < BM; i += THREADS) {
+        const int v = min(v0 + m0 + i, a.V - 1);
+        s->bias[i] = !a.bias ? 0.f : a.bf32 ? ((const float *)a.bias)[v] : ld_elem<DT>((const E *)a.bias + v);
     }
-#pragma unroll
-    for (int j = 0; j < Core::FN; ++j) {
-        const int col = wn + 32 * j + (lane & 31), k = n0 + col;
-        const long long y = k < T ? a.target[a.rows.row(k)] : -1;
-        const int rel = y >= vb && y < a.V && y < vb + Core::WM ? (int)(y - vb) : -1;
-        if (__any(rel >= 0)) {
-            float z = 0.f;
-            bool mine = false;                                    // (the other half has the other rows of four)
-#pragma unroll
-            for (int i = 0; i < Core::FM; ++i) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const bool it = rel == 32 * i + (r & 3) + 8 * (r >> 2);
-                    z = it ? c.acc[i][j][r] : z;
-                    mine |= it;
-                }
-            }
-            if (mine) a.zt[k] = z;
+    for (int i = threadIdx.x; i < BN; i += THREADS) {
+        const int k = n0 + i;
+        int rel = -2;                                             // -2: no row, or an ignored one
+        float m = 0.f, sum = 1.f, co = 0.f;
+        if (k < T) {
+            const long long y = a.target[a.rows.row(k)];
+            if (y != a.ignore) rel = y >= (long long)v0 + m0 && y < (long long)v0 + m0 + BM && y < a.V ? (int)(y - v0 - m0) : -1;
+            if (grad) { m = a.stat[2 * (size_t)k]; sum = a.stat[2 * (size_t)k + 1]; co = a.coef[k]; }
         }
-        float sz = 0.f;
-        if (whole) {
-            if (a.smooth != 0.f) {
-#pragma unroll
-                for (int i = 0; i < Core::FM; ++i) {
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) sz += c.acc[i][j][r];
-                }
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < Core::FM; ++i) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const bool past = vb + 32 * i + (r & 3) + 8 * (r >> 2) >= a.V;
-                    sz += past ? 0.f : c.acc[i][j][r];
-                    c.acc[i][j][r] = past ? -INFINITY : c.acc[i][j][r];
-                }
-            }
-        }
-        sz = half_sum(sz);
-        float m = -INFINITY, s = 0.f;
-#pragma unroll
-        for (int i = 0; i < Core::FM; ++i) {
-#pragma unroll
-            for (int r = 0; r < 16; r += 2) m = max3f(m, c.acc[i][j][r], c.acc[i][j][r + 1]);
-        }
-        float lo, hi;
-        half_pair(m, lo, hi);
-        m = fmaxf(lo, hi);
-        const float mf = m == -INFINITY ? 0.f : m, ref = mf * LOG2E;
-        if (__any(lce_far<DT>(m) && y != a.ignore)) {            // (not for what an ignored row holds: the others' bits stay)
-#pragma unroll
-            for (int i = 0; i < Core::FM; ++i) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) s += __builtin_amdgcn_exp2f((c.acc[i][j][r] - mf) * LOG2E);
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < Core::FM; ++i) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) s += __builtin_amdgcn_exp2f(fmaf(c.acc[i][j][r], LOG2E, -ref));
-            }
-        }
-        s = half_sum(s);
-        if (half == 0) {
-            float *o = sh + ((wave % WGM) * BN + col) * 3;
-            o[0] = m; o[1] = s; o[2] = sz;
-        }
-    }
-    __syncthreads();
-    for (int col = threadIdx.x; col < BN; col += Core::THREADS) {
-        const int k = n0 + col;
-        if (k >= T) continue;
-        float m = sh[col * 3], s = sh[col * 3 + 1], sz = sh[col * 3 + 2];
-#pragma unroll
-        for (int w = 1; w < WGM; ++w) {
-            const float *o = sh + (w * BN + col) * 3;
-            lce_join(m, s, o[0], o[1]);
-            sz += o[2];
-        }
-        const size_t at = (size_t)tm * a.T + k;
-        *(f32x2 *)(a.pm + 2 * at) = f32x2{m, s};
-        if (a.smooth != 0.f) a.ps[at] = sz;
+        s->rel[i] = rel;
+        if (grad) { s->m[i] = m; s->ks[i] = co / sum; s->kf[i] = co * (a.smooth / (float)a.V); s->co[i] = co; }
     }
 }
 
-// One kept row a group of 8 lanes: joins its tiles, in fp64; stat (T,2) = max, sum; row (T) = every row's loss.
+// The epilogues cost vector instructions that the matrix pipe waits for (128 values a lane of the large tile): what only
+// some tiles need (the target's logit, classes past V, smoothing) is asked once a wave, and an exponential is one FMA and
+// one v_exp_f32.  A workgroup walks over tiles: the next one's loads run under the epilogue.
+template <int DT, int BM, int BN, int WGM, int WGN, int PIPE>
+__global__ __launch_bounds__(WGM * WGN * 64, 2) void lce_stats_kernel(const LceArgs a) {
+    typedef LceCore<DT, false, false, BM, BN, WGM, WGN, PIPE> Core;
+    typedef LceSide<BM, BN> Side;
+    extern __shared__ __align__(16) char smem[];
+    Side *side = (Side *)(smem + Core::LDS);
+    float *sh = (float *)(side + 2);                              // [WGM][BN][3]
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+    const int wm = (wave % WGM) * Core::WM, wn = (wave / WGM) * Core::WN;
+    const int T = a.rows.count(), nt = (T + BN - 1) / BN, total = a.mt * nt;
+    const int *list = a.packed ? nullptr : a.rows.list();
+    int at = blockIdx.x, tm, tn, flip = 0;
+    if (at >= total) return;
+    LceOperand w = a.w;
+    w.p = (const typename elem<DT>::t *)a.w.p + (long long)a.v0 * a.w.ld;
+    Core c;
+    lce_tile_of(at, a.mt, nt, tm, tn);
+    lce_side<DT, BM, BN, Core::THREADS>(a, side, a.v0, tm * BM, tn * BN, T, false);
+    c.start(smem, w, a.x, list, tm * BM, a.vc, tn * BN, T, 0, a.D);
+    while (true) {
+        const int m0 = tm * BM, n0 = tn * BN, here = a.mt0 + tm;
+        c.finish(smem, w.ld, a.x.ld);
+        const Side *s = side + flip;
+        at += gridDim.x; flip ^= 1;
+        if (at < total) {
+            lce_tile_of(at, a.mt, nt, tm, tn);
+            lce_side<DT, BM, BN, Core::THREADS>(a, side + flip, a.v0, tm * BM, tn * BN, T, false);
+            c.start(smem, w, a.x, list, tm * BM, a.vc, tn * BN, T, 0, a.D);
+        }
+        const int vl = wm + 4 * half;                             // the lane's row 0 in the tile
+        if (a.bias) {
+#pragma unroll
+            for (int i = 0; i < Core::FM; ++i) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const f32x4 b = *(const f32x4 *)(s->bias + vl + 32 * i + 8 * q);
+#pragma unroll
+                    for (int j = 0; j < Core::FN; ++j) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) c.acc[i][j][4 * q + e] += b[e];
+                    }
+                }
+            }
+        }
+        const bool whole = m0 + BM <= a.vc;
+#pragma unroll
+        for (int j = 0; j < Core::FN; ++j) {
+            const int col = wn + 32 * j + (lane & 31), k = n0 + col, rel = s->rel[col], mine = rel - vl;
+            if (__any(mine >= 0 && mine < Core::WM)) {
+                float z = 0.f;
+                bool found = false;                               // (the other half has the other rows of four)
+#pragma unroll
+                for (int i = 0; i < Core::FM; ++i) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const bool it = mine == 32 * i + (r & 3) + 8 * (r >> 2);
+                        z = it ? c.acc[i][j][r] : z;
+                        found |= it;
+                    }
+                }
+                if (found) a.zt[k] = z;
+            }
+            float sz = 0.f;
+            if (whole) {
+                if (a.smooth != 0.f) {
+#pragma unroll
+                    for (int i = 0; i < Core::FM; ++i) {
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) sz += c.acc[i][j][r];
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < Core::FM; ++i) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const bool past = m0 + vl + 32 * i + (r & 3) + 8 * (r >> 2) >= a.vc;
+                        sz += past ? 0.f : c.acc[i][j][r];
+                        c.acc[i][j][r] = past ? -INFINITY : c.acc[i][j][r];
+                    }
+                }
+            }
+            sz = half_sum(sz);
+            float m = -INFINITY, e = 0.f;
+#pragma unroll
+            for (int i = 0; i < Core::FM; ++i) {
+#pragma unroll
+                for (int r = 0; r < 16; r += 2) m = max3f(m, c.acc[i][j][r], c.acc[i][j][r + 1]);
+            }
+            float lo, hi;
+            half_pair(m, lo, hi);
+            m = fmaxf(lo, hi);
+            const float mf = m == -INFINITY ? 0.f : m;
+            if (__any(lce_far<DT>(m) && rel != -2)) {             // (not for what an ignored row holds: the others' bits stay)
+#pragma unroll
+                for (int i = 0; i < Core::FM; ++i) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) e += __builtin_amdgcn_exp2f((c.acc[i][j][r] - mf) * LOG2E);
+                }
+            } else {
+                const float ref = mf * LOG2E;
+#pragma unroll
+                for (int i = 0; i < Core::FM; ++i) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) e += __builtin_amdgcn_exp2f(fmaf(c.acc[i][j][r], LOG2E, -ref));
+                }
+            }
+            e = half_sum(e);
+            if (half == 0) {
+                float *o = sh + ((wave % WGM) * BN + col) * 3;
+                o[0] = m; o[1] = e; o[2] = sz;
+            }
+        }
+        lce_lds_barrier();
+        for (int col = threadIdx.x; col < BN; col += Core::THREADS) {
+            const int k = n0 + col;
+            if (k >= T) continue;
+            float m = sh[col * 3], e = sh[col * 3 + 1], sz = sh[col * 3 + 2];
+#pragma unroll
+            for (int w = 1; w < WGM; ++w) {
+                const float *o = sh + (w * BN + col) * 3;
+                lce_join(m, e, o[0], o[1]);
+                sz += o[2];
+            }
+            const size_t to = (size_t)here * a.T + k;
+            *(f32x2 *)(a.pm + 2 * to) = f32x2{m, e};
+            if (a.smooth != 0.f) a.ps[to] = sz;
+        }
+        if (at >= total) return;
+    }
+}
+
+// One row a group of 32 lanes: joins its tiles, in fp64; stat (T,2) = max, sum of the kept rows; row (T) = every row's loss.
 __global__ __launch_bounds__(256) void lce_join_kernel(const LceArgs a, float *__restrict__ stat, float *__restrict__ row) {
-    __shared__ double sh[8][32][2];
-    __shared__ float shm[8][32];
-    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5, t = blockIdx.x * 32 + tx;
+    __shared__ double sh[32][8][2];
+    __shared__ float shm[32][8];
+    const int tx = threadIdx.x & 7, ty = threadIdx.x >> 3, t = blockIdx.x * 8 + tx;
     const int place = t < a.T ? a.rows.place(t) : -1;
     float m = -INFINITY;
     double s = 0.0, sz = 0.0;
     if (place >= 0) {
-        for (int k = ty; k < a.mt; k += 8) {
+        for (int k = ty; k < a.mt; k += 32) {
             const size_t at = (size_t)k * a.T + place;
             const f32x2 p = *(const f32x2 *)(a.pm + 2 * at);
             const float M = fmaxf(m, p[0]), ref = M == -INFINITY ? 0.f : M;
@@ -270,10 +293,10 @@ __global__ __launch_bounds__(256) void lce_join_kernel(const LceArgs a, float *_
     if (ty || t >= a.T) return;
     if (place < 0) { row[t] = 0.f; return; }
     float M = m;
-    for (int k = 1; k < 8; ++k) M = fmaxf(M, shm[k][tx]);
+    for (int k = 1; k < 32; ++k) M = fmaxf(M, shm[k][tx]);
     const float ref = M == -INFINITY ? 0.f : M;
     s = sz = 0.0;
-    for (int k = 0; k < 8; ++k) { s += sh[k][tx][0] * (double)expf(shm[k][tx] - ref); sz += sh[k][tx][1]; }
+    for (int k = 0; k < 32; ++k) { s += sh[k][tx][0] * (double)expf(shm[k][tx] - ref); sz += sh[k][tx][1]; }
     stat[2 * (size_t)place] = M; stat[2 * (size_t)place + 1] = (float)s;
     const long long y = a.target[t];
     double l = 0.0;
@@ -356,105 +379,104 @@ __global__ __launch_bounds__(1024) void lce_coef_kernel(const float *__restrict_
 template <int DT, int BM, int BN, int WGM, int WGN, int PIPE>
 __global__ __launch_bounds__(WGM * WGN * 64, 2) void lce_grad_kernel(const LceArgs a) {
     typedef LceCore<DT, false, false, BM, BN, WGM, WGN, PIPE> Core;
+    typedef LceSide<BM, BN> Side;
     typedef typename elem<DT>::t E;
     extern __shared__ __align__(16) char smem[];
+    Side *side = (Side *)(smem + Core::LDS);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
     const int wm = (wave % WGM) * Core::WM, wn = (wave / WGM) * Core::WN;
-    const int T = a.rows.count(), nt = (T + BN - 1) / BN;
-    if ((int)blockIdx.x >= a.mt * nt) return;
-    int tm, tn;
-    lce_tile_of(blockIdx.x, a.mt, nt, tm, tn);
-    const int m0 = tm * BM, n0 = tn * BN;
+    const int T = a.rows.count(), nt = (T + BN - 1) / BN, total = a.mt * nt;
     LceOperand w = a.w;
     w.p = (const E *)a.w.p + (long long)a.v0 * a.w.ld;
+    int at = blockIdx.x, tm, tn, flip = 0;
+    if (at >= total) return;
     Core c;
-    c.run(smem, w, a.x, nullptr, m0, a.vc, n0, T, 0, a.D);
-    const int vb = m0 + wm + 4 * half;                            // the piece's class of the lane's row 0
-    const bool whole = m0 + BM <= a.vc;
-    float m[Core::FN], ks[Core::FN], kf[Core::FN], co[Core::FN];
-    bool far = false;
+    lce_tile_of(at, a.mt, nt, tm, tn);
+    lce_side<DT, BM, BN, Core::THREADS>(a, side, a.v0, tm * BM, tn * BN, T, true);
+    c.start(smem, w, a.x, nullptr, tm * BM, a.vc, tn * BN, T, 0, a.D);
+    while (true) {
+        const int m0 = tm * BM, n0 = tn * BN;
+        c.finish(smem, w.ld, a.x.ld);
+        const Side *s = side + flip;
+        at += gridDim.x; flip ^= 1;
+        if (at < total) {
+            lce_tile_of(at, a.mt, nt, tm, tn);
+            lce_side<DT, BM, BN, Core::THREADS>(a, side + flip, a.v0, tm * BM, tn * BN, T, true);
+            c.start(smem, w, a.x, nullptr, tm * BM, a.vc, tn * BN, T, 0, a.D);
+        }
+        const int vl = wm + 4 * half;                             // the lane's row 0 in the tile
+        if (a.bias) {
 #pragma unroll
-    for (int j = 0; j < Core::FN; ++j) {
-        const int k = min(n0 + wn + 32 * j + (lane & 31), T - 1);
-        co[j] = a.coef[k];
-        m[j] = a.stat[2 * (size_t)k];
-        ks[j] = co[j] / a.stat[2 * (size_t)k + 1];
-        kf[j] = co[j] * (a.smooth / (float)a.V);
-        far |= lce_far<DT>(m[j]) && co[j] != 0.f;
-    }
-    far = __any(far);
+            for (int i = 0; i < Core::FM; ++i) {
 #pragma unroll
-    for (int i = 0; i < Core::FM; ++i) {
+                for (int q = 0; q < 4; ++q) {
+                    const f32x4 b = *(const f32x4 *)(s->bias + vl + 32 * i + 8 * q);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            float b[4] = {0.f, 0.f, 0.f, 0.f};
-            if (a.bias) lce_bias4<DT>(a, a.v0 + vb + 32 * i + 8 * q, whole, b);
+                    for (int j = 0; j < Core::FN; ++j) {
 #pragma unroll
-            for (int j = 0; j < Core::FN; ++j) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) c.acc[i][j][4 * q + e] += b[e];
+                        for (int e = 0; e < 4; ++e) c.acc[i][j][4 * q + e] += b[e];
+                    }
+                }
             }
         }
-    }
+        const bool whole = m0 + BM <= a.vc;
 #pragma unroll
-    for (int j = 0; j < Core::FN; ++j) {
-        const float ref = m[j] * LOG2E;
-        if (far) {
+        for (int j = 0; j < Core::FN; ++j) {
+            const int col = wn + 32 * j + (lane & 31), k = n0 + col, mine = s->rel[col] - vl;
+            const float m = s->m[col], ks = s->ks[col], kf = s->kf[col], co = s->co[col];
+            float ref = m * LOG2E;
+            if (__any(lce_far<DT>(m) && co != 0.f)) {
+                ref = 0.f;
+#pragma unroll
+                for (int i = 0; i < Core::FM; ++i) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) c.acc[i][j][r] -= m;
+                }
+            }
 #pragma unroll
             for (int i = 0; i < Core::FM; ++i) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
-                    c.acc[i][j][r] = fmaf(__builtin_amdgcn_exp2f((c.acc[i][j][r] - m[j]) * LOG2E), ks[j], -kf[j]);
+                    c.acc[i][j][r] = fmaf(__builtin_amdgcn_exp2f(fmaf(c.acc[i][j][r], LOG2E, -ref)), ks, -kf);
             }
-        } else {
+            if (__any(mine >= 0 && mine < Core::WM)) {
+                const float hit = co * (1.f - a.smooth);
 #pragma unroll
-            for (int i = 0; i < Core::FM; ++i) {
+                for (int i = 0; i < Core::FM; ++i) {
 #pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    c.acc[i][j][r] = fmaf(__builtin_amdgcn_exp2f(fmaf(c.acc[i][j][r], LOG2E, -ref)), ks[j], -kf[j]);
+                    for (int r = 0; r < 16; ++r) c.acc[i][j][r] -= mine == 32 * i + (r & 3) + 8 * (r >> 2) ? hit : 0.f;
+                }
             }
-        }
-    }
+            // rows without a weight (ignored ones that are still here among them) have no gradient, whatever they hold
+            const bool none = co == 0.f;
+            if (__any(none) || !whole) {
 #pragma unroll
-    for (int j = 0; j < Core::FN; ++j) {
-        const int k = n0 + wn + 32 * j + (lane & 31);
-        const long long y = k < T ? a.target[a.rows.row(k)] - a.v0 : -1;
-        const int rel = y >= vb && y < vb + Core::WM ? (int)(y - vb) : -1;
-        const float hit = co[j] * (1.f - a.smooth);
-        if (__any(rel >= 0)) {
+                for (int i = 0; i < Core::FM; ++i) {
 #pragma unroll
-            for (int i = 0; i < Core::FM; ++i) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) if (rel == 32 * i + (r & 3) + 8 * (r >> 2)) c.acc[i][j][r] -= hit;
+                    for (int r = 0; r < 16; ++r)
+                        c.acc[i][j][r] = none || m0 + vl + 32 * i + (r & 3) + 8 * (r >> 2) >= a.vc ? 0.f : c.acc[i][j][r];
+                }
             }
-        }
-        // rows without a weight (ignored ones that are still here among them) have no gradient, whatever they hold
-        const bool none = co[j] == 0.f;
-        if (__any(none) || !whole) {
+            if (k < T) {                                          // (alike in both halves: lce_pair's lanes stay together)
+                E *g = (E *)a.g + (size_t)k * a.ldg + m0 + wm;
 #pragma unroll
-            for (int i = 0; i < Core::FM; ++i) {
+                for (int i = 0; i < Core::FM; ++i) {
+                    const f32x16 &v = c.acc[i][j];
+                    if constexpr (DT == PNGPD_F32) {
 #pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if (none || vb + 32 * i + (r & 3) + 8 * (r >> 2) >= a.vc) c.acc[i][j][r] = 0.f;
-            }
-        }
-        if (k >= T) continue;                                     // (T - 1's partner lane leaves with it: both hold row k)
-        E *g = (E *)a.g + (size_t)k * a.ldg + m0 + wm;
+                        for (int q = 0; q < 4; ++q)
+                            *(f32x4 *)(g + 32 * i + 8 * q + 4 * half) = f32x4{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
+                    } else {
 #pragma unroll
-        for (int i = 0; i < Core::FM; ++i) {
-            const f32x16 &v = c.acc[i][j];
-            if constexpr (DT == PNGPD_F32) {
-#pragma unroll
-                for (int q = 0; q < 4; ++q)
-                    *(f32x4 *)(g + 32 * i + 8 * q + 4 * half) = f32x4{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
-            } else {
-#pragma unroll
-                for (int q = 0; q < 4; q += 2)
-                    *(uint4 *)(g + 32 * i + 8 * (q + half)) =
-                        lce_pair(lce_half4<DT>(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]),
-                                 lce_half4<DT>(v[4 * q + 4], v[4 * q + 5], v[4 * q + 6], v[4 * q + 7]));
+                        for (int q = 0; q < 4; q += 2)
+                            *(uint4 *)(g + 32 * i + 8 * (q + half)) =
+                                lce_pair(lce_half4<DT>(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]),
+                                         lce_half4<DT>(v[4 * q + 4], v[4 * q + 5], v[4 * q + 6], v[4 * q + 7]));
+                    }
+                }
             }
         }
+        if (at >= total) return;
     }
 }
 
@@ -537,7 +559,8 @@ __global__ __launch_bounds__(WGM * WGN * 64, 2) void lce_out_kernel(const LceOut
     const int m0 = tm * BM, n0 = tn * BN;
     const long long k0 = split * a.kper, k1 = k0 + a.kper < K ? k0 + a.kper : K;
     Core c;
-    c.run(smem, a.a, a.b, nullptr, m0, a.M, n0, N, k0, k1);
+    c.start(smem, a.a, a.b, nullptr, m0, a.M, n0, N, k0, k1);
+    c.finish(smem, a.a.ld, a.b.ld);
     const float sc = a.part ? 1.f : *a.scale;
 #pragma unroll
     for (int j = 0; j < Core::FN; ++j) {
@@ -645,20 +668,30 @@ static inline bool lce_plain(const Lce *a, const void *p, long long ld, long lon
     return lce_dp(a) == a->D && !((uintptr_t)p & 15) && (ld * es) % 16 == 0 && (double)ld * es * (double)reach < 4e9;
 }
 
-// tile shapes: 0 = 256 x 128, 1 = 64 x 64, 2 = 64 x 32
-static const int LCE_BM[3] = {256, 64, 64}, LCE_BN[3] = {128, 64, 32};
-#define LCE_SHAPE0 256, 128, 2, 2, 3
-#define LCE_SHAPE1 64, 64, 2, 2, 4
-#define LCE_SHAPE2 64, 32, 2, 1, 4
+// tile shapes: 0 = 256 x 256, 1 = 64 x 64, 2 = 64 x 32
+static const int LCE_BM[3] = {256, 64, 64}, LCE_BN[3] = {256, 64, 32};
+#define LCE_SHAPE0 256, 256, 2, 4, 2
+#define LCE_SHAPE1 64, 64, 2, 2, 3
+#define LCE_SHAPE2 64, 32, 2, 1, 3
 static inline int lce_cdiv(long long a, int b) { return (int)((a + b - 1) / b); }
 // The large tile needs a workgroup for every CU; the narrow one is for rows that would leave half of 64 unused.
 static int lce_shape(long long M, long long N) {
     if (N <= 32) return 2;
-    return (long long)lce_cdiv(M, 256) * lce_cdiv(N, 128) >= 256 ? 0 : 1;
+    return (long long)lce_cdiv(M, 256) * lce_cdiv(N, 256) >= 256 ? 0 : 1;
+}
+
+// Of `n` classes, those that the large tile takes: whole rounds of 256 workgroups (one a CU) of `other` tiles each.  What is
+// left of a round goes to the 64 x 64 tile where it is less than 0.4 of one: that tile is 2.5 times slower an operation but
+// spreads over all CUs (1024 rows, 50,000 classes: 3.06 rounds take 3.2 tiles' time in place of 4).
+static int lce_cut(int n, int other) {
+    const long long tiles = (long long)lce_cdiv(n, 256) * other, rounds = tiles / 256;
+    if (!rounds || tiles % 256 == 0 || tiles % 256 >= 102) return n;
+    const long long cut = rounds * 256 / other * 256;
+    return cut < n ? (int)cut : n;
 }
 
 struct LcePlan {
-    int Dp, fshape, fmt, padx, padw;
+    int Dp, fshape, fmt, fcut, padx, padw;
     int piece, ldg, gshape, xshape, splits, wshape;
     int share, shares;                     // db: rows of a share, shares
     long long kper;
@@ -677,7 +710,8 @@ static LcePlan lce_plan(const Lce *a, bool bwd) {
         p.padx = !lce_plain(a, a->x, a->ldx, a->rows ? a->T : 256);
         if (p.padx) p.o_x = take((size_t)a->T * p.Dp * es);
         p.fshape = lce_shape(a->V, a->T);
-        p.fmt = lce_cdiv(a->V, LCE_BM[p.fshape]);
+        p.fcut = p.fshape ? a->V : lce_cut(a->V, lce_cdiv(a->T, 256));
+        p.fmt = lce_cdiv(p.fcut, LCE_BM[p.fshape]) + lce_cdiv(a->V - p.fcut, LCE_BM[1]);
         p.o_part = take((size_t)p.fmt * a->T * 8);
         if (a->smoothing != 0.f) p.o_ps = take((size_t)p.fmt * a->T * 4);
         p.o_zt = take((size_t)a->T * 4);
@@ -692,14 +726,14 @@ static LcePlan lce_plan(const Lce *a, bool bwd) {
         if (most < 256) most = 256;
         const long long n = ((long long)a->V + most - 1) / most;
         p.piece = (int)((((long long)a->V + n - 1) / n + 255) / 256 * 256);
-        p.ldg = p.piece;
+        p.ldg = p.piece + (es == 2 ? 128 : 64);
         p.gshape = lce_shape(p.piece, a->T);
         p.o_g = take((size_t)a->T * p.ldg * es);
-        p.wshape = lce_shape(p.Dp, p.piece) ? 1 : 0;
+        p.wshape = (long long)lce_cdiv(p.Dp, 256) * lce_cdiv(p.piece, 256) >= 192 ? 0 : 1;
         // dx: few tiles and a long k: cut k until there are about 512 workgroups, of at least 256 classes
         p.xshape = a->T <= 32 ? 2 : a->T >= 128 && p.Dp >= 256 ? 0 : 1;
         const long long tiles = (long long)lce_cdiv(p.Dp, LCE_BM[p.xshape]) * lce_cdiv(a->T, LCE_BN[p.xshape]);
-        long long s = 512 / tiles;
+        long long s = (p.xshape == 0 ? 256 : 512) / tiles;
         if (s > p.piece / 256) s = p.piece / 256;
         if (s < 1) s = 1;
         p.kper = (((long long)p.piece + s - 1) / s + 63) / 64 * 64;
@@ -731,16 +765,20 @@ template <class K, class A> static int lce_launch(K kernel, int lds, long long g
     hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(threads), lds, st, a);
     return pngpd_launch_status();
 }
-template <int DT, bool GRAD, int BM, int BN, int WGM, int WGN, int PIPE> static int lce_z_shape(LceArgs &a, int M, hipStream_t st) {
-    constexpr int lds = LceCore<DT, false, false, BM, BN, WGM, WGN, PIPE>::LDS;
-    a.mt = lce_cdiv(M, BM);
-    const long long grid = (long long)a.mt * lce_cdiv(a.T, BN);
+template <int DT, bool GRAD, int BM, int BN, int WGM, int WGN, int PIPE> static int lce_z_shape(LceArgs &a, hipStream_t st) {
+    constexpr int lds = LceCore<DT, false, false, BM, BN, WGM, WGN, PIPE>::LDS + 2 * (int)sizeof(LceSide<BM, BN>) + WGM * BN * 12;
+    static_assert(lds <= 160 * 1024, "LDS of a CU");
+    a.mt = lce_cdiv(a.vc, BM);
+    // as many workgroups as run at once (256 CUs), walking over the tiles
+    const long long tiles = (long long)a.mt * lce_cdiv(a.T, BN), most = 256ll * (160 * 1024 / lds < 4 ? 160 * 1024 / lds : 4);
+    if (tiles > 0x7fffffffll - most) return PNGPD_ERR_UNSUPPORTED;
+    const long long grid = tiles < most ? tiles : most;
     if constexpr (GRAD) return lce_launch(lce_grad_kernel<DT, BM, BN, WGM, WGN, PIPE>, lds, grid, WGM * WGN * 64, a, st);
     else return lce_launch(lce_stats_kernel<DT, BM, BN, WGM, WGN, PIPE>, lds, grid, WGM * WGN * 64, a, st);
 }
-template <int DT, bool GRAD> static int lce_z(LceArgs &a, int shape, int M, hipStream_t st) {
-    return shape == 0 ? lce_z_shape<DT, GRAD, LCE_SHAPE0>(a, M, st) : shape == 1 ? lce_z_shape<DT, GRAD, LCE_SHAPE1>(a, M, st)
-                                                                                : lce_z_shape<DT, GRAD, LCE_SHAPE2>(a, M, st);
+template <int DT, bool GRAD> static int lce_z(LceArgs &a, int shape, hipStream_t st) {
+    return shape == 0 ? lce_z_shape<DT, GRAD, LCE_SHAPE0>(a, st) : shape == 1 ? lce_z_shape<DT, GRAD, LCE_SHAPE1>(a, st)
+                                                                             : lce_z_shape<DT, GRAD, LCE_SHAPE2>(a, st);
 }
 template <int DT, bool BMC, int BM, int BN, int WGM, int WGN, int PIPE> static int lce_out_shape(LceOut &a, hipStream_t st) {
     a.mt = lce_cdiv(a.M, BM); a.nt = lce_cdiv(a.no, BN);
@@ -777,10 +815,16 @@ template <int DT> static int lce_forward(const Lce *a, const LcePlan &p, hipStre
     if (p.padw) { lce_copy<DT>(a, a->w, a->ldw, a->V, 0, k.rows, ws + p.o_w, st); k.w = LceOperand{ws + p.o_w, p.Dp}; }
     k.D = p.Dp;
     k.pm = (float *)(ws + p.o_part); k.ps = (float *)(ws + p.o_ps); k.zt = (float *)(ws + p.o_zt);
-    int rc = lce_z<DT, false>(k, p.fshape, a->V, st);
+    k.vc = p.fcut;
+    int rc = lce_z<DT, false>(k, p.fshape, st);
     if (rc) return rc;
+    if (p.fcut < a->V) {
+        k.v0 = p.fcut; k.vc = a->V - p.fcut; k.mt0 = k.mt;
+        if ((rc = lce_z<DT, false>(k, 1, st))) return rc;
+    }
+    k.mt = p.fmt;
     float *row = a->reduction == PNGPD_REDUCE_NONE ? a->loss : (float *)(ws + p.o_row);
-    hipLaunchKernelGGL(lce_join_kernel, dim3((unsigned)((a->T + 31) / 32)), dim3(256), 0, st, k, a->stat, row);
+    hipLaunchKernelGGL(lce_join_kernel, dim3((unsigned)((a->T + 7) / 8)), dim3(256), 0, st, k, a->stat, row);
     if (a->reduction != PNGPD_REDUCE_NONE)
         hipLaunchKernelGGL(lce_loss_kernel, dim3(1), dim3(1024), 0, st, row, k.target, k.ignore, a->T, a->reduction, a->loss, a->kept);
     return pngpd_launch_status();
@@ -798,35 +842,46 @@ template <int DT> static int lce_backward(const Lce *a, const LcePlan &p, hipStr
     float *coef = (float *)(ws + p.o_coef), *scale = (float *)(ws + p.o_scale), *part = (float *)(ws + p.o_dx);
     hipLaunchKernelGGL(lce_coef_kernel, dim3(1), dim3(1024), 0, st, a->dloss, a->kept, k.target, k.ignore, k.rows, a->V, a->reduction,
                        DT == PNGPD_F16 ? 32768.f : 1.f, coef, scale);
-    k.stat = a->stat; k.coef = coef; k.g = ws + p.o_g; k.ldg = p.ldg;
+    k.stat = a->stat; k.coef = coef; k.ldg = p.ldg;
     for (int v0 = 0; v0 < a->V; v0 += p.piece) {
-        k.v0 = v0; k.vc = a->V - v0 < p.piece ? a->V - v0 : p.piece;
-        const int cols = (k.vc + 63) / 64 * 64;                    // columns of g that are written (zeros past vc)
-        int rc = lce_z<DT, true>(k, p.gshape, k.vc, st);
+        const int vc = a->V - v0 < p.piece ? a->V - v0 : p.piece;
+        const int cols = (vc + 63) / 64 * 64;                      // columns of g that are written (zeros past vc)
+        const int gcut = p.gshape ? vc : lce_cut(vc, lce_cdiv(a->T, 256));
+        k.v0 = v0; k.vc = gcut; k.g = ws + p.o_g;
+        int rc = lce_z<DT, true>(k, p.gshape, st);
         if (rc) return rc;
+        if (gcut < vc) {
+            k.v0 = v0 + gcut; k.vc = vc - gcut; k.g = (E *)(ws + p.o_g) + gcut;
+            if ((rc = lce_z<DT, true>(k, 1, st))) return rc;
+        }
+        const E *g = (const E *)(ws + p.o_g);
         const E *w = (const E *)k.w.p + (long long)v0 * k.w.ld;
         if (a->db) {
             float *sums = (float *)(ws + p.o_db);
             void *db = a->bias_dtype == PNGPD_F32 ? (void *)((float *)a->db + v0) : (void *)((E *)a->db + v0);
             hipLaunchKernelGGL(lce_db_kernel<DT>, dim3((unsigned)lce_cdiv(cols, DT == PNGPD_F32 ? 32 : 64), p.shares), dim3(256), 0, st,
-                               k.g, k.rows, p.ldg, p.share, cols, sums);
-            hipLaunchKernelGGL(lce_db_join_kernel<DT>, dim3((unsigned)lce_cdiv(k.vc, 256)), dim3(256), 0, st, sums, p.shares, p.ldg,
-                               k.vc, scale, db, a->bias_dtype == PNGPD_F32);
+                               g, k.rows, p.ldg, p.share, cols, sums);
+            hipLaunchKernelGGL(lce_db_join_kernel<DT>, dim3((unsigned)lce_cdiv(vc, 256)), dim3(256), 0, st, sums, p.shares, p.ldg,
+                               vc, scale, db, a->bias_dtype == PNGPD_F32);
         }
         if (a->dx) {
             LceOut o = {};
-            o.a = LceOperand{w, k.w.ld}; o.b = LceOperand{k.g, p.ldg}; o.rows = k.rows;
-            o.M = p.Dp; o.N = -1; o.mo = a->D; o.no = a->T; o.K = k.vc; o.kper = p.kper; o.splits = p.splits;
+            o.a = LceOperand{w, k.w.ld}; o.b = LceOperand{g, p.ldg}; o.rows = k.rows;
+            o.M = p.Dp; o.N = -1; o.mo = a->D; o.no = a->T; o.K = vc; o.kper = p.kper; o.splits = p.splits;
             o.part = part; o.add = v0 > 0; o.scale = scale;
             if ((rc = lce_out<DT, false>(o, p.xshape, st))) return rc;
         }
         if (a->dw) {
-            LceOut o = {};
-            o.a = LceOperand{k.x.p, p.Dp}; o.b = LceOperand{k.g, p.ldg}; o.rows = k.rows;
-            o.M = p.Dp; o.N = cols; o.mo = a->D; o.no = k.vc; o.K = -1; o.kper = a->T; o.splits = 1;
-            o.out = (E *)a->dw + (long long)v0 * a->D; o.ldo = a->D; o.scale = scale;
-            o.vec = (a->D * (long long)sizeof(E)) % 16 == 0 && !((uintptr_t)a->dw & 15);
-            if ((rc = lce_out<DT, true>(o, p.wshape, st))) return rc;
+            const int wcut = p.wshape ? vc : lce_cut(vc, lce_cdiv(p.Dp, 256));
+            for (int c0 = 0; c0 < vc; c0 = c0 ? vc : wcut) {       // the large tile's classes, then the rest
+                const int c1 = c0 ? vc : wcut;
+                LceOut o = {};
+                o.a = LceOperand{k.x.p, p.Dp}; o.b = LceOperand{g + c0, p.ldg}; o.rows = k.rows;
+                o.M = p.Dp; o.N = (c1 == vc ? cols : c1) - c0; o.mo = a->D; o.no = c1 - c0; o.K = -1; o.kper = a->T; o.splits = 1;
+                o.out = (E *)a->dw + (long long)(v0 + c0) * a->D; o.ldo = a->D; o.scale = scale;
+                o.vec = (a->D * (long long)sizeof(E)) % 16 == 0 && !((uintptr_t)a->dw & 15);
+                if ((rc = lce_out<DT, true>(o, c0 ? 1 : p.wshape, st))) return rc;
+            }
         }
     }
     if (a->dx) {

@@ -10,11 +10,12 @@
 // v_mfma_f32_32x32x* holds one column n and 16 rows m in runs of four — softmax statistics of a row of logits reduce
 // inside a lane, and stores are 8 or 16 bytes.
 //
-// A K tile (64 bytes of k: 32 of 16 bits, 16 of 32) of both operands goes from global memory straight into LDS
-// (global_load_lds_dwordx4, no registers, the address a scalar base that walks along k plus a 32-bit lane offset that
-// stays), PIPE - 1 tiles ahead of the matrix instructions, one barrier a tile; two workgroups of the large tile share a
-// CU, so one's barrier and epilogue hide behind the other's products.  The LDS destination of that load is lane after
-// lane, so the XOR swizzle against bank conflicts is put on the SOURCE: slot p of LDS row r holds chunk p ^ f(r).
+// A K tile (128 bytes of k: 64 of 16 bits, 32 of 32, four steps of the matrix instructions) of both operands goes from
+// global memory straight into LDS (global_load_lds_dwordx4, no registers, the address a scalar base that walks along k
+// plus a 32-bit lane offset that stays), up to PIPE - 1 tiles ahead of the matrix instructions.  A wave reads the
+// fragments of a step while the products of the step before run; the one barrier of a tile stands before its last
+// step, which has its fragments.  The LDS destination of that load is lane after lane, so the XOR swizzle
+// against bank conflicts is put on the SOURCE: slot p of LDS row r holds chunk p ^ f(r).
 //   KC: fragments are ds_read_b128 (8 or 4 consecutive k of a row);
 //   MC, 16 bits: ds_read_b64_tr_b16, which transposes a [4 k][16 m] block over 16 lanes; 32 bits: ds_read_b32 per k.
 // (Measured: no bank conflict in any of the three products.)
@@ -30,7 +31,9 @@ typedef __bf16 lce_bf16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) lce_bf16x4 lds_lce_bf16x4;
 typedef __attribute__((address_space(3))) char lds_char;
 
-#define LCE_KB 64                          // bytes of k in a tile
+#define LCE_KB 128                         // bytes of k in a tile: a cache line of every row of a KC operand
+#define LCE_BAND 4                         // n tiles of a band (lce_tile_of)
+
 struct LceOperand {
     const void *p;
     long long ld;                          // elements from row to row
@@ -47,11 +50,17 @@ template <int N> __device__ __forceinline__ void lce_wait_barrier() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(N) : "memory");
 }
 
-// for a pipeline of DEPTH tiles of LOADS loads each: the oldest tile has landed, `younger` of the others are on their way
-template <int LOADS, int DEPTH> __device__ __forceinline__ void lce_wait_tile(int younger) {
-    if (DEPTH >= 3 && younger >= 2) lce_wait_barrier<2 * LOADS>();
-    else if (DEPTH >= 2 && younger >= 1) lce_wait_barrier<LOADS>();
-    else lce_wait_barrier<0>();
+// all but the youngest tiles' loads have landed: of MOST tiles that may be on their way behind the one waited for, `n` are
+template <int LOADS, int MOST> __device__ __forceinline__ void lce_wait_tile(int n) {
+    if (MOST >= 3 && n >= 3) lce_wait_barrier<3 * LOADS>();
+    else if (MOST >= 2 && n == 2) lce_wait_barrier<2 * LOADS>();
+    else if (MOST >= 1 && n == 1) lce_wait_barrier<LOADS>();
+    else if (n <= 0) lce_wait_barrier<0>();
+    else lce_wait_barrier<MOST * LOADS>();
+}
+// LDS is settled between the waves; loads on their way stay so
+__device__ __forceinline__ void lce_lds_barrier() {
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" : : : "memory");
 }
 
 __device__ __align__(16) unsigned lce_zero[4];       // what a chunk past the end of k reads
@@ -66,7 +75,7 @@ template <int DT, bool MC, int ROWS, int THREADS> struct LceTile {
     unsigned off[LOADS];                   // bytes from there to the lane's chunks (below 4 GiB: the host sees to it)
 
     static __device__ __forceinline__ int swz(int row) {
-        if constexpr (!MC) return (row >> 2) & 3;
+        if constexpr (!MC) return (row >> 1) & 7;
         else if constexpr (DT == PNGPD_F32) return RB >= 256 ? ((row >> 2) & 1) << 3 : 0;
         else return RB >= 256 ? (row & 3) << 2 : RB == 128 ? ((row >> 1) & 1) << 2 : 0;
     }
@@ -142,20 +151,58 @@ template <int DT> __device__ __forceinline__ f32x16 lce_mma(const f32x4 &a, cons
     }
 }
 
-// The accumulators of one workgroup's tile: BM x BN, WGM x WGN waves, PIPE tiles of k in LDS.  k in [k0, k1).
+// One workgroup's tile: BM x BN, WGM x WGN waves, PIPE tiles of k in LDS.  start() sends the first loads on their way (the
+// LDS is free from the end of finish() on, so the next tile's may run under this one's epilogue), finish() does the rest.
 template <int DT, bool AMC, bool BMC, int BM, int BN, int WGM, int WGN, int PIPE> struct LceCore {
     static constexpr int THREADS = WGM * WGN * 64, WM = BM / WGM, WN = BN / WGN, FM = WM / 32, FN = WN / 32;
     typedef LceTile<DT, AMC, BM, THREADS> TA;
     typedef LceTile<DT, BMC, BN, THREADS> TB;
-    static constexpr int STAGE = TA::BYTES + TB::BYTES, LDS = PIPE * STAGE, BK = TA::BK;
-    static_assert(PIPE >= 2 && PIPE <= 4, "lce_wait_tile counts up to three tiles");
+    static constexpr int STAGE = TA::BYTES + TB::BYTES, LDS = PIPE * STAGE, BK = TA::BK, LOADS = TA::LOADS + TB::LOADS;
+    static_assert(PIPE >= 2 && PIPE <= 5, "lce_wait_tile counts up to three tiles");
+    static constexpr int STEPS = LCE_KB / 32;
     f32x16 acc[FM][FN];
+    TA ta;
+    TB tb;
+    long long left;                        // k that the next tile to load has
+    int tiles, stage;                      // tiles of k; where the next one goes
+    unsigned lds0;
 
-    __device__ __forceinline__ void run(char *smem, const LceOperand &a, const LceOperand &b, const int *rows, int m0, int M,
-                                        int n0, int N, long long k0, long long k1) {
+    __device__ __forceinline__ void load(long long lda, long long ldb) {
+        const int l = left < BK ? (int)left : BK;
+        ta.load(lds0 + stage * STAGE, l, lda);
+        tb.load(lds0 + stage * STAGE + TA::BYTES, l, ldb);
+        left -= BK;
+        stage = stage == PIPE - 1 ? 0 : stage + 1;
+    }
+    // k in [k0, k1)
+    __device__ __forceinline__ void start(char *smem, const LceOperand &a, const LceOperand &b, const int *rows, int m0, int M,
+                                          int n0, int N, long long k0, long long k1) {
+        lds0 = (unsigned)(uintptr_t)(lds_char *)smem;
+        ta.init(a, nullptr, m0, M, k0);
+        tb.init(b, rows, n0, N, k0);
+        left = k1 - k0;
+        tiles = left > 0 ? (int)((left + BK - 1) / BK) : 0;
+        stage = 0;
+#pragma unroll
+        for (int t = 0; t < PIPE - 1; ++t) if (t < tiles) load(a.ld, b.ld);
+    }
+    __device__ __forceinline__ void frags(f32x4 (&fa)[FM], f32x4 (&fb)[FN], const char *sa, int wm, int wn, int s, int lane) {
+        const char *sb = sa + TA::BYTES;
+#pragma unroll
+        for (int j = 0; j < FN; ++j) fb[j] = TB::frag(sb, wn + 32 * j, s, lane);
+#pragma unroll
+        for (int i = 0; i < FM; ++i) fa[i] = TA::frag(sa, wm + 32 * i, s, lane);
+    }
+    __device__ __forceinline__ void products(const f32x4 (&fa)[FM], const f32x4 (&fb)[FN]) {
+#pragma unroll
+        for (int i = 0; i < FM; ++i) {
+#pragma unroll
+            for (int j = 0; j < FN; ++j) acc[i][j] = lce_mma<DT>(fa[i], fb[j], acc[i][j]);
+        }
+    }
+    __device__ __forceinline__ void finish(const char *smem, long long lda, long long ldb) {
         const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
         const int wm = (wave % WGM) * WM, wn = (wave / WGM) * WN;
-        const unsigned lds0 = (unsigned)(uintptr_t)(lds_char *)smem;
 #pragma unroll
         for (int i = 0; i < FM; ++i) {
 #pragma unroll
@@ -164,41 +211,26 @@ template <int DT, bool AMC, bool BMC, int BM, int BN, int WGM, int WGN, int PIPE
                 for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
             }
         }
-        TA ta;
-        TB tb;
-        ta.init(a, nullptr, m0, M, k0);
-        tb.init(b, rows, n0, N, k0);
-        long long left = k1 - k0;                                  // k that the next tile to load has
-        const int tiles = left > 0 ? (int)((left + BK - 1) / BK) : 0;
-        auto load = [&](int stage) {
-            const int l = left < BK ? (int)left : BK;
-            ta.load(lds0 + stage * STAGE, l, a.ld);
-            tb.load(lds0 + stage * STAGE + TA::BYTES, l, b.ld);
-            left -= BK;
-        };
-#pragma unroll
-        for (int t = 0; t < PIPE - 1; ++t) if (t < tiles) load(t);
+        if (tiles == 0) { lce_wait_barrier<0>(); return; }
+        f32x4 fa[2][FM], fb[2][FN];
+        lce_wait_tile<LOADS, PIPE - 2>(tiles - 1);
+        frags(fa[0], fb[0], smem, wm, wn, 0, lane);
         int cur = 0;
         for (int t = 0; t < tiles; ++t) {
-            lce_wait_tile<TA::LOADS + TB::LOADS, PIPE - 1>(tiles - 1 - t);      // tile t is there, t - 1's LDS is free
-            if (t + PIPE - 1 < tiles) load(cur ? cur - 1 : PIPE - 1);
-            const char *sa = smem + cur * STAGE, *sb = sa + TA::BYTES;
+            const char *sa = smem + cur * STAGE;
             cur = cur == PIPE - 1 ? 0 : cur + 1;
+            if (t + PIPE - 1 < tiles) load(lda, ldb);              // over tile t - 1, which every wave has read
 #pragma unroll
-            for (int s = 0; s < LCE_KB / 32; ++s) {
-                f32x4 fa[FM], fb[FN];
-#pragma unroll
-                for (int j = 0; j < FN; ++j) fb[j] = TB::frag(sb, wn + 32 * j, s, lane);
-#pragma unroll
-                for (int i = 0; i < FM; ++i) fa[i] = TA::frag(sa, wm + 32 * i, s, lane);
-#pragma unroll
-                for (int i = 0; i < FM; ++i) {
-#pragma unroll
-                    for (int j = 0; j < FN; ++j) acc[i][j] = lce_mma<DT>(fa[i], fb[j], acc[i][j]);
-                }
+            for (int s = 0; s + 1 < STEPS; ++s) {
+                frags(fa[(s + 1) & 1], fb[(s + 1) & 1], sa, wm, wn, s + 1, lane);
+                products(fa[s & 1], fb[s & 1]);
+                __builtin_amdgcn_sched_barrier(0);
             }
+            lce_wait_tile<LOADS, PIPE - 2>(tiles - 2 - t);         // tile t + 1 is there, tile t is read
+            if (t + 1 < tiles) frags(fa[0], fb[0], smem + cur * STAGE, wm, wn, 0, lane);
+            products(fa[1], fb[1]);
+            __builtin_amdgcn_sched_barrier(0);
         }
-        lce_wait_barrier<0>();                                     // the epilogue may use the LDS
     }
 };
 
@@ -208,7 +240,7 @@ __device__ __forceinline__ void lce_tile_of(int i, int mt, int nt, int &m, int &
     const int per = (mt * nt) >> 3;
     int w = i;
     if (i < per * 8) w = (i & 7) * per + (i >> 3);
-    const int band = w / (8 * mt), r = w - band * 8 * mt;
-    const int wide = nt - band * 8 < 8 ? nt - band * 8 : 8;
-    m = r / wide; n = band * 8 + r % wide;
+    const int band = w / (LCE_BAND * mt), r = w - band * LCE_BAND * mt;
+    const int wide = nt - band * LCE_BAND < LCE_BAND ? nt - band * LCE_BAND : LCE_BAND;
+    m = r / wide; n = band * LCE_BAND + r % wide;
 }
