@@ -20,6 +20,8 @@
 #include "pngpd_common.h"
 #include "pngpd_types.h"
 
+#define SLAB_THREADS 512                // of a slab's workgroup: two share a CU, one loads while the other computes
+
 struct GnArgs {
     const void *x, *dy, *w, *b;
     void *y, *dx;
@@ -96,39 +98,33 @@ __device__ __forceinline__ void load_rows(Col<DT, VEC> (&q)[K], const typename e
 
 // ---------------------------------------------------------------- activations
 // Phi(z), the normal distribution, and e = exp(-z^2/2): erf by Abramowitz & Stegun 7.1.26 (|error| < 1.5e-7), whose
-// exponential is the density's too; ~16 instructions where erff takes both its branches in a divergent wave.
+// exponential is the density's too; 14 instructions where erff takes both its branches in a divergent wave.
 __device__ __forceinline__ float phi_cdf(float z, float &e) {
-    const float a = fabsf(z) * 0.70710678118654752f;
-    const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, a, 1.f));
-    e = __expf(-0.5f * z * z);
-    const float p = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
-    const float tail = 0.5f * p * e;
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f * 0.70710678118654752f, fabsf(z), 1.f));
+    e = __builtin_amdgcn_exp2f(z * z * (-0.5f * 1.44269504088896340736f));
+    const float p = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 0.5f * 1.061405429f, 0.5f * -1.453152027f), 0.5f * 1.421413741f),
+                                     0.5f * -0.284496736f), 0.5f * 0.254829592f);
+    const float tail = p * e;
     return z < 0.f ? tail : 1.f - tail;
 }
-__device__ __forceinline__ float act_value(int act, float z) {
-    float e;
-    switch (act) {
-    case PNGPD_ACT_RELU: return z < 0.f ? 0.f : z;                    // NaN passes
-    case PNGPD_ACT_SILU: return z * __builtin_amdgcn_rcpf(1.f + __expf(-z));
-    case PNGPD_ACT_GELU: return z * phi_cdf(z, e);
-    default: return z;
-    }
+__device__ __forceinline__ float sigmoid(float z) {
+    return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * -1.44269504088896340736f));
 }
-// act'(z) for relu takes its own z (see gn_slope)
-__device__ __forceinline__ float act_slope(int act, float z) {
-    float e, s;
-    switch (act) {
-    case PNGPD_ACT_SILU: s = __builtin_amdgcn_rcpf(1.f + __expf(-z)); return s * fmaf(z, 1.f - s, 1.f);
-    case PNGPD_ACT_GELU: s = phi_cdf(z, e); return fmaf(z * 0.39894228040143268f, e, s);
-    default: return 1.f;
-    }
+// ACT: PNGPD_ACT_*
+template <int ACT> __device__ __forceinline__ float act_value(float z) {
+    float e;
+    if constexpr (ACT == PNGPD_ACT_RELU) return z < 0.f ? 0.f : z;                  // NaN passes
+    else if constexpr (ACT == PNGPD_ACT_SILU) return z * sigmoid(z);
+    else if constexpr (ACT == PNGPD_ACT_GELU) return z * phi_cdf(z, e);
+    else return z;
 }
 
-// What a thread keeps of its column: w, b and, for each of SUB groups it touches, the statistics.  SUB = 1: the column
-// lies inside one group (Cg a multiple of VEC); SUB = VEC: every element may belong to another one.
+// What a thread keeps of its column: w, b and, for each of the SUB groups it touches, the statistics.  SUB = 1: the column
+// lies inside one group (Cg a multiple of VEC); 2: it is two whole groups; VEC: every element may belong to another one.
 template <int VEC, int SUB> struct ColPar {
     float w[VEC], b[VEC];
-    double mean[SUB], rstd[SUB];
+    float mean[SUB], rstd[SUB];
+    static __device__ __forceinline__ int sub(int e) { return e * SUB / VEC; }
 };
 template <int DT, int VEC, int SUB>
 __device__ __forceinline__ void load_wb(const GnArgs &a, int c, int n, ColPar<VEC, SUB> &p) {
@@ -146,30 +142,32 @@ template <int VEC, int SUB>
 __device__ __forceinline__ void load_stats(const GnArgs &a, const double *st, int c, int n, int g0, ColPar<VEC, SUB> &p) {
 #pragma unroll
     for (int e = 0; e < SUB; ++e) {
-        p.mean[e] = 0.0; p.rstd[e] = 0.0;
-        if (e < n) {
-            const int g = (c + e) / a.Cg - g0;
-            p.mean[e] = st[2 * g]; p.rstd[e] = st[2 * g + 1];
+        p.mean[e] = 0.f; p.rstd[e] = 0.f;
+        const int at = e * (VEC / SUB);
+        if (at < n) {
+            const int g = (c + at) / a.Cg - g0;
+            p.mean[e] = (float)st[2 * g]; p.rstd[e] = (float)st[2 * g + 1];
         }
     }
 }
-template <int VEC, int SUB>
-__device__ __forceinline__ void gn_apply(const GnArgs &a, const ColPar<VEC, SUB> &p, const float (&x)[VEC], float (&y)[VEC]) {
+template <int ACT, int VEC, int SUB>
+__device__ __forceinline__ void gn_apply(const ColPar<VEC, SUB> &p, const float (&x)[VEC], float (&y)[VEC]) {
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
-        const int s = SUB == 1 ? 0 : e;
-        y[e] = act_value(a.act, fmaf((x[e] - (float)p.mean[s]) * (float)p.rstd[s], p.w[e], p.b[e]));
+        const int s = p.sub(e);
+        y[e] = act_value<ACT>(fmaf((x[e] - p.mean[s]) * p.rstd[s], p.w[e], p.b[e]));
     }
 }
-// dz and xh of one element
-template <int VEC, int SUB>
-__device__ __forceinline__ float gn_dz(const GnArgs &a, const ColPar<VEC, SUB> &p, int e, float x, float dy, float &xh) {
-    const int s = SUB == 1 ? 0 : e;
-    xh = (x - (float)p.mean[s]) * (float)p.rstd[s];
-    if (a.act == PNGPD_ACT_NONE) return dy;
-    if (a.act == PNGPD_ACT_RELU)
-        return fma(((double)x - p.mean[s]) * p.rstd[s], (double)p.w[e], (double)p.b[e]) <= 0.0 ? 0.f : dy;
-    return dy * act_slope(a.act, fmaf(xh, p.w[e], p.b[e]));
+// dz of one element; st: the fp64 statistics (mean, rstd) of its group, for relu's slope
+template <int ACT>
+__device__ __forceinline__ float gn_dz(float x, float xh, float dy, float w, float b, const double *st) {
+    if constexpr (ACT == PNGPD_ACT_NONE) return dy;
+    else if constexpr (ACT == PNGPD_ACT_RELU) return fma(((double)x - st[0]) * st[1], (double)w, (double)b) <= 0.0 ? 0.f : dy;
+    else {
+        const float z = fmaf(xh, w, b);
+        if constexpr (ACT == PNGPD_ACT_SILU) { const float s = sigmoid(z); return dy * (s * fmaf(z, 1.f - s, 1.f)); }
+        else { float e; const float s = phi_cdf(z, e); return dy * fmaf(z * 0.39894228040143268f, e, s); }
+    }
 }
 
 // sum over the lanes of a wave that hold the same column (lane ^ (1 << lx), ... )
@@ -192,8 +190,8 @@ __device__ __forceinline__ int slab_item(int i, int ranges, int total) {
 }
 
 // ---------------------------------------------------------------------------------------------- slab form
-template <int DT, int VEC, int SUB, int RPT>
-__global__ __launch_bounds__(1024) void gn_fwd_slab_kernel(const GnArgs a) {
+template <int DT, int VEC, int SUB, int RPT, int ACT>
+__global__ __launch_bounds__(SLAB_THREADS) void gn_fwd_slab_kernel(const GnArgs a) {
     typedef typename elem<DT>::t T;
     extern __shared__ double sh[];
     const int tid = threadIdx.x, X = 1 << a.lx, tx = tid & (X - 1), ty = tid >> a.lx, TY = blockDim.x >> a.lx;
@@ -215,7 +213,7 @@ __global__ __launch_bounds__(1024) void gn_fwd_slab_kernel(const GnArgs a) {
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
                 const double v = (double)q[i].get(e);
-                const int k = SUB == 1 ? 0 : e;
+                const int k = p.sub(e);
                 s[k] += v; s2[k] = fma(v, v, s2[k]);
             }
         }
@@ -232,7 +230,7 @@ __global__ __launch_bounds__(1024) void gn_fwd_slab_kernel(const GnArgs a) {
     }
     double *st = sh + 2 * (size_t)waves * units;
     __syncthreads();
-    const int upg = SUB == 1 ? a.Cg / VEC : a.Cg;       // units of a group
+    const int upg = a.Cg * SUB / VEC;                     // units of a group
     const double m = (double)a.N * a.Cg;
     for (int g = wave; g < gn; g += waves) {
         double u = 0.0, v = 0.0;
@@ -262,15 +260,17 @@ __global__ __launch_bounds__(1024) void gn_fwd_slab_kernel(const GnArgs a) {
             float v[VEC], o[VEC];
 #pragma unroll
             for (int e = 0; e < VEC; ++e) v[e] = q[i].get(e);
-            gn_apply(a, p, v, o);
+            gn_apply<ACT>(p, v, o);
             Col<DT, VEC>::store(y + (size_t)row * a.C, o, n);
         }
     }
 }
 
-template <int DT, int VEC, int SUB, int RPT>
-__global__ __launch_bounds__(1024) void gn_bwd_slab_kernel(const GnArgs a) {
+// dz stays in registers (float32) between the sums and dx where its slope is dear (silu, gelu); none and relu take dy again.
+template <int DT, int VEC, int SUB, int RPT, int ACT>
+__global__ __launch_bounds__(SLAB_THREADS) void gn_bwd_slab_kernel(const GnArgs a) {
     typedef typename elem<DT>::t T;
+    constexpr bool KEEP = ACT == PNGPD_ACT_SILU || ACT == PNGPD_ACT_GELU;
     extern __shared__ double sh[];
     const int tid = threadIdx.x, X = 1 << a.lx, tx = tid & (X - 1), ty = tid >> a.lx, TY = blockDim.x >> a.lx;
     const int waves = blockDim.x >> 6, wave = tid >> 6, lane = tid & 63;
@@ -279,13 +279,14 @@ __global__ __launch_bounds__(1024) void gn_bwd_slab_kernel(const GnArgs a) {
     const int c = c0 + tx * VEC, n = max(0, min(VEC, c1 - c));
     const T *x = (const T *)a.x + (long long)b * a.sB + c;
     const T *dy = (const T *)a.dy + (size_t)b * a.N * a.C + c;
+    const double *stats = a.stats + 2 * ((size_t)b * a.G + g0);
     Col<DT, VEC> q[RPT], d[RPT];
     load_rows<RPT>(q, x, a.sN, ty, TY, a.N, n);
     load_rows<RPT>(d, dy, a.C, ty, TY, a.N, n);
     ColPar<VEC, SUB> p;
     load_wb<DT>(a, c, n, p);
-    load_stats(a, a.stats + 2 * ((size_t)b * a.G + g0), c, n, g0, p);
-    float A[VEC], Bs[VEC];
+    load_stats(a, stats, c, n, g0, p);
+    float A[VEC], Bs[VEC], keep[KEEP ? RPT : 1][VEC];
 #pragma unroll
     for (int e = 0; e < VEC; ++e) { A[e] = 0.f; Bs[e] = 0.f; }
 #pragma unroll
@@ -293,8 +294,11 @@ __global__ __launch_bounds__(1024) void gn_bwd_slab_kernel(const GnArgs a) {
         if (ty + i * TY < a.N) {
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
-                float xh;
-                const float dz = gn_dz(a, p, e, q[i].get(e), d[i].get(e), xh);
+                const int k = p.sub(e);
+                const float xv = q[i].get(e), xh = (xv - p.mean[k]) * p.rstd[k];
+                const double *st = stats + 2 * (ACT == PNGPD_ACT_RELU ? (c + min(e, max(n, 1) - 1)) / a.Cg - g0 : 0);
+                const float dz = gn_dz<ACT>(xv, xh, d[i].get(e), p.w[e], p.b[e], st);
+                if constexpr (KEEP) keep[i][e] = dz;
                 A[e] += dz; Bs[e] = fmaf(dz, xh, Bs[e]);
             }
         }
@@ -338,7 +342,7 @@ __global__ __launch_bounds__(1024) void gn_bwd_slab_kernel(const GnArgs a) {
     float S1[SUB], S2[SUB];
 #pragma unroll
     for (int e = 0; e < SUB; ++e) {
-        const int g = (c + min(e, n - 1)) / a.Cg - g0;
+        const int g = (c + min(e * (VEC / SUB), n - 1)) / a.Cg - g0;
         S1[e] = (float)st[2 * g]; S2[e] = (float)st[2 * g + 1];
     }
     T *dx = (T *)a.dx + (size_t)b * a.N * a.C + c;
@@ -349,10 +353,13 @@ __global__ __launch_bounds__(1024) void gn_bwd_slab_kernel(const GnArgs a) {
             float o[VEC];
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
-                const int s = SUB == 1 ? 0 : e;
-                float xh;
-                const float dz = gn_dz(a, p, e, q[i].get(e), d[i].get(e), xh);
-                o[e] = (float)p.rstd[s] * (fmaf(dz, p.w[e], -S1[s]) - xh * S2[s]);
+                const int k = p.sub(e);
+                const float xv = q[i].get(e), xh = (xv - p.mean[k]) * p.rstd[k];
+                float dz;
+                if constexpr (KEEP) dz = keep[i][e];
+                else dz = gn_dz<ACT>(xv, xh, d[i].get(e), p.w[e], p.b[e],
+                                     stats + 2 * (ACT == PNGPD_ACT_RELU ? (c + min(e, n - 1)) / a.Cg - g0 : 0));
+                o[e] = p.rstd[k] * (fmaf(dz, p.w[e], -S1[k]) - xh * S2[k]);
             }
             Col<DT, VEC>::store(dx + (size_t)row * a.C, o, n);
         }
@@ -390,7 +397,7 @@ __global__ __launch_bounds__(256) void gn_fwd_part_kernel(const GnArgs a) {
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) {
                     const double v = (double)q[i].get(e);
-                    const int k = SUB == 1 ? 0 : e;
+                    const int k = e * SUB / VEC;
                     s[k] += v; s2[k] = fma(v, v, s2[k]);
                 }
             }
@@ -407,7 +414,7 @@ __global__ __launch_bounds__(256) void gn_fwd_part_kernel(const GnArgs a) {
         }
     }
     __syncthreads();
-    const int per = SUB == 1 ? VEC : 1, total = a.C / per;          // channels of a unit, units of a row
+    const int per = VEC / SUB, total = a.C / per;                   // channels of a unit, units of a row
     double *out = a.part + 2 * ((size_t)b * a.S + sp) * total;
     for (int k = tid; k < units; k += 256) {
         const int u = col * units + k;
@@ -443,7 +450,7 @@ __global__ __launch_bounds__(256) void gn_stats_kernel(const GnArgs a, int per) 
     }
 }
 
-template <int DT, int VEC, int SUB>
+template <int DT, int VEC, int SUB, int ACT>
 __global__ __launch_bounds__(256) void gn_fwd_apply_kernel(const GnArgs a) {
     typedef typename elem<DT>::t T;
     const int tid = threadIdx.x, X = 1 << a.lx, tx = tid & (X - 1), ty = tid >> a.lx, TY = 256 >> a.lx;
@@ -454,7 +461,8 @@ __global__ __launch_bounds__(256) void gn_fwd_apply_kernel(const GnArgs a) {
     const int r0 = sp * a.rows, r1 = min(a.N, r0 + a.rows);
     ColPar<VEC, SUB> p;
     load_wb<DT>(a, c, n, p);
-    load_stats(a, a.stats + 2 * (size_t)b * a.G, c, n, 0, p);
+    const double *stats = a.stats + 2 * (size_t)b * a.G;
+    load_stats(a, stats, c, n, 0, p);
     const T *x = (const T *)a.x + (long long)b * a.sB + c;
     T *y = (T *)a.y + (size_t)b * a.N * a.C + c;
     for (int row = r0 + ty; row < r1; row += 4 * TY) {
@@ -466,14 +474,14 @@ __global__ __launch_bounds__(256) void gn_fwd_apply_kernel(const GnArgs a) {
                 float v[VEC], o[VEC];
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) v[e] = q[i].get(e);
-                gn_apply(a, p, v, o);
+                gn_apply<ACT>(p, v, o);
                 Col<DT, VEC>::store(y + (size_t)(row + i * TY) * a.C, o, n);
             }
         }
     }
 }
 
-template <int DT, int VEC, int SUB>
+template <int DT, int VEC, int SUB, int ACT>
 __global__ __launch_bounds__(256) void gn_bwd_part_kernel(const GnArgs a) {
     typedef typename elem<DT>::t T;
     extern __shared__ double sh[];
@@ -486,7 +494,8 @@ __global__ __launch_bounds__(256) void gn_bwd_part_kernel(const GnArgs a) {
     const int r0 = sp * a.rows, r1 = min(a.N, r0 + a.rows);
     ColPar<VEC, SUB> p;
     load_wb<DT>(a, c, n, p);
-    load_stats(a, a.stats + 2 * (size_t)b * a.G, c, n, 0, p);
+    const double *stats = a.stats + 2 * (size_t)b * a.G;
+    load_stats(a, stats, c, n, 0, p);
     const T *x = (const T *)a.x + (long long)b * a.sB + c;
     const T *dy = (const T *)a.dy + (size_t)b * a.N * a.C + c;
     float A[VEC], Bs[VEC];
@@ -502,8 +511,10 @@ __global__ __launch_bounds__(256) void gn_bwd_part_kernel(const GnArgs a) {
                 if (row + i * TY < r1) {
 #pragma unroll
                     for (int e = 0; e < VEC; ++e) {
-                        float xh;
-                        const float dz = gn_dz(a, p, e, q[i].get(e), d[i].get(e), xh);
+                        const int k = p.sub(e);
+                        const float xv = q[i].get(e), xh = (xv - p.mean[k]) * p.rstd[k];
+                        const float dz = gn_dz<ACT>(xv, xh, d[i].get(e), p.w[e], p.b[e],
+                                                    stats + 2 * (ACT == PNGPD_ACT_RELU ? (c + min(e, n - 1)) / a.Cg : 0));
                         A[e] += dz; Bs[e] = fmaf(dz, xh, Bs[e]);
                     }
                 }
@@ -531,46 +542,52 @@ __global__ __launch_bounds__(256) void gn_bwd_part_kernel(const GnArgs a) {
     }
 }
 
-// one workgroup a (sample, group): the channels' A, B over the cuts, then the group's S1, S2.  A wave takes 16 channels x
-// 4 cuts at a time.
-template <int DT>
-__global__ __launch_bounds__(256) void gn_bwd_join_kernel(const GnArgs a) {
-    __shared__ double sh[4][2];
-    const int b = blockIdx.x / a.G, g = blockIdx.x - b * a.G, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const float *in = (const float *)a.part + 2 * ((size_t)b * a.S * a.C + (size_t)g * a.Cg);
-    double gu = 0.0, gv = 0.0;
-    for (int k0 = wave * 16; k0 < a.Cg; k0 += 64) {
-        const int k = k0 + (lane & 15);
-        double u = 0.0, v = 0.0;
-        if (k < a.Cg) {
-            for (int s = lane >> 4; s < a.S; s += 4) {
-                const float *o = in + 2 * ((size_t)s * a.C + k);
-                u += (double)o[0]; v += (double)o[1];
-            }
-        }
-        u += __shfl_xor(u, 16); v += __shfl_xor(v, 16);
-        u += __shfl_xor(u, 32); v += __shfl_xor(v, 32);
-        if (k < a.Cg && lane < 16) {
-            const int c = g * a.Cg + k;
-            if (a.ab) {
-                float *o = a.ab + 2 * ((size_t)b * a.C + c);
-                o[0] = (float)u; o[1] = (float)v;
-            }
-            const float w = !a.w ? 1.f : a.wf32 ? ((const float *)a.w)[c] : ld_elem<DT>((const typename elem<DT>::t *)a.w + c);
-            gu += u * w; gv += v * w;
+// the channels' A, B of a sample over its cuts: 32 channels x 32 cut lanes a workgroup
+__global__ __launch_bounds__(1024) void gn_bwd_join_kernel(const GnArgs a) {
+    __shared__ double sh[32][32][2];
+    const int cx = threadIdx.x & 31, sy = threadIdx.x >> 5, blocks = (a.C + 31) / 32;
+    const int b = blockIdx.x / blocks, c = (blockIdx.x - b * blocks) * 32 + cx;
+    const float *in = (const float *)a.part + 2 * ((size_t)b * a.S * a.C + c);
+    double u = 0.0, v = 0.0;
+    if (c < a.C) {
+#pragma unroll 4
+        for (int s = sy; s < a.S; s += 32) {
+            const f32x2 o = *(const f32x2 *)(in + 2 * (size_t)s * a.C);
+            u += (double)o[0]; v += (double)o[1];
         }
     }
-    gu = wave_sum(gu); gv = wave_sum(gv);
-    if (lane == 0) { sh[wave][0] = gu; sh[wave][1] = gv; }
+    sh[sy][cx][0] = u; sh[sy][cx][1] = v;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        const double m = (double)a.N * a.Cg;
-        a.gsum[2 * (size_t)blockIdx.x] = (float)(((sh[0][0] + sh[1][0]) + (sh[2][0] + sh[3][0])) / m);
-        a.gsum[2 * (size_t)blockIdx.x + 1] = (float)(((sh[0][1] + sh[1][1]) + (sh[2][1] + sh[3][1])) / m);
+    for (int k = 16; k >= 1; k >>= 1) {
+        if (sy < k) { sh[sy][cx][0] += sh[sy + k][cx][0]; sh[sy][cx][1] += sh[sy + k][cx][1]; }
+        __syncthreads();
+    }
+    if (sy == 0 && c < a.C) {
+        float *o = a.ab + 2 * ((size_t)b * a.C + c);
+        o[0] = (float)sh[0][cx][0]; o[1] = (float)sh[0][cx][1];
     }
 }
 
-template <int DT, int VEC, int SUB>
+// one wave a (sample, group): S1, S2 from its channels' A, B
+template <int DT>
+__global__ __launch_bounds__(64) void gn_bwd_group_kernel(const GnArgs a) {
+    const int b = blockIdx.x / a.G, g = blockIdx.x - b * a.G;
+    double u = 0.0, v = 0.0;
+    for (int k = threadIdx.x; k < a.Cg; k += 64) {
+        const int c = g * a.Cg + k;
+        const float *o = a.ab + 2 * ((size_t)b * a.C + c);
+        const float w = !a.w ? 1.f : a.wf32 ? ((const float *)a.w)[c] : ld_elem<DT>((const typename elem<DT>::t *)a.w + c);
+        u += (double)o[0] * w; v += (double)o[1] * w;
+    }
+    u = wave_sum(u); v = wave_sum(v);
+    if (threadIdx.x == 0) {
+        const double m = (double)a.N * a.Cg;
+        a.gsum[2 * (size_t)blockIdx.x] = (float)(u / m);
+        a.gsum[2 * (size_t)blockIdx.x + 1] = (float)(v / m);
+    }
+}
+
+template <int DT, int VEC, int SUB, int ACT>
 __global__ __launch_bounds__(256) void gn_bwd_apply_kernel(const GnArgs a) {
     typedef typename elem<DT>::t T;
     const int tid = threadIdx.x, X = 1 << a.lx, tx = tid & (X - 1), ty = tid >> a.lx, TY = 256 >> a.lx;
@@ -581,11 +598,12 @@ __global__ __launch_bounds__(256) void gn_bwd_apply_kernel(const GnArgs a) {
     const int r0 = sp * a.rows, r1 = min(a.N, r0 + a.rows);
     ColPar<VEC, SUB> p;
     load_wb<DT>(a, c, n, p);
-    load_stats(a, a.stats + 2 * (size_t)b * a.G, c, n, 0, p);
+    const double *stats = a.stats + 2 * (size_t)b * a.G;
+    load_stats(a, stats, c, n, 0, p);
     float S1[SUB], S2[SUB];
 #pragma unroll
     for (int e = 0; e < SUB; ++e) {
-        const float *o = a.gsum + 2 * ((size_t)b * a.G + (c + min(e, n - 1)) / a.Cg);
+        const float *o = a.gsum + 2 * ((size_t)b * a.G + (c + min(e * (VEC / SUB), n - 1)) / a.Cg);
         S1[e] = o[0]; S2[e] = o[1];
     }
     const T *x = (const T *)a.x + (long long)b * a.sB + c;
@@ -601,10 +619,11 @@ __global__ __launch_bounds__(256) void gn_bwd_apply_kernel(const GnArgs a) {
                 float o[VEC];
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) {
-                    const int s = SUB == 1 ? 0 : e;
-                    float xh;
-                    const float dz = gn_dz(a, p, e, q[i].get(e), d[i].get(e), xh);
-                    o[e] = (float)p.rstd[s] * (fmaf(dz, p.w[e], -S1[s]) - xh * S2[s]);
+                    const int k = p.sub(e);
+                    const float xv = q[i].get(e), xh = (xv - p.mean[k]) * p.rstd[k];
+                    const float dz = gn_dz<ACT>(xv, xh, d[i].get(e), p.w[e], p.b[e],
+                                                stats + 2 * (ACT == PNGPD_ACT_RELU ? (c + min(e, n - 1)) / a.Cg : 0));
+                    o[e] = p.rstd[k] * (fmaf(dz, p.w[e], -S1[k]) - xh * S2[k]);
                 }
                 Col<DT, VEC>::store(dx + (size_t)(row + i * TY) * a.C, o, n);
             }
@@ -647,9 +666,10 @@ static GnPlan gn_plan(int B, int N, int C, int G, int dt, int bwd) {
     GnPlan p;
     const int Cg = C / G, e = dt == PNGPD_F32 ? 4 : 2, wide = 16 / e;
     p.vec = C >= wide ? wide : 1;
-    p.sub = Cg % p.vec == 0 ? 1 : p.vec;
+    p.sub = Cg % p.vec == 0 ? 1 : 2 * Cg == p.vec ? 2 : p.vec;
     // slab: columns of a range = 128 bytes of a row (whole cache lines), or one group where that is more (up to 512
-    // bytes); halved, down to 32 bytes, while the rows do not fit or the card (256 CUs) is not filled
+    // bytes); halved, down to 32 bytes, while the rows do not fit or there are fewer than 512 workgroups (two a CU: one
+    // loads while the other computes).  Rows of a thread: 64 registers of x forward, x and dz (or dy) backward.
     p.slab = 0; p.gpr = p.ranges = p.threads = p.rpt = 0;
     const int most = bwd ? 8 : 16;
     for (int bytes = 128; bytes >= 32; bytes >>= 1) {
@@ -661,17 +681,17 @@ static GnPlan gn_plan(int B, int N, int C, int G, int dt, int bwd) {
         if (lx > 5) break;
         const int ranges = (G + gpr - 1) / gpr;
         const long long need = ((long long)N + most - 1) / most << lx;
-        if (need <= 1024) {
+        if (need <= SLAB_THREADS) {
             p.slab = 1; p.gpr = gpr; p.ranges = ranges; p.lx = lx;
-            if ((long long)B * ranges >= 256) break;
+            if ((long long)B * ranges >= 512) break;
         }
         if (gpr == 1) break;
     }
     if (p.slab) {
-        // as many threads as there are rows for, up to 1024; then the rows a thread holds
+        // as many threads as there are rows for, up to SLAB_THREADS; then the rows a thread holds
         long long t = (long long)N << p.lx;
         int th = 64;
-        while (th < t && th < 1024) th <<= 1;
+        while (th < t && th < SLAB_THREADS) th <<= 1;
         p.threads = th;
         int r = (int)(((long long)N + (th >> p.lx) - 1) / (th >> p.lx));
         p.rpt = r <= 2 ? 2 : r <= 4 ? 4 : r <= 8 ? 8 : 16;
@@ -682,9 +702,9 @@ static GnPlan gn_plan(int B, int N, int C, int G, int dt, int bwd) {
         p.lx = log2_up(cols);
         if (p.lx > 6) p.lx = 6;
         p.cols = (cols + (1 << p.lx) - 1) >> p.lx;
-        // cuts: 2048 workgroups (8 a CU), of at least 4 rows a thread
+        // cuts: 1024 workgroups (4 a CU), of at least 4 rows a thread
         const int TY = 256 >> p.lx;
-        long long S = 2048 / ((long long)B * p.cols);
+        long long S = 1024 / ((long long)B * p.cols);
         const long long top = ((long long)N + 4 * TY - 1) / (4 * TY);
         if (S > top) S = top;
         if (S < 1) S = 1;
@@ -696,7 +716,7 @@ static GnPlan gn_plan(int B, int N, int C, int G, int dt, int bwd) {
 
 static size_t gn_part_bytes(const GnPlan &p, int B, int C, int bwd) {
     if (p.slab) return 0;
-    return (size_t)B * p.S * (bwd ? (size_t)C * 8 : (size_t)(p.sub == 1 ? C / p.vec : C) * 16);
+    return (size_t)B * p.S * (bwd ? (size_t)C * 8 : (size_t)(C / (p.vec / p.sub)) * 16);
 }
 
 // workgroups of one launch past the grid's (and the kernels' int) range
@@ -710,46 +730,75 @@ static bool gn_bad(const void *x, int dt, int B, int N, int C, int G, int act, c
            act < PNGPD_ACT_NONE || act > PNGPD_ACT_GELU || !(eps >= 0.f) || (wdt != PNGPD_F32 && wdt != dt);
 }
 
-template <int DT, int VEC, int SUB>
+template <class K> static int gn_slab_launch(K kernel, const GnArgs &a, const GnPlan &p, size_t lds, hipStream_t st) {
+    const int rc = pngpd_allow_lds((const void *)kernel, lds);
+    if (rc) return rc;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(a.B * p.ranges)), dim3(p.threads), lds, st, a);
+    return PNGPD_OK;
+}
+
+template <int DT, int VEC, int SUB, int ACT>
 static int gn_fwd_launch(GnArgs &a, const GnPlan &p, hipStream_t st) {
     if (p.slab) {
         const size_t lds = (size_t)(p.threads / 64) * (1 << p.lx) * SUB * 16 + (size_t)p.gpr * 16;
-#define GN_SLAB(R) { const int rc = pngpd_allow_lds((const void *)gn_fwd_slab_kernel<DT, VEC, SUB, R>, lds); if (rc) return rc; \
-        hipLaunchKernelGGL((gn_fwd_slab_kernel<DT, VEC, SUB, R>), dim3((unsigned)(a.B * p.ranges)), dim3(p.threads), lds, st, a); }
-        if (p.rpt == 2) GN_SLAB(2) else if (p.rpt == 4) GN_SLAB(4) else if (p.rpt == 8) GN_SLAB(8) else GN_SLAB(16)
-#undef GN_SLAB
-        return pngpd_launch_status();
+        const int rc = p.rpt == 2 ? gn_slab_launch(gn_fwd_slab_kernel<DT, VEC, SUB, 2, ACT>, a, p, lds, st)
+                     : p.rpt == 4 ? gn_slab_launch(gn_fwd_slab_kernel<DT, VEC, SUB, 4, ACT>, a, p, lds, st)
+                     : p.rpt == 8 ? gn_slab_launch(gn_fwd_slab_kernel<DT, VEC, SUB, 8, ACT>, a, p, lds, st)
+                                  : gn_slab_launch(gn_fwd_slab_kernel<DT, VEC, SUB, 16, ACT>, a, p, lds, st);
+        return rc ? rc : pngpd_launch_status();
     }
     const dim3 grid((unsigned)(p.cols * p.S * a.B));
     hipLaunchKernelGGL((gn_fwd_part_kernel<DT, VEC, SUB>), grid, dim3(256), (size_t)4 * (1 << p.lx) * SUB * 16, st, a);
-    hipLaunchKernelGGL(gn_stats_kernel, dim3((unsigned)(a.B * a.G)), dim3(256), 0, st, a, SUB == 1 ? VEC : 1);
-    hipLaunchKernelGGL((gn_fwd_apply_kernel<DT, VEC, SUB>), grid, dim3(256), 0, st, a);
+    hipLaunchKernelGGL(gn_stats_kernel, dim3((unsigned)(a.B * a.G)), dim3(256), 0, st, a, VEC / SUB);
+    hipLaunchKernelGGL((gn_fwd_apply_kernel<DT, VEC, SUB, ACT>), grid, dim3(256), 0, st, a);
     return pngpd_launch_status();
 }
 
-template <int DT, int VEC, int SUB>
+template <int DT, int VEC, int SUB, int ACT>
 static int gn_bwd_launch(GnArgs &a, const GnPlan &p, void *dw, void *db, hipStream_t st) {
     if (p.slab) {
         const size_t chans = (size_t)(1 << p.lx) * VEC;
         const size_t lds = (size_t)(p.threads / 64) * chans * 8 + chans * 16 + (size_t)p.gpr * 16;
-#define GN_SLAB(R) { const int rc = pngpd_allow_lds((const void *)gn_bwd_slab_kernel<DT, VEC, SUB, R>, lds); if (rc) return rc; \
-        hipLaunchKernelGGL((gn_bwd_slab_kernel<DT, VEC, SUB, R>), dim3((unsigned)(a.B * p.ranges)), dim3(p.threads), lds, st, a); }
-        if (p.rpt == 2) GN_SLAB(2) else if (p.rpt == 4) GN_SLAB(4) else GN_SLAB(8)
-#undef GN_SLAB
+        const int rc = p.rpt == 2 ? gn_slab_launch(gn_bwd_slab_kernel<DT, VEC, SUB, 2, ACT>, a, p, lds, st)
+                     : p.rpt == 4 ? gn_slab_launch(gn_bwd_slab_kernel<DT, VEC, SUB, 4, ACT>, a, p, lds, st)
+                                  : gn_slab_launch(gn_bwd_slab_kernel<DT, VEC, SUB, 8, ACT>, a, p, lds, st);
+        if (rc) return rc;
     } else {
         const dim3 grid((unsigned)(p.cols * p.S * a.B));
-        hipLaunchKernelGGL((gn_bwd_part_kernel<DT, VEC, SUB>), grid, dim3(256), (size_t)4 * (1 << p.lx) * VEC * 8, st, a);
-        hipLaunchKernelGGL(gn_bwd_join_kernel<DT>, dim3((unsigned)(a.B * a.G)), dim3(256), 0, st, a);
-        if (a.dx) hipLaunchKernelGGL((gn_bwd_apply_kernel<DT, VEC, SUB>), grid, dim3(256), 0, st, a);
+        hipLaunchKernelGGL((gn_bwd_part_kernel<DT, VEC, SUB, ACT>), grid, dim3(256), (size_t)4 * (1 << p.lx) * VEC * 8, st, a);
+        hipLaunchKernelGGL(gn_bwd_join_kernel, dim3((unsigned)(a.B * ((a.C + 31) / 32))), dim3(1024), 0, st, a);
+        if (a.dx) {
+            hipLaunchKernelGGL(gn_bwd_group_kernel<DT>, dim3((unsigned)(a.B * a.G)), dim3(64), 0, st, a);
+            hipLaunchKernelGGL((gn_bwd_apply_kernel<DT, VEC, SUB, ACT>), grid, dim3(256), 0, st, a);
+        }
     }
-    if (a.ab) hipLaunchKernelGGL(gn_dwdb_kernel<DT>, dim3((unsigned)((a.C + 15) / 16)), dim3(1024), 0, st, a, dw, db);
+    if (dw || db) hipLaunchKernelGGL(gn_dwdb_kernel<DT>, dim3((unsigned)((a.C + 15) / 16)), dim3(1024), 0, st, a, dw, db);
     return pngpd_launch_status();
 }
 
-#define GN_DISPATCH(call) \
-    if (dtype == PNGPD_F32) return p.vec == 1 ? call(PNGPD_F32, 1, 1) : p.sub == 1 ? call(PNGPD_F32, 4, 1) : call(PNGPD_F32, 4, 4); \
-    if (dtype == PNGPD_BF16) return p.vec == 1 ? call(PNGPD_BF16, 1, 1) : p.sub == 1 ? call(PNGPD_BF16, 8, 1) : call(PNGPD_BF16, 8, 8); \
-    return p.vec == 1 ? call(PNGPD_F16, 1, 1) : p.sub == 1 ? call(PNGPD_F16, 8, 1) : call(PNGPD_F16, 8, 8);
+template <int DT, int VEC, int SUB>
+static int gn_launch(GnArgs &a, const GnPlan &p, bool bwd, void *dw, void *db, hipStream_t st) {
+#define GN_ACT(A) case A: return bwd ? gn_bwd_launch<DT, VEC, SUB, A>(a, p, dw, db, st) : gn_fwd_launch<DT, VEC, SUB, A>(a, p, st)
+    switch (a.act) {
+        GN_ACT(PNGPD_ACT_NONE);
+        GN_ACT(PNGPD_ACT_RELU);
+        GN_ACT(PNGPD_ACT_SILU);
+        GN_ACT(PNGPD_ACT_GELU);
+    }
+#undef GN_ACT
+    return PNGPD_ERR_INVALID_ARG;
+}
+template <int DT, int VEC>
+static int gn_launch_vec(GnArgs &a, const GnPlan &p, bool bwd, void *dw, void *db, hipStream_t st) {
+    if (p.vec == 1) return gn_launch<DT, 1, 1>(a, p, bwd, dw, db, st);
+    return p.sub == 1 ? gn_launch<DT, VEC, 1>(a, p, bwd, dw, db, st) : p.sub == 2 ? gn_launch<DT, VEC, 2>(a, p, bwd, dw, db, st)
+                                                                              : gn_launch<DT, VEC, VEC>(a, p, bwd, dw, db, st);
+}
+static int gn_launch_type(GnArgs &a, int dtype, const GnPlan &p, bool bwd, void *dw, void *db, hipStream_t st) {
+    return dtype == PNGPD_F32 ? gn_launch_vec<PNGPD_F32, 4>(a, p, bwd, dw, db, st)
+         : dtype == PNGPD_BF16 ? gn_launch_vec<PNGPD_BF16, 8>(a, p, bwd, dw, db, st)
+                               : gn_launch_vec<PNGPD_F16, 8>(a, p, bwd, dw, db, st);
+}
 
 extern "C" {
 
@@ -772,10 +821,7 @@ int pngpd_group_norm_fwd(const void *x, int dtype, int B, int N, int C, long lon
     a.x = x; a.w = w; a.b = b; a.y = y; a.stats = stats; a.part = (double *)workspace;
     a.sB = stride_b; a.sN = stride_n; a.B = B; a.N = N; a.C = C; a.G = G; a.Cg = C / G; a.act = act;
     a.wf32 = wdtype == PNGPD_F32; a.eps = eps; a.lx = p.lx; a.gpr = p.gpr; a.ranges = p.ranges; a.cols = p.cols; a.S = p.S; a.rows = p.rows;
-    hipStream_t st = (hipStream_t)stream;
-#define GN_CALL(D, V, U) gn_fwd_launch<D, V, U>(a, p, st)
-    GN_DISPATCH(GN_CALL)
-#undef GN_CALL
+    return gn_launch_type(a, dtype, p, false, nullptr, nullptr, (hipStream_t)stream);
 }
 
 int pngpd_group_norm_bwd(const void *x, int dtype, int B, int N, int C, long long stride_b, long long stride_n, int G,
@@ -791,14 +837,11 @@ int pngpd_group_norm_bwd(const void *x, int dtype, int B, int N, int C, long lon
     char *ws = (char *)workspace;
     const size_t part = (gn_part_bytes(p, B, C, 1) + 255) & ~(size_t)255;
     a.x = x; a.dy = dy; a.w = w; a.b = b; a.dx = dx; a.stats = (double *)stats; a.part = (double *)ws;
-    a.ab = dw || db ? (float *)(ws + part) : nullptr;
+    a.ab = dw || db || !p.slab ? (float *)(ws + part) : nullptr;
     a.gsum = (float *)(ws + part + (((size_t)B * C * 8 + 255) & ~(size_t)255));
     a.sB = stride_b; a.sN = stride_n; a.B = B; a.N = N; a.C = C; a.G = G; a.Cg = C / G; a.act = act;
     a.wf32 = wdtype == PNGPD_F32; a.eps = eps; a.lx = p.lx; a.gpr = p.gpr; a.ranges = p.ranges; a.cols = p.cols; a.S = p.S; a.rows = p.rows;
-    hipStream_t st = (hipStream_t)stream;
-#define GN_CALL(D, V, U) gn_bwd_launch<D, V, U>(a, p, dw, db, st)
-    GN_DISPATCH(GN_CALL)
-#undef GN_CALL
+    return gn_launch_type(a, dtype, p, true, dw, db, (hipStream_t)stream);
 }
 
 }  // extern "C"
