@@ -89,8 +89,7 @@ __device__ __forceinline__ uint4 lce_pair(uint2 x, uint2 y) {
     return make_uint4(a[0], b[0], a[1], b[1]);
 }
 template <int DT> __device__ __forceinline__ uint2 lce_half4(float a, float b, float c, float d) {
-    return make_uint2((unsigned)f_to_half(DT, a) | ((unsigned)f_to_half(DT, b) << 16),
-                      (unsigned)f_to_half(DT, c) | ((unsigned)f_to_half(DT, d) << 16));
+    return make_uint2(pk_half<DT>(a, b), pk_half<DT>(c, d));
 }
 
 // 2^((z - m) log2 e) is one FMA, z log2 e - (m log2 e), where the rounding of the product in brackets is small: an error of

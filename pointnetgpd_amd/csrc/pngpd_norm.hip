@@ -22,6 +22,10 @@
 
 #define SLAB_THREADS 512                // of a slab's workgroup: two share a CU, one loads while the other computes
 
+#ifndef GN_FWD_T
+#define GN_FWD_T 512
+#define GN_BWD_T 512
+#endif
 struct GnArgs {
     const void *x, *dy, *w, *b;
     void *y, *dx;
@@ -61,13 +65,38 @@ template <int DT, int VEC> struct Col {
             }
         }
     }
+    // adds the values (and their squares) of each SUB-th part to s, s2.  16 bits: the squares are exact in float32, and so
+    // are sums of a part's four or eight but for a rounding; from there on fp64 (1.5 instructions a value, not 4).
+    template <int SUB> __device__ __forceinline__ void sums(double (&s)[SUB], double (&s2)[SUB]) const {
+        if constexpr (DT != PNGPD_F32 && VEC > 1 && SUB <= 2) {
+            constexpr int W = WORDS / SUB;
+            const unsigned one = DT == PNGPD_BF16 ? 0x3f803f80u : 0x3c003c00u;
+#pragma unroll
+            for (int k = 0; k < SUB; ++k) {
+                float u = 0.f, v = 0.f;
+#pragma unroll
+                for (int i = 0; i < W; ++i) {
+                    u = dot_half<DT>(q[k * W + i], one, u);
+                    v = dot_half<DT>(q[k * W + i], q[k * W + i], v);
+                }
+                s[k] += (double)u; s2[k] += (double)v;
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const double v = (double)get(e);
+                const int k = e * SUB / VEC;
+                s[k] += v; s2[k] = fma(v, v, s2[k]);
+            }
+        }
+    }
     static __device__ __forceinline__ void store(typename elem<DT>::t *p, const float (&v)[VEC], int n) {
         if (VEC > 1 && n == VEC) {
             unsigned o[WORDS];
 #pragma unroll
             for (int i = 0; i < WORDS; ++i) {
                 if constexpr (DT == PNGPD_F32) o[i] = __float_as_uint(v[i]);
-                else o[i] = (unsigned)f_to_half(DT, v[(2 * i) % VEC]) | ((unsigned)f_to_half(DT, v[(2 * i + 1) % VEC]) << 16);
+                else o[i] = pk_half<DT>(v[(2 * i) % VEC], v[(2 * i + 1) % VEC]);
             }
             __builtin_memcpy(p, o, 16);
             return;
@@ -121,9 +150,11 @@ template <int ACT> __device__ __forceinline__ float act_value(float z) {
 
 // What a thread keeps of its column: w, b and, for each of the SUB groups it touches, the statistics.  SUB = 1: the column
 // lies inside one group (Cg a multiple of VEC); 2: it is two whole groups; VEC: every element may belong to another one.
+// xh = x r + mr and z = x w' + b' (fold()) are one FMA each; r, mr, w', b' come from fp64 and are rounded once, an error of
+// 2^-24 (|x| + |mean|) rstd like that of subtracting a rounded mean.
 template <int VEC, int SUB> struct ColPar {
     float w[VEC], b[VEC];
-    float mean[SUB], rstd[SUB];
+    float r[SUB], mr[SUB];                 // rstd, -mean rstd
     static __device__ __forceinline__ int sub(int e) { return e * SUB / VEC; }
 };
 template <int DT, int VEC, int SUB>
@@ -137,26 +168,32 @@ __device__ __forceinline__ void load_wb(const GnArgs &a, int c, int n, ColPar<VE
         }
     }
 }
-// statistics of the column's groups out of st (mean, rstd pairs), whose first entry is group g0
-template <int VEC, int SUB>
+// statistics of the column's groups out of st (mean, rstd pairs), whose first entry is group g0; fold: w, b become w', b'
+template <bool FOLD, int VEC, int SUB>
 __device__ __forceinline__ void load_stats(const GnArgs &a, const double *st, int c, int n, int g0, ColPar<VEC, SUB> &p) {
 #pragma unroll
-    for (int e = 0; e < SUB; ++e) {
-        p.mean[e] = 0.f; p.rstd[e] = 0.f;
-        const int at = e * (VEC / SUB);
+    for (int k = 0; k < SUB; ++k) {
+        const int at = k * (VEC / SUB);
+        double mean = 0.0, rstd = 0.0;
         if (at < n) {
             const int g = (c + at) / a.Cg - g0;
-            p.mean[e] = (float)st[2 * g]; p.rstd[e] = (float)st[2 * g + 1];
+            mean = st[2 * g]; rstd = st[2 * g + 1];
+        }
+        p.r[k] = (float)rstd; p.mr[k] = (float)(-mean * rstd);
+        if constexpr (FOLD) {
+#pragma unroll
+            for (int e = at; e < at + VEC / SUB; ++e) {
+                const double w = rstd * (double)p.w[e];
+                p.b[e] = (float)((double)p.b[e] - mean * w);
+                p.w[e] = (float)w;
+            }
         }
     }
 }
 template <int ACT, int VEC, int SUB>
 __device__ __forceinline__ void gn_apply(const ColPar<VEC, SUB> &p, const float (&x)[VEC], float (&y)[VEC]) {
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-        const int s = p.sub(e);
-        y[e] = act_value<ACT>(fmaf((x[e] - p.mean[s]) * p.rstd[s], p.w[e], p.b[e]));
-    }
+    for (int e = 0; e < VEC; ++e) y[e] = act_value<ACT>(fmaf(x[e], p.w[e], p.b[e]));
 }
 // dz of one element; st: the fp64 statistics (mean, rstd) of its group, for relu's slope
 template <int ACT>
@@ -168,6 +205,47 @@ __device__ __forceinline__ float gn_dz(float x, float xh, float dy, float w, flo
         if constexpr (ACT == PNGPD_ACT_SILU) { const float s = sigmoid(z); return dy * (s * fmaf(z, 1.f - s, 1.f)); }
         else { float e; const float s = phi_cdf(z, e); return dy * fmaf(z * 0.39894228040143268f, e, s); }
     }
+}
+// dx = rstd (w dz - S1 - xh S2) = dz w r + x k1 + k0
+template <int VEC, int SUB> struct DxPar {
+    float wr[VEC], k0[SUB], k1[SUB];
+    // S: (S1, S2) of the column's groups in turn
+    __device__ __forceinline__ void set(const ColPar<VEC, SUB> &p, int k, double S1, double S2) {
+        const double r = (double)p.r[k], mr = (double)p.mr[k];
+        k1[k] = (float)(-r * r * S2);
+        k0[k] = (float)(-r * (S1 + mr * S2));
+#pragma unroll
+        for (int e = k * (VEC / SUB); e < (k + 1) * (VEC / SUB); ++e) wr[e] = p.w[e] * p.r[k];
+    }
+    __device__ __forceinline__ float dx(int e, float x, float dz) const {
+        const int k = ColPar<VEC, SUB>::sub(e);
+        return fmaf(dz, wr[e], fmaf(x, k1[k], k0[k]));
+    }
+};
+
+// Sums of NV values of each column (tx) over the workgroup's rows: res[v X + tx], in LDS (NV (threads + 64) values of
+// scratch before res).  Every thread writes its values, conflict-free, and a group of lanes adds a column's up: NV reads and
+// a few exchanges a thread, where sums over lanes alone exchange every value log2 times.  Fixed order.
+template <class T, int NV> __device__ __forceinline__ T *cols_sum(T *sh, const T (&v)[NV], int lx) {
+    const int tid = threadIdx.x, threads = blockDim.x, X = 1 << lx, TY = threads >> lx, pitch = TY + (64 >> lx);
+    const int tx = tid & (X - 1), ty = tid >> lx;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) sh[(i * X + tx) * pitch + ty] = v[i];
+    __syncthreads();
+    const int outs = NV * X;
+    T *res = sh + NV * (threads + 64);
+    int L = threads / outs;                               // lanes of an output (a power of two)
+    if (L > 64) L = 64;
+    if (L < 1) L = 1;
+    for (int o = tid / L; o < outs; o += threads / L) {
+        const T *c = sh + o * pitch;
+        T u = 0;
+        for (int k = tid & (L - 1); k < TY; k += L) u += c[k];
+        for (int k = 1; k < L; k <<= 1) u += __shfl_xor(u, k);
+        if ((tid & (L - 1)) == 0) res[o] = u;
+    }
+    __syncthreads();
+    return res;
 }
 
 // sum over the lanes of a wave that hold the same column (lane ^ (1 << lx), ... )
@@ -204,40 +282,24 @@ __global__ __launch_bounds__(SLAB_THREADS) void gn_fwd_slab_kernel(const GnArgs 
     load_rows<RPT>(q, x, a.sN, ty, TY, a.N, n);
     ColPar<VEC, SUB> p;
     load_wb<DT>(a, c, n, p);
-    double s[SUB], s2[SUB];
+    double s[SUB], s2[SUB], all[2 * SUB];
 #pragma unroll
     for (int e = 0; e < SUB; ++e) { s[e] = 0.0; s2[e] = 0.0; }
 #pragma unroll
     for (int i = 0; i < RPT; ++i) {
-        if (ty + i * TY < a.N) {
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                const double v = (double)q[i].get(e);
-                const int k = p.sub(e);
-                s[k] += v; s2[k] = fma(v, v, s2[k]);
-            }
-        }
+        if (ty + i * TY < a.N) q[i].sums(s, s2);
     }
-    // per wave: (X * SUB) units of (sum, sum of squares)
-    const int units = X * SUB;
 #pragma unroll
-    for (int e = 0; e < SUB; ++e) {
-        const double u = lanes_sum(s[e], a.lx), v = lanes_sum(s2[e], a.lx);
-        if (lane < X) {
-            double *o = sh + 2 * ((size_t)wave * units + tx * SUB + e);
-            o[0] = u; o[1] = v;
-        }
-    }
-    double *st = sh + 2 * (size_t)waves * units;
-    __syncthreads();
-    const int upg = a.Cg * SUB / VEC;                     // units of a group
+    for (int e = 0; e < SUB; ++e) { all[2 * e] = s[e]; all[2 * e + 1] = s2[e]; }
+    const double *res = cols_sum(sh, all, a.lx);          // [2 * part + {sum, squares}][column]
+    double *st = sh + 2 * SUB * (blockDim.x + 64) + 2 * SUB * X;
+    const int upg = a.Cg * SUB / VEC;                     // parts of a group
     const double m = (double)a.N * a.Cg;
     for (int g = wave; g < gn; g += waves) {
         double u = 0.0, v = 0.0;
-        for (int k = lane; k < waves * upg; k += 64) {
-            const int w = k / upg, j = k - w * upg;
-            const double *o = sh + 2 * ((size_t)w * units + g * upg + j);
-            u += o[0]; v += o[1];
+        for (int k = lane; k < upg; k += 64) {
+            const int j = g * upg + k, col = j / SUB, part = j - col * SUB;
+            u += res[2 * part * X + col]; v += res[(2 * part + 1) * X + col];
         }
         u = wave_sum(u); v = wave_sum(v);
         if (lane == 0) {
@@ -251,7 +313,7 @@ __global__ __launch_bounds__(SLAB_THREADS) void gn_fwd_slab_kernel(const GnArgs 
         }
     }
     __syncthreads();
-    load_stats(a, st, c, n, g0, p);
+    load_stats<true>(a, st, c, n, g0, p);
     T *y = (T *)a.y + (size_t)b * a.N * a.C + c;
 #pragma unroll
     for (int i = 0; i < RPT; ++i) {
@@ -285,7 +347,7 @@ __global__ __launch_bounds__(SLAB_THREADS) void gn_bwd_slab_kernel(const GnArgs 
     load_rows<RPT>(d, dy, a.C, ty, TY, a.N, n);
     ColPar<VEC, SUB> p;
     load_wb<DT>(a, c, n, p);
-    load_stats(a, stats, c, n, g0, p);
+    load_stats<false>(a, stats, c, n, g0, p);
     float A[VEC], Bs[VEC], keep[KEEP ? RPT : 1][VEC];
 #pragma unroll
     for (int e = 0; e < VEC; ++e) { A[e] = 0.f; Bs[e] = 0.f; }
@@ -295,7 +357,7 @@ __global__ __launch_bounds__(SLAB_THREADS) void gn_bwd_slab_kernel(const GnArgs 
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
                 const int k = p.sub(e);
-                const float xv = q[i].get(e), xh = (xv - p.mean[k]) * p.rstd[k];
+                const float xv = q[i].get(e), xh = fmaf(xv, p.r[k], p.mr[k]);
                 const double *st = stats + 2 * (ACT == PNGPD_ACT_RELU ? (c + min(e, max(n, 1) - 1)) / a.Cg - g0 : 0);
                 const float dz = gn_dz<ACT>(xv, xh, d[i].get(e), p.w[e], p.b[e], st);
                 if constexpr (KEEP) keep[i][e] = dz;
@@ -303,31 +365,22 @@ __global__ __launch_bounds__(SLAB_THREADS) void gn_bwd_slab_kernel(const GnArgs 
             }
         }
     }
-    const int chans = X * VEC;
-    float *shf = (float *)sh;                            // [wave][chans][2]
+    float all[2 * VEC];
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-        const float u = lanes_sum(A[e], a.lx), v = lanes_sum(Bs[e], a.lx);
-        if (lane < X) {
-            float *o = shf + 2 * ((size_t)wave * chans + tx * VEC + e);
-            o[0] = u; o[1] = v;
-        }
-    }
-    double *ch = sh + (size_t)waves * chans;             // [chans][2]: w A, w B
-    double *st = ch + 2 * (size_t)chans;                 // [gn][2]: S1, S2
-    __syncthreads();
+    for (int e = 0; e < VEC; ++e) { all[2 * e] = A[e]; all[2 * e + 1] = Bs[e]; }
+    const float *res = cols_sum((float *)sh, all, a.lx);  // [2 * e + {A, B}][column]
+    const int chans = X * VEC;
+    double *ch = sh + (VEC * (blockDim.x + 64) + chans);  // [chans][2]: w A, w B   (behind 2 VEC (threads + 64 + X) floats)
+    double *st = ch + 2 * (size_t)chans;                  // [gn][2]: S1, S2
     for (int k = tid; k < c1 - c0; k += blockDim.x) {
-        double u = 0.0, v = 0.0;
-        for (int w = 0; w < waves; ++w) {
-            const float *o = shf + 2 * ((size_t)w * chans + k);
-            u += (double)o[0]; v += (double)o[1];
-        }
+        const int col = k / VEC, e = k - col * VEC;
+        const float u = res[2 * e * X + col], v = res[(2 * e + 1) * X + col];
         if (a.ab) {
             float *o = a.ab + 2 * ((size_t)b * a.C + c0 + k);
-            o[0] = (float)u; o[1] = (float)v;
+            o[0] = u; o[1] = v;
         }
         const float w = !a.w ? 1.f : a.wf32 ? ((const float *)a.w)[c0 + k] : ld_elem<DT>((const T *)a.w + c0 + k);
-        ch[2 * k] = u * w; ch[2 * k + 1] = v * w;
+        ch[2 * k] = (double)u * w; ch[2 * k + 1] = (double)v * w;
     }
     __syncthreads();
     const double m = (double)a.N * a.Cg;
@@ -339,11 +392,11 @@ __global__ __launch_bounds__(SLAB_THREADS) void gn_bwd_slab_kernel(const GnArgs 
     }
     __syncthreads();
     if (n == 0 || !a.dx) return;
-    float S1[SUB], S2[SUB];
+    DxPar<VEC, SUB> dp;
 #pragma unroll
-    for (int e = 0; e < SUB; ++e) {
-        const int g = (c + min(e * (VEC / SUB), n - 1)) / a.Cg - g0;
-        S1[e] = (float)st[2 * g]; S2[e] = (float)st[2 * g + 1];
+    for (int k = 0; k < SUB; ++k) {
+        const int g = (c + min(k * (VEC / SUB), n - 1)) / a.Cg - g0;
+        dp.set(p, k, st[2 * g], st[2 * g + 1]);
     }
     T *dx = (T *)a.dx + (size_t)b * a.N * a.C + c;
 #pragma unroll
@@ -353,13 +406,12 @@ __global__ __launch_bounds__(SLAB_THREADS) void gn_bwd_slab_kernel(const GnArgs 
             float o[VEC];
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
-                const int k = p.sub(e);
-                const float xv = q[i].get(e), xh = (xv - p.mean[k]) * p.rstd[k];
+                const float xv = q[i].get(e);
                 float dz;
                 if constexpr (KEEP) dz = keep[i][e];
-                else dz = gn_dz<ACT>(xv, xh, d[i].get(e), p.w[e], p.b[e],
+                else dz = gn_dz<ACT>(xv, 0.f, d[i].get(e), p.w[e], p.b[e],
                                      stats + 2 * (ACT == PNGPD_ACT_RELU ? (c + min(e, n - 1)) / a.Cg - g0 : 0));
-                o[e] = p.rstd[k] * (fmaf(dz, p.w[e], -S1[k]) - xh * S2[k]);
+                o[e] = dp.dx(e, xv, dz);
             }
             Col<DT, VEC>::store(dx + (size_t)row * a.C, o, n);
         }
@@ -393,14 +445,7 @@ __global__ __launch_bounds__(256) void gn_fwd_part_kernel(const GnArgs a) {
         load_rows<4>(q, x, a.sN, row, TY, r1, n, row);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            if (row + i * TY < r1) {
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    const double v = (double)q[i].get(e);
-                    const int k = e * SUB / VEC;
-                    s[k] += v; s2[k] = fma(v, v, s2[k]);
-                }
-            }
+            if (row + i * TY < r1) q[i].sums(s, s2);
         }
     }
     // X <= 64: the rows of a wave by shuffles, the four waves through LDS
@@ -462,7 +507,7 @@ __global__ __launch_bounds__(256) void gn_fwd_apply_kernel(const GnArgs a) {
     ColPar<VEC, SUB> p;
     load_wb<DT>(a, c, n, p);
     const double *stats = a.stats + 2 * (size_t)b * a.G;
-    load_stats(a, stats, c, n, 0, p);
+    load_stats<true>(a, stats, c, n, 0, p);
     const T *x = (const T *)a.x + (long long)b * a.sB + c;
     T *y = (T *)a.y + (size_t)b * a.N * a.C + c;
     for (int row = r0 + ty; row < r1; row += 4 * TY) {
@@ -495,7 +540,7 @@ __global__ __launch_bounds__(256) void gn_bwd_part_kernel(const GnArgs a) {
     ColPar<VEC, SUB> p;
     load_wb<DT>(a, c, n, p);
     const double *stats = a.stats + 2 * (size_t)b * a.G;
-    load_stats(a, stats, c, n, 0, p);
+    load_stats<false>(a, stats, c, n, 0, p);
     const T *x = (const T *)a.x + (long long)b * a.sB + c;
     const T *dy = (const T *)a.dy + (size_t)b * a.N * a.C + c;
     float A[VEC], Bs[VEC];
@@ -512,7 +557,7 @@ __global__ __launch_bounds__(256) void gn_bwd_part_kernel(const GnArgs a) {
 #pragma unroll
                     for (int e = 0; e < VEC; ++e) {
                         const int k = p.sub(e);
-                        const float xv = q[i].get(e), xh = (xv - p.mean[k]) * p.rstd[k];
+                        const float xv = q[i].get(e), xh = fmaf(xv, p.r[k], p.mr[k]);
                         const float dz = gn_dz<ACT>(xv, xh, d[i].get(e), p.w[e], p.b[e],
                                                     stats + 2 * (ACT == PNGPD_ACT_RELU ? (c + min(e, n - 1)) / a.Cg : 0));
                         A[e] += dz; Bs[e] = fmaf(dz, xh, Bs[e]);
@@ -599,12 +644,12 @@ __global__ __launch_bounds__(256) void gn_bwd_apply_kernel(const GnArgs a) {
     ColPar<VEC, SUB> p;
     load_wb<DT>(a, c, n, p);
     const double *stats = a.stats + 2 * (size_t)b * a.G;
-    load_stats(a, stats, c, n, 0, p);
-    float S1[SUB], S2[SUB];
+    load_stats<false>(a, stats, c, n, 0, p);
+    DxPar<VEC, SUB> dp;
 #pragma unroll
-    for (int e = 0; e < SUB; ++e) {
-        const float *o = a.gsum + 2 * ((size_t)b * a.G + (c + min(e * (VEC / SUB), n - 1)) / a.Cg);
-        S1[e] = o[0]; S2[e] = o[1];
+    for (int k = 0; k < SUB; ++k) {
+        const float *o = a.gsum + 2 * ((size_t)b * a.G + (c + min(k * (VEC / SUB), n - 1)) / a.Cg);
+        dp.set(p, k, (double)o[0], (double)o[1]);
     }
     const T *x = (const T *)a.x + (long long)b * a.sB + c;
     const T *dy = (const T *)a.dy + (size_t)b * a.N * a.C + c;
@@ -620,10 +665,10 @@ __global__ __launch_bounds__(256) void gn_bwd_apply_kernel(const GnArgs a) {
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) {
                     const int k = p.sub(e);
-                    const float xv = q[i].get(e), xh = (xv - p.mean[k]) * p.rstd[k];
+                    const float xv = q[i].get(e), xh = fmaf(xv, p.r[k], p.mr[k]);
                     const float dz = gn_dz<ACT>(xv, xh, d[i].get(e), p.w[e], p.b[e],
                                                 stats + 2 * (ACT == PNGPD_ACT_RELU ? (c + min(e, n - 1)) / a.Cg : 0));
-                    o[e] = p.rstd[k] * (fmaf(dz, p.w[e], -S1[k]) - xh * S2[k]);
+                    o[e] = dp.dx(e, xv, dz);
                 }
                 Col<DT, VEC>::store(dx + (size_t)(row + i * TY) * a.C, o, n);
             }
@@ -671,27 +716,29 @@ static GnPlan gn_plan(int B, int N, int C, int G, int dt, int bwd) {
     // bytes); halved, down to 32 bytes, while the rows do not fit or there are fewer than 512 workgroups (two a CU: one
     // loads while the other computes).  Rows of a thread: 64 registers of x forward, x and dz (or dy) backward.
     p.slab = 0; p.gpr = p.ranges = p.threads = p.rpt = 0;
-    const int most = bwd ? 8 : 16;
-    for (int bytes = 128; bytes >= 32; bytes >>= 1) {
-        int gpr = bytes / e / Cg;
-        if (gpr < 1) gpr = 1;
-        if (gpr > G) gpr = G;
-        const int cols = (gpr * Cg + p.vec - 1) / p.vec;
-        const int lx = log2_up(cols);
-        if (lx > 5) break;
-        const int ranges = (G + gpr - 1) / gpr;
-        const long long need = ((long long)N + most - 1) / most << lx;
-        if (need <= SLAB_THREADS) {
-            p.slab = 1; p.gpr = gpr; p.ranges = ranges; p.lx = lx;
-            if ((long long)B * ranges >= 512) break;
+    const int most_threads = bwd ? GN_BWD_T : GN_FWD_T;
+    for (int most = 8; most <= (bwd ? 8 : 16) && !p.slab; most *= 2) {
+        for (int bytes = 128; bytes >= 32; bytes >>= 1) {
+            int gpr = bytes / e / Cg;
+            if (gpr < 1) gpr = 1;
+            if (gpr > G) gpr = G;
+            const int cols = (gpr * Cg + p.vec - 1) / p.vec;
+            const int lx = log2_up(cols);
+            if (lx > 5) break;
+            const int ranges = (G + gpr - 1) / gpr;
+            const long long need = ((long long)N + most - 1) / most << lx;
+            if (need <= most_threads) {
+                p.slab = 1; p.gpr = gpr; p.ranges = ranges; p.lx = lx;
+                if ((long long)B * ranges >= 512) break;
+            }
+            if (gpr == 1) break;
         }
-        if (gpr == 1) break;
     }
     if (p.slab) {
         // as many threads as there are rows for, up to SLAB_THREADS; then the rows a thread holds
         long long t = (long long)N << p.lx;
         int th = 64;
-        while (th < t && th < SLAB_THREADS) th <<= 1;
+        while (th < t && th < most_threads) th <<= 1;
         p.threads = th;
         int r = (int)(((long long)N + (th >> p.lx) - 1) / (th >> p.lx));
         p.rpt = r <= 2 ? 2 : r <= 4 ? 4 : r <= 8 ? 8 : 16;
@@ -740,7 +787,7 @@ template <class K> static int gn_slab_launch(K kernel, const GnArgs &a, const Gn
 template <int DT, int VEC, int SUB, int ACT>
 static int gn_fwd_launch(GnArgs &a, const GnPlan &p, hipStream_t st) {
     if (p.slab) {
-        const size_t lds = (size_t)(p.threads / 64) * (1 << p.lx) * SUB * 16 + (size_t)p.gpr * 16;
+        const size_t lds = (size_t)2 * SUB * (p.threads + 64 + (1 << p.lx)) * 8 + (size_t)p.gpr * 16;
         const int rc = p.rpt == 2 ? gn_slab_launch(gn_fwd_slab_kernel<DT, VEC, SUB, 2, ACT>, a, p, lds, st)
                      : p.rpt == 4 ? gn_slab_launch(gn_fwd_slab_kernel<DT, VEC, SUB, 4, ACT>, a, p, lds, st)
                      : p.rpt == 8 ? gn_slab_launch(gn_fwd_slab_kernel<DT, VEC, SUB, 8, ACT>, a, p, lds, st)
@@ -758,7 +805,7 @@ template <int DT, int VEC, int SUB, int ACT>
 static int gn_bwd_launch(GnArgs &a, const GnPlan &p, void *dw, void *db, hipStream_t st) {
     if (p.slab) {
         const size_t chans = (size_t)(1 << p.lx) * VEC;
-        const size_t lds = (size_t)(p.threads / 64) * chans * 8 + chans * 16 + (size_t)p.gpr * 16;
+        const size_t lds = (size_t)2 * VEC * (p.threads + 64) * 4 + chans * 8 + chans * 16 + (size_t)p.gpr * 16;
         const int rc = p.rpt == 2 ? gn_slab_launch(gn_bwd_slab_kernel<DT, VEC, SUB, 2, ACT>, a, p, lds, st)
                      : p.rpt == 4 ? gn_slab_launch(gn_bwd_slab_kernel<DT, VEC, SUB, 4, ACT>, a, p, lds, st)
                                   : gn_slab_launch(gn_bwd_slab_kernel<DT, VEC, SUB, 8, ACT>, a, p, lds, st);
