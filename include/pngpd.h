@@ -475,7 +475,7 @@ int pngpd_adam_step_inc(float *step_dev, void *stream);
 /* Global norm of n gradients and their clipping in place: *total_norm = the 2-norm (norm_kind 2), the 1-norm (1) or the
  * largest magnitude (0) over every element of every tensor; then g *= min(1, max_norm / (*total_norm + 1e-6)).
  * g, numel, dtype: HOST arrays (dtype NULL: all float32); tensors dense, each aligned to its element, none overlapping
- * another; an empty one may be NULL.  Sums in fp64, in a fixed order.  A NaN or infinite gradient gives a norm of NaN or
+ * another (PNGPD_ERR_UNSUPPORTED); an empty one may be NULL.  Sums in fp64, in a fixed order.  A NaN or infinite gradient gives a norm of NaN or
  * infinity and reaches the gradients through the factor.  max_norm infinite: the norm alone.  Two launches a 128 tensors. */
 size_t pngpd_grad_clip_workspace_bytes(int n);
 int pngpd_grad_clip(void *const *g, const long long *numel, const int *dtype, int n, int norm_kind, float max_norm,
@@ -524,7 +524,7 @@ int pngpd_lce_bwd(const pngpd_lce_t *a, void *stream);
  *   w, b (C) of wdtype (= dtype or PNGPD_F32), each NULL: 1 / 0;  dw, db likewise, each NULL: not wanted; dx NULL: same
  *   stats (B,G,2) fp64 = mean, 1/sqrt(var + eps): written by the forward call, read by the backward one
  * The backward call takes the forward's x, w, b, act.  Deterministic; no row or channel count is special.           */
-size_t pngpd_group_norm_workspace_bytes(int B, int N, int C, int G, int dtype, int backward);
+size_t pngpd_group_norm_workspace_bytes(int B, int N, int C, int G, int dtype, int act, int backward);
 int pngpd_group_norm_fwd(const void *x, int dtype, int B, int N, int C, long long stride_b, long long stride_n, int G,
                          const void *w, const void *b, int wdtype, float eps, int act, void *y, double *stats,
                          void *workspace, size_t workspace_bytes, void *stream);

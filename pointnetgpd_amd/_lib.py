@@ -170,7 +170,7 @@ SIGNATURES = {
                                                            ctypes.c_double, ctypes.c_float, ctypes.c_float, c_void,
                                                            ctypes.c_float, c_void, ctypes.c_float, c_void, c_void,
                                                            ctypes.c_size_t, c_void]),
-    "pngpd_group_norm_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int] * 6),
+    "pngpd_group_norm_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int] * 7),
     "pngpd_group_norm_fwd": (ctypes.c_int, [c_void] + [ctypes.c_int] * 4 + [ctypes.c_longlong] * 2 +
                              [ctypes.c_int, c_void, c_void, ctypes.c_int, ctypes.c_float, ctypes.c_int, c_void, c_void,
                               c_void, ctypes.c_size_t, c_void]),
@@ -294,6 +294,12 @@ def device_guard(device):
     hipSetDevice round trips per kernel launch, which is most of a launch's host time at B = 1."""
     import torch
     return _NULL if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def raw_stream(device):
+    """The current stream of ``device`` as an integer; torch.cuda.current_stream builds a Stream object first (2 us)."""
+    import torch
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def check(code, what):

@@ -12,6 +12,9 @@
 // fp64 partial sums: the squares of float32 / bfloat16 gradients leave float32's range at 1.8e19 and below 1e-23; the
 // conversion and the fp64 FMA (half the fp32 rate) stay under the time of the loads.
 // Measured on the clip / Adam cases of the design table.
+#include <algorithm>
+#include <vector>
+
 #include "pngpd_common.h"
 #include "pngpd_types.h"
 
@@ -257,16 +260,22 @@ static int clip_norm(void *const *g, const long long *numel, const int *dtype, i
     return rc;
 }
 
-// total chunks, or -1 when an argument is wrong (a tensor of more than 2^31 chunks of one table included)
+// total chunks; -1 when an argument is wrong (more than 2^31 chunks included), -2 when two tensors share memory
 static long long clip_check(void *const *g, const long long *numel, const int *dtype, int n) {
     if (n < 0 || (n > 0 && (!g || !numel))) return -1;
     long long chunks = 0;
+    std::vector<std::pair<uintptr_t, uintptr_t>> spans;
+    try { spans.reserve(n); } catch (...) { return -1; }
     for (int i = 0; i < n; ++i) {
         const int dt = dtype ? dtype[i] : PNGPD_F32;
         if (numel[i] < 0 || (numel[i] && !g[i]) || dt < PNGPD_F32 || dt > PNGPD_F16) return -1;
         if ((uintptr_t)g[i] & (dt == PNGPD_F32 ? 3 : 1)) return -1;
         chunks += clip_chunks(numel[i]);
+        if (numel[i]) spans.emplace_back((uintptr_t)g[i], (uintptr_t)g[i] + (uintptr_t)numel[i] * (dt == PNGPD_F32 ? 4 : 2));
     }
+    std::sort(spans.begin(), spans.end());
+    for (size_t i = 1; i < spans.size(); ++i)
+        if (spans[i - 1].second > spans[i].first) return -2;
     return chunks < (1ll << 31) ? chunks : -1;
 }
 
@@ -279,6 +288,7 @@ size_t pngpd_grad_clip_workspace_bytes(int n) {
 int pngpd_grad_clip(void *const *g, const long long *numel, const int *dtype, int n, int norm_kind, float max_norm,
                     float *total_norm, void *workspace, size_t workspace_bytes, void *stream) {
     const long long chunks = clip_check(g, numel, dtype, n);
+    if (chunks == -2) return PNGPD_ERR_UNSUPPORTED;
     if (chunks < 0 || !total_norm || norm_kind < KIND_INF || norm_kind > KIND_L2 || !(max_norm >= 0.f))
         return PNGPD_ERR_INVALID_ARG;
     if (!workspace || ((uintptr_t)workspace & 7) || workspace_bytes < pngpd_grad_clip_workspace_bytes(n)) return PNGPD_ERR_WORKSPACE;

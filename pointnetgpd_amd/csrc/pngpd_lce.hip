@@ -270,64 +270,24 @@ __global__ __launch_bounds__(WGM * WGN * 64, 2) void lce_stats_kernel(const LceA
 }
 
 // One row a group of 32 lanes: joins its tiles, in fp64; stat (T,2) = max, sum of the kept rows; row (T) = every row's loss.
-__global__ __launch_bounds__(256) void lce_join_kernel(const LceArgs a, float *__restrict__ stat, float *__restrict__ row) {
-    __shared__ double sh[32][8][2];
-    __shared__ float shm[32][8];
-    const int tx = threadIdx.x & 7, ty = threadIdx.x >> 3, t = blockIdx.x * 8 + tx;
-    const int place = t < a.T ? a.rows.place(t) : -1;
-    float m = -INFINITY;
-    double s = 0.0, sz = 0.0;
-    if (place >= 0) {
-        for (int k = ty; k < a.mt; k += 32) {
-            const size_t at = (size_t)k * a.T + place;
-            const f32x2 p = *(const f32x2 *)(a.pm + 2 * at);
-            const float M = fmaxf(m, p[0]), ref = M == -INFINITY ? 0.f : M;
-            s = s * (double)expf(m - ref) + (double)p[1] * (double)expf(p[0] - ref);
-            m = M;
-            if (a.smooth != 0.f) sz += (double)a.ps[at];
-        }
-    }
-    shm[ty][tx] = m; sh[ty][tx][0] = s; sh[ty][tx][1] = sz;
-    __syncthreads();
-    if (ty || t >= a.T) return;
-    if (place < 0) { row[t] = 0.f; return; }
-    float M = m;
-    for (int k = 1; k < 32; ++k) M = fmaxf(M, shm[k][tx]);
-    const float ref = M == -INFINITY ? 0.f : M;
-    s = sz = 0.0;
-    for (int k = 0; k < 32; ++k) { s += sh[k][tx][0] * (double)expf(shm[k][tx] - ref); sz += sh[k][tx][1]; }
-    stat[2 * (size_t)place] = M; stat[2 * (size_t)place + 1] = (float)s;
-    const long long y = a.target[t];
-    double l = 0.0;
-    if (y != a.ignore) {
-        if (y < 0 || y >= a.V) l = NAN;                            // a class that does not exist: as loud as a value can be
-        else {
-            // differences from the maximum first: beside a maximum of 1e30 the logarithm would be lost
-            l = log(s) + (1.0 - (double)a.smooth) * ((double)M - (double)a.zt[place]);
-            if (a.smooth != 0.f) l += (double)a.smooth * ((double)M - sz / a.V);
-        }
-    }
-    row[t] = (float)l;
-}
-
+// A grid of one workgroup (few rows) walks over all of them and goes on to the loss.
+#define LCE_FEW 64
 __device__ __forceinline__ double lce_block_sum(double v, double *sh) {
     for (int k = 32; k >= 1; k >>= 1) v += __shfl_xor(v, k);
     __syncthreads();
     if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
     __syncthreads();
     double s = 0.0;
-    for (int k = 0; k < 16; ++k) s += sh[k];
+    for (int k = 0; k < (int)(blockDim.x >> 6); ++k) s += sh[k];
     return s;
 }
 
 // kept rows; loss = their sum or mean (a mean over none is NaN)
-__global__ __launch_bounds__(1024) void lce_loss_kernel(const float *__restrict__ row, const long long *__restrict__ target,
-                                                        long long ignore, int T, int reduction, float *__restrict__ loss,
-                                                        float *__restrict__ kept) {
+__device__ __forceinline__ void lce_loss(const float *row, const LceArgs &a, int reduction, float *loss, float *kept) {
     __shared__ double sh[16];
     double s = 0.0, n = 0.0;
-    for (int t = threadIdx.x; t < T; t += 1024) {
-        if (target[t] != ignore) n += 1.0;
+    for (int t = threadIdx.x; t < a.T; t += blockDim.x) {
+        if (a.target[t] != a.ignore) n += 1.0;
         s += (double)row[t];
     }
     s = lce_block_sum(s, sh);
@@ -338,40 +298,102 @@ __global__ __launch_bounds__(1024) void lce_loss_kernel(const float *__restrict_
         if (reduction == PNGPD_REDUCE_SUM) *loss = (float)s;
     }
 }
+__global__ __launch_bounds__(1024) void lce_loss_kernel(const LceArgs a, const float *row, int reduction, float *loss, float *kept) {
+    lce_loss(row, a, reduction, loss, kept);
+}
 
-// coef (T) = c_t over the largest finite |c_t| (times up, the factor of the type's range), scale = what gives c_t back
-__global__ __launch_bounds__(1024) void lce_coef_kernel(const float *__restrict__ dloss, const float *__restrict__ kept,
-                                                        const long long *__restrict__ target, long long ignore, LceRows rows,
-                                                        int V, int reduction, float up, float *__restrict__ coef,
-                                                        float *__restrict__ scale) {
-    const int T = rows.T;
-    __shared__ float sh[16];
+// ROWS rows a workgroup and turn
+template <int ROWS>
+__global__ __launch_bounds__(ROWS * 32) void lce_join_kernel(const LceArgs a, float *stat, float *row, int reduction, float *loss,
+                                                             float *kept) {
+    __shared__ double sh[32][ROWS][2];
+    __shared__ float shm[32][ROWS];
+    const int tx = threadIdx.x % ROWS, ty = threadIdx.x / ROWS;
+    for (int t0 = blockIdx.x * ROWS; t0 < a.T; t0 += gridDim.x * ROWS) {
+        const int t = t0 + tx, place = t < a.T ? a.rows.place(t) : -1;
+        float m = -INFINITY;
+        double s = 0.0, sz = 0.0;
+        if (place >= 0) {
+#pragma unroll 4
+            for (int k = ty; k < a.mt; k += 32) {
+                const size_t at = (size_t)k * a.T + place;
+                const f32x2 p = *(const f32x2 *)(a.pm + 2 * at);
+                const float M = fmaxf(m, p[0]), ref = M == -INFINITY ? 0.f : M;
+                s = s * (double)expf(m - ref) + (double)p[1] * (double)expf(p[0] - ref);
+                m = M;
+                if (a.smooth != 0.f) sz += (double)a.ps[at];
+            }
+        }
+        __syncthreads();
+        shm[ty][tx] = m; sh[ty][tx][0] = s; sh[ty][tx][1] = sz;
+        __syncthreads();
+        if (ty || t >= a.T) continue;
+        if (place < 0) { row[t] = 0.f; continue; }
+        float M = m;
+        for (int k = 1; k < 32; ++k) M = fmaxf(M, shm[k][tx]);
+        const float ref = M == -INFINITY ? 0.f : M;
+        s = sz = 0.0;
+        for (int k = 0; k < 32; ++k) { s += sh[k][tx][0] * (double)expf(shm[k][tx] - ref); sz += sh[k][tx][1]; }
+        stat[2 * (size_t)place] = M; stat[2 * (size_t)place + 1] = (float)s;
+        const long long y = a.target[t];
+        double l = 0.0;
+        if (y != a.ignore) {
+            if (y < 0 || y >= a.V) l = NAN;                        // a class that does not exist: as loud as a value can be
+            else {
+                // differences from the maximum first: beside a maximum of 1e30 the logarithm would be lost
+                l = log(s) + (1.0 - (double)a.smooth) * ((double)M - (double)a.zt[place]);
+                if (a.smooth != 0.f) l += (double)a.smooth * ((double)M - sz / a.V);
+            }
+        }
+        row[t] = (float)l;
+    }
+    if (gridDim.x == 1) {
+        __threadfence_block();
+        __syncthreads();
+        lce_loss(row, a, reduction, loss, kept);
+    }
+}
+
+struct LceCoef {
+    const float *dloss, *kept;
+    const long long *target;
+    long long ignore;
+    LceRows rows;
+    int V, reduction;
+    float up;
+    float *coef, *scale;
+};
+// coef (T) = c_t over the largest finite |c_t| (times up, the factor of the type's range), scale = what gives c_t back.  One
+// workgroup of 256.
+__device__ __forceinline__ void lce_coef(const LceCoef &a) {
+    __shared__ float sh[4];
+    const int T = a.rows.T;
     float top = 1.f;
-    if (reduction == PNGPD_REDUCE_NONE) {
+    if (a.reduction == PNGPD_REDUCE_NONE) {
         top = 0.f;
-        for (int t = threadIdx.x; t < T; t += 1024) {
-            const float c = fabsf(dloss[t]);
-            if (c < INFINITY && target[t] != ignore) top = fmaxf(top, c);
+        for (int t = threadIdx.x; t < T; t += 256) {
+            const float c = fabsf(a.dloss[t]);
+            if (c < INFINITY && a.target[t] != a.ignore) top = fmaxf(top, c);
         }
         for (int k = 32; k >= 1; k >>= 1) top = fmaxf(top, __shfl_xor(top, k));
         if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = top;
         __syncthreads();
-        for (int k = 0; k < 16; ++k) top = fmaxf(top, sh[k]);
+        top = fmaxf(fmaxf(sh[0], sh[1]), fmaxf(sh[2], sh[3]));
         if (top == 0.f) top = 1.f;
     }
-    for (int t = threadIdx.x; t < T; t += 1024) {
-        const long long y = target[t];
-        float c = reduction == PNGPD_REDUCE_NONE ? dloss[t] / top * up : up;
-        if (y == ignore) c = 0.f;
-        else if (y < 0 || y >= V) c = NAN;
-        const int k = rows.place(t);
-        if (k >= 0) coef[k] = c;
+    for (int t = threadIdx.x; t < T; t += 256) {
+        const long long y = a.target[t];
+        float c = a.reduction == PNGPD_REDUCE_NONE ? a.dloss[t] / top * a.up : a.up;
+        if (y == a.ignore) c = 0.f;
+        else if (y < 0 || y >= a.V) c = NAN;
+        const int k = a.rows.place(t);
+        if (k >= 0) a.coef[k] = c;
     }
     if (threadIdx.x == 0) {
-        float s = top / up;
-        if (reduction == PNGPD_REDUCE_SUM) s = *dloss / up;
-        if (reduction == PNGPD_REDUCE_MEAN) s = *kept > 0.f ? *dloss / *kept / up : 0.f;     // no row, no gradient
-        *scale = s;
+        float s = top / a.up;
+        if (a.reduction == PNGPD_REDUCE_SUM) s = *a.dloss / a.up;
+        if (a.reduction == PNGPD_REDUCE_MEAN) s = *a.kept > 0.f ? *a.dloss / *a.kept / a.up : 0.f;    // no row, no gradient
+        *a.scale = s;
     }
 }
 
@@ -483,7 +505,8 @@ __global__ __launch_bounds__(WGM * WGN * 64, 2) void lce_grad_kernel(const LceAr
 // workgroup's share; the shares' sums (S, ldg) in float32, then one thread a class.
 template <int DT>
 __global__ __launch_bounds__(256) void lce_db_kernel(const void *__restrict__ gp, LceRows rows, int ldg, int share, int cols,
-                                                     float *__restrict__ out) {
+                                                     float *__restrict__ out, const float *__restrict__ scale,
+                                                     void *__restrict__ db, int vc, int f32) {
     constexpr int EPC = DT == PNGPD_F32 ? 4 : 8, X = 8;           // 8 chunks by 32 rows
     __shared__ float sh[32][X * EPC + 1];
     const int T = rows.count(), cx = threadIdx.x % X, ry = threadIdx.x / X, v = (blockIdx.x * X + cx) * EPC;
@@ -511,7 +534,13 @@ __global__ __launch_bounds__(256) void lce_db_kernel(const void *__restrict__ gp
         float u = 0.f;
         for (int k = 0; k < 32; ++k) u += sh[k][threadIdx.x];
         const int col = blockIdx.x * X * EPC + threadIdx.x;
-        if (col < cols) out[(size_t)blockIdx.y * ldg + col] = u;
+        if (gridDim.y > 1) {
+            if (col < cols) out[(size_t)blockIdx.y * ldg + col] = u;
+        } else if (col < vc) {                                     // one share: done
+            u *= *scale;
+            if (f32) ((float *)db)[col] = u;
+            else st_elem<DT>((typename elem<DT>::t *)db + col, u);
+        }
     }
 }
 template <int DT>
@@ -617,8 +646,10 @@ __global__ __launch_bounds__(256) void lce_dx_kernel(const float *__restrict__ p
     const long long t = q / per;
     const int d = (int)(q - t * per) * 4, k = rows.place((int)t);
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    if (k >= 0)
+    if (k >= 0) {
+#pragma unroll 8
         for (int s = 0; s < splits; ++s) v += *(const f32x4 *)(part + ((size_t)s * rows.T + k) * Dp + d);
+    }
     const float sc = *scale;
     E *o = (E *)dx + t * D + d;
 #pragma unroll
@@ -627,15 +658,16 @@ __global__ __launch_bounds__(256) void lce_dx_kernel(const float *__restrict__ p
 
 // dst (R,Dp) = src (R,D) with zeros behind; with `mask` the kept rows only, in their places (all of them, in order: a row
 // of zeros where the target is ignored — what such a row holds is nobody's, a NaN there must not meet g's zeros in a
-// product).  One 16-byte chunk of dst a thread.
+// product).  One 16-byte chunk of dst a thread.  coef.coef: the first workgroup makes the coefficients in its place.
 template <int DT>
 __global__ __launch_bounds__(256) void lce_copy_kernel(const void *__restrict__ src, long long ld, int D, int Dp, long long R,
                                                        int mask, LceRows rows, const long long *__restrict__ target,
-                                                       long long ignore, void *__restrict__ dst) {
+                                                       long long ignore, void *__restrict__ dst, const LceCoef coef) {
     typedef typename elem<DT>::t E;
     constexpr int EPC = 16 / (int)sizeof(E);
-    const int per = Dp / EPC;
-    const long long q = (long long)blockIdx.x * 256 + threadIdx.x;
+    const int per = Dp / EPC, first = coef.coef ? 1 : 0;
+    if (first && blockIdx.x == 0) { lce_coef(coef); return; }
+    const long long q = (long long)(blockIdx.x - first) * 256 + threadIdx.x;
     if (q >= R * per) return;
     const long long k = q / per;
     const int d = (int)(q - k * per) * EPC;
@@ -791,11 +823,12 @@ template <int DT, bool BMC> static int lce_out(LceOut &a, int shape, hipStream_t
 }
 
 template <int DT>
-static void lce_copy(const Lce *a, const void *src, long long ld, long long R, int mask, LceRows rows, void *dst, hipStream_t st) {
+static void lce_copy(const Lce *a, const void *src, long long ld, long long R, int mask, LceRows rows, void *dst, hipStream_t st,
+                     const LceCoef &coef = LceCoef{}) {
     const int Dp = lce_dp(a);
     const long long n = R * (Dp * lce_esize(DT) / 16);
-    hipLaunchKernelGGL(lce_copy_kernel<DT>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, src, ld, a->D, Dp, R, mask, rows,
-                       (const long long *)a->target, (long long)a->ignore_index, dst);
+    hipLaunchKernelGGL(lce_copy_kernel<DT>, dim3((unsigned)((n + 255) / 256 + (coef.coef != nullptr))), dim3(256), 0, st, src, ld, a->D, Dp, R,
+                       mask, rows, (const long long *)a->target, (long long)a->ignore_index, dst, coef);
 }
 
 static LceArgs lce_args(const Lce *a) {
@@ -823,9 +856,13 @@ template <int DT> static int lce_forward(const Lce *a, const LcePlan &p, hipStre
     }
     k.mt = p.fmt;
     float *row = a->reduction == PNGPD_REDUCE_NONE ? a->loss : (float *)(ws + p.o_row);
-    hipLaunchKernelGGL(lce_join_kernel, dim3((unsigned)((a->T + 7) / 8)), dim3(256), 0, st, k, a->stat, row);
+    if (a->T <= LCE_FEW) {
+        hipLaunchKernelGGL(lce_join_kernel<32>, dim3(1), dim3(1024), 0, st, k, a->stat, row, a->reduction, a->loss, a->kept);
+        return pngpd_launch_status();
+    }
+    hipLaunchKernelGGL(lce_join_kernel<8>, dim3((unsigned)((a->T + 7) / 8)), dim3(256), 0, st, k, a->stat, row, a->reduction, a->loss, a->kept);
     if (a->reduction != PNGPD_REDUCE_NONE)
-        hipLaunchKernelGGL(lce_loss_kernel, dim3(1), dim3(1024), 0, st, row, k.target, k.ignore, a->T, a->reduction, a->loss, a->kept);
+        hipLaunchKernelGGL(lce_loss_kernel, dim3(1), dim3(1024), 0, st, k, row, a->reduction, a->loss, a->kept);
     return pngpd_launch_status();
 }
 
@@ -833,14 +870,13 @@ template <int DT> static int lce_backward(const Lce *a, const LcePlan &p, hipStr
     typedef typename elem<DT>::t E;
     char *ws = (char *)a->workspace;
     LceArgs k = lce_args(a);
-    lce_copy<DT>(a, a->x, a->ldx, a->T, 1, k.rows, ws + p.o_x, st);
+    float *coef = (float *)(ws + p.o_coef), *scale = (float *)(ws + p.o_scale), *part = (float *)(ws + p.o_dx);
+    lce_copy<DT>(a, a->x, a->ldx, a->T, 1, k.rows, ws + p.o_x, st,
+                 LceCoef{a->dloss, a->kept, k.target, k.ignore, k.rows, a->V, a->reduction, DT == PNGPD_F16 ? 32768.f : 1.f, coef, scale});
     k.x = LceOperand{ws + p.o_x, p.Dp};
     k.packed = 1;
     if (p.padw) { lce_copy<DT>(a, a->w, a->ldw, a->V, 0, k.rows, ws + p.o_w, st); k.w = LceOperand{ws + p.o_w, p.Dp}; }
     k.D = p.Dp;
-    float *coef = (float *)(ws + p.o_coef), *scale = (float *)(ws + p.o_scale), *part = (float *)(ws + p.o_dx);
-    hipLaunchKernelGGL(lce_coef_kernel, dim3(1), dim3(1024), 0, st, a->dloss, a->kept, k.target, k.ignore, k.rows, a->V, a->reduction,
-                       DT == PNGPD_F16 ? 32768.f : 1.f, coef, scale);
     k.stat = a->stat; k.coef = coef; k.ldg = p.ldg;
     for (int v0 = 0; v0 < a->V; v0 += p.piece) {
         const int vc = a->V - v0 < p.piece ? a->V - v0 : p.piece;
@@ -859,8 +895,8 @@ template <int DT> static int lce_backward(const Lce *a, const LcePlan &p, hipStr
             float *sums = (float *)(ws + p.o_db);
             void *db = a->bias_dtype == PNGPD_F32 ? (void *)((float *)a->db + v0) : (void *)((E *)a->db + v0);
             hipLaunchKernelGGL(lce_db_kernel<DT>, dim3((unsigned)lce_cdiv(cols, DT == PNGPD_F32 ? 32 : 64), p.shares), dim3(256), 0, st,
-                               g, k.rows, p.ldg, p.share, cols, sums);
-            hipLaunchKernelGGL(lce_db_join_kernel<DT>, dim3((unsigned)lce_cdiv(vc, 256)), dim3(256), 0, st, sums, p.shares, p.ldg,
+                               g, k.rows, p.ldg, p.share, cols, sums, scale, db, vc, a->bias_dtype == PNGPD_F32);
+            if (p.shares > 1) hipLaunchKernelGGL(lce_db_join_kernel<DT>, dim3((unsigned)lce_cdiv(vc, 256)), dim3(256), 0, st, sums, p.shares, p.ldg,
                                vc, scale, db, a->bias_dtype == PNGPD_F32);
         }
         if (a->dx) {

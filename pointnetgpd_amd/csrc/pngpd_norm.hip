@@ -22,10 +22,6 @@
 
 #define SLAB_THREADS 512                // of a slab's workgroup: two share a CU, one loads while the other computes
 
-#ifndef GN_FWD_T
-#define GN_FWD_T 512
-#define GN_BWD_T 512
-#endif
 struct GnArgs {
     const void *x, *dy, *w, *b;
     void *y, *dx;
@@ -676,29 +672,27 @@ __global__ __launch_bounds__(256) void gn_bwd_apply_kernel(const GnArgs a) {
     }
 }
 
-// db_c, dw_c = the samples' A_c, B_c summed in fp64: 16 channels x 64 sample lanes a workgroup
+// db_c, dw_c = the samples' A_c, B_c summed in fp64: 4 channels x 64 sample lanes a workgroup
 template <int DT>
-__global__ __launch_bounds__(1024) void gn_dwdb_kernel(const GnArgs a, void *dw, void *db) {
-    __shared__ double sh[64][16][2];
-    const int cx = threadIdx.x & 15, ry = threadIdx.x >> 4, c = blockIdx.x * 16 + cx;
+__global__ __launch_bounds__(256) void gn_dwdb_kernel(const GnArgs a, void *dw, void *db) {
+    __shared__ double sh[64][4][2];
+    const int cx = threadIdx.x & 3, ry = threadIdx.x >> 2, c = blockIdx.x * 4 + cx;
     double u = 0.0, v = 0.0;
     if (c < a.C) {
+#pragma unroll 4
         for (int b = ry; b < a.B; b += 64) {
-            const float *o = a.ab + 2 * ((size_t)b * a.C + c);
+            const f32x2 o = *(const f32x2 *)(a.ab + 2 * ((size_t)b * a.C + c));
             u += (double)o[0]; v += (double)o[1];
         }
     }
     sh[ry][cx][0] = u; sh[ry][cx][1] = v;
     __syncthreads();
-    for (int k = 32; k >= 1; k >>= 1) {
-        if (ry < k) { sh[ry][cx][0] += sh[ry + k][cx][0]; sh[ry][cx][1] += sh[ry + k][cx][1]; }
-        __syncthreads();
-    }
-    if (ry == 0 && c < a.C) {
-        const float A = (float)sh[0][cx][0], B = (float)sh[0][cx][1];
-        if (db) { if (a.wf32) ((float *)db)[c] = A; else st_elem<DT>((typename elem<DT>::t *)db + c, A); }
-        if (dw) { if (a.wf32) ((float *)dw)[c] = B; else st_elem<DT>((typename elem<DT>::t *)dw + c, B); }
-    }
+    if (threadIdx.x >= 8) return;
+    double s = 0.0;
+    const int j = threadIdx.x >> 2;                       // 0: db of channel cx, 1: dw
+    for (int k = 0; k < 64; ++k) s += sh[k][cx][j];
+    void *to = j ? dw : db;
+    if (to && c < a.C) { if (a.wf32) ((float *)to)[c] = (float)s; else st_elem<DT>((typename elem<DT>::t *)to + c, (float)s); }
 }
 
 // ---------------------------------------------------------------------------------------------- plan
@@ -707,7 +701,7 @@ struct GnPlan { int vec, sub, slab, lx, gpr, ranges, threads, rpt, cols, S, rows
 
 static inline int log2_up(int n) { int k = 0; while ((1 << k) < n) ++k; return k; }
 
-static GnPlan gn_plan(int B, int N, int C, int G, int dt, int bwd) {
+static GnPlan gn_plan(int B, int N, int C, int G, int dt, int act, int bwd) {
     GnPlan p;
     const int Cg = C / G, e = dt == PNGPD_F32 ? 4 : 2, wide = 16 / e;
     p.vec = C >= wide ? wide : 1;
@@ -716,7 +710,10 @@ static GnPlan gn_plan(int B, int N, int C, int G, int dt, int bwd) {
     // bytes); halved, down to 32 bytes, while the rows do not fit or there are fewer than 512 workgroups (two a CU: one
     // loads while the other computes).  Rows of a thread: 64 registers of x forward, x and dz (or dy) backward.
     p.slab = 0; p.gpr = p.ranges = p.threads = p.rpt = 0;
-    const int most_threads = bwd ? GN_BWD_T : GN_FWD_T;
+    // 160 registers a thread where dz is kept for eight 16-bit channels: one workgroup of 512 a CU, three of 256 (bf16, 1024
+    // samples of 1024 x 128: 322 and 292 us); otherwise 512 threads, on wider pieces of a row (float32, 64 x 750 x 128:
+    // 19.7 and 23.7 us)
+    const int most_threads = bwd && dt != PNGPD_F32 && act >= PNGPD_ACT_SILU ? SLAB_THREADS / 2 : SLAB_THREADS;
     for (int most = 8; most <= (bwd ? 8 : 16) && !p.slab; most *= 2) {
         for (int bytes = 128; bytes >= 32; bytes >>= 1) {
             int gpr = bytes / e / Cg;
@@ -819,7 +816,7 @@ static int gn_bwd_launch(GnArgs &a, const GnPlan &p, void *dw, void *db, hipStre
             hipLaunchKernelGGL((gn_bwd_apply_kernel<DT, VEC, SUB, ACT>), grid, dim3(256), 0, st, a);
         }
     }
-    if (dw || db) hipLaunchKernelGGL(gn_dwdb_kernel<DT>, dim3((unsigned)((a.C + 15) / 16)), dim3(1024), 0, st, a, dw, db);
+    if (dw || db) hipLaunchKernelGGL(gn_dwdb_kernel<DT>, dim3((unsigned)((a.C + 3) / 4)), dim3(256), 0, st, a, dw, db);
     return pngpd_launch_status();
 }
 
@@ -849,9 +846,9 @@ static int gn_launch_type(GnArgs &a, int dtype, const GnPlan &p, bool bwd, void 
 
 extern "C" {
 
-size_t pngpd_group_norm_workspace_bytes(int B, int N, int C, int G, int dtype, int backward) {
+size_t pngpd_group_norm_workspace_bytes(int B, int N, int C, int G, int dtype, int act, int backward) {
     if (B <= 0 || N <= 0 || C <= 0 || G <= 0 || C % G || dtype < PNGPD_F32 || dtype > PNGPD_F16) return 0;
-    const GnPlan p = gn_plan(B, N, C, G, dtype, backward != 0);
+    const GnPlan p = gn_plan(B, N, C, G, dtype, act, backward != 0);
     size_t n = (gn_part_bytes(p, B, C, backward != 0) + 255) & ~(size_t)255;
     if (backward) n += (((size_t)B * C * 8 + 255) & ~(size_t)255) + (p.slab ? 0 : (size_t)B * G * 8);
     return n;
@@ -861,9 +858,9 @@ int pngpd_group_norm_fwd(const void *x, int dtype, int B, int N, int C, long lon
                          const void *w, const void *b, int wdtype, float eps, int act, void *y, double *stats,
                          void *workspace, size_t workspace_bytes, void *stream) {
     if (gn_bad(x, dtype, B, N, C, G, act, w, wdtype, eps) || !y || !stats) return PNGPD_ERR_INVALID_ARG;
-    const GnPlan p = gn_plan(B, N, C, G, dtype, 0);
+    const GnPlan p = gn_plan(B, N, C, G, dtype, act, 0);
     if (gn_too_many(p, B, G)) return PNGPD_ERR_UNSUPPORTED;
-    if (workspace_bytes < pngpd_group_norm_workspace_bytes(B, N, C, G, dtype, 0) || (!p.slab && !workspace)) return PNGPD_ERR_WORKSPACE;
+    if (workspace_bytes < pngpd_group_norm_workspace_bytes(B, N, C, G, dtype, act, 0) || (!p.slab && !workspace)) return PNGPD_ERR_WORKSPACE;
     GnArgs a = {};
     a.x = x; a.w = w; a.b = b; a.y = y; a.stats = stats; a.part = (double *)workspace;
     a.sB = stride_b; a.sN = stride_n; a.B = B; a.N = N; a.C = C; a.G = G; a.Cg = C / G; a.act = act;
@@ -877,9 +874,9 @@ int pngpd_group_norm_bwd(const void *x, int dtype, int B, int N, int C, long lon
                          void *stream) {
     if (gn_bad(x, dtype, B, N, C, G, act, w, wdtype, eps) || !stats || !dy) return PNGPD_ERR_INVALID_ARG;
     if (!dx && !dw && !db) return PNGPD_OK;
-    const GnPlan p = gn_plan(B, N, C, G, dtype, 1);
+    const GnPlan p = gn_plan(B, N, C, G, dtype, act, 1);
     if (gn_too_many(p, B, G)) return PNGPD_ERR_UNSUPPORTED;
-    if (workspace_bytes < pngpd_group_norm_workspace_bytes(B, N, C, G, dtype, 1) || !workspace) return PNGPD_ERR_WORKSPACE;
+    if (workspace_bytes < pngpd_group_norm_workspace_bytes(B, N, C, G, dtype, act, 1) || !workspace) return PNGPD_ERR_WORKSPACE;
     GnArgs a = {};
     char *ws = (char *)workspace;
     const size_t part = (gn_part_bytes(p, B, C, 1) + 255) & ~(size_t)255;

@@ -125,8 +125,6 @@ _GRAD_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # PNG
 
 def _dense(t):
     """Whether t's elements fill one range of memory, each once (a permutation of a contiguous tensor)."""
-    if t.is_contiguous():
-        return True
     want = 1
     for stride, size in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n > 1):
         if stride != want:
@@ -155,38 +153,47 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
         raise ValueError(f"clip_grad_norm_: max_norm must not be negative, got {max_norm}")
     if norm_type not in _NORM_KINDS:
         raise ValueError(f"clip_grad_norm_: norm_type must be 2, 1 or inf, got {norm_type}")
-    grads = [p.grad for p in params if p.grad is not None]
+    grads = [g for g in [p.grad for p in params] if g is not None]
     if not grads:
         return torch.tensor(0.0)
-    dev = grads[0].device
-    if any(g.device != dev for g in grads):
-        raise RuntimeError("clip_grad_norm_: the gradients are on more than one device")
-    if dev.type != "cuda":
+    index = grads[0].get_device()
+    if index < 0:
+        if any(g.get_device() >= 0 for g in grads):
+            raise RuntimeError("clip_grad_norm_: the gradients are on more than one device")
         return torch.nn.utils.clip_grad_norm_(params, max_norm, norm_type, error_if_nonfinite)
+    work, ptr, num, typ = [], [], [], []
     for g in grads:
-        if g.layout != torch.strided or g.dtype not in _GRAD_TYPES:
+        if g.get_device() != index:
+            raise RuntimeError("clip_grad_norm_: the gradients are on more than one device")
+        t = _GRAD_TYPES.get(g.dtype)
+        if t is None or g.layout is not torch.strided:
             raise RuntimeError("clip_grad_norm_: expected dense float32, bfloat16 or float16 gradients, got "
                                f"{g.dtype}, {g.layout}")
-        if 0 in g.stride() and any(st == 0 and k > 1 for st, k in zip(g.stride(), g.shape)):
-            raise RuntimeError("clip_grad_norm_: a gradient's elements share memory (an expanded tensor)")
-    # a gradient with gaps (a column of a wider buffer) is clipped in a copy and written back
-    work = [g if _dense(g) else g.contiguous() for g in grads]
-    spans = sorted((g.data_ptr(), g.numel() * g.element_size()) for g in work if g.numel())
-    if any(a + n > b for (a, n), (b, _) in zip(spans, spans[1:])) or len(set(map(id, grads))) != len(grads):
-        raise RuntimeError("clip_grad_norm_: two of the gradients share memory (a parameter listed twice?)")
-    n = len(work)
+        if not g.is_contiguous():
+            if any(st == 0 and k > 1 for st, k in zip(g.stride(), g.shape)):
+                raise RuntimeError("clip_grad_norm_: a gradient's elements share memory (an expanded tensor)")
+            if not _dense(g):              # gaps (a column of a wider buffer): clipped in a copy and written back
+                if any(g is o for o in grads[:len(work)]):
+                    raise RuntimeError("clip_grad_norm_: two of the gradients share memory (a parameter listed twice?)")
+                work.append(g := g.contiguous())
+                ptr.append(g.data_ptr()); num.append(g.numel()); typ.append(t)
+                continue
+        work.append(g)
+        ptr.append(g.data_ptr()); num.append(g.numel()); typ.append(t)
+    n, dev = len(work), grads[0].device
     lib = _lib.load()
     total = torch.empty((), device=dev, dtype=torch.float32)
     nbytes = lib.pngpd_grad_clip_workspace_bytes(n)
     ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
-    ptr = (ctypes.c_void_p * n)(*[g.data_ptr() for g in work])
-    num = (ctypes.c_longlong * n)(*[g.numel() for g in work])
-    typ = (ctypes.c_int * n)(*[_GRAD_TYPES[g.dtype] for g in work])
-    stream = torch.cuda.current_stream(dev).cuda_stream
+    ptr, num, typ = (ctypes.c_void_p * n)(*ptr), (ctypes.c_longlong * n)(*num), (ctypes.c_int * n)(*typ)
+    stream = _lib.raw_stream(dev)
     with _lib.device_guard(dev):
         for bound in (math.inf, max_norm) if error_if_nonfinite else (max_norm,):       # inf: the norm alone
-            _lib.check(lib.pngpd_grad_clip(ptr, num, typ, n, _NORM_KINDS[norm_type], bound, total.data_ptr(), ws.data_ptr(),
-                                           nbytes, stream), "grad_clip")
+            code = lib.pngpd_grad_clip(ptr, num, typ, n, _NORM_KINDS[norm_type], bound, total.data_ptr(), ws.data_ptr(),
+                                       nbytes, stream)
+            if code == 3:                  # PNGPD_ERR_UNSUPPORTED
+                raise RuntimeError("clip_grad_norm_: two of the gradients share memory (a parameter listed twice?)")
+            _lib.check(code, "grad_clip")
             if error_if_nonfinite and not math.isfinite(float(total)):
                 raise RuntimeError(f"clip_grad_norm_: the norm of the gradients is {float(total)}; nothing was clipped")
     for g, c in zip(grads, work):

@@ -16,7 +16,6 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .ops import _call
 
 ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # PNGPD_F32, PNGPD_BF16, PNGPD_F16
@@ -35,52 +34,68 @@ def _bytes(dev, n):
 
 
 def _same_device(ref, name, *others):
+    index = ref.get_device()
     for n, t in others:
-        if t is not None and t.device != ref.device:
+        if t is not None and t.get_device() != index:
             raise RuntimeError(f"{name}: {n} is on {t.device}, the input on {ref.device}")
 
 
 # --------------------------------------------------------------------------------------------- group norm + activation
-class GroupNormActFn(torch.autograd.Function):
-    """(B,N,C) with adjacent channels -> (B,N,C) contiguous."""
+def _gn_call(entry, backward, x, w, b, groups, eps, act, stats, *ptrs):
+    """One C call; ``ptrs``: the pointers between stats (forward: y before it) and the workspace.  Lean on purpose: at one
+    cloud the host's time is the operator's."""
+    lib, dev = _lib.load(), x.device
+    B, N, C = x.shape
+    dt = DTYPES[x.dtype]
+    wdt = DTYPES[w.dtype] if w is not None else DTYPES[b.dtype] if b is not None else dt
+    nbytes = lib.pngpd_group_norm_workspace_bytes(B, N, C, groups, dt, act, backward)
+    ws = _bytes(dev, nbytes).data_ptr() if nbytes else None      # (freed on return: the stream orders its next user)
+    head = (x.data_ptr(), dt, B, N, C, x.stride(0), x.stride(1), groups, None if w is None else w.data_ptr(),
+            None if b is None else b.data_ptr(), wdt, eps, act)
+    with _lib.device_guard(dev):
+        if backward:
+            code = lib.pngpd_group_norm_bwd(*head, stats.data_ptr(), *ptrs, ws, nbytes, _lib.raw_stream(dev))
+        else:
+            code = lib.pngpd_group_norm_fwd(*head, *ptrs, stats.data_ptr(), ws, nbytes, _lib.raw_stream(dev))
+    if code:
+        _lib.check(code, entry)
 
+
+def _group_norm_fwd(x, w, b, groups, eps, act):
+    """(B,N,C) with adjacent channels -> y (B,N,C) contiguous, stats (B,G,2) float64."""
+    B, N, C = x.shape
+    y = torch.empty((B, N, C), device=x.device, dtype=x.dtype)
+    stats = torch.empty((B, groups, 2), device=x.device, dtype=torch.float64)
+    if x.numel():
+        _gn_call("group_norm_fwd", 0, x, w, b, groups, eps, act, stats, y.data_ptr())
+    return y, stats
+
+
+class GroupNormActFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, b, groups, eps, act):
-        B, N, C = x.shape
-        y = torch.empty(B, N, C, device=x.device, dtype=x.dtype)
-        ctx.groups, ctx.eps, ctx.act, ctx.has = groups, eps, act, (w is not None, b is not None)
-        stats = torch.empty(B, groups, 2, device=x.device, dtype=torch.float64)
-        w, b = (t.detach().contiguous() if t is not None else None for t in (w, b))
-        if x.numel():
-            dt = DTYPES[x.dtype]
-            wdt = next((DTYPES[t.dtype] for t in (w, b) if t is not None), dt)
-            nbytes = _lib.load().pngpd_group_norm_workspace_bytes(B, N, C, groups, dt, 0)
-            _call("pngpd_group_norm_fwd", x, x.data_ptr(), dt, B, N, C, x.stride(0), x.stride(1), groups, w, b, wdt, eps,
-                  act, y, stats, _bytes(x.device, nbytes), nbytes)
-        ctx.save_for_backward(x, stats, *(t for t in (w, b) if t is not None))
+        y, stats = _group_norm_fwd(x, w, b, groups, eps, act)
+        ctx.args = (groups, eps, act)
+        ctx.save_for_backward(x, w, b, stats)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        x, stats, *wb = ctx.saved_tensors
-        w = wb.pop(0) if ctx.has[0] else None
-        b = wb.pop(0) if ctx.has[1] else None
-        B, N, C = x.shape
+        x, w, b, stats = ctx.saved_tensors
         need = ctx.needs_input_grad
-        dx = torch.empty(B, N, C, device=x.device, dtype=x.dtype) if need[0] else None
+        dx = torch.empty(x.shape, device=x.device, dtype=x.dtype) if need[0] else None
         dw = torch.empty_like(w) if need[1] else None
         db = torch.empty_like(b) if need[2] else None
-        if not x.numel():
+        if x.numel():
+            if not dy.is_contiguous():
+                dy = dy.contiguous()
+            _gn_call("group_norm_bwd", 1, x, w, b, *ctx.args, stats, dy.data_ptr(),
+                     *(None if t is None else t.data_ptr() for t in (dx, dw, db)))
+        else:
             for t in (dw, db):
                 if t is not None:
                     t.zero_()
-            return dx, dw, db, None, None, None
-        dt = DTYPES[x.dtype]
-        wdt = next((DTYPES[t.dtype] for t in (w, b) if t is not None), dt)
-        nbytes = _lib.load().pngpd_group_norm_workspace_bytes(B, N, C, ctx.groups, dt, 1)
-        _call("pngpd_group_norm_bwd", x, x.data_ptr(), dt, B, N, C, x.stride(0), x.stride(1), ctx.groups, w, b, wdt,
-              ctx.eps, ctx.act, stats, dy.contiguous(), dx, dw, db, _bytes(x.device, nbytes), nbytes)
         return dx, dw, db, None, None, None
 
 
@@ -119,7 +134,7 @@ def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, act="none"):
     N = 1
     for n in x.shape[1:-1]:
         N *= n
-    v = x.reshape(x.shape[0], N, C)
+    v = x if x.dim() == 3 else x.reshape(x.shape[0], N, C)
     if not x.is_cuda:
         return _group_norm_act_aten(v, groups, weight, bias, eps, act).reshape(x.shape)
     _dtype(x, "group_norm_act: x")
@@ -132,7 +147,12 @@ def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, act="none"):
         raise RuntimeError("group_norm_act: more than 2^31 - 1 samples or positions")
     if v.stride(2) != 1 and C > 1:
         v = v.contiguous()
-    return GroupNormActFn.apply(v, weight, bias, groups, eps, ACTIVATIONS[act]).view(x.shape)
+    weight, bias = (t if t is None or t.is_contiguous() else t.contiguous() for t in (weight, bias))
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (v, weight, bias)):
+        y = GroupNormActFn.apply(v, weight, bias, groups, eps, ACTIVATIONS[act])
+    else:
+        y = _group_norm_fwd(v, weight, bias, groups, eps, ACTIVATIONS[act])[0]
+    return y if y.shape == x.shape else y.view(x.shape)
 
 
 # ------------------------------------------------------------------------------------------------ linear cross entropy
@@ -145,58 +165,56 @@ def _lce_call(entry, a, ref, backward):
     ws = _bytes(dev, lib.pngpd_lce_workspace_bytes(ctypes.addressof(a), backward))
     a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
     with _lib.device_guard(dev):
-        _lib.check(getattr(lib, entry)(ctypes.addressof(a), torch.cuda.current_stream(dev).cuda_stream), entry)
+        _lib.check(getattr(lib, entry)(ctypes.addressof(a), _lib.raw_stream(dev)), entry)
+
+
+def _lce_args(scalars, x, w, bias, target, stat, kept, rows):
+    (T, D), ld = x.shape, [t.stride(0) if t.shape[0] > 1 else t.shape[1] for t in (x, w)]
+    dt = DTYPES[x.dtype]
+    reduction, ignore_index, smoothing = scalars
+    return _lib.LceArgs(x=x.data_ptr(), w=w.data_ptr(), bias=None if bias is None else bias.data_ptr(), target=target.data_ptr(),
+                        ldx=ld[0], ldw=ld[1], ignore_index=ignore_index, T=T, D=D, V=w.shape[0], dtype=dt,
+                        bias_dtype=dt if bias is None else DTYPES[bias.dtype], reduction=reduction, smoothing=smoothing,
+                        stat=stat.data_ptr(), kept=kept.data_ptr(), rows=None if rows is None else rows.data_ptr())
+
+
+def _lce_fwd(x, w, bias, target, scalars):
+    """-> loss and what the backward pass reads."""
+    dev, T = x.device, x.shape[0]
+    stat = torch.empty(2 * T + 1, device=dev, dtype=torch.float32)             # (T,2), then the kept rows' number
+    n = _lib.load().pngpd_lce_rows_ints(T)
+    rows = torch.empty(n, device=dev, dtype=torch.int32) if n else None
+    loss = torch.empty((T,) if scalars[0] == 0 else (), device=dev, dtype=torch.float32)
+    a = _lce_args(scalars, x, w, bias, target, stat, stat[2 * T:], rows)
+    a.loss = loss.data_ptr()
+    _lce_call("pngpd_lce_fwd", a, x, 0)
+    return loss, stat, rows
 
 
 class LinearCrossEntropyFn(torch.autograd.Function):
     """x (T,D), w (V,D), target (T) -> loss (T) or (); T, V, D > 0, channels adjacent."""
 
     @staticmethod
-    def forward(ctx, x, w, bias, target, reduction, ignore_index, smoothing):
-        dev, f32 = x.device, torch.float32
-        T, D = x.shape
-        bias = bias.detach().contiguous() if bias is not None else None
-        stat, kept = torch.empty(T, 2, device=dev, dtype=f32), torch.empty((), device=dev, dtype=f32)
-        loss = torch.empty((T,) if reduction == 0 else (), device=dev, dtype=f32)
-        n = _lib.load().pngpd_lce_rows_ints(T)
-        rows = torch.empty(n, device=dev, dtype=torch.int32) if n else None
-        ctx.scalars = (reduction, ignore_index, smoothing)
-        ctx.has = (bias is not None, rows is not None)
-        ctx.save_for_backward(x, w, target, stat, kept, *(t for t in (bias, rows) if t is not None))
-        a = LinearCrossEntropyFn._args(ctx.scalars, x, w, bias, target, stat, kept, rows)
-        a.loss = loss.data_ptr()
-        _lce_call("pngpd_lce_fwd", a, x, 0)
+    def forward(ctx, x, w, bias, target, scalars):
+        loss, stat, rows = _lce_fwd(x, w, bias, target, scalars)
+        ctx.scalars = scalars
+        ctx.save_for_backward(x, w, bias, target, stat, rows)
         return loss
-
-    @staticmethod
-    def _args(scalars, x, w, bias, target, stat, kept, rows):
-        a = _lib.LceArgs()
-        a.rows = None if rows is None else rows.data_ptr()
-        a.x, a.w, a.target, a.stat, a.kept = (t.data_ptr() for t in (x, w, target, stat, kept))
-        a.bias = None if bias is None else bias.data_ptr()
-        (a.T, a.D), a.V = x.shape, w.shape[0]
-        a.ldx, a.ldw = (t.stride(0) if t.shape[0] > 1 else t.shape[1] for t in (x, w))
-        a.dtype = DTYPES[x.dtype]
-        a.bias_dtype = a.dtype if bias is None else DTYPES[bias.dtype]
-        a.reduction, a.ignore_index, a.smoothing = scalars
-        return a
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dloss):
-        x, w, target, stat, kept, *more = ctx.saved_tensors
-        bias = more.pop(0) if ctx.has[0] else None
-        rows = more.pop(0) if ctx.has[1] else None
+        x, w, bias, target, stat, rows = ctx.saved_tensors
         need = ctx.needs_input_grad
         dloss = dloss.float().contiguous()
         dx = torch.empty(x.shape, device=x.device, dtype=x.dtype) if need[0] else None
         dw = torch.empty(w.shape, device=x.device, dtype=w.dtype) if need[1] else None
-        db = torch.empty_like(bias) if bias is not None and need[2] else None
-        a = LinearCrossEntropyFn._args(ctx.scalars, x, w, bias, target, stat, kept, rows)
+        db = torch.empty_like(bias) if need[2] else None
+        a = _lce_args(ctx.scalars, x, w, bias, target, stat, stat[2 * x.shape[0]:], rows)
         a.dloss = dloss.data_ptr()
         a.dx, a.dw, a.db = (None if t is None else t.data_ptr() for t in (dx, dw, db))
         _lce_call("pngpd_lce_bwd", a, x, 1)
-        return dx, dw, db, None, None, None, None
+        return dx, dw, db, None, None
 
 
 def linear_cross_entropy(x, weight, target, bias=None, reduction="mean", ignore_index=-100, label_smoothing=0.0):
@@ -245,6 +263,11 @@ def linear_cross_entropy(x, weight, target, bias=None, reduction="mean", ignore_
         raise RuntimeError("linear_cross_entropy: more than 2^31 - 257 rows, classes or channels")
     rows = [v if (v.shape[1] == 1 or v.stride(1) == 1) and (v.shape[0] == 1 or v.stride(0) >= v.shape[1]) else v.contiguous()
             for v in (x.reshape(-1, D), weight)]
-    loss = LinearCrossEntropyFn.apply(rows[0], rows[1], bias, target.reshape(-1).contiguous(), REDUCTIONS[reduction],
-                                      ignore_index, label_smoothing)
+    if bias is not None and not bias.is_contiguous():
+        bias = bias.contiguous()
+    target_rows, scalars = target.reshape(-1).contiguous(), (REDUCTIONS[reduction], ignore_index, label_smoothing)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (*rows, bias)):
+        loss = LinearCrossEntropyFn.apply(*rows, bias, target_rows, scalars)
+    else:
+        loss = _lce_fwd(*rows, bias, target_rows, scalars)[0]
     return loss.reshape(target.shape) if reduction == "none" else loss

@@ -71,6 +71,7 @@ def test_c_entries_check_their_arguments():
     assert clip(t=(ctypes.c_int * 2)(0, 7)) == INV and clip(n=(ctypes.c_longlong * 2)(4, -1)) == INV
     assert clip(g=(ctypes.c_void_p * 2)(P, None)) == INV and clip(g=(ctypes.c_void_p * 2)(P + 1, P + 64)) == INV
     assert clip(g=(ctypes.c_void_p * 2)(P + 2, P + 64)) == INV                           # float32 at a 2-byte address
+    assert clip(g=(ctypes.c_void_p * 2)(P, P + 12)) == clip(g=(ctypes.c_void_p * 2)(P, P)) == 3    # they share memory
     assert clip(ws=None) == WS and clip(b=nb - 1) == WS and clip(ws=P + 4) == WS
     off = (ctypes.c_longlong * 1)(64)
     adam = lambda p=P, o=off, n=one, k=1, mx=1.0, tot=P, ws=P, b=nb, step=1.0: lib.pngpd_adam_flat_clip(
@@ -88,11 +89,11 @@ def test_c_entries_check_their_arguments():
         assert f(eps=math.nan) == INV and f(act=4) == INV and f(act=-1) == INV and f(st=None) == INV
     assert fwd(y=None) == INV and bwd(dy=None) == INV and bwd(ws=None) == WS and bwd(b=0) == WS
     assert fwd(N=50000, ws=None) == WS and fwd(N=50000, b=0) == WS
-    assert lib.pngpd_group_norm_workspace_bytes(2, 3, 8, 3, 0, 0) == 0
+    assert lib.pngpd_group_norm_workspace_bytes(2, 3, 8, 3, 0, 0, 0) == 0
     # every plan's workspace covers what it cuts: positive wherever the backward pass keeps per-sample sums
     for dt in (0, 1, 2):
         for B, N, C, G in [(1, 1, 1, 1), (3, 50000, 17, 1), (1024, 1024, 128, 32), (1, 50000, 1024, 32), (9, 77, 1000, 1)]:
-            assert lib.pngpd_group_norm_workspace_bytes(B, N, C, G, dt, 1) >= B * C * 8
+            assert min(lib.pngpd_group_norm_workspace_bytes(B, N, C, G, dt, act, 1) for act in range(4)) >= B * C * 8
 
 
 def test_command_refuses_a_negative_clip():
