@@ -126,7 +126,8 @@ __global__ __launch_bounds__(256) void grad_scale_kernel(const ClipTable t, int 
                                                          int nparts, float max_norm, float *__restrict__ total) {
     const float c = clip_factor(kind, part, nparts, 1.0, max_norm, total);
     if (c == 1.f) return;
-    for (int ch = blockIdx.x; ch < t.first[t.count]; ch += gridDim.x) {
+    // from the end: the norm's launch read that last, and up to 256 MB of it are still in the last-level cache
+    for (int ch = t.first[t.count] - 1 - (int)blockIdx.x; ch >= 0; ch -= gridDim.x) {
         const int i = clip_find(t, ch);
         const long long at = (long long)(ch - t.first[i]) * CLIP_CHUNK;
         const long long left = t.n[i] - at;
@@ -199,7 +200,8 @@ __global__ __launch_bounds__(256) void adam_flat_clip_kernel(const AdamArgs a) {
     const float step_size = (a.lr_dev ? *a.lr_dev : a.lr) / (a.step_dev ? bc[0] : a.bc1);
     const float bc2s = a.step_dev ? bc[1] : a.bc2s;
     const long long quads = a.n >> 2;
-    for (long long q = (long long)blockIdx.x * 256 + threadIdx.x; q < quads; q += (long long)gridDim.x * 256) {
+    // from the end, as grad_scale_kernel
+    for (long long q = quads - 1 - ((long long)blockIdx.x * 256 + threadIdx.x); q >= 0; q -= (long long)gridDim.x * 256) {
         f32x4 pv = ((const f32x4 *)a.p)[q], mv = ((const f32x4 *)a.m)[q], vv = ((const f32x4 *)a.v)[q];
         const f32x4 gv = ((const f32x4 *)a.g)[q];
 #pragma unroll

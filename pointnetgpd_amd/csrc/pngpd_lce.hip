@@ -324,28 +324,32 @@ __global__ __launch_bounds__(ROWS * 32) void lce_join_kernel(const LceArgs a, fl
                 if (a.smooth != 0.f) sz += (double)a.ps[at];
             }
         }
-        __syncthreads();
+        __syncthreads();                                          // (the turn before has read its parts)
         shm[ty][tx] = m; sh[ty][tx][0] = s; sh[ty][tx][1] = sz;
         __syncthreads();
-        if (ty || t >= a.T) continue;
-        if (place < 0) { row[t] = 0.f; continue; }
+        // the other way round: a row's 32 parts in 32 lanes
+        const int lane = threadIdx.x & 31, u = t0 + threadIdx.x / 32, at = u < a.T ? a.rows.place(u) : -1;
+        m = shm[lane][threadIdx.x / 32]; s = sh[lane][threadIdx.x / 32][0]; sz = sh[lane][threadIdx.x / 32][1];
         float M = m;
-        for (int k = 1; k < 32; ++k) M = fmaxf(M, shm[k][tx]);
-        const float ref = M == -INFINITY ? 0.f : M;
-        s = sz = 0.0;
-        for (int k = 0; k < 32; ++k) { s += sh[k][tx][0] * (double)expf(shm[k][tx] - ref); sz += sh[k][tx][1]; }
-        stat[2 * (size_t)place] = M; stat[2 * (size_t)place + 1] = (float)s;
-        const long long y = a.target[t];
+#pragma unroll
+        for (int k = 16; k >= 1; k >>= 1) M = fmaxf(M, __shfl_xor(M, k));
+        s *= (double)expf(m - (M == -INFINITY ? 0.f : M));
+#pragma unroll
+        for (int k = 16; k >= 1; k >>= 1) { s += __shfl_xor(s, k); sz += __shfl_xor(sz, k); }
+        if (lane || u >= a.T) continue;
+        if (at < 0) { row[u] = 0.f; continue; }
+        stat[2 * (size_t)at] = M; stat[2 * (size_t)at + 1] = (float)s;
+        const long long y = a.target[u];
         double l = 0.0;
         if (y != a.ignore) {
             if (y < 0 || y >= a.V) l = NAN;                        // a class that does not exist: as loud as a value can be
             else {
                 // differences from the maximum first: beside a maximum of 1e30 the logarithm would be lost
-                l = log(s) + (1.0 - (double)a.smooth) * ((double)M - (double)a.zt[place]);
+                l = log(s) + (1.0 - (double)a.smooth) * ((double)M - (double)a.zt[at]);
                 if (a.smooth != 0.f) l += (double)a.smooth * ((double)M - sz / a.V);
             }
         }
-        row[t] = (float)l;
+        row[u] = (float)l;
     }
     if (gridDim.x == 1) {
         __threadfence_block();
@@ -702,8 +706,8 @@ static inline bool lce_plain(const Lce *a, const void *p, long long ld, long lon
 // tile shapes: 0 = 256 x 256, 1 = 64 x 64, 2 = 64 x 32
 static const int LCE_BM[3] = {256, 64, 64}, LCE_BN[3] = {256, 64, 32};
 #define LCE_SHAPE0 256, 256, 2, 4, 2
-#define LCE_SHAPE1 64, 64, 2, 2, 3
-#define LCE_SHAPE2 64, 32, 2, 1, 3
+#define LCE_SHAPE1 64, 64, 2, 2, 4
+#define LCE_SHAPE2 64, 32, 2, 1, 5
 static inline int lce_cdiv(long long a, int b) { return (int)((a + b - 1) / b); }
 // The large tile needs a workgroup for every CU; the narrow one is for rows that would leave half of 64 unused.
 static int lce_shape(long long M, long long N) {

@@ -146,11 +146,11 @@ template <int ACT> __device__ __forceinline__ float act_value(float z) {
 
 // What a thread keeps of its column: w, b and, for each of the SUB groups it touches, the statistics.  SUB = 1: the column
 // lies inside one group (Cg a multiple of VEC); 2: it is two whole groups; VEC: every element may belong to another one.
-// xh = x r + mr and z = x w' + b' (fold()) are one FMA each; r, mr, w', b' come from fp64 and are rounded once, an error of
-// 2^-24 (|x| + |mean|) rstd like that of subtracting a rounded mean.
+// With d = x - (the mean rounded to float32), xh = d r + c and z = d w' + b' (FOLD) are one FMA each; c and b' hold what the
+// rounded mean leaves out, so the error is of |d|'s size and not of the mean's (two nearly equal values make a group too).
 template <int VEC, int SUB> struct ColPar {
     float w[VEC], b[VEC];
-    float r[SUB], mr[SUB];                 // rstd, -mean rstd
+    float m[SUB], r[SUB], c[SUB];          // mean, rstd, -(mean - m) rstd
     static __device__ __forceinline__ int sub(int e) { return e * SUB / VEC; }
 };
 template <int DT, int VEC, int SUB>
@@ -175,13 +175,14 @@ __device__ __forceinline__ void load_stats(const GnArgs &a, const double *st, in
             const int g = (c + at) / a.Cg - g0;
             mean = st[2 * g]; rstd = st[2 * g + 1];
         }
-        p.r[k] = (float)rstd; p.mr[k] = (float)(-mean * rstd);
+        p.m[k] = (float)mean; p.r[k] = (float)rstd;
+        const double c = -(mean - (double)p.m[k]) * rstd;
+        p.c[k] = (float)c;
         if constexpr (FOLD) {
 #pragma unroll
             for (int e = at; e < at + VEC / SUB; ++e) {
-                const double w = rstd * (double)p.w[e];
-                p.b[e] = (float)((double)p.b[e] - mean * w);
-                p.w[e] = (float)w;
+                p.b[e] = (float)((double)p.b[e] + c * (double)p.w[e]);
+                p.w[e] = (float)(rstd * (double)p.w[e]);
             }
         }
     }
@@ -189,7 +190,7 @@ __device__ __forceinline__ void load_stats(const GnArgs &a, const double *st, in
 template <int ACT, int VEC, int SUB>
 __device__ __forceinline__ void gn_apply(const ColPar<VEC, SUB> &p, const float (&x)[VEC], float (&y)[VEC]) {
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) y[e] = act_value<ACT>(fmaf(x[e], p.w[e], p.b[e]));
+    for (int e = 0; e < VEC; ++e) y[e] = act_value<ACT>(fmaf(x[e] - p.m[p.sub(e)], p.w[e], p.b[e]));
 }
 // dz of one element; st: the fp64 statistics (mean, rstd) of its group, for relu's slope
 template <int ACT>
@@ -202,20 +203,20 @@ __device__ __forceinline__ float gn_dz(float x, float xh, float dy, float w, flo
         else { float e; const float s = phi_cdf(z, e); return dy * fmaf(z * 0.39894228040143268f, e, s); }
     }
 }
-// dx = rstd (w dz - S1 - xh S2) = dz w r + x k1 + k0
+// dx = rstd (w dz - S1 - xh S2) = dz w r + d k1 + k0
 template <int VEC, int SUB> struct DxPar {
     float wr[VEC], k0[SUB], k1[SUB];
     // S: (S1, S2) of the column's groups in turn
     __device__ __forceinline__ void set(const ColPar<VEC, SUB> &p, int k, double S1, double S2) {
-        const double r = (double)p.r[k], mr = (double)p.mr[k];
+        const double r = (double)p.r[k];
         k1[k] = (float)(-r * r * S2);
-        k0[k] = (float)(-r * (S1 + mr * S2));
+        k0[k] = (float)(-r * (S1 + (double)p.c[k] * S2));
 #pragma unroll
         for (int e = k * (VEC / SUB); e < (k + 1) * (VEC / SUB); ++e) wr[e] = p.w[e] * p.r[k];
     }
-    __device__ __forceinline__ float dx(int e, float x, float dz) const {
+    __device__ __forceinline__ float dx(int e, float d, float dz) const {
         const int k = ColPar<VEC, SUB>::sub(e);
-        return fmaf(dz, wr[e], fmaf(x, k1[k], k0[k]));
+        return fmaf(dz, wr[e], fmaf(d, k1[k], k0[k]));
     }
 };
 
@@ -353,7 +354,7 @@ __global__ __launch_bounds__(SLAB_THREADS) void gn_bwd_slab_kernel(const GnArgs 
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
                 const int k = p.sub(e);
-                const float xv = q[i].get(e), xh = fmaf(xv, p.r[k], p.mr[k]);
+                const float xv = q[i].get(e), xh = fmaf(xv - p.m[k], p.r[k], p.c[k]);
                 const double *st = stats + 2 * (ACT == PNGPD_ACT_RELU ? (c + min(e, max(n, 1) - 1)) / a.Cg - g0 : 0);
                 const float dz = gn_dz<ACT>(xv, xh, d[i].get(e), p.w[e], p.b[e], st);
                 if constexpr (KEEP) keep[i][e] = dz;
@@ -403,11 +404,12 @@ __global__ __launch_bounds__(SLAB_THREADS) void gn_bwd_slab_kernel(const GnArgs 
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
                 const float xv = q[i].get(e);
+                const int k = p.sub(e);
                 float dz;
                 if constexpr (KEEP) dz = keep[i][e];
                 else dz = gn_dz<ACT>(xv, 0.f, d[i].get(e), p.w[e], p.b[e],
                                      stats + 2 * (ACT == PNGPD_ACT_RELU ? (c + min(e, n - 1)) / a.Cg - g0 : 0));
-                o[e] = dp.dx(e, xv, dz);
+                o[e] = dp.dx(e, xv - p.m[k], dz);
             }
             Col<DT, VEC>::store(dx + (size_t)row * a.C, o, n);
         }
@@ -553,7 +555,7 @@ __global__ __launch_bounds__(256) void gn_bwd_part_kernel(const GnArgs a) {
 #pragma unroll
                     for (int e = 0; e < VEC; ++e) {
                         const int k = p.sub(e);
-                        const float xv = q[i].get(e), xh = fmaf(xv, p.r[k], p.mr[k]);
+                        const float xv = q[i].get(e), xh = fmaf(xv - p.m[k], p.r[k], p.c[k]);
                         const float dz = gn_dz<ACT>(xv, xh, d[i].get(e), p.w[e], p.b[e],
                                                     stats + 2 * (ACT == PNGPD_ACT_RELU ? (c + min(e, n - 1)) / a.Cg : 0));
                         A[e] += dz; Bs[e] = fmaf(dz, xh, Bs[e]);
@@ -661,10 +663,10 @@ __global__ __launch_bounds__(256) void gn_bwd_apply_kernel(const GnArgs a) {
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) {
                     const int k = p.sub(e);
-                    const float xv = q[i].get(e), xh = fmaf(xv, p.r[k], p.mr[k]);
+                    const float xv = q[i].get(e), xh = fmaf(xv - p.m[k], p.r[k], p.c[k]);
                     const float dz = gn_dz<ACT>(xv, xh, d[i].get(e), p.w[e], p.b[e],
                                                 stats + 2 * (ACT == PNGPD_ACT_RELU ? (c + min(e, n - 1)) / a.Cg : 0));
-                    o[e] = dp.dx(e, xv, dz);
+                    o[e] = dp.dx(e, xv - p.m[k], dz);
                 }
                 Col<DT, VEC>::store(dx + (size_t)(row + i * TY) * a.C, o, n);
             }

@@ -178,6 +178,18 @@ def test_nan_stays_in_its_group(shape, groups):
         assert got[n][:k].isnan().all() and torch.equal(got[n][k:], clean[n][k:]), n
 
 
+@pytest.mark.parametrize("shape,groups", [((922, 2, 8), 8), ((50, 1, 24), 12), ((300, 3, 40), 40)])
+def test_groups_of_few_values(shape, groups):
+    """Two or three values a group, some of them nearly equal: far from the mean's size, near each other."""
+    x, w, b, dy = data(shape, torch.float32, 17)
+    compare(x, w, b, groups, "none", dy)
+    got = run(x, w, b, groups, "none", dy)
+    want = reference(x, dy, w, b, groups, "none")
+    # the differences x - mean are exact but for their own rounding, whatever the mean: 2^-21 covers eight of them
+    assert (got["dw"].double() - want["dw"][0]).norm() <= 2.0 ** -21 * want["dw"][0].norm()
+    assert (got["y"].double() - want["y"][0]).norm() <= 2.0 ** -21 * want["y"][0].norm()
+
+
 def test_constant_group():
     """No spread: xh is 0, y is act(b), and the gradients are finite."""
     x = torch.full((2, 30, 16), 3.0, device="cuda")
