@@ -697,7 +697,9 @@ static inline size_t lce_up(size_t n) { return (n + 255) & ~(size_t)255; }
 static inline int lce_esize(int dt) { return dt == PNGPD_F32 ? 4 : 2; }
 static inline int lce_dp(const Lce *a) { const int c = 16 / lce_esize(a->dtype); return (a->D + c - 1) / c * c; }
 // rows that the loads can take as they are: 16-byte aligned, D a whole number of chunks, and `reach` of them within the
-// 4 GiB of a lane's offset
+// 4 GiB of a lane's offset (a tile's 256, or all where the kept rows are picked out of them; copied, they are packed, and
+// LCE_MOST_D keeps a tile's within)
+#define LCE_MOST_D (1 << 22)
 static inline bool lce_plain(const Lce *a, const void *p, long long ld, long long reach) {
     const int es = lce_esize(a->dtype);
     return lce_dp(a) == a->D && !((uintptr_t)p & 15) && (ld * es) % 16 == 0 && (double)ld * es * (double)reach < 4e9;
@@ -722,7 +724,7 @@ static int lce_cut(int n, int other) {
     const long long tiles = (long long)lce_cdiv(n, 256) * other, rounds = tiles / 256;
     if (!rounds || tiles % 256 == 0 || tiles % 256 >= 102) return n;
     const long long cut = rounds * 256 / other * 256;
-    return cut < n ? (int)cut : n;
+    return cut > 0 && cut < n ? (int)cut : n;
 }
 
 struct LcePlan {
@@ -847,7 +849,11 @@ template <int DT> static int lce_forward(const Lce *a, const LcePlan &p, hipStre
     char *ws = (char *)a->workspace;
     LceArgs k = lce_args(a);
     if (a->rows) hipLaunchKernelGGL(lce_rows_kernel, dim3(1), dim3(1024), 0, st, k.target, k.ignore, a->T, a->rows);
-    if (p.padx) { lce_copy<DT>(a, a->x, a->ldx, a->T, 0, k.rows, ws + p.o_x, st); k.x = LceOperand{ws + p.o_x, p.Dp}; }
+    if (p.padx) {
+        lce_copy<DT>(a, a->x, a->ldx, a->T, 1, k.rows, ws + p.o_x, st);
+        k.x = LceOperand{ws + p.o_x, p.Dp};
+        k.packed = 1;
+    }
     if (p.padw) { lce_copy<DT>(a, a->w, a->ldw, a->V, 0, k.rows, ws + p.o_w, st); k.w = LceOperand{ws + p.o_w, p.Dp}; }
     k.D = p.Dp;
     k.pm = (float *)(ws + p.o_part); k.ps = (float *)(ws + p.o_ps); k.zt = (float *)(ws + p.o_zt);
@@ -941,6 +947,7 @@ size_t pngpd_lce_workspace_bytes(const pngpd_lce_t *a, int backward) {
 
 int pngpd_lce_fwd(const pngpd_lce_t *a, void *stream) {
     if (lce_bad(a) || !a->loss) return PNGPD_ERR_INVALID_ARG;
+    if (a->D > LCE_MOST_D) return PNGPD_ERR_UNSUPPORTED;
     const LcePlan p = lce_plan(a, false);
     if (!a->workspace || ((uintptr_t)a->workspace & 255) || a->workspace_bytes < p.bytes) return PNGPD_ERR_WORKSPACE;
     hipStream_t st = (hipStream_t)stream;
@@ -951,6 +958,7 @@ int pngpd_lce_fwd(const pngpd_lce_t *a, void *stream) {
 
 int pngpd_lce_bwd(const pngpd_lce_t *a, void *stream) {
     if (lce_bad(a) || !a->dloss || (a->db && !a->bias)) return PNGPD_ERR_INVALID_ARG;
+    if (a->D > LCE_MOST_D) return PNGPD_ERR_UNSUPPORTED;
     if (!a->dx && !a->dw && !a->db) return PNGPD_OK;
     const LcePlan p = lce_plan(a, true);
     if (!a->workspace || ((uintptr_t)a->workspace & 255) || a->workspace_bytes < p.bytes) return PNGPD_ERR_WORKSPACE;

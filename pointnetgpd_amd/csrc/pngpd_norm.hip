@@ -766,13 +766,14 @@ static size_t gn_part_bytes(const GnPlan &p, int B, int C, int bwd) {
 }
 
 // workgroups of one launch past the grid's (and the kernels' int) range
-static bool gn_too_many(const GnPlan &p, int B, int G) {
+static bool gn_too_many(const GnPlan &p, int B, int C, int G) {
     const long long most = 0x7fffffffll;
-    return p.slab ? (long long)B * p.ranges > most : (long long)p.cols * p.S * B > most || (long long)B * G > most;
+    return p.slab ? (long long)B * p.ranges > most
+                  : (long long)p.cols * p.S * B > most || (long long)B * G > most || (long long)B * ((C + 31) / 32) > most;
 }
 
 static bool gn_bad(const void *x, int dt, int B, int N, int C, int G, int act, const void *w, int wdt, float eps) {
-    return !x || dt < PNGPD_F32 || dt > PNGPD_F16 || B <= 0 || N <= 0 || C <= 0 || G <= 0 || C % G ||
+    return !x || dt < PNGPD_F32 || dt > PNGPD_F16 || B <= 0 || N <= 0 || N > (1 << 30) || C <= 0 || C > (1 << 30) || G <= 0 || C % G ||
            act < PNGPD_ACT_NONE || act > PNGPD_ACT_GELU || !(eps >= 0.f) || (wdt != PNGPD_F32 && wdt != dt);
 }
 
@@ -861,7 +862,7 @@ int pngpd_group_norm_fwd(const void *x, int dtype, int B, int N, int C, long lon
                          void *workspace, size_t workspace_bytes, void *stream) {
     if (gn_bad(x, dtype, B, N, C, G, act, w, wdtype, eps) || !y || !stats) return PNGPD_ERR_INVALID_ARG;
     const GnPlan p = gn_plan(B, N, C, G, dtype, act, 0);
-    if (gn_too_many(p, B, G)) return PNGPD_ERR_UNSUPPORTED;
+    if (gn_too_many(p, B, C, G)) return PNGPD_ERR_UNSUPPORTED;
     if (workspace_bytes < pngpd_group_norm_workspace_bytes(B, N, C, G, dtype, act, 0) || (!p.slab && !workspace)) return PNGPD_ERR_WORKSPACE;
     GnArgs a = {};
     a.x = x; a.w = w; a.b = b; a.y = y; a.stats = stats; a.part = (double *)workspace;
@@ -877,7 +878,7 @@ int pngpd_group_norm_bwd(const void *x, int dtype, int B, int N, int C, long lon
     if (gn_bad(x, dtype, B, N, C, G, act, w, wdtype, eps) || !stats || !dy) return PNGPD_ERR_INVALID_ARG;
     if (!dx && !dw && !db) return PNGPD_OK;
     const GnPlan p = gn_plan(B, N, C, G, dtype, act, 1);
-    if (gn_too_many(p, B, G)) return PNGPD_ERR_UNSUPPORTED;
+    if (gn_too_many(p, B, C, G)) return PNGPD_ERR_UNSUPPORTED;
     if (workspace_bytes < pngpd_group_norm_workspace_bytes(B, N, C, G, dtype, act, 1) || !workspace) return PNGPD_ERR_WORKSPACE;
     GnArgs a = {};
     char *ws = (char *)workspace;

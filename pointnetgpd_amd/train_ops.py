@@ -143,8 +143,8 @@ def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, act="none"):
             raise RuntimeError(f"group_norm_act: {n} must be of x's type ({x.dtype}) or float32, got {t.dtype}")
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
         raise RuntimeError("group_norm_act: weight and bias must be of one type")
-    if max(v.shape[:2]) >= 2 ** 31:
-        raise RuntimeError("group_norm_act: more than 2^31 - 1 samples or positions")
+    if v.shape[0] >= 2 ** 31 or max(N, C) > 2 ** 30:
+        raise RuntimeError("group_norm_act: more than 2^31 - 1 samples, 2^30 positions or 2^30 channels")
     if v.stride(2) != 1 and C > 1:
         v = v.contiguous()
     weight, bias = (t if t is None or t.is_contiguous() else t.contiguous() for t in (weight, bias))
@@ -259,8 +259,8 @@ def linear_cross_entropy(x, weight, target, bias=None, reduction="mean", ignore_
     _dtype(x, "linear_cross_entropy: x")
     if bias is not None and bias.dtype not in (x.dtype, torch.float32):
         raise RuntimeError(f"linear_cross_entropy: bias must be of x's type ({x.dtype}) or float32, got {bias.dtype}")
-    if max(V, D, target.numel()) >= 2 ** 31 - 256:
-        raise RuntimeError("linear_cross_entropy: more than 2^31 - 257 rows, classes or channels")
+    if max(V, target.numel()) >= 2 ** 31 - 256 or D > 2 ** 22:
+        raise RuntimeError("linear_cross_entropy: more than 2^31 - 257 rows or classes, or 2^22 channels")
     rows = [v if (v.shape[1] == 1 or v.stride(1) == 1) and (v.shape[0] == 1 or v.stride(0) >= v.shape[1]) else v.contiguous()
             for v in (x.reshape(-1, D), weight)]
     if bias is not None and not bias.is_contiguous():

@@ -241,3 +241,11 @@ def test_same_bits_streams_and_graph(shape, groups):
         eager = run(x, w, b, groups, "gelu", dy)
         torch.cuda.synchronize()
         assert all(torch.equal(held[n], eager[n]) for n in eager), k
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_small_values(dtype):
+    """Features under the type's normal range (float16: 6e-5), where eps is what scales them."""
+    x, w, b, dy = data((3, 200, 64), dtype, 18)
+    compare((x.float() * 1e-5 + 3e-5).to(dtype), w, b, 8, "none", dy)
+    compare((x.float() * 1e-5 + 3e-5).repeat(1, 40, 1).to(dtype), w, b, 1, "none", dy.repeat(1, 40, 1))

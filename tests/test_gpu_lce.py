@@ -123,6 +123,28 @@ def test_pieces():
     compare(*args, reduction="none", smooth=0.1)
 
 
+def test_rows_far_apart():
+    """Rows whose last lies over 4 GiB from the first: no lane's offset may wrap, picked out of all rows or copied."""
+    T, D, ld = 1030, 64, 2_100_000
+    big = torch.empty(T * ld, device="cuda", dtype=BF16)
+    x, w, b, y, c = data(T, D, 300, BF16, 16)
+    far = big.as_strided((T, D), (ld, 1))
+    far.copy_(x)
+    assert T * ld * 2 > 2 ** 32
+    a, f = run(x, w, b, y, c, "none", 0.0), run(far, w, b, y, c, "none", 0.0)
+    assert all(torch.equal(a[k], f[k]) for k in a)
+    wfar = big.as_strided((300, D), (ld * 3, 1))
+    wfar.copy_(w)
+    f = run(x, wfar, b, y, c, "none", 0.0)
+    assert all(torch.equal(a[k], f[k]) for k in a)
+
+
+@pytest.mark.parametrize("T,V", [(80_000, 300), (70_000, 256), (600, 17_000)])
+def test_rounds_that_do_not_divide(T, V):
+    """More tiles across the rows than one round of workgroups takes, and a remainder for the small tile."""
+    compare(*data(T, 32, V, BF16, 17), reduction="sum", smooth=0.0)
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_strides_shapes_and_bias_types(dtype):
     g = torch.Generator(device="cuda").manual_seed(3)

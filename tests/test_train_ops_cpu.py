@@ -44,6 +44,46 @@ def test_group_norm_act_cpu(act):
     assert group_norm_act(torch.randn(2, 3, 4, 8).bfloat16(), 2, act=act).dtype == torch.bfloat16
 
 
+def test_linear_cross_entropy_refusals():
+    from pointnetgpd_amd.train_ops import linear_cross_entropy
+    x, w, y, b = torch.randn(4, 8), torch.randn(5, 8), torch.tensor([0, 1, 2, 4]), torch.zeros(5)
+    with pytest.raises(RuntimeError, match="do not fit"):
+        linear_cross_entropy(x, w[:, :7], y)
+    with pytest.raises(RuntimeError, match="do not fit"):
+        linear_cross_entropy(x, w, y[:3])
+    with pytest.raises(RuntimeError, match="shape"):
+        linear_cross_entropy(x, w[0], y)
+    with pytest.raises(RuntimeError, match="int64"):
+        linear_cross_entropy(x, w, y.int())
+    with pytest.raises(RuntimeError, match="bias"):
+        linear_cross_entropy(x, w, y, bias=b[:4])
+    with pytest.raises(RuntimeError, match="float64|float32"):
+        linear_cross_entropy(x.double(), w, y)
+    with pytest.raises(RuntimeError, match="no classes"):
+        linear_cross_entropy(x, w[:0], y)
+    with pytest.raises(ValueError, match="reduction"):
+        linear_cross_entropy(x, w, y, reduction="batchmean")
+    for bad in (-0.1, 1.1, math.nan):
+        with pytest.raises(ValueError, match="label_smoothing"):
+            linear_cross_entropy(x, w, y, label_smoothing=bad)
+
+
+@pytest.mark.parametrize("reduction", ["none", "mean", "sum"])
+def test_linear_cross_entropy_cpu(reduction):
+    from pointnetgpd_amd.train_ops import linear_cross_entropy
+    F = torch.nn.functional
+    g = torch.Generator().manual_seed(0)
+    x = torch.randn(2, 6, 8, generator=g, dtype=torch.double, requires_grad=True)
+    w, b = torch.randn(9, 8, generator=g, dtype=torch.double), torch.randn(9, generator=g, dtype=torch.double)
+    y = torch.randint(0, 9, (2, 6), generator=g)
+    y[0, 2] = -100
+    got = linear_cross_entropy(x, w, y, bias=b, reduction=reduction, label_smoothing=0.1)
+    want = F.cross_entropy(F.linear(x, w, b).flatten(0, 1), y.flatten(), reduction=reduction, label_smoothing=0.1).reshape(got.shape)
+    torch.testing.assert_close(got, want)
+    torch.testing.assert_close(torch.autograd.grad(got.sum(), x), torch.autograd.grad(want.sum(), x))
+    assert linear_cross_entropy(x.detach().bfloat16(), w.bfloat16(), y).dtype == torch.float32
+
+
 def test_clip_grad_norm_cpu():
     from pointnetgpd_amd.optim import clip_grad_norm_
     p = torch.nn.Parameter(torch.zeros(3))
@@ -94,6 +134,37 @@ def test_c_entries_check_their_arguments():
     for dt in (0, 1, 2):
         for B, N, C, G in [(1, 1, 1, 1), (3, 50000, 17, 1), (1024, 1024, 128, 32), (1, 50000, 1024, 32), (9, 77, 1000, 1)]:
             assert min(lib.pngpd_group_norm_workspace_bytes(B, N, C, G, dt, act, 1) for act in range(4)) >= B * C * 8
+
+
+def test_loss_entries_check_their_arguments():
+    import ctypes
+    from pointnetgpd_amd import _lib
+    lib = _lib.load()
+
+    def args(**k):
+        f = dict(x=256, w=256, target=256, ldx=8, ldw=8, ignore_index=-100, T=4, D=8, V=5, dtype=0, bias_dtype=0, reduction=1,
+                 smoothing=0.0, stat=256, kept=256, loss=256, dloss=256, dx=256, dw=256, workspace=256, workspace_bytes=1 << 24)
+        return _lib.LceArgs(**{**f, **k})
+    for entry, own in ((lib.pngpd_lce_fwd, "loss"), (lib.pngpd_lce_bwd, "dloss")):
+        def call(**k):
+            a = args(**k)                                          # (lives until the entry has returned)
+            return entry(ctypes.addressof(a), None)
+        assert entry(None, None) == INV
+        for bad in (dict(x=None), dict(w=None), dict(target=None), dict(T=0), dict(D=0), dict(V=0), dict(T=-1), dict(dtype=3),
+                    dict(bias_dtype=1), dict(reduction=3), dict(smoothing=1.5), dict(smoothing=math.nan), dict(ldx=7), dict(ldw=7),
+                    dict(stat=None), dict(kept=None), dict(rows=256), dict(T=512), {own: None}):
+            assert call(**bad) == INV, bad
+        assert call(workspace=None) == WS and call(workspace_bytes=16) == WS and call(workspace=264) == WS
+        assert call(D=(1 << 22) + 8, ldx=1 << 23, ldw=1 << 23) == 3
+    assert call(db=256) == INV                                                                  # a gradient of no bias
+    assert lib.pngpd_lce_rows_ints(511) == 0 and lib.pngpd_lce_rows_ints(512) == 1025
+    a = args(T=0)
+    assert lib.pngpd_lce_workspace_bytes(ctypes.addressof(a), 0) == 0
+    # a piece's gradient of the logits is bounded: 256 MB, or 256 classes of all rows
+    for T, V, D in ((8192, 100000, 1024), (100000, 100000, 64), (1, 1000000, 64)):
+        a = args(T=T, V=V, D=D, ldx=D, ldw=D, dtype=1, bias_dtype=1, rows=256 if T >= 512 else None)
+        n = lib.pngpd_lce_workspace_bytes(ctypes.addressof(a), 1)
+        assert T * D * 2 < n < (256 << 20) + T * (256 + 128) * 2 + 16 * T * D * 4 + 1024 * 4 * D * 4 + (8 << 20) + 64 * V
 
 
 def test_command_refuses_a_negative_clip():
