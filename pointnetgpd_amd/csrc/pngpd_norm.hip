@@ -7,8 +7,8 @@
 //     S1 = sum_c w_c A_c / m      S2 = sum_c w_c B_c / m      dx = rstd (w_c dz - S1 - xh S2)
 //
 // Memory-bound: x is read and y written once forward, x and dy read and dx written once backward.  Two forms:
-//   * slab: one workgroup owns the N rows of a few whole groups of one sample (64 to 512 bytes of a row) and holds
-//     them in REGISTERS between the sums and the output: each byte moves once, one launch;
+//   * slab: one workgroup owns the N rows of a few whole groups of one sample (32 bytes of a row to all of it; of short
+//     samples, several) and holds them in REGISTERS between the sums and the output: each byte moves once, one launch;
 //   * split: groups too large for that (a 50,000-point scene) are cut along N over workgroups: partial sums, a tiny
 //     launch that joins them, a second walk over the data.
 // A thread owns a fixed 16-byte column of channels, so w, b and the group's statistics sit in its registers, and the
@@ -26,14 +26,17 @@ struct GnArgs {
     const void *x, *dy, *w, *b;
     void *y, *dx;
     double *stats;                 // (B,G,2): mean, rstd
-    float *ab;                     // (B,C,2): A, B of the sample
+    float *ab;                     // (nab,C,2): A, B of a sample, or of the samples of one workgroup
     double *part;                  // split form: (B,S,units,2) sums;  backward: (B,S,C,2) as float
     float *gsum;                   // split form, backward: (B,G,2): S1, S2
+    float *folded;                 // (fold,C,2): A, B of GN_FOLD neighbours of ab
     long long sB, sN;              // strides of x (elements)
     int B, N, C, G, Cg, act, wf32; // wf32: w, b are float32 (else of x's type)
     float eps;
     int lx;                        // log2 of the columns of a workgroup
     int gpr, ranges;               // slab: groups of a workgroup, workgroups of a sample
+    int spw, cps;                  // slab: samples side by side in a workgroup, columns of one of them
+    int per, nab;                  // slab, backward: times that a workgroup takes spw samples; rows of ab
     int cols, S, rows;             // split: column blocks, cuts of N, rows of one
 };
 
@@ -220,7 +223,7 @@ template <int VEC, int SUB> struct DxPar {
     }
 };
 
-// Sums of NV values of each column (tx) over the workgroup's rows: res[v X + tx], in LDS (NV (threads + 64) values of
+// Sums of NV values of each column (tx) over the workgroup's rows: res[tx NV + v], in LDS (NV (threads + 64) values of
 // scratch before res).  Every thread writes its values, conflict-free, and a group of lanes adds a column's up: NV reads and
 // a few exchanges a thread, where sums over lanes alone exchange every value log2 times.  Fixed order.
 template <class T, int NV> __device__ __forceinline__ T *cols_sum(T *sh, const T (&v)[NV], int lx) {
@@ -239,7 +242,7 @@ template <class T, int NV> __device__ __forceinline__ T *cols_sum(T *sh, const T
         T u = 0;
         for (int k = tid & (L - 1); k < TY; k += L) u += c[k];
         for (int k = 1; k < L; k <<= 1) u += __shfl_xor(u, k);
-        if ((tid & (L - 1)) == 0) res[o] = u;
+        if ((tid & (L - 1)) == 0) res[(o & (X - 1)) * NV + (o >> lx)] = u;
     }
     __syncthreads();
     return res;
@@ -256,6 +259,13 @@ __device__ __forceinline__ double wave_sum(double v) {
     return v;
 }
 
+// lanes that add up n values together: a power of two of at least n, at most a wave; as its logarithm
+__device__ __forceinline__ int lanes_for(int n) { return n <= 1 ? 0 : min(6, 32 - __clz(n - 1)); }
+__device__ __forceinline__ double part_sum(double v, int ll) {
+    for (int k = 1; k < 1 << ll; k <<= 1) v += __shfl_xor(v, k);
+    return v;
+}
+
 // ranges of one sample stay on one XCD (workgroup i runs on XCD i % 8): neighbouring ranges share cache lines
 __device__ __forceinline__ int slab_item(int i, int ranges, int total) {
     const int whole = total / (8 * ranges) * (8 * ranges);
@@ -265,15 +275,18 @@ __device__ __forceinline__ int slab_item(int i, int ranges, int total) {
 }
 
 // ---------------------------------------------------------------------------------------------- slab form
-template <int DT, int VEC, int SUB, int RPT, int ACT>
+// MANY: a.spw samples side by side.  Otherwise the sample is the same in all lanes, and so are the addresses' bases (float32,
+// 1024 samples of 1024 x 128: 253 us, and 313 with a base in every lane).
+template <int DT, int VEC, int SUB, int RPT, int ACT, bool MANY>
 __global__ __launch_bounds__(SLAB_THREADS) void gn_fwd_slab_kernel(const GnArgs a) {
     typedef typename elem<DT>::t T;
     extern __shared__ double sh[];
     const int tid = threadIdx.x, X = 1 << a.lx, tx = tid & (X - 1), ty = tid >> a.lx, TY = blockDim.x >> a.lx;
-    const int waves = blockDim.x >> 6, wave = tid >> 6, lane = tid & 63;
-    const int item = slab_item(blockIdx.x, a.ranges, a.B * a.ranges), b = item / a.ranges, r = item - b * a.ranges;
+    const int item = slab_item(blockIdx.x, a.ranges, gridDim.x), ib = item / a.ranges, r = item - ib * a.ranges;
     const int g0 = r * a.gpr, gn = min(a.gpr, a.G - g0), c0 = g0 * a.Cg, c1 = c0 + gn * a.Cg;
-    const int c = c0 + tx * VEC, n = max(0, min(VEC, c1 - c));
+    const int sb = MANY ? tx / a.cps : 0, c = c0 + (tx - sb * a.cps) * VEC;
+    const int b0 = MANY ? ib * a.spw : ib, b = b0 + sb, have = MANY ? min(a.spw, a.B - b0) : 1;
+    const int n = sb < have ? max(0, min(VEC, c1 - c)) : 0;
     const T *x = (const T *)a.x + (long long)b * a.sB + c;
     Col<DT, VEC> q[RPT];                                  // rows past the last one: row 0 again, never used
     load_rows<RPT>(q, x, a.sN, ty, TY, a.N, n);
@@ -288,29 +301,31 @@ __global__ __launch_bounds__(SLAB_THREADS) void gn_fwd_slab_kernel(const GnArgs 
     }
 #pragma unroll
     for (int e = 0; e < SUB; ++e) { all[2 * e] = s[e]; all[2 * e + 1] = s2[e]; }
-    const double *res = cols_sum(sh, all, a.lx);          // [2 * part + {sum, squares}][column]
+    const double *res = cols_sum(sh, all, a.lx);          // [column][part][sum, squares]
     double *st = sh + 2 * SUB * (blockDim.x + 64) + 2 * SUB * X;
     const int upg = a.Cg * SUB / VEC;                     // parts of a group
     const double m = (double)a.N * a.Cg;
-    for (int g = wave; g < gn; g += waves) {
+    const int ll = lanes_for(upg), lane = tid & ((1 << ll) - 1);
+    for (int i = tid >> ll; i < have * gn; i += blockDim.x >> ll) {
+        const int is = MANY ? i / gn : 0, g = i - is * gn;
         double u = 0.0, v = 0.0;
-        for (int k = lane; k < upg; k += 64) {
-            const int j = g * upg + k, col = j / SUB, part = j - col * SUB;
-            u += res[2 * part * X + col]; v += res[(2 * part + 1) * X + col];
+        for (int k = lane; k < upg; k += 1 << ll) {
+            const double *o = res + 2 * ((size_t)is * a.cps * SUB + g * upg + k);
+            u += o[0]; v += o[1];
         }
-        u = wave_sum(u); v = wave_sum(v);
+        u = part_sum(u, ll); v = part_sum(v, ll);
         if (lane == 0) {
             const double mean = u / m;
             double var = v / m - mean * mean;
             var = var < 0.0 ? 0.0 : var;                  // NaN passes
             const double rstd = 1.0 / sqrt(var + (double)a.eps);
-            st[2 * g] = mean; st[2 * g + 1] = rstd;
-            double *o = a.stats + 2 * ((size_t)b * a.G + g0 + g);
+            st[2 * i] = mean; st[2 * i + 1] = rstd;
+            double *o = a.stats + 2 * ((size_t)(b0 + is) * a.G + g0 + g);
             o[0] = mean; o[1] = rstd;
         }
     }
     __syncthreads();
-    load_stats<true>(a, st, c, n, g0, p);
+    load_stats<true>(a, st + 2 * sb * gn, c, n, g0, p);
     T *y = (T *)a.y + (size_t)b * a.N * a.C + c;
 #pragma unroll
     for (int i = 0; i < RPT; ++i) {
@@ -325,17 +340,18 @@ __global__ __launch_bounds__(SLAB_THREADS) void gn_fwd_slab_kernel(const GnArgs 
     }
 }
 
-// dz stays in registers (float32) between the sums and dx where its slope is dear (silu, gelu); none and relu take dy again.
-template <int DT, int VEC, int SUB, int RPT, int ACT>
-__global__ __launch_bounds__(SLAB_THREADS) void gn_bwd_slab_kernel(const GnArgs a) {
+// The samples b0 .. b0 + have - 1 (without MANY: one); dz stays in registers (float32) between the sums and dx where its
+// slope is dear (silu, gelu); none and relu take dy again.  sum: A, B of the channels tid + i threads over the samples so far.
+template <int DT, int VEC, int SUB, int RPT, int ACT, bool MANY>
+__device__ __forceinline__ void gn_bwd_samples(const GnArgs &a, double *sh, int ib, int r, int b0, int have, bool first, bool last,
+                                               double (&sum)[MANY ? VEC : 1][2]) {
     typedef typename elem<DT>::t T;
     constexpr bool KEEP = ACT == PNGPD_ACT_SILU || ACT == PNGPD_ACT_GELU;
-    extern __shared__ double sh[];
     const int tid = threadIdx.x, X = 1 << a.lx, tx = tid & (X - 1), ty = tid >> a.lx, TY = blockDim.x >> a.lx;
-    const int waves = blockDim.x >> 6, wave = tid >> 6, lane = tid & 63;
-    const int item = slab_item(blockIdx.x, a.ranges, a.B * a.ranges), b = item / a.ranges, r = item - b * a.ranges;
-    const int g0 = r * a.gpr, gn = min(a.gpr, a.G - g0), c0 = g0 * a.Cg, c1 = c0 + gn * a.Cg;
-    const int c = c0 + tx * VEC, n = max(0, min(VEC, c1 - c));
+    const int g0 = r * a.gpr, gn = min(a.gpr, a.G - g0), c0 = g0 * a.Cg, c1 = c0 + gn * a.Cg, nc = c1 - c0;
+    const int sb = MANY ? tx / a.cps : 0, c = c0 + (tx - sb * a.cps) * VEC, b = b0 + sb;
+    const int n = sb < have ? max(0, min(VEC, c1 - c)) : 0;
+    double *st = sh + VEC * (blockDim.x + 64 + X);        // [samples][gn][2]: S1, S2   (behind 2 VEC (threads + 64 + X) floats)
     const T *x = (const T *)a.x + (long long)b * a.sB + c;
     const T *dy = (const T *)a.dy + (size_t)b * a.N * a.C + c;
     const double *stats = a.stats + 2 * ((size_t)b * a.G + g0);
@@ -350,12 +366,12 @@ __global__ __launch_bounds__(SLAB_THREADS) void gn_bwd_slab_kernel(const GnArgs 
     for (int e = 0; e < VEC; ++e) { A[e] = 0.f; Bs[e] = 0.f; }
 #pragma unroll
     for (int i = 0; i < RPT; ++i) {
-        if (ty + i * TY < a.N) {
+        if (ty + i * TY < a.N && n > 0) {
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
                 const int k = p.sub(e);
                 const float xv = q[i].get(e), xh = fmaf(xv - p.m[k], p.r[k], p.c[k]);
-                const double *st = stats + 2 * (ACT == PNGPD_ACT_RELU ? (c + min(e, max(n, 1) - 1)) / a.Cg - g0 : 0);
+                const double *st = stats + 2 * (ACT == PNGPD_ACT_RELU ? (c + min(e, n - 1)) / a.Cg - g0 : 0);
                 const float dz = gn_dz<ACT>(xv, xh, d[i].get(e), p.w[e], p.b[e], st);
                 if constexpr (KEEP) keep[i][e] = dz;
                 A[e] += dz; Bs[e] = fmaf(dz, xh, Bs[e]);
@@ -365,53 +381,81 @@ __global__ __launch_bounds__(SLAB_THREADS) void gn_bwd_slab_kernel(const GnArgs 
     float all[2 * VEC];
 #pragma unroll
     for (int e = 0; e < VEC; ++e) { all[2 * e] = A[e]; all[2 * e + 1] = Bs[e]; }
-    const float *res = cols_sum((float *)sh, all, a.lx);  // [2 * e + {A, B}][column]
-    const int chans = X * VEC;
-    double *ch = sh + (VEC * (blockDim.x + 64) + chans);  // [chans][2]: w A, w B   (behind 2 VEC (threads + 64 + X) floats)
-    double *st = ch + 2 * (size_t)chans;                  // [gn][2]: S1, S2
-    for (int k = tid; k < c1 - c0; k += blockDim.x) {
-        const int col = k / VEC, e = k - col * VEC;
-        const float u = res[2 * e * X + col], v = res[(2 * e + 1) * X + col];
-        if (a.ab) {
-            float *o = a.ab + 2 * ((size_t)b * a.C + c0 + k);
-            o[0] = u; o[1] = v;
-        }
-        const float w = !a.w ? 1.f : a.wf32 ? ((const float *)a.w)[c0 + k] : ld_elem<DT>((const T *)a.w + c0 + k);
-        ch[2 * k] = (double)u * w; ch[2 * k + 1] = (double)v * w;
-    }
-    __syncthreads();
-    const double m = (double)a.N * a.Cg;
-    for (int g = wave; g < gn; g += waves) {
-        double u = 0.0, v = 0.0;
-        for (int k = lane; k < a.Cg; k += 64) { u += ch[2 * (g * a.Cg + k)]; v += ch[2 * (g * a.Cg + k) + 1]; }
-        u = wave_sum(u); v = wave_sum(v);
-        if (lane == 0) { st[2 * g] = u / m; st[2 * g + 1] = v / m; }
-    }
-    __syncthreads();
-    if (n == 0 || !a.dx) return;
-    DxPar<VEC, SUB> dp;
+    const float *res = cols_sum((float *)sh, all, a.lx);  // [column][e][A, B]
 #pragma unroll
-    for (int k = 0; k < SUB; ++k) {
-        const int g = (c + min(k * (VEC / SUB), n - 1)) / a.Cg - g0;
-        dp.set(p, k, st[2 * g], st[2 * g + 1]);
-    }
-    T *dx = (T *)a.dx + (size_t)b * a.N * a.C + c;
-#pragma unroll
-    for (int i = 0; i < RPT; ++i) {
-        const int row = ty + i * TY;
-        if (row < a.N) {
-            float o[VEC];
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                const float xv = q[i].get(e);
-                const int k = p.sub(e);
-                float dz;
-                if constexpr (KEEP) dz = keep[i][e];
-                else dz = gn_dz<ACT>(xv, 0.f, d[i].get(e), p.w[e], p.b[e],
-                                     stats + 2 * (ACT == PNGPD_ACT_RELU ? (c + min(e, n - 1)) / a.Cg - g0 : 0));
-                o[e] = dp.dx(e, xv - p.m[k], dz);
+    for (int i = 0; i < (MANY ? VEC : 1); ++i) {
+        for (int k = tid + i * blockDim.x; k < nc; k += MANY ? nc : blockDim.x) {
+            double u = MANY && !first ? sum[i][0] : 0.0, v = MANY && !first ? sum[i][1] : 0.0;
+            for (int is = 0; is < have; ++is) {
+                const float *o = res + 2 * (is * a.cps * VEC + k);
+                u += (double)o[0]; v += (double)o[1];
             }
-            Col<DT, VEC>::store(dx + (size_t)row * a.C, o, n);
+            if constexpr (MANY) { sum[i][0] = u; sum[i][1] = v; }
+            if (a.ab && last) {
+                float *o = a.ab + 2 * ((size_t)ib * a.C + c0 + k);
+                o[0] = (float)u; o[1] = (float)v;
+            }
+        }
+    }
+    const double m = (double)a.N * a.Cg;
+    const int ll = lanes_for(a.Cg), lane = tid & ((1 << ll) - 1);
+    for (int i = tid >> ll; i < have * gn; i += blockDim.x >> ll) {
+        const int is = MANY ? i / gn : 0, g = i - is * gn;
+        const float *o = res + 2 * (is * a.cps * VEC + g * a.Cg);
+        double u = 0.0, v = 0.0;
+        for (int k = lane; k < a.Cg; k += 1 << ll) {
+            const int ch = c0 + g * a.Cg + k;
+            const double w = !a.w ? 1.f : a.wf32 ? ((const float *)a.w)[ch] : ld_elem<DT>((const T *)a.w + ch);
+            u += (double)o[2 * k] * w; v += (double)o[2 * k + 1] * w;
+        }
+        u = part_sum(u, ll); v = part_sum(v, ll);
+        if (lane == 0) { st[2 * i] = u / m; st[2 * i + 1] = v / m; }
+    }
+    __syncthreads();
+    if (n > 0 && a.dx) {
+        DxPar<VEC, SUB> dp;
+#pragma unroll
+        for (int k = 0; k < SUB; ++k) {
+            const int g = sb * gn + (c + min(k * (VEC / SUB), n - 1)) / a.Cg - g0;
+            dp.set(p, k, st[2 * g], st[2 * g + 1]);
+        }
+        T *dx = (T *)a.dx + (size_t)b * a.N * a.C + c;
+#pragma unroll
+        for (int i = 0; i < RPT; ++i) {
+            const int row = ty + i * TY;
+            if (row < a.N) {
+                float o[VEC];
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    const float xv = q[i].get(e);
+                    const int k = p.sub(e);
+                    float dz;
+                    if constexpr (KEEP) dz = keep[i][e];
+                    else dz = gn_dz<ACT>(xv, 0.f, d[i].get(e), p.w[e], p.b[e],
+                                         stats + 2 * (ACT == PNGPD_ACT_RELU ? (c + min(e, n - 1)) / a.Cg - g0 : 0));
+                    o[e] = dp.dx(e, xv - p.m[k], dz);
+                }
+                Col<DT, VEC>::store(dx + (size_t)row * a.C, o, n);
+            }
+        }
+    }
+}
+
+// MANY: a workgroup takes spw samples a.per times and keeps its A, B over them (fp64): of many samples of a few rows each the
+// sums would otherwise be larger than the data.
+template <int DT, int VEC, int SUB, int RPT, int ACT, bool MANY>
+__global__ __launch_bounds__(SLAB_THREADS) void gn_bwd_slab_kernel(const GnArgs a) {
+    extern __shared__ double sh[];
+    const int item = slab_item(blockIdx.x, a.ranges, gridDim.x), ib = item / a.ranges, r = item - ib * a.ranges;
+    double sum[MANY ? VEC : 1][2];
+    if constexpr (!MANY) gn_bwd_samples<DT, VEC, SUB, RPT, ACT, MANY>(a, sh, ib, r, ib, 1, true, true, sum);
+    else {
+        const long long span = (long long)a.per * a.spw, from = ib * span, to = min((long long)a.B, from + span);
+#pragma unroll 1
+        for (long long b0 = from; b0 < to; b0 += a.spw) {
+            gn_bwd_samples<DT, VEC, SUB, RPT, ACT, MANY>(a, sh, ib, r, (int)b0, (int)min((long long)a.spw, to - b0), b0 == from,
+                                                         b0 + a.spw >= to, sum);
+            __syncthreads();                              // the next samples' sums go where these are read
         }
     }
 }
@@ -585,17 +629,18 @@ __global__ __launch_bounds__(256) void gn_bwd_part_kernel(const GnArgs a) {
     }
 }
 
-// the channels' A, B of a sample over its cuts: 32 channels x 32 cut lanes a workgroup
-__global__ __launch_bounds__(1024) void gn_bwd_join_kernel(const GnArgs a) {
+// the channels' A, B over `per` neighbours (a sample's cuts, or samples): in (total,C,2), out (total / per, rounded up, C, 2);
+// 32 channels x 32 lanes of neighbours a workgroup
+__global__ __launch_bounds__(1024) void gn_bwd_join_kernel(const float *in, float *out, int C, int total, int per) {
     __shared__ double sh[32][32][2];
-    const int cx = threadIdx.x & 31, sy = threadIdx.x >> 5, blocks = (a.C + 31) / 32;
-    const int b = blockIdx.x / blocks, c = (blockIdx.x - b * blocks) * 32 + cx;
-    const float *in = (const float *)a.part + 2 * ((size_t)b * a.S * a.C + c);
+    const int cx = threadIdx.x & 31, sy = threadIdx.x >> 5, blocks = (C + 31) / 32;
+    const int j = blockIdx.x / blocks, c = (blockIdx.x - j * blocks) * 32 + cx, s0 = j * per, n = min(per, total - s0);
+    in += 2 * ((size_t)s0 * C + c);
     double u = 0.0, v = 0.0;
-    if (c < a.C) {
+    if (c < C) {
 #pragma unroll 4
-        for (int s = sy; s < a.S; s += 32) {
-            const f32x2 o = *(const f32x2 *)(in + 2 * (size_t)s * a.C);
+        for (int s = sy; s < n; s += 32) {
+            const f32x2 o = *(const f32x2 *)(in + 2 * (size_t)s * C);
             u += (double)o[0]; v += (double)o[1];
         }
     }
@@ -605,8 +650,8 @@ __global__ __launch_bounds__(1024) void gn_bwd_join_kernel(const GnArgs a) {
         if (sy < k) { sh[sy][cx][0] += sh[sy + k][cx][0]; sh[sy][cx][1] += sh[sy + k][cx][1]; }
         __syncthreads();
     }
-    if (sy == 0 && c < a.C) {
-        float *o = a.ab + 2 * ((size_t)b * a.C + c);
+    if (sy == 0 && c < C) {
+        float *o = out + 2 * ((size_t)j * C + c);
         o[0] = (float)sh[0][cx][0]; o[1] = (float)sh[0][cx][1];
     }
 }
@@ -674,16 +719,16 @@ __global__ __launch_bounds__(256) void gn_bwd_apply_kernel(const GnArgs a) {
     }
 }
 
-// db_c, dw_c = the samples' A_c, B_c summed in fp64: 4 channels x 64 sample lanes a workgroup
+// db_c, dw_c = the A_c, B_c of ab (n,C,2) summed in fp64: 4 channels x 64 lanes a workgroup
 template <int DT>
-__global__ __launch_bounds__(256) void gn_dwdb_kernel(const GnArgs a, void *dw, void *db) {
+__global__ __launch_bounds__(256) void gn_dwdb_kernel(const GnArgs a, const float *ab, int n, void *dw, void *db) {
     __shared__ double sh[64][4][2];
     const int cx = threadIdx.x & 3, ry = threadIdx.x >> 2, c = blockIdx.x * 4 + cx;
     double u = 0.0, v = 0.0;
     if (c < a.C) {
 #pragma unroll 4
-        for (int b = ry; b < a.B; b += 64) {
-            const f32x2 o = *(const f32x2 *)(a.ab + 2 * ((size_t)b * a.C + c));
+        for (int b = ry; b < n; b += 64) {
+            const f32x2 o = *(const f32x2 *)(ab + 2 * ((size_t)b * a.C + c));
             u += (double)o[0]; v += (double)o[1];
         }
     }
@@ -699,7 +744,8 @@ __global__ __launch_bounds__(256) void gn_dwdb_kernel(const GnArgs a, void *dw, 
 
 // ---------------------------------------------------------------------------------------------- plan
 // rpt rows a thread can hold: forward 16 (64 registers of data), backward 8 of x and of dy.
-struct GnPlan { int vec, sub, slab, lx, gpr, ranges, threads, rpt, cols, S, rows; };
+#define GN_FOLD 256
+struct GnPlan { int vec, sub, slab, lx, gpr, ranges, spw, cps, threads, rpt, per, nab, fold, cols, S, rows; };
 
 static inline int log2_up(int n) { int k = 0; while ((1 << k) < n) ++k; return k; }
 
@@ -709,9 +755,11 @@ static GnPlan gn_plan(int B, int N, int C, int G, int dt, int act, int bwd) {
     p.vec = C >= wide ? wide : 1;
     p.sub = Cg % p.vec == 0 ? 1 : 2 * Cg == p.vec ? 2 : p.vec;
     // slab: columns of a range = 128 bytes of a row (whole cache lines), or one group where that is more (up to 512
-    // bytes); halved, down to 32 bytes, while the rows do not fit or there are fewer than 512 workgroups (two a CU: one
-    // loads while the other computes).  Rows of a thread: 64 registers of x forward, x and dz (or dy) backward.
+    // columns: 1000 samples of 60 x 1000 in one group, bf16, forward + backward: 233 us, cut by rows 318); halved, down to
+    // 32 bytes, while the rows do not fit or there are fewer than 512 workgroups (two a CU: one loads while the other
+    // computes).  Rows of a thread: 64 registers of x forward, x and dz (or dy) backward.
     p.slab = 0; p.gpr = p.ranges = p.threads = p.rpt = 0;
+    p.per = p.spw = 1; p.nab = B; p.cps = 0;
     // 160 registers a thread where dz is kept for eight 16-bit channels: one workgroup of 512 a CU, three of 256 (bf16, 1024
     // samples of 1024 x 128: 322 and 292 us); otherwise 512 threads, on wider pieces of a row (float32, 64 x 750 x 128:
     // 19.7 and 23.7 us)
@@ -723,7 +771,7 @@ static GnPlan gn_plan(int B, int N, int C, int G, int dt, int act, int bwd) {
             if (gpr > G) gpr = G;
             const int cols = (gpr * Cg + p.vec - 1) / p.vec;
             const int lx = log2_up(cols);
-            if (lx > 5) break;
+            if (lx > 9) break;
             const int ranges = (G + gpr - 1) / gpr;
             const long long need = ((long long)N + most - 1) / most << lx;
             if (need <= most_threads) {
@@ -731,6 +779,20 @@ static GnPlan gn_plan(int B, int N, int C, int G, int dt, int act, int bwd) {
                 if ((long long)B * ranges >= 512) break;
             }
             if (gpr == 1) break;
+        }
+    }
+    // more than 16 workgroups a CU, of a few rows each: wider ranges, then several samples side by side, up to 256 columns
+    // (100,000 samples of 1 x 64, bf16, forward: 256 and 24 us; 20,000 of 1 x 1024 in 32 groups, forward + backward: 1311 and 406)
+    while (p.slab && p.ranges > 1 && (long long)B * p.ranges > 4096 && (long long)N << p.lx <= 128) {
+        p.gpr = p.gpr * 2 > G ? G : p.gpr * 2;
+        p.ranges = (G + p.gpr - 1) / p.gpr;
+        p.lx = log2_up((p.gpr * Cg + p.vec - 1) / p.vec);
+    }
+    if (p.slab) {
+        p.cps = (p.gpr * Cg + p.vec - 1) / p.vec;
+        while (p.ranges == 1 && B / p.spw > 4096 && (long long)N << p.lx <= 128) {
+            p.spw *= 2;
+            p.lx = log2_up(p.spw * p.cps);
         }
     }
     if (p.slab) {
@@ -741,6 +803,10 @@ static GnPlan gn_plan(int B, int N, int C, int G, int dt, int act, int bwd) {
         p.threads = th;
         int r = (int)(((long long)N + (th >> p.lx) - 1) / (th >> p.lx));
         p.rpt = r <= 2 ? 2 : r <= 4 ? 4 : r <= 8 ? 8 : 16;
+        // backward of one row or two a thread: 4096 workgroups, each taking more samples in turn
+        const long long sets = ((long long)B + p.spw - 1) / p.spw;
+        if (bwd && p.rpt == 2 && sets * p.ranges > 4096) p.per = (int)((sets * p.ranges + 4095) / 4096);
+        p.nab = (int)((sets + p.per - 1) / p.per);
         p.cols = p.S = p.rows = 0;
     }
     if (!p.slab) {
@@ -757,13 +823,18 @@ static GnPlan gn_plan(int B, int N, int C, int G, int dt, int act, int bwd) {
         p.rows = (int)(((long long)N + S - 1) / S);
         p.S = (N + p.rows - 1) / p.rows;
     }
+    // dw, db of thousands of sums: GN_FOLD of them at a time first (a second launch, but whole cache lines)
+    p.fold = p.nab >= 2048 ? (p.nab + GN_FOLD - 1) / GN_FOLD : 0;
     return p;
 }
 
 static size_t gn_part_bytes(const GnPlan &p, int B, int C, int bwd) {
-    if (p.slab) return 0;
+    if (p.slab || (bwd && p.S == 1)) return 0;            // one cut: its sums are the sample's
     return (size_t)B * p.S * (bwd ? (size_t)C * 8 : (size_t)(C / (p.vec / p.sub)) * 16);
 }
+
+static size_t gn_ab_bytes(const GnPlan &p, int C) { return ((size_t)p.nab * C * 8 + 255) & ~(size_t)255; }
+static size_t gn_gsum_bytes(const GnPlan &p, int B, int G) { return p.slab ? 0 : ((size_t)B * G * 8 + 255) & ~(size_t)255; }
 
 // workgroups of one launch past the grid's (and the kernels' int) range
 static bool gn_too_many(const GnPlan &p, int B, int C, int G) {
@@ -780,18 +851,19 @@ static bool gn_bad(const void *x, int dt, int B, int N, int C, int G, int act, c
 template <class K> static int gn_slab_launch(K kernel, const GnArgs &a, const GnPlan &p, size_t lds, hipStream_t st) {
     const int rc = pngpd_allow_lds((const void *)kernel, lds);
     if (rc) return rc;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)(a.B * p.ranges)), dim3(p.threads), lds, st, a);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(p.nab * p.ranges)), dim3(p.threads), lds, st, a);
     return PNGPD_OK;
 }
 
 template <int DT, int VEC, int SUB, int ACT>
 static int gn_fwd_launch(GnArgs &a, const GnPlan &p, hipStream_t st) {
     if (p.slab) {
-        const size_t lds = (size_t)2 * SUB * (p.threads + 64 + (1 << p.lx)) * 8 + (size_t)p.gpr * 16;
-        const int rc = p.rpt == 2 ? gn_slab_launch(gn_fwd_slab_kernel<DT, VEC, SUB, 2, ACT>, a, p, lds, st)
-                     : p.rpt == 4 ? gn_slab_launch(gn_fwd_slab_kernel<DT, VEC, SUB, 4, ACT>, a, p, lds, st)
-                     : p.rpt == 8 ? gn_slab_launch(gn_fwd_slab_kernel<DT, VEC, SUB, 8, ACT>, a, p, lds, st)
-                                  : gn_slab_launch(gn_fwd_slab_kernel<DT, VEC, SUB, 16, ACT>, a, p, lds, st);
+        const size_t lds = (size_t)2 * SUB * (p.threads + 64 + (1 << p.lx)) * 8 + (size_t)p.spw * p.gpr * 16;
+        const int rc = p.spw > 1  ? gn_slab_launch(gn_fwd_slab_kernel<DT, VEC, SUB, 2, ACT, true>, a, p, lds, st)
+                     : p.rpt == 2 ? gn_slab_launch(gn_fwd_slab_kernel<DT, VEC, SUB, 2, ACT, false>, a, p, lds, st)
+                     : p.rpt == 4 ? gn_slab_launch(gn_fwd_slab_kernel<DT, VEC, SUB, 4, ACT, false>, a, p, lds, st)
+                     : p.rpt == 8 ? gn_slab_launch(gn_fwd_slab_kernel<DT, VEC, SUB, 8, ACT, false>, a, p, lds, st)
+                                  : gn_slab_launch(gn_fwd_slab_kernel<DT, VEC, SUB, 16, ACT, false>, a, p, lds, st);
         return rc ? rc : pngpd_launch_status();
     }
     const dim3 grid((unsigned)(p.cols * p.S * a.B));
@@ -803,23 +875,32 @@ static int gn_fwd_launch(GnArgs &a, const GnPlan &p, hipStream_t st) {
 
 template <int DT, int VEC, int SUB, int ACT>
 static int gn_bwd_launch(GnArgs &a, const GnPlan &p, void *dw, void *db, hipStream_t st) {
+    const int blocks = (a.C + 31) / 32;                   // of a join, for one output row
     if (p.slab) {
-        const size_t chans = (size_t)(1 << p.lx) * VEC;
-        const size_t lds = (size_t)2 * VEC * (p.threads + 64) * 4 + chans * 8 + chans * 16 + (size_t)p.gpr * 16;
-        const int rc = p.rpt == 2 ? gn_slab_launch(gn_bwd_slab_kernel<DT, VEC, SUB, 2, ACT>, a, p, lds, st)
-                     : p.rpt == 4 ? gn_slab_launch(gn_bwd_slab_kernel<DT, VEC, SUB, 4, ACT>, a, p, lds, st)
-                                  : gn_slab_launch(gn_bwd_slab_kernel<DT, VEC, SUB, 8, ACT>, a, p, lds, st);
+        const bool many = p.per > 1 || p.spw > 1;
+        const size_t lds = (size_t)2 * VEC * (p.threads + 64 + (1 << p.lx)) * 4 + (size_t)p.spw * p.gpr * 16;
+        const int rc = many       ? gn_slab_launch(gn_bwd_slab_kernel<DT, VEC, SUB, 2, ACT, true>, a, p, lds, st)
+                     : p.rpt == 2 ? gn_slab_launch(gn_bwd_slab_kernel<DT, VEC, SUB, 2, ACT, false>, a, p, lds, st)
+                     : p.rpt == 4 ? gn_slab_launch(gn_bwd_slab_kernel<DT, VEC, SUB, 4, ACT, false>, a, p, lds, st)
+                                  : gn_slab_launch(gn_bwd_slab_kernel<DT, VEC, SUB, 8, ACT, false>, a, p, lds, st);
         if (rc) return rc;
     } else {
         const dim3 grid((unsigned)(p.cols * p.S * a.B));
         hipLaunchKernelGGL((gn_bwd_part_kernel<DT, VEC, SUB, ACT>), grid, dim3(256), (size_t)4 * (1 << p.lx) * VEC * 8, st, a);
-        hipLaunchKernelGGL(gn_bwd_join_kernel, dim3((unsigned)(a.B * ((a.C + 31) / 32))), dim3(1024), 0, st, a);
+        if (p.S > 1) hipLaunchKernelGGL(gn_bwd_join_kernel, dim3((unsigned)(a.B * blocks)), dim3(1024), 0, st, (const float *)a.part, a.ab, a.C, a.B * p.S, p.S);
         if (a.dx) {
             hipLaunchKernelGGL(gn_bwd_group_kernel<DT>, dim3((unsigned)(a.B * a.G)), dim3(64), 0, st, a);
             hipLaunchKernelGGL((gn_bwd_apply_kernel<DT, VEC, SUB, ACT>), grid, dim3(256), 0, st, a);
         }
     }
-    if (dw || db) hipLaunchKernelGGL(gn_dwdb_kernel<DT>, dim3((unsigned)((a.C + 3) / 4)), dim3(256), 0, st, a, dw, db);
+    if (dw || db) {
+        const float *ab = a.ab;
+        if (p.fold) {
+            hipLaunchKernelGGL(gn_bwd_join_kernel, dim3((unsigned)(p.fold * blocks)), dim3(1024), 0, st, ab, a.folded, a.C, p.nab, GN_FOLD);
+            ab = a.folded;
+        }
+        hipLaunchKernelGGL(gn_dwdb_kernel<DT>, dim3((unsigned)((a.C + 3) / 4)), dim3(256), 0, st, a, ab, p.fold ? p.fold : p.nab, dw, db);
+    }
     return pngpd_launch_status();
 }
 
@@ -853,7 +934,7 @@ size_t pngpd_group_norm_workspace_bytes(int B, int N, int C, int G, int dtype, i
     if (B <= 0 || N <= 0 || C <= 0 || G <= 0 || C % G || dtype < PNGPD_F32 || dtype > PNGPD_F16) return 0;
     const GnPlan p = gn_plan(B, N, C, G, dtype, act, backward != 0);
     size_t n = (gn_part_bytes(p, B, C, backward != 0) + 255) & ~(size_t)255;
-    if (backward) n += (((size_t)B * C * 8 + 255) & ~(size_t)255) + (p.slab ? 0 : (size_t)B * G * 8);
+    if (backward) n += gn_ab_bytes(p, C) + gn_gsum_bytes(p, B, G) + (size_t)p.fold * C * 8;
     return n;
 }
 
@@ -865,6 +946,7 @@ int pngpd_group_norm_fwd(const void *x, int dtype, int B, int N, int C, long lon
     if (gn_too_many(p, B, C, G)) return PNGPD_ERR_UNSUPPORTED;
     if (workspace_bytes < pngpd_group_norm_workspace_bytes(B, N, C, G, dtype, act, 0) || (!p.slab && !workspace)) return PNGPD_ERR_WORKSPACE;
     GnArgs a = {};
+    a.spw = p.spw; a.cps = p.cps;
     a.x = x; a.w = w; a.b = b; a.y = y; a.stats = stats; a.part = (double *)workspace;
     a.sB = stride_b; a.sN = stride_n; a.B = B; a.N = N; a.C = C; a.G = G; a.Cg = C / G; a.act = act;
     a.wf32 = wdtype == PNGPD_F32; a.eps = eps; a.lx = p.lx; a.gpr = p.gpr; a.ranges = p.ranges; a.cols = p.cols; a.S = p.S; a.rows = p.rows;
@@ -885,7 +967,10 @@ int pngpd_group_norm_bwd(const void *x, int dtype, int B, int N, int C, long lon
     const size_t part = (gn_part_bytes(p, B, C, 1) + 255) & ~(size_t)255;
     a.x = x; a.dy = dy; a.w = w; a.b = b; a.dx = dx; a.stats = (double *)stats; a.part = (double *)ws;
     a.ab = dw || db || !p.slab ? (float *)(ws + part) : nullptr;
-    a.gsum = (float *)(ws + part + (((size_t)B * C * 8 + 255) & ~(size_t)255));
+    a.gsum = (float *)(ws + part + gn_ab_bytes(p, C));
+    a.folded = (float *)(ws + part + gn_ab_bytes(p, C) + gn_gsum_bytes(p, B, G));
+    a.per = p.per; a.nab = p.nab; a.spw = p.spw; a.cps = p.cps;
+    if (!p.slab && p.S == 1) a.part = (double *)a.ab;
     a.sB = stride_b; a.sN = stride_n; a.B = B; a.N = N; a.C = C; a.G = G; a.Cg = C / G; a.act = act;
     a.wf32 = wdtype == PNGPD_F32; a.eps = eps; a.lx = p.lx; a.gpr = p.gpr; a.ranges = p.ranges; a.cols = p.cols; a.S = p.S; a.rows = p.rows;
     return gn_launch_type(a, dtype, p, true, dw, db, (hipStream_t)stream);

@@ -249,3 +249,23 @@ def test_small_values(dtype):
     x, w, b, dy = data((3, 200, 64), dtype, 18)
     compare((x.float() * 1e-5 + 3e-5).to(dtype), w, b, 8, "none", dy)
     compare((x.float() * 1e-5 + 3e-5).repeat(1, 40, 1).to(dtype), w, b, 1, "none", dy.repeat(1, 40, 1))
+
+
+@pytest.mark.parametrize("shape,groups", [((4500, 1, 40), 5), ((8209, 3, 24), 2), ((5003, 1, 2000), 250), ((33001, 2, 6), 6),
+                                          ((2100, 1, 5000), 1), ((9001, 1, 7), 1), ((4097, 40, 8), 1)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_many_samples_of_few_rows(shape, groups, dtype):
+    """Samples share a workgroup, the last one has fewer, and a sample's NaN stays in it."""
+    x, w, b, dy = data(shape, dtype, 31, shift=0.3)
+    got = compare(x, w, b, groups, "silu", dy)
+    at = shape[0] - 2
+    x[at, 0, -1] = float("nan")
+    bad = run(x, w, b, groups, "silu", dy)
+    k = shape[2] // groups
+    for name in ("y", "dx"):
+        assert bad[name][at, :, -k:].isnan().all(), name
+        rest = torch.ones(shape, dtype=torch.bool, device="cuda")
+        rest[at, :, -k:] = False
+        assert torch.equal(bad[name][rest], got[name][rest]), name
+    for name in ("dw", "db"):
+        assert bad[name][-k:].isnan().all() and torch.equal(bad[name][:-k], got[name][:-k]), name
