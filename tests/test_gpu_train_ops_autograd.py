@@ -1,0 +1,134 @@
+"""The training operators as nodes of an autograd graph: what autograd lets a user do with a node gives the same bits as the
+plain call, or an error."""
+import threading
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def cases():
+    from pointnetgpd_amd.train_ops import group_norm_act, linear_cross_entropy
+    g = torch.Generator(device="cuda").manual_seed(4)
+    r = lambda *s: torch.randn(*s, generator=g, device="cuda")
+    y = torch.randint(0, 300, (600,), generator=g, device="cuda")
+    y[::7] = -100
+    norm = lambda x, w, b: group_norm_act(x, 4, w, b, act="silu")
+    return {"norm": (norm, (r(5, 70, 24), r(24), r(24)), r(5, 70, 24)),
+            "norm_split": (norm, (r(1, 20000, 64), r(64), r(64)), r(1, 20000, 64)),
+            "loss": (lambda x, w, b: linear_cross_entropy(x, w, y, bias=b), (r(600, 40), r(300, 40), r(300)), r(1)[0]),
+            "loss_rows": (lambda x, w, b: linear_cross_entropy(x, w, y[:9], bias=b, reduction="none", label_smoothing=0.1),
+                          (r(9, 40), r(300, 40), r(300)), r(9))}
+
+
+NAMES = ("norm", "norm_split", "loss", "loss_rows")
+
+
+def leaves(ts):
+    return [t.clone().requires_grad_() for t in ts]
+
+
+def plain(fn, ts, up):
+    ls = leaves(ts)
+    out = fn(*ls)
+    return out.detach(), torch.autograd.grad(out, ls, up)
+
+
+def same(a, b):
+    assert len(a) == len(b) and all(torch.equal(u, v) for u, v in zip(a, b))
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_twice_through_one_graph(name):
+    fn, ts, up = cases()[name]
+    want = plain(fn, ts, up)[1]
+    ls = leaves(ts)
+    out = fn(*ls)
+    same(torch.autograd.grad(out, ls, up, retain_graph=True), want)
+    same(torch.autograd.grad(out, ls, up, retain_graph=True), want)
+    same(torch.autograd.grad(out, ls[1:], up), want[1:])
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_create_graph(name):
+    """First derivatives as ever; differentiating them again is an error, not a silent zero."""
+    fn, ts, up = cases()[name]
+    want = plain(fn, ts, up)[1]
+    ls = leaves(ts)
+    got = torch.autograd.grad(fn(*ls), ls, up, create_graph=True)
+    same([t.detach() for t in got], want)
+    with pytest.raises(RuntimeError):
+        sum(t.sum() for t in got).backward()
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_saved_tensors_moved_by_hooks(name):
+    """Offloaded to the host and brought back elsewhere on the device."""
+    fn, ts, up = cases()[name]
+    want = plain(fn, ts, up)[1]
+    ls = leaves(ts)
+    with torch.autograd.graph.save_on_cpu():
+        out = fn(*ls)
+    hold = [torch.full_like(t, float("nan")) for t in ts]                # the addresses differ
+    same(torch.autograd.grad(out, ls, up), want)
+    del hold
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_checkpoint(name):
+    from torch.utils.checkpoint import checkpoint
+    fn, ts, up = cases()[name]
+    want = plain(fn, ts, up)[1]
+    ls = leaves(ts)
+    same(torch.autograd.grad(checkpoint(fn, *ls, use_reentrant=False), ls, up), want)
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_input_changed_in_place_is_refused(name):
+    fn, ts, up = cases()[name]
+    ls = leaves(ts)
+    out = fn(*ls)
+    with torch.no_grad():
+        ls[0].mul_(2.0)
+    with pytest.raises(RuntimeError, match="inplace"):
+        torch.autograd.grad(out, ls, up)
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_two_threads_share_a_graph(name):
+    fn, ts, up = cases()[name]
+    want = plain(fn, ts, up)[1]
+    ls = leaves(ts)
+    out = fn(*ls)
+    torch.cuda.synchronize()
+    got, errors = [None] * 4, []
+
+    def work(i):
+        try:
+            for _ in range(5):
+                got[i] = torch.autograd.grad(out, ls, up, retain_graph=True)
+        except Exception as e:                                           # reported by the main thread
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    torch.cuda.synchronize()
+    assert not errors, errors
+    for g in got:
+        same(g, want)
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_forward_under_no_grad_and_detached_inputs(name):
+    fn, ts, up = cases()[name]
+    want = plain(fn, ts, up)[0]
+    with torch.no_grad():
+        out = fn(*leaves(ts))
+    assert not out.requires_grad and torch.equal(out, want)
+    with torch.inference_mode():
+        assert torch.equal(fn(*ts), want)
+    ls = leaves(ts)
+    got = torch.autograd.grad(fn(ls[0].detach(), ls[1], ls[2].detach()), ls[1], up)
+    same(got, plain(fn, ts, up)[1][1:2])
