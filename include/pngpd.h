@@ -496,7 +496,7 @@ int pngpd_adam_flat_clip(float *p, const float *g, float *m, float *v, const lon
  * Rows' channels adjacent; ldx, ldw in elements, any (rows at 16-byte addresses of whole 16 bytes are read in place,
  * others are copied into the workspace first).  A target outside [0,V) that is not ignore_index gives a NaN loss and NaN
  * gradients.  Deterministic.  The workspace is bounded in V (a piece's gradient of the logits, 256 MB at most unless 256
- * classes of all rows take more).
+ * classes of all rows take more).  T and V below 2^30, D up to 2^22.
  *   forward   writes stat (T,2), kept (1) and rows (pngpd_lce_rows_ints(T) values, NULL where that is 0: the list of the
  *             rows that are not ignored), which the backward call reads, and loss: (T), or one value
  *   backward  reads dloss (T, or one value); dx (T,D), dw (V,D), db (V) contiguous, each NULL: not wanted             */

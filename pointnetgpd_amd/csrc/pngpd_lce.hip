@@ -14,6 +14,10 @@
 // the device, and the workgroups past them leave.
 // float16 holds g times 2^15 (|g| <= 1: below 65504, and its normal range then reaches down to 2e-9, under 1/V); the
 // coefficients c_t are scaled to at most 1 the same way; both factors come back in float32 on the way out.
+// Measured (bf16; a large library product reaches 1250 TFLOP/s on this card): 6,550 kept rows of 8192, D 1024, V 100,000: statistics
+// 1.33 ms = 1010 TFLOP/s; of each of 7 pieces g 222 us = 860, dx's product 224 us = 860, dW's 208 us = 920, db 28 us: 5.9 ms in
+// all.  No LDS bank conflict; of the statistics' time the epilogue is 17 %, rows a power of two apart cost 12 % (1088
+// elements apart 1467 us in place of 1660, all rows).  64 rows, D 256, V 6500, float32: eight launches of 3 to 13 us.
 #include "pngpd_lce_gemm.h"
 
 #define LCE_PIECE_BYTES (256ll << 20)      // a piece's g
@@ -945,9 +949,12 @@ size_t pngpd_lce_workspace_bytes(const pngpd_lce_t *a, int backward) {
     return lce_bad(a) ? 0 : lce_plan(a, backward != 0).bytes;
 }
 
+// row numbers and places of the kept rows are ints behind one another: 1 + 2 T of them
+static bool lce_too_many(const Lce *a) { return a->D > LCE_MOST_D || a->T >= 1 << 30 || a->V >= 1 << 30; }
+
 int pngpd_lce_fwd(const pngpd_lce_t *a, void *stream) {
     if (lce_bad(a) || !a->loss) return PNGPD_ERR_INVALID_ARG;
-    if (a->D > LCE_MOST_D) return PNGPD_ERR_UNSUPPORTED;
+    if (lce_too_many(a)) return PNGPD_ERR_UNSUPPORTED;
     const LcePlan p = lce_plan(a, false);
     if (!a->workspace || ((uintptr_t)a->workspace & 255) || a->workspace_bytes < p.bytes) return PNGPD_ERR_WORKSPACE;
     hipStream_t st = (hipStream_t)stream;
@@ -958,7 +965,7 @@ int pngpd_lce_fwd(const pngpd_lce_t *a, void *stream) {
 
 int pngpd_lce_bwd(const pngpd_lce_t *a, void *stream) {
     if (lce_bad(a) || !a->dloss || (a->db && !a->bias)) return PNGPD_ERR_INVALID_ARG;
-    if (a->D > LCE_MOST_D) return PNGPD_ERR_UNSUPPORTED;
+    if (lce_too_many(a)) return PNGPD_ERR_UNSUPPORTED;
     if (!a->dx && !a->dw && !a->db) return PNGPD_OK;
     const LcePlan p = lce_plan(a, true);
     if (!a->workspace || ((uintptr_t)a->workspace & 255) || a->workspace_bytes < p.bytes) return PNGPD_ERR_WORKSPACE;

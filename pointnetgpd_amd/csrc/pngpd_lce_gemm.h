@@ -235,7 +235,7 @@ template <int DT, bool AMC, bool BMC, int BM, int BN, int WGM, int WGN, int PIPE
 };
 
 // Workgroup -> tile.  Workgroup i runs on XCD i % 8: each XCD takes a contiguous stretch of a walk over the tiles that
-// goes down bands of 8 n tiles, so the operands of its running workgroups overlap in its own L2.  (i < mt * nt)
+// goes down bands of LCE_BAND n tiles, so the operands of its running workgroups overlap in its own L2.  (i < mt * nt)
 __device__ __forceinline__ void lce_tile_of(int i, int mt, int nt, int &m, int &n) {
     const int per = (mt * nt) >> 3;
     int w = i;

@@ -20,6 +20,7 @@ import ctypes
 import math
 import weakref
 
+import numpy as np
 import torch
 from torch.utils.weak import WeakIdKeyDictionary
 
@@ -133,6 +134,33 @@ def _dense(t):
     return True
 
 
+class _Span:
+    """t's addresses for numpy (which does not read them)."""
+
+    def __init__(self, t):
+        e = t.element_size()
+        self.__array_interface__ = dict(version=3, typestr=f"|V{e}", data=(t.data_ptr(), False), shape=tuple(t.shape),
+                                        strides=tuple(st * e for st in t.stride()))
+
+
+def _share_memory(grads):
+    """Whether two of the gradients, some with gaps, have an element in common (those without are compared by the C call)."""
+    spans = []
+    for g in grads:
+        if g.numel():
+            reach = sum(st * (n - 1) for st, n in zip(g.stride(), g.shape)) + 1
+            spans.append((g.data_ptr(), g.data_ptr() + reach * g.element_size(), _dense(g), g))
+    spans.sort(key=lambda s: s[:2])
+    near = []                                  # those that reach past the start of the one at hand
+    for s in spans:
+        near = [o for o in near if o[1] > s[0]]
+        for o in near:
+            if not (o[2] and s[2]) and np.shares_memory(np.asarray(_Span(o[3])), np.asarray(_Span(s[3]))):
+                return True
+        near.append(s)
+    return False
+
+
 @torch.no_grad()
 def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
     """Clip the gradients of ``parameters`` (a tensor or an iterable of tensors; those without ``.grad`` are passed over)
@@ -161,7 +189,7 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
         if any(g.get_device() >= 0 for g in grads):
             raise RuntimeError("clip_grad_norm_: the gradients are on more than one device")
         return torch.nn.utils.clip_grad_norm_(params, max_norm, norm_type, error_if_nonfinite)
-    work, ptr, num, typ = [], [], [], []
+    work, ptr, num, typ, gaps = [], [], [], [], False
     for g in grads:
         if g.get_device() != index:
             raise RuntimeError("clip_grad_norm_: the gradients are on more than one device")
@@ -173,13 +201,12 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
             if any(st == 0 and k > 1 for st, k in zip(g.stride(), g.shape)):
                 raise RuntimeError("clip_grad_norm_: a gradient's elements share memory (an expanded tensor)")
             if not _dense(g):              # gaps (a column of a wider buffer): clipped in a copy and written back
-                if any(g is o for o in grads[:len(work)]):
-                    raise RuntimeError("clip_grad_norm_: two of the gradients share memory (a parameter listed twice?)")
-                work.append(g := g.contiguous())
-                ptr.append(g.data_ptr()); num.append(g.numel()); typ.append(t)
-                continue
+                g = g.contiguous()
+                gaps = True
         work.append(g)
         ptr.append(g.data_ptr()); num.append(g.numel()); typ.append(t)
+    if gaps and _share_memory(grads):
+        raise RuntimeError("clip_grad_norm_: two of the gradients share memory (a parameter listed twice?)")
     n, dev = len(work), grads[0].device
     lib = _lib.load()
     total = torch.empty((), device=dev, dtype=torch.float32)

@@ -288,8 +288,8 @@ def linear_cross_entropy(x, weight, target, bias=None, reduction="mean", ignore_
     _dtype(x, "linear_cross_entropy: x")
     if bias is not None and bias.dtype not in (x.dtype, torch.float32):
         raise RuntimeError(f"linear_cross_entropy: bias must be of x's type ({x.dtype}) or float32, got {bias.dtype}")
-    if max(V, target.numel()) >= 2 ** 31 - 256 or D > 2 ** 22:
-        raise RuntimeError("linear_cross_entropy: more than 2^31 - 257 rows or classes, or 2^22 channels")
+    if max(V, target.numel()) >= 2 ** 30 or D > 2 ** 22:
+        raise RuntimeError("linear_cross_entropy: more than 2^30 - 1 rows or classes, or 2^22 channels")
     rows = [v if (v.shape[1] == 1 or v.stride(1) == 1) and (v.shape[0] == 1 or v.stride(0) >= v.shape[1]) else v.contiguous()
             for v in (x.reshape(-1, D), weight)]
     if bias is not None and not bias.is_contiguous():

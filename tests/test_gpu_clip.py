@@ -295,3 +295,23 @@ def test_classifier_step_eager_and_graphed():
         torch.cuda.synchronize()
         assert torch.equal(l0.detach(), l1) and torch.equal(o0.grad_norm, o1.grad_norm) and o0.grad_norm > 0.05
         assert torch.equal(o0.flat_p, o1.flat_p)
+
+
+def test_gradients_with_gaps_that_overlap():
+    """Views of one buffer as other tensor objects: refused before anything is written; columns that are apart are clipped."""
+    from pointnetgpd_amd.optim import clip_grad_norm_
+    buf = torch.randn(50, 9, device="cuda")
+    want = buf.clone()
+    ps = [torch.nn.Parameter(torch.zeros(50, device="cuda")) for _ in range(2)]
+    ps[0].grad, ps[1].grad = buf[:, 4], buf[:, 4]
+    with pytest.raises(RuntimeError, match="share memory"):
+        clip_grad_norm_(ps, 0.1)
+    assert torch.equal(buf, want)
+    ps[1].grad = buf[:, 5]
+    norm = clip_grad_norm_(ps, 0.1)
+    exact = want[:, 4:6].double().norm()
+    assert abs(norm.double() - exact) <= 2.0 ** -23 * exact
+    keep = [0, 1, 2, 3, 6, 7, 8]
+    assert torch.equal(buf[:, keep], want[:, keep])
+    scaled = want[:, 4:6].double() * (0.1 / (exact + 1e-6))             # the factor and the product are rounded once each, the norm too
+    assert ((buf[:, 4:6].double() - scaled).abs() <= 2.0 ** -22 * scaled.abs()).all()

@@ -156,6 +156,7 @@ def test_loss_entries_check_their_arguments():
             assert call(**bad) == INV, bad
         assert call(workspace=None) == WS and call(workspace_bytes=16) == WS and call(workspace=264) == WS
         assert call(D=(1 << 22) + 8, ldx=1 << 23, ldw=1 << 23) == 3
+        assert call(T=1 << 30, rows=256) == call(V=1 << 30) == 3
     assert call(db=256) == INV                                                                  # a gradient of no bias
     assert lib.pngpd_lce_rows_ints(511) == 0 and lib.pngpd_lce_rows_ints(512) == 1025
     a = args(T=0)
@@ -171,3 +172,19 @@ def test_command_refuses_a_negative_clip():
     from pointnetgpd_amd import mains
     with pytest.raises(SystemExit, match="clip-grad"):
         mains.run("1v", ["--mode", "train", "--clip-grad", "-1"])
+
+
+def test_gradients_with_gaps_that_share_memory():
+    """The host's check: interleaved columns are apart, overlapping ones and a column of a listed buffer are not."""
+    from pointnetgpd_amd.optim import _share_memory
+    for dt in (torch.float32, torch.bfloat16):
+        buf, other = torch.zeros(40, 12, dtype=dt), torch.zeros(7, dtype=dt)
+        assert not _share_memory([buf[:, k] for k in range(12)] + [other])
+        assert not _share_memory([buf[:, :5], buf[:, 5:8], buf[:, 9:], buf[3, 8:9], other[:0]])
+        assert not _share_memory([buf[::2, :5], buf[1::2, 2:7], buf[::2, 5:], buf[1::2, 7:]])
+        assert _share_memory([buf[:, 3], other, buf[:, 3]])
+        assert _share_memory([buf[:, :5], buf[:, 4:8]])
+        assert _share_memory([buf, buf[7:, 2]])
+        assert _share_memory([other, buf[:, 6], buf[11]])
+        wide = buf.view(20, 24)[:, ::5].t()                 # columns 0, 5, 10 of the even rows, 3 and 8 of the odd ones
+    assert _share_memory([wide, buf[::3, 1:4]]) and not _share_memory([wide, buf[::3, 1:3]])
