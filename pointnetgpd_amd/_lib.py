@@ -302,6 +302,17 @@ def raw_stream(device):
     return torch._C._cuda_getCurrentRawStream(device.index)
 
 
+def call_on(device, fn, *args):
+    """``fn(*args, stream)`` with ``device`` current and its current stream: ``device_guard`` and ``raw_stream`` without the
+    Python calls of a context that is not needed (5 us of a small operator's 60)."""
+    import torch
+    index = device.index
+    if torch._C._cuda_getDevice() == index:
+        return fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    with torch.cuda.device(device):
+        return fn(*args, torch._C._cuda_getCurrentRawStream(index))
+
+
 def check(code, what):
     if code != 0:
         msg = load().pngpd_strerror(code).decode()

@@ -30,7 +30,7 @@ def _dtype(t, name):
 def _bytes(dev, n):
     """Workspace of one call.  Taken from the caching allocator each time, never kept: two captured graphs must not
     share one, and the allocator orders its reuse by stream."""
-    return torch.empty(max(int(n), 1), device=dev, dtype=torch.uint8)
+    return torch.empty(n, device=dev, dtype=torch.uint8)
 
 
 def _same_device(ref, name, *others):
@@ -44,7 +44,8 @@ def _same_device(ref, name, *others):
 # The backward passes run on autograd's own thread, often on a far core: the same Python costs up to four times there what it
 # costs in the forward pass.  So what a backward call needs besides addresses and strides is settled in the forward pass, and
 # its node enters no context that it does not need (forward + backward of 64 rows against 6500 classes 175 -> 155 us with the
-# thread on a far core, 102 -> 93 on a near one; a small group norm 134 -> 125 and 67 -> 65).
+# thread on a far core, 102 -> 93 on a near one; a small group norm 134 -> 125 and 67 -> 65; without the context that
+# call_on spares, 147 and 118 on a far core).
 def _once(backward):
     """``once_differentiable(backward)`` where the call itself may be differentiated (create_graph), else ``backward``."""
     guarded = once_differentiable(backward)
@@ -54,10 +55,10 @@ def _once(backward):
 def _gn_call(fn, entry, dev, dims, nbytes, x, w, b, *ptrs):
     """One C call; ``dims``: see ``_gn_dims``; ``ptrs``: the pointers between act and the workspace."""
     dt, B, N, C, groups, wdt, eps, act = dims
-    ws = _bytes(dev, nbytes).data_ptr() if nbytes else None      # (freed on return: the stream orders its next user)
-    with _lib.device_guard(dev):
-        code = fn(x.data_ptr(), dt, B, N, C, x.stride(0), x.stride(1), groups, None if w is None else w.data_ptr(),
-                  None if b is None else b.data_ptr(), wdt, eps, act, *ptrs, ws, nbytes, _lib.raw_stream(dev))
+    ws = _bytes(dev, nbytes) if nbytes else None      # held until the launches are queued: another thread may allocate meanwhile
+    sB, sN, _ = x.stride()
+    code = _lib.call_on(dev, fn, x.data_ptr(), dt, B, N, C, sB, sN, groups, None if w is None else w.data_ptr(),
+                        None if b is None else b.data_ptr(), wdt, eps, act, *ptrs, None if ws is None else ws.data_ptr(), nbytes)
     if code:
         _lib.check(code, entry)
 
@@ -181,8 +182,7 @@ def _lce_call(fn, entry, a, nbytes, dev):
     """One C call on ``dev`` and its current stream with a workspace of its own."""
     ws = _bytes(dev, nbytes)
     a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes
-    with _lib.device_guard(dev):
-        code = fn(ctypes.addressof(a), _lib.raw_stream(dev))
+    code = _lib.call_on(dev, fn, ctypes.addressof(a))
     if code:
         _lib.check(code, entry)
 

@@ -132,3 +132,23 @@ def test_forward_under_no_grad_and_detached_inputs(name):
     ls = leaves(ts)
     got = torch.autograd.grad(fn(ls[0].detach(), ls[1], ls[2].detach()), ls[1], up)
     same(got, plain(fn, ts, up)[1][1:2])
+
+
+def test_threads_on_one_stream():
+    """Calls of four threads on one stream, each with its own inputs: the workspace of a call is its own until it is queued."""
+    fns = [cases()[n] for n in ("norm_split", "loss", "norm_split", "norm")]
+    wants = [plain(*c) for c in fns]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        fn, ts, up = fns[i]
+        for _ in range(30):
+            out, grads = plain(fn, ts, up)
+            if not (torch.equal(out, wants[i][0]) and all(torch.equal(u, v) for u, v in zip(grads, wants[i][1]))):
+                bad.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not bad, bad
