@@ -16,8 +16,9 @@
 // coefficients c_t are scaled to at most 1 the same way; both factors come back in float32 on the way out.
 // Measured (bf16; a large library product reaches 1250 TFLOP/s on this card): 6,550 kept rows of 8192, D 1024, V 100,000: statistics
 // 1.33 ms = 1010 TFLOP/s; of each of 7 pieces g 222 us = 860, dx's product 224 us = 860, dW's 208 us = 920, db 28 us: 5.9 ms in
-// all.  No LDS bank conflict; of the statistics' time the epilogue is 17 %, rows a power of two apart cost 12 % (1088
-// elements apart 1467 us in place of 1660, all rows).  64 rows, D 256, V 6500, float32: eight launches of 3 to 13 us.
+// all.  No LDS bank conflict; of the statistics' time the epilogue is 17 %; rows of x or W other than a power of two apart
+// change nothing (1480 us at 1024 and at 1088 elements, all rows).  64 rows, D 256, V 6500, float32: eight launches of 3 to
+// 13 us.
 #include "pngpd_lce_gemm.h"
 
 #define LCE_PIECE_BYTES (256ll << 20)      // a piece's g
