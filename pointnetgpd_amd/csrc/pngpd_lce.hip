@@ -19,9 +19,12 @@
 // all.  No LDS bank conflict; of the statistics' time the epilogue is 17 %; rows of x or W other than a power of two apart
 // change nothing (1480 us at 1024 and at 1088 elements, all rows).  64 rows, D 256, V 6500, float32: eight launches of 3 to
 // 13 us.
+#include <algorithm>
+
 #include "pngpd_lce_gemm.h"
 
 #define LCE_PIECE_BYTES (256ll << 20)      // a piece's g
+#define LCE_PIECE_MOST (1ll << 30)         // where a round of dW's large tiles over the CUs takes more
 
 #define LCE_ROWS 512                       // below, dropping rows does not drop enough tiles to pay for the list's launch
 #define LOG2E 1.44269504088896340736f
@@ -734,9 +737,8 @@ static int lce_cut(int n, int other) {
 
 struct LcePlan {
     int Dp, fshape, fmt, fcut, padx, padw;
-    int piece, ldg, gshape, xshape, splits, wshape;
+    int piece, large, ldg, xshape, splits; // classes of a piece, at most of the last one
     int share, shares;                     // db: rows of a share, shares
-    long long kper;
     size_t o_part, o_ps, o_zt, o_row, o_x, o_w, o_coef, o_scale, o_g, o_dx, o_db, bytes;
 };
 
@@ -763,23 +765,26 @@ static LcePlan lce_plan(const Lce *a, bool bwd) {
         p.o_x = take((size_t)a->T * p.Dp * es);
         p.o_coef = take((size_t)a->T * 4);
         p.o_scale = take(4);
-        // a piece: g of at most LCE_PIECE_BYTES, at least 256 classes, pieces of one size
-        long long most = LCE_PIECE_BYTES / ((long long)a->T * es) / 256 * 256;
-        if (most < 256) most = 256;
-        const long long n = ((long long)a->V + most - 1) / most;
-        p.piece = (int)((((long long)a->V + n - 1) / n + 255) / 256 * 256);
-        p.ldg = p.piece + (es == 2 ? 128 : 64);
-        p.gshape = lce_shape(p.piece, a->T);
+        // a piece: g of at most LCE_PIECE_BYTES, at least 256 classes; pieces whose dW is whole rounds of the large tile over
+        // the CUs (up to a quarter of one more in the last), or of one size where not even one round fits (8192 rows, a fifth
+        // of them ignored, 100,000 classes, D 1024: PIECENEW us, and 5930 in seven pieces of 224 tiles)
+        long long most = LCE_PIECE_BYTES / ((long long)a->T * es) / 256;
+        if (most < 1) most = 1;
+        const long long across_d = lce_cdiv(p.Dp, 256), fit = 256 / across_d;
+        if (most < fit && (long long)a->T * fit * 256 * es <= LCE_PIECE_MOST) most = fit;
+        const long long rounds = most * across_d / 256;
+        const long long tiles_v = lce_cdiv(a->V, 256), n = (tiles_v + most - 1) / most;
+        p.piece = (int)(n == 1 || !rounds ? (tiles_v + n - 1) / n : std::max(1ll, 256 * rounds / across_d)) * 256;
+        const int rest = a->V % p.piece;
+        p.large = a->V > p.piece && rest < p.piece / 4 ? p.piece + (rest + 255) / 256 * 256 : p.piece;
+        p.ldg = p.large + (es == 2 ? 128 : 64);
         p.o_g = take((size_t)a->T * p.ldg * es);
-        p.wshape = (long long)lce_cdiv(p.Dp, 256) * lce_cdiv(p.piece, 256) >= 192 ? 0 : 1;
         // dx: few tiles and a long k: cut k until there are about 512 workgroups, of at least 256 classes
         p.xshape = a->T <= 32 ? 2 : a->T >= 128 && p.Dp >= 256 ? 0 : 1;
         const long long tiles = (long long)lce_cdiv(p.Dp, LCE_BM[p.xshape]) * lce_cdiv(a->T, LCE_BN[p.xshape]);
         long long s = (p.xshape == 0 ? 256 : 512) / tiles;
         if (s > p.piece / 256) s = p.piece / 256;
-        if (s < 1) s = 1;
-        p.kper = (((long long)p.piece + s - 1) / s + 63) / 64 * 64;
-        p.splits = (int)(((long long)p.piece + p.kper - 1) / p.kper);
+        p.splits = s < 1 ? 1 : (int)s;
         p.o_dx = take((size_t)p.splits * a->T * p.Dp * 4);
         // db: about 1024 workgroups
         const long long across = lce_cdiv(p.piece, es == 4 ? 32 : 64);
@@ -893,12 +898,13 @@ template <int DT> static int lce_backward(const Lce *a, const LcePlan &p, hipStr
     if (p.padw) { lce_copy<DT>(a, a->w, a->ldw, a->V, 0, k.rows, ws + p.o_w, st); k.w = LceOperand{ws + p.o_w, p.Dp}; }
     k.D = p.Dp;
     k.stat = a->stat; k.coef = coef; k.ldg = p.ldg;
-    for (int v0 = 0; v0 < a->V; v0 += p.piece) {
-        const int vc = a->V - v0 < p.piece ? a->V - v0 : p.piece;
+    for (int v0 = 0, vc; v0 < a->V; v0 += vc) {
+        vc = a->V - v0 <= p.large ? a->V - v0 : p.piece;
+        const int gshape = lce_shape(vc, a->T), wshape = (long long)lce_cdiv(p.Dp, 256) * lce_cdiv(vc, 256) >= 192 ? 0 : 1;
         const int cols = (vc + 63) / 64 * 64;                      // columns of g that are written (zeros past vc)
-        const int gcut = p.gshape ? vc : lce_cut(vc, lce_cdiv(a->T, 256));
+        const int gcut = gshape ? vc : lce_cut(vc, lce_cdiv(a->T, 256));
         k.v0 = v0; k.vc = gcut; k.g = ws + p.o_g;
-        int rc = lce_z<DT, true>(k, p.gshape, st);
+        int rc = lce_z<DT, true>(k, gshape, st);
         if (rc) return rc;
         if (gcut < vc) {
             k.v0 = v0 + gcut; k.vc = vc - gcut; k.g = (E *)(ws + p.o_g) + gcut;
@@ -917,12 +923,12 @@ template <int DT> static int lce_backward(const Lce *a, const LcePlan &p, hipStr
         if (a->dx) {
             LceOut o = {};
             o.a = LceOperand{w, k.w.ld}; o.b = LceOperand{g, p.ldg}; o.rows = k.rows;
-            o.M = p.Dp; o.N = -1; o.mo = a->D; o.no = a->T; o.K = vc; o.kper = p.kper; o.splits = p.splits;
+            o.M = p.Dp; o.N = -1; o.mo = a->D; o.no = a->T; o.K = vc; o.kper = ((long long)vc + 64 * p.splits - 1) / (64 * p.splits) * 64; o.splits = p.splits;
             o.part = part; o.add = v0 > 0; o.scale = scale;
             if ((rc = lce_out<DT, false>(o, p.xshape, st))) return rc;
         }
         if (a->dw) {
-            const int wcut = p.wshape ? vc : lce_cut(vc, lce_cdiv(p.Dp, 256));
+            const int wcut = wshape ? vc : lce_cut(vc, lce_cdiv(p.Dp, 256));
             for (int c0 = 0; c0 < vc; c0 = c0 ? vc : wcut) {       // the large tile's classes, then the rest
                 const int c1 = c0 ? vc : wcut;
                 LceOut o = {};
@@ -930,7 +936,7 @@ template <int DT> static int lce_backward(const Lce *a, const LcePlan &p, hipStr
                 o.M = p.Dp; o.N = (c1 == vc ? cols : c1) - c0; o.mo = a->D; o.no = c1 - c0; o.K = -1; o.kper = a->T; o.splits = 1;
                 o.out = (E *)a->dw + (long long)(v0 + c0) * a->D; o.ldo = a->D; o.scale = scale;
                 o.vec = (a->D * (long long)sizeof(E)) % 16 == 0 && !((uintptr_t)a->dw & 15);
-                if ((rc = lce_out<DT, true>(o, c0 ? 1 : p.wshape, st))) return rc;
+                if ((rc = lce_out<DT, true>(o, c0 ? 1 : wshape, st))) return rc;
             }
         }
     }

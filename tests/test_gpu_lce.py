@@ -123,6 +123,13 @@ def test_pieces():
     compare(*args, reduction="none", smooth=0.1)
 
 
+@pytest.mark.parametrize("T,D,V,dtype", [(8192, 1000, 17300, BF16), (8192, 1000, 22400, F16), (4096, 1024, 40000, F32),
+                                         (9000, 300, 70000, BF16)])
+def test_pieces_of_whole_rounds(T, D, V, dtype):
+    """The last piece a little larger than the others, a good deal smaller, and pieces of one size."""
+    compare(*data(T, D, V, dtype, 12), reduction="none", smooth=0.0)
+
+
 def test_rows_far_apart():
     """Rows whose last lies over 4 GiB from the first: no lane's offset may wrap, picked out of all rows or copied."""
     T, D, ld = 1030, 64, 2_100_000
