@@ -99,7 +99,8 @@ def compare(x, w, b, y, c, reduction="mean", smooth=0.0, ignore=-100):
 
 # (T, D, V): single rows, classes and channels; odd channels (copied rows); tiles' edges; the large tiles; cut sums
 SHAPES = [(1, 1, 2), (1, 256, 6500), (2, 8, 1), (3, 17, 5), (33, 40, 65), (64, 256, 6500), (31, 250, 999), (130, 129, 777),
-          (257, 64, 1000), (1000, 96, 9000), (2500, 264, 4097), (5, 1024, 30001), (4097, 48, 2050), (300, 520, 20000)]
+          (257, 64, 1000), (1000, 96, 9000), (2500, 264, 4097), (5, 1024, 30001), (4097, 48, 2050), (300, 520, 20000),
+          (500, 760, 8150), (1030, 300, 12100)]
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
