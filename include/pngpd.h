@@ -490,15 +490,18 @@ int pngpd_adam_flat_clip(float *p, const float *g, float *m, float *v, const lon
                          const float *step_dev, float gscale, const float *gdiv_dev, float max_norm, float *total_norm,
                          void *workspace, size_t workspace_bytes, void *stream);
 
-/* Softmax cross entropy of a linear classifier, z = x W^T + bias, whose logits are never kept:
+/* Softmax cross entropy of a linear classifier, z = x W^T + bias, for any number of classes:
  *   loss_t = log sum_v exp(z[t,v]) - (1 - smoothing) z[t,target_t] - smoothing mean_v z[t,v],  0 where target_t is ignore_index
  * (F.nll_loss(F.log_softmax(F.linear(x, W, bias))), main_1v.py:73-74 with pointnet.py:193-194, for a head of any width).
  * Rows' channels adjacent; ldx, ldw in elements, any (rows at 16-byte addresses of whole 16 bytes are read in place,
  * others are copied into the workspace first).  A target outside [0,V) that is not ignore_index gives a NaN loss and NaN
- * gradients.  Deterministic.  The workspace is bounded in V (a piece's gradient of the logits, 256 MB at most unless 256
- * classes of all rows take more).  T and V below 2^30, D up to 2^22.
+ * gradients.  Deterministic.  The workspace is bounded in V: a piece's gradient of the logits, 256 MB at most unless 256
+ * classes of all rows take more, or up to 1 GB where that lets dW's product fill the CUs.  T and V below 2^30, D up to 2^22.
  *   forward   writes stat (T,2), kept (1) and rows (pngpd_lce_rows_ints(T) values, NULL where that is 0: the list of the
- *             rows that are not ignored), which the backward call reads, and loss: (T), or one value
+ *             rows that are not ignored), which the backward call reads, and loss: (T), or one value; and z, where it is
+ *             not NULL (pngpd_lce_z_bytes of room, 0: must be NULL): the logits in float32, only where reading them again
+ *             costs less than computing them again, which the backward call does where z is NULL, and at most 1 GB (float32
+ *             inputs; 256 MB otherwise)
  *   backward  reads dloss (T, or one value); dx (T,D), dw (V,D), db (V) contiguous, each NULL: not wanted             */
 typedef struct pngpd_lce {
     const void *x, *w, *bias;      /* (T,D), (V,D) of dtype; (V) of bias_dtype (= dtype or PNGPD_F32), NULL: none  */
@@ -508,12 +511,14 @@ typedef struct pngpd_lce {
     float smoothing;
     float *stat, *kept, *loss;
     int *rows;
+    float *z;                      /* 16-byte aligned                                                              */
     const float *dloss;
     void *dx, *dw, *db;
     void *workspace;               /* 256-byte aligned; pngpd_lce_workspace_bytes of the same descriptor           */
     size_t workspace_bytes;
 } pngpd_lce_t;
 size_t pngpd_lce_rows_ints(int T);
+size_t pngpd_lce_z_bytes(int T, int D, int V, int dtype);
 size_t pngpd_lce_workspace_bytes(const pngpd_lce_t *a, int backward);
 int pngpd_lce_fwd(const pngpd_lce_t *a, void *stream);
 int pngpd_lce_bwd(const pngpd_lce_t *a, void *stream);

@@ -61,7 +61,7 @@ class LceArgs(ctypes.Structure):
     """``pngpd_lce_t`` of include/pngpd.h."""
     _fields_ = ([(n, _P) for n in ("x", "w", "bias", "target")] + [(n, ctypes.c_int64) for n in ("ldx", "ldw", "ignore_index")] +
                 [(n, _I) for n in ("T", "D", "V", "dtype", "bias_dtype", "reduction")] + [("smoothing", _F)] +
-                [(n, _P) for n in ("stat", "kept", "loss", "rows", "dloss", "dx", "dw", "db", "workspace")] + [("workspace_bytes", _Z)])
+                [(n, _P) for n in ("stat", "kept", "loss", "rows", "z", "dloss", "dx", "dw", "db", "workspace")] + [("workspace_bytes", _Z)])
 
 
 # name -> (restype, argtypes); mirrors include/pngpd.h one-to-one (checked by tests).
@@ -160,6 +160,7 @@ SIGNATURES = {
     "pngpd_adam_step_inc": (ctypes.c_int, [c_void, c_void]),
     # ---- gradient clipping, group norm + activation, linear cross entropy
     "pngpd_lce_rows_ints": (ctypes.c_size_t, [ctypes.c_int]),
+    "pngpd_lce_z_bytes": (ctypes.c_size_t, [ctypes.c_int] * 4),
     "pngpd_lce_workspace_bytes": (ctypes.c_size_t, [c_void, ctypes.c_int]),
     "pngpd_lce_fwd": (ctypes.c_int, [c_void, c_void]),
     "pngpd_lce_bwd": (ctypes.c_int, [c_void, c_void]),

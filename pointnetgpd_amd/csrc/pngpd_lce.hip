@@ -1,4 +1,4 @@
-// Linear + softmax cross entropy over many classes, the logits never kept, with its gradient.
+// Linear + softmax cross entropy over many classes, the logits not kept (but for few of them: lce_keeps), with its gradient.
 //
 //   z = x W^T + b  (T,V)     m_t = max_v z     s_t = sum_v exp(z - m_t)     lse_t = m_t + log s_t
 //   loss_t = lse_t - (1 - e) z[t, y_t] - e mean_v z          (0 where y_t = ignore_index)
@@ -9,7 +9,8 @@
 // tiles of a row.  Backward: z is computed again, a piece of the vocabulary at a time; the piece's g (rounded once to the
 // inputs' type, as the operand of the matrix instructions has to be) lives in a workspace of bounded size, and two products
 // turn it into the piece's dW and its share of dx.  8 T D V operations for both directions where keeping T V logits takes
-// 6: the price of not keeping them.  Bound by the matrix cores for T in the hundreds and above, by reading W below.
+// 6: the price of not keeping them, which pays for 16 bits; float32's matrix rate makes keeping them the better way, up to 1 GB.
+// Bound by the matrix cores for T in the hundreds and above, by reading W below.
 // Rows whose target is ignored are left out of the products (from LCE_ROWS rows on): a list of the kept ones is made on
 // the device, and the workgroups past them leave.
 // float16 holds g times 2^15 (|g| <= 1: below 65504, and its normal range then reaches down to 2e-9, under 1/V); the
@@ -51,6 +52,8 @@ struct LceArgs {
     float smooth;
     float *pm, *ps, *zt;                   // forward: (mt,T,2) max / sum, (mt,T) sum of z, (T) z at the target
     const float *stat, *coef;              // backward: (T,2) max / sum, (T)
+    float *z;                              // (T, ldz) the logits kept for the backward pass, or NULL
+    int ldz;
     void *g;
     int v0, vc, ldg;                       // the launch's classes (g starts at the first one)
 };                                         // (T above, but for target: by place among the kept rows)
@@ -193,6 +196,18 @@ __global__ __launch_bounds__(WGM * WGN * 64, 2) void lce_stats_kernel(const LceA
 #pragma unroll
         for (int j = 0; j < Core::FN; ++j) {
             const int col = wn + 32 * j + (lane & 31), k = n0 + col, rel = s->rel[col], mine = rel - vl;
+            if constexpr (DT == PNGPD_F32 || BM < 256) {          // (lce_keeps: of 16 bits not with the large tile)
+                if (a.z && k < T) {
+                    float *z = a.z + (size_t)k * a.ldz + a.v0 + m0 + vl;
+#pragma unroll
+                    for (int i = 0; i < Core::FM; ++i) {
+#pragma unroll
+                        for (int q = 0; q < 4; ++q)
+                            *(f32x4 *)(z + 32 * i + 8 * q) = f32x4{c.acc[i][j][4 * q], c.acc[i][j][4 * q + 1],
+                                                                   c.acc[i][j][4 * q + 2], c.acc[i][j][4 * q + 3]};
+                    }
+                }
+            }
             if (__any(mine >= 0 && mine < Core::WM)) {
                 float z = 0.f;
                 bool found = false;                               // (the other half has the other rows of four)
@@ -513,6 +528,27 @@ __global__ __launch_bounds__(WGM * WGN * 64, 2) void lce_grad_kernel(const LceAr
     }
 }
 
+// lce_grad_kernel's epilogue on kept logits: four classes a thread, 1024 of one row a workgroup.
+template <int DT>
+__global__ __launch_bounds__(256) void lce_kept_grad_kernel(const LceArgs a, int cols) {
+    typedef typename elem<DT>::t E;
+    const int per = (cols + 1023) / 1024, k = blockIdx.x / per, v = (blockIdx.x - k * per) * 1024 + threadIdx.x * 4;
+    if (k >= a.rows.count() || v >= cols) return;
+    const float m = a.stat[2 * (size_t)k], co = a.coef[k], ks = co / a.stat[2 * (size_t)k + 1], kf = co * (a.smooth / (float)a.V);
+    const long long y = a.target[a.rows.row(k)] - a.v0;           // (an ignored row's co is 0)
+    const f32x4 z = *(const f32x4 *)(a.z + (size_t)k * a.ldz + a.v0 + v);
+    float g[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const float p = lce_far<DT>(m) ? __builtin_amdgcn_exp2f((z[e] - m) * LOG2E) : __builtin_amdgcn_exp2f(fmaf(z[e], LOG2E, -(m * LOG2E)));
+        g[e] = fmaf(p, ks, -kf) - (y == v + e ? co * (1.f - a.smooth) : 0.f);
+        if (co == 0.f || v + e >= a.vc) g[e] = 0.f;
+    }
+    E *o = (E *)a.g + (size_t)k * a.ldg + v;
+    if constexpr (DT == PNGPD_F32) *(f32x4 *)o = f32x4{g[0], g[1], g[2], g[3]};
+    else *(uint2 *)o = lce_half4<DT>(g[0], g[1], g[2], g[3]);
+}
+
 // db of a piece: column sums of g (as rounded), in two steps.  A thread takes 16 bytes of a row and every 32nd row of the
 // workgroup's share; the shares' sums (S, ldg) in float32, then one thread a class.
 template <int DT>
@@ -810,7 +846,8 @@ static bool lce_bad(const Lce *a) {
     return !a || !a->x || !a->w || !a->target || a->T <= 0 || a->D <= 0 || a->V <= 0 || a->dtype < PNGPD_F32 || a->dtype > PNGPD_F16 ||
            a->ldx < (a->T > 1 ? a->D : 0) || a->ldw < (a->V > 1 ? a->D : 0) || (a->bias_dtype != PNGPD_F32 && a->bias_dtype != a->dtype) ||
            a->reduction < PNGPD_REDUCE_NONE || a->reduction > PNGPD_REDUCE_SUM || !(a->smoothing >= 0.f && a->smoothing <= 1.f) ||
-           !a->stat || !a->kept || !a->rows != !pngpd_lce_rows_ints(a->T);
+           !a->stat || !a->kept || !a->rows != !pngpd_lce_rows_ints(a->T) ||
+           (a->z && (((uintptr_t)a->z & 15) || !pngpd_lce_z_bytes(a->T, a->D, a->V, a->dtype)));
 }
 
 template <class K, class A> static int lce_launch(K kernel, int lds, long long grid, int threads, const A &a, hipStream_t st) {
@@ -856,11 +893,21 @@ static void lce_copy(const Lce *a, const void *src, long long ld, long long R, i
                        mask, rows, (const long long *)a->target, (long long)a->ignore_index, dst, coef);
 }
 
+static inline int lce_ldz(int V) { return (V + 255) / 256 * 256; }
+// Whether the logits are kept, in float32, where they are few: written and read they are 8 bytes a logit at the memory's rate
+// (1.6 ps); computed again 2 D operations at the matrix cores' (float32: 0.014 ps D), or W is read again for few rows (2 D
+// bytes of 16 bits a class).  (Forward + backward, float32, 1024 x 2048 x 12,000: 1369
+// us, computed again 1752; bf16, 200 x 800 x 40,000: 163 and 169.)
+static bool lce_keeps(int T, int D, int V, int dt) {
+    const long long bytes = (long long)T * lce_ldz(V) * 4;
+    return dt == PNGPD_F32 ? D >= 128 && bytes <= LCE_PIECE_MOST : 4ll * T <= D && bytes <= LCE_PIECE_BYTES && lce_shape(V, T) != 0;
+}
 static LceArgs lce_args(const Lce *a) {
     LceArgs k = {};
     k.x = LceOperand{a->x, a->ldx}; k.w = LceOperand{a->w, a->ldw}; k.rows = LceRows{a->rows, a->T};
     k.bias = a->bias; k.bf32 = a->bias_dtype == PNGPD_F32; k.target = (const long long *)a->target; k.ignore = a->ignore_index;
     k.T = a->T; k.D = a->D; k.V = a->V; k.smooth = a->smoothing;
+    k.z = a->z; k.ldz = lce_ldz(a->V);
     return k;
 }
 
@@ -914,9 +961,16 @@ template <int DT> static int lce_backward(const Lce *a, const LcePlan &p, hipStr
         const int cols = (vc + 63) / 64 * 64;                      // columns of g that are written (zeros past vc)
         const int gcut = gshape ? vc : lce_cut(vc, lce_cdiv(a->T, 256));
         k.v0 = v0; k.vc = gcut; k.g = ws + p.o_g;
-        int rc = lce_z<DT, true>(k, gshape, st);
+        int rc;
+        if (a->z) {
+            k.vc = vc;
+            const long long grid = (long long)a->T * ((cols + 1023) / 1024);
+            if (grid > 0x7fffffffll) return PNGPD_ERR_UNSUPPORTED;
+            hipLaunchKernelGGL(lce_kept_grad_kernel<DT>, dim3((unsigned)grid), dim3(256), 0, st, k, cols);
+            rc = pngpd_launch_status();
+        } else rc = lce_z<DT, true>(k, gshape, st);
         if (rc) return rc;
-        if (gcut < vc) {
+        if (!a->z && gcut < vc) {
             k.v0 = v0 + gcut; k.vc = vc - gcut; k.g = (E *)(ws + p.o_g) + gcut;
             if ((rc = lce_z<DT, true>(k, 1, st))) return rc;
         }
@@ -961,6 +1015,11 @@ template <int DT> static int lce_backward(const Lce *a, const LcePlan &p, hipStr
 extern "C" {
 
 size_t pngpd_lce_rows_ints(int T) { return T < LCE_ROWS ? 0 : 2 * (size_t)T + 1; }
+
+size_t pngpd_lce_z_bytes(int T, int D, int V, int dtype) {
+    if (T <= 0 || D <= 0 || V <= 0 || V >= 1 << 30 || dtype < PNGPD_F32 || dtype > PNGPD_F16 || !lce_keeps(T, D, V, dtype)) return 0;
+    return (size_t)T * lce_ldz(V) * 4;
+}
 
 size_t pngpd_lce_workspace_bytes(const pngpd_lce_t *a, int backward) {
     return lce_bad(a) ? 0 : lce_plan(a, backward != 0).bytes;

@@ -4,7 +4,7 @@
                              (PointNetGPD/model/pointnet.py:29-31,144-147) needs two samples a rank and keeps statistics of
                              its replica; this one's are of each sample alone.
 * ``linear_cross_entropy`` — the loss of a linear classifier of any width, F.nll_loss(F.log_softmax(F.linear(...)))
-                             (main_1v.py:73-74, pointnet.py:193-194), without its logits ever being kept: codebooks of
+                             (main_1v.py:73-74, pointnet.py:193-194), without rows x classes of logits in memory: codebooks of
                              grasps, one class for each point of a scene.
 
 CUDA tensors run the HIP kernels of libpngpd (a missing library raises), CPU tensors the same formulas in ATen operations.
@@ -187,31 +187,34 @@ def _lce_call(fn, entry, a, nbytes, dev):
         _lib.check(code, entry)
 
 
-def _lce_args(scalars, x, w, bias, target, stat, rows):
+def _lce_args(scalars, x, w, bias, target, stat, rows, z):
     (T, D), ld = x.shape, [t.stride(0) if t.shape[0] > 1 else t.shape[1] for t in (x, w)]
     dt, at = DTYPES[x.dtype], stat.data_ptr()
     reduction, ignore_index, smoothing = scalars
     return _lib.LceArgs(x=x.data_ptr(), w=w.data_ptr(), bias=None if bias is None else bias.data_ptr(), target=target.data_ptr(),
                         ldx=ld[0], ldw=ld[1], ignore_index=ignore_index, T=T, D=D, V=w.shape[0], dtype=dt,
                         bias_dtype=dt if bias is None else DTYPES[bias.dtype], reduction=reduction, smoothing=smoothing,
-                        stat=at, kept=at + 8 * T, rows=None if rows is None else rows.data_ptr())
+                        stat=at, kept=at + 8 * T, rows=None if rows is None else rows.data_ptr(),
+                        z=None if z is None else z.data_ptr())
 
 
-def _lce_fwd(x, w, bias, target, scalars):
-    """-> loss, what the backward pass reads, the call's arguments."""
+def _lce_fwd(x, w, bias, target, scalars, train):
+    """-> loss, what the backward pass reads (``train``), the call's arguments."""
     lib, dev, T = _lib.load(), x.device, x.shape[0]
     stat = torch.empty(2 * T + 1, device=dev, dtype=torch.float32)             # (T,2), then the kept rows' number
     n = lib.pngpd_lce_rows_ints(T)
     rows = torch.empty(n, device=dev, dtype=torch.int32) if n else None
+    n = lib.pngpd_lce_z_bytes(T, x.shape[1], w.shape[0], DTYPES[x.dtype]) if train else 0
+    z = torch.empty(n // 4, device=dev, dtype=torch.float32) if n else None
     loss = torch.empty((T,) if scalars[0] == 0 else (), device=dev, dtype=torch.float32)
-    a = _lce_args(scalars, x, w, bias, target, stat, rows)
+    a = _lce_args(scalars, x, w, bias, target, stat, rows, z)
     a.loss = loss.data_ptr()
     _lce_call(lib.pngpd_lce_fwd, "pngpd_lce_fwd", a, lib.pngpd_lce_workspace_bytes(ctypes.addressof(a), 0), dev)
-    return loss, stat, rows, a
+    return loss, (stat, rows, z), a
 
 
 def _lce_bwd(ctx, dloss):
-    x, w, bias, target, stat, rows = saved = ctx.saved_tensors
+    x, w, bias, target, stat, rows, z = saved = ctx.saved_tensors
     made, where, nbytes, dev = ctx.call
     need = ctx.needs_input_grad
     if not dloss.is_contiguous():
@@ -219,7 +222,7 @@ def _lce_bwd(ctx, dloss):
     if tuple(0 if t is None else t.data_ptr() for t in saved) == where:
         a = _lib.LceArgs.from_buffer_copy(made)                                # a copy: two threads may run one node
     else:                                                                      # saved tensors that a hook has moved
-        a = _lce_args(ctx.scalars, x, w, bias, target, stat, rows)
+        a = _lce_args(ctx.scalars, x, w, bias, target, stat, rows, z)
         nbytes = _lib.load().pngpd_lce_workspace_bytes(ctypes.addressof(a), 1)
     dx = torch.empty_like(x, memory_format=torch.contiguous_format) if need[0] else None
     dw = torch.empty_like(w, memory_format=torch.contiguous_format) if need[1] else None
@@ -235,8 +238,8 @@ class LinearCrossEntropyFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, w, bias, target, scalars):
-        loss, stat, rows, a = _lce_fwd(x, w, bias, target, scalars)
-        saved = (x, w, bias, target, stat, rows)
+        loss, made, a = _lce_fwd(x, w, bias, target, scalars, True)
+        saved = (x, w, bias, target, *made)
         ctx.scalars = scalars
         ctx.call = (a, tuple(0 if t is None else t.data_ptr() for t in saved),
                     _lib.load().pngpd_lce_workspace_bytes(ctypes.addressof(a), 1), x.device)
@@ -249,7 +252,8 @@ class LinearCrossEntropyFn(torch.autograd.Function):
 def linear_cross_entropy(x, weight, target, bias=None, reduction="mean", ignore_index=-100, label_smoothing=0.0):
     """``F.cross_entropy(F.linear(x, weight, bias), target, ...)`` without the logits: x (..., D), weight (V, D), target
     (...) int64, bias (V) or None.  The forward pass reduces the logits tile by tile, the backward pass computes them again
-    a piece of the classes at a time, so memory grows with the rows and not with rows x classes.
+    a piece of the classes at a time, so memory grows with the rows and not with rows x classes (float32 logits of up to
+    1 GB, and those of a few rows of 16 bits up to 256 MB, are kept for the backward pass: reading them is the faster way).
 
     Returns float32: a scalar for ``reduction`` "mean" (over the rows whose target is not ``ignore_index``; NaN if there is
     none, with zero gradients) or "sum", target's shape for "none".  Ignored rows have loss 0 and no gradient, whatever
@@ -298,5 +302,5 @@ def linear_cross_entropy(x, weight, target, bias=None, reduction="mean", ignore_
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (*rows, bias)):
         loss = LinearCrossEntropyFn.apply(*rows, bias, target_rows, scalars)
     else:
-        loss = _lce_fwd(*rows, bias, target_rows, scalars)[0]
+        loss = _lce_fwd(*rows, bias, target_rows, scalars, False)[0]
     return loss.reshape(target.shape) if reduction == "none" else loss

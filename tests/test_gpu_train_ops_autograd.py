@@ -19,10 +19,13 @@ def cases():
             "norm_split": (norm, (r(1, 20000, 64), r(64), r(64)), r(1, 20000, 64)),
             "loss": (lambda x, w, b: linear_cross_entropy(x, w, y, bias=b), (r(600, 40), r(300, 40), r(300)), r(1)[0]),
             "loss_rows": (lambda x, w, b: linear_cross_entropy(x, w, y[:9], bias=b, reduction="none", label_smoothing=0.1),
-                          (r(9, 40), r(300, 40), r(300)), r(9))}
+                          (r(9, 40), r(300, 40), r(300)), r(9)),
+            "loss_kept": (lambda x, w, b: linear_cross_entropy(x, w, y, bias=b), (r(600, 160), r(300, 160), r(300)), r(1)[0]),
+            "loss_few": (lambda x, w, b: linear_cross_entropy(x, w, y[:9], bias=b, reduction="sum"),
+                         tuple(t.bfloat16() for t in (r(9, 40), r(300, 40), r(300))), r(1)[0])}      # (their logits are kept)
 
 
-NAMES = ("norm", "norm_split", "loss", "loss_rows")
+NAMES = ("norm", "norm_split", "loss", "loss_rows", "loss_kept", "loss_few")
 
 
 def leaves(ts):
@@ -136,7 +139,7 @@ def test_forward_under_no_grad_and_detached_inputs(name):
 
 def test_threads_on_one_stream():
     """Calls of four threads on one stream, each with its own inputs: the workspace of a call is its own until it is queued."""
-    fns = [cases()[n] for n in ("norm_split", "loss", "norm_split", "norm")]
+    fns = [cases()[n] for n in ("norm_split", "loss", "loss_kept", "norm")]
     wants = [plain(*c) for c in fns]
     torch.cuda.synchronize()
     bad = []
@@ -152,3 +155,30 @@ def test_threads_on_one_stream():
     [t.start() for t in threads]
     [t.join() for t in threads]
     assert not bad, bad
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_captured_and_replayed(name):
+    """Forward and backward in one graph, replayed over new inputs with eager calls in between."""
+    fn, ts, up = cases()[name]
+    ls = leaves(ts)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            torch.autograd.grad(fn(*ls), ls, up)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = fn(*ls)
+        grads = torch.autograd.grad(out, ls, up)
+    for i in range(4):
+        with torch.no_grad():
+            new = [t * (1 + 0.25 * i) for t in ts]
+            for t, v in zip(ls, new):
+                t.copy_(v)
+        want = plain(fn, new, up)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out.detach(), want[0])
+        same(grads, want[1])

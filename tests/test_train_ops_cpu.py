@@ -152,13 +152,18 @@ def test_loss_entries_check_their_arguments():
         assert entry(None, None) == INV
         for bad in (dict(x=None), dict(w=None), dict(target=None), dict(T=0), dict(D=0), dict(V=0), dict(T=-1), dict(dtype=3),
                     dict(bias_dtype=1), dict(reduction=3), dict(smoothing=1.5), dict(smoothing=math.nan), dict(ldx=7), dict(ldw=7),
-                    dict(stat=None), dict(kept=None), dict(rows=256), dict(T=512), {own: None}):
+                    dict(stat=None), dict(kept=None), dict(rows=256), dict(T=512), {own: None},
+                    dict(z=256), dict(z=264, D=128, ldx=128, ldw=128)):
             assert call(**bad) == INV, bad
         assert call(workspace=None) == WS and call(workspace_bytes=16) == WS and call(workspace=264) == WS
         assert call(D=(1 << 22) + 8, ldx=1 << 23, ldw=1 << 23) == 3
         assert call(T=1 << 30, rows=256) == call(V=1 << 30) == 3
     assert call(db=256) == INV                                                                  # a gradient of no bias
     assert lib.pngpd_lce_rows_ints(511) == 0 and lib.pngpd_lce_rows_ints(512) == 1025
+    kept = lib.pngpd_lce_z_bytes                                   # float32 of whole 256 classes; 0: not kept
+    assert kept(64, 256, 6500, 0) == 64 * 6656 * 4 and kept(64, 127, 6500, 0) == 0 == kept(8192, 1024, 40000, 0)
+    assert kept(9, 40, 300, 1) == 9 * 512 * 4 and kept(11, 40, 300, 1) == kept(0, 8, 8, 0) == kept(4, 256, 8, 3) == 0
+    assert kept(8192, 1024, 32768, 0) == 1 << 30 and kept(512, 4096, 200000, 2) == 0
     a = args(T=0)
     assert lib.pngpd_lce_workspace_bytes(ctypes.addressof(a), 0) == 0
     # a piece's gradient of the logits is bounded: 256 MB, or 256 classes of all rows
