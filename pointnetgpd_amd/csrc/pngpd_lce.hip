@@ -16,10 +16,10 @@
 // float16 holds g times 2^15 (|g| <= 1: below 65504, and its normal range then reaches down to 2e-9, under 1/V); the
 // coefficients c_t are scaled to at most 1 the same way; both factors come back in float32 on the way out.
 // Measured (bf16; a large library product reaches 1250 TFLOP/s on this card): 6,550 kept rows of 8192, D 1024, V 100,000: statistics
-// 1.33 ms = 1010 TFLOP/s; of each of 6 pieces g 261 us = 860, dx's product 268 us = 840, dW's 223 us (and 99 for the classes past
-// its rounds) = 930, db 33 us: 5.7 ms in all.  No LDS bank conflict; of the statistics' time the epilogue is 17 %; rows of x or W other than a power of two apart
-// change nothing (1480 us at 1024 and at 1088 elements, all rows).  64 rows, D 256, V 6500, float32: eight launches of 3 to
-// 13 us.
+// 1.33 ms = 1010 TFLOP/s; of each of 6 pieces g 261 us = 860, dx's product 268 us = 840, dW's 223 us (and 99 for the classes
+// past its rounds) = 930, db 33 us: 5.7 ms in all.  No LDS bank conflict; of the statistics' time the epilogue is 17 %; rows of x
+// or W other than a power of two apart change nothing (1480 us at 1024 and at 1088 elements, all rows).  64 rows, D 256, V 6500,
+// float32: eight launches of 3 to 13 us.
 #include <algorithm>
 
 #include "pngpd_lce_gemm.h"
@@ -540,7 +540,7 @@ __global__ __launch_bounds__(256) void lce_kept_grad_kernel(const LceArgs a, int
     float g[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        const float p = lce_far<DT>(m) ? __builtin_amdgcn_exp2f((z[e] - m) * LOG2E) : __builtin_amdgcn_exp2f(fmaf(z[e], LOG2E, -(m * LOG2E)));
+        const float p = __builtin_amdgcn_exp2f(lce_far<DT>(m) ? (z[e] - m) * LOG2E : fmaf(z[e], LOG2E, -(m * LOG2E)));
         g[e] = fmaf(p, ks, -kf) - (y == v + e ? co * (1.f - a.smooth) : 0.f);
         if (co == 0.f || v + e >= a.vc) g[e] = 0.f;
     }
@@ -810,8 +810,9 @@ static LcePlan lce_plan(const Lce *a, bool bwd) {
         p.o_coef = take((size_t)a->T * 4);
         p.o_scale = take(4);
         // a piece: g of at most LCE_PIECE_BYTES, at least 256 classes; pieces whose dW is whole rounds of the large tile over
-        // the CUs (up to a quarter of one more in the last), or of one size where not even one round fits (forward + backward of 8192 rows, D 1024,
-        // 33,000 classes, bf16: 2.42 ms, and 3.66 in pieces of one size; D 512, 60,000 classes: 2.38 and 3.71)
+        // the CUs (up to a quarter of one more in the last), or of one size where not even one round fits (forward + backward
+        // of 8192 rows, D 1024, 33,000 classes, bf16: 2.42 ms, and 3.66 in pieces of one size; D 512, 60,000 classes: 2.38 and
+        // 3.71)
         long long most = LCE_PIECE_BYTES / ((long long)a->T * es) / 256;
         if (most < 1) most = 1;
         const long long across_d = lce_cdiv(p.Dp, 256), fit = 256 / across_d;
@@ -987,7 +988,8 @@ template <int DT> static int lce_backward(const Lce *a, const LcePlan &p, hipStr
         if (a->dx) {
             LceOut o = {};
             o.a = LceOperand{w, k.w.ld}; o.b = LceOperand{g, p.ldg}; o.rows = k.rows;
-            o.M = p.Dp; o.N = -1; o.mo = a->D; o.no = a->T; o.K = vc; o.kper = ((long long)vc + 64 * p.splits - 1) / (64 * p.splits) * 64; o.splits = p.splits;
+            o.M = p.Dp; o.N = -1; o.mo = a->D; o.no = a->T; o.K = vc; o.splits = p.splits;
+            o.kper = ((long long)vc + 64 * p.splits - 1) / (64 * p.splits) * 64;
             o.part = part; o.add = v0 > 0; o.scale = scale;
             if ((rc = lce_out<DT, false>(o, p.xshape, st))) return rc;
         }
