@@ -20,7 +20,7 @@
 // Measured (a large copy reaches 4.9 TB/s on this card): bf16, 1024 samples of 1024 x 128 in 32 groups, gelu: forward 168 us
 // (537 MB, 3.2 TB/s), backward 285 us (805 MB, 2.8 TB/s; a workgroup's 32-byte pieces of a row reach memory with 23 % more
 // writes); float32, 64 of 750 x 128: 16 and 19 + 4 us; fp16, one sample of 50,000 x 1024: forward 17 + 6 + 37 us, backward
-// 46 + 5 + 5 + 60 + 5 (102 MB a walk; the second walk finds part of it in the last-level cache).
+// 46 + 6 + 59 (102 MB a walk; the second walk finds part of it in the last-level cache).
 #include "pngpd_common.h"
 #include "pngpd_types.h"
 
@@ -28,7 +28,7 @@
 
 struct GnArgs {
     const void *x, *dy, *w, *b;
-    void *y, *dx;
+    void *y, *dx, *dw, *db;        // dw, db: where A, B of one row of ab are theirs, or NULL
     double *stats;                 // (B,G,2): mean, rstd
     float *ab;                     // (nab,C,2): A, B of a sample, or of the samples of one workgroup
     double *part;                  // split form: (B,S,units,2) sums;  backward: (B,S,C,2) as float
@@ -344,6 +344,12 @@ __global__ __launch_bounds__(SLAB_THREADS) void gn_fwd_slab_kernel(const GnArgs 
     }
 }
 
+// a channel's gradient, of w's and b's type; to NULL: none
+template <int DT> __device__ __forceinline__ void gn_store(const GnArgs &a, void *to, size_t c, float v) {
+    if (!to) return;
+    if (a.wf32) ((float *)to)[c] = v; else st_elem<DT>((typename elem<DT>::t *)to + c, v);
+}
+
 // The samples b0 .. b0 + have - 1 (without MANY: one); dz stays in registers (float32) between the sums and dx where its
 // slope is dear (silu, gelu); none and relu take dy again.  sum: A, B of the channels tid + i threads over the samples so far.
 template <int DT, int VEC, int SUB, int RPT, int ACT, bool MANY>
@@ -396,8 +402,9 @@ __device__ __forceinline__ void gn_bwd_samples(const GnArgs &a, double *sh, int 
             }
             if constexpr (MANY) { sum[i][0] = u; sum[i][1] = v; }
             if (a.ab && last) {
-                float *o = a.ab + 2 * ((size_t)ib * a.C + c0 + k);
-                o[0] = (float)u; o[1] = (float)v;
+                const size_t ch = (size_t)ib * a.C + c0 + k;
+                a.ab[2 * ch] = (float)u; a.ab[2 * ch + 1] = (float)v;
+                gn_store<DT>(a, a.db, ch, (float)u); gn_store<DT>(a, a.dw, ch, (float)v);
             }
         }
     }
@@ -634,8 +641,11 @@ __global__ __launch_bounds__(256) void gn_bwd_part_kernel(const GnArgs a) {
 }
 
 // the channels' A, B over `per` neighbours (a sample's cuts, or samples): in (total,C,2), out (total / per, rounded up, C, 2);
-// 32 channels x 32 lanes of neighbours a workgroup
-__global__ __launch_bounds__(1024) void gn_bwd_join_kernel(const float *in, float *out, int C, int total, int per) {
+// 32 channels x 32 lanes of neighbours a workgroup.  sums: S1, S2 of the groups too (Cg divides 32), in the place of
+// gn_bwd_group_kernel; dw, db of an only sample, in the place of gn_dwdb_kernel (one sample of 50,000 x 1024: 5 us each).
+template <int DT>
+__global__ __launch_bounds__(1024) void gn_bwd_join_kernel(const GnArgs a, const float *in, float *out, int total, int per, int sums) {
+    const int C = a.C;
     __shared__ double sh[32][32][2];
     const int cx = threadIdx.x & 31, sy = threadIdx.x >> 5, blocks = (C + 31) / 32;
     const int j = blockIdx.x / blocks, c = (blockIdx.x - j * blocks) * 32 + cx, s0 = j * per, n = min(per, total - s0);
@@ -654,9 +664,21 @@ __global__ __launch_bounds__(1024) void gn_bwd_join_kernel(const float *in, floa
         if (sy < k) { sh[sy][cx][0] += sh[sy + k][cx][0]; sh[sy][cx][1] += sh[sy + k][cx][1]; }
         __syncthreads();
     }
-    if (sy == 0 && c < C) {
+    if (sy) return;
+    const float A = (float)sh[0][cx][0], B = (float)sh[0][cx][1];
+    if (c < C) {
         float *o = out + 2 * ((size_t)j * C + c);
-        o[0] = (float)sh[0][cx][0]; o[1] = (float)sh[0][cx][1];
+        o[0] = A; o[1] = B;
+        if (a.nab == 1) { gn_store<DT>(a, a.db, c, A); gn_store<DT>(a, a.dw, c, B); }
+    }
+    if (!sums) return;
+    const double w = c >= C || !a.w ? 1.f : a.wf32 ? ((const float *)a.w)[c] : ld_elem<DT>((const typename elem<DT>::t *)a.w + c);
+    double S1 = (double)A * w, S2 = (double)B * w;        // (lanes past C: whole groups of them)
+    for (int k = 1; k < a.Cg; k <<= 1) { S1 += __shfl_xor(S1, k); S2 += __shfl_xor(S2, k); }
+    if (c < C && cx % a.Cg == 0) {
+        const double m = (double)a.N * a.Cg;
+        float *o = a.gsum + 2 * ((size_t)j * a.G + c / a.Cg);
+        o[0] = (float)(S1 / m); o[1] = (float)(S2 / m);
     }
 }
 
@@ -743,7 +765,7 @@ __global__ __launch_bounds__(256) void gn_dwdb_kernel(const GnArgs a, const floa
     const int j = threadIdx.x >> 2;                       // 0: db of channel cx, 1: dw
     for (int k = 0; k < 64; ++k) s += sh[k][cx][j];
     void *to = j ? dw : db;
-    if (to && c < a.C) { if (a.wf32) ((float *)to)[c] = (float)s; else st_elem<DT>((typename elem<DT>::t *)to + c, (float)s); }
+    if (c < a.C) gn_store<DT>(a, to, c, (float)s);
 }
 
 // ---------------------------------------------------------------------------------------------- plan
@@ -880,6 +902,8 @@ static int gn_fwd_launch(GnArgs &a, const GnPlan &p, hipStream_t st) {
 template <int DT, int VEC, int SUB, int ACT>
 static int gn_bwd_launch(GnArgs &a, const GnPlan &p, void *dw, void *db, hipStream_t st) {
     const int blocks = (a.C + 31) / 32;                   // of a join, for one output row
+    if (p.nab == 1) { a.dw = dw; a.db = db; }
+    bool done = p.slab && p.nab == 1;                     // dw, db are written
     if (p.slab) {
         const bool many = p.per > 1 || p.spw > 1;
         const size_t lds = (size_t)2 * VEC * (p.threads + 64 + (1 << p.lx)) * 4 + (size_t)p.spw * p.gpr * 16;
@@ -891,19 +915,23 @@ static int gn_bwd_launch(GnArgs &a, const GnPlan &p, void *dw, void *db, hipStre
     } else {
         const dim3 grid((unsigned)(p.cols * p.S * a.B));
         hipLaunchKernelGGL((gn_bwd_part_kernel<DT, VEC, SUB, ACT>), grid, dim3(256), (size_t)4 * (1 << p.lx) * VEC * 8, st, a);
-        if (p.S > 1) hipLaunchKernelGGL(gn_bwd_join_kernel, dim3((unsigned)(a.B * blocks)), dim3(1024), 0, st, (const float *)a.part, a.ab, a.C, a.B * p.S, p.S);
+        const bool joined = p.S > 1, sums = joined && a.dx && 32 % a.Cg == 0;
+        done = joined && p.nab == 1;
+        if (joined) hipLaunchKernelGGL(gn_bwd_join_kernel<DT>, dim3((unsigned)(a.B * blocks)), dim3(1024), 0, st, a, (const float *)a.part,
+                                       a.ab, a.B * p.S, p.S, (int)sums);
         if (a.dx) {
-            hipLaunchKernelGGL(gn_bwd_group_kernel<DT>, dim3((unsigned)(a.B * a.G)), dim3(64), 0, st, a);
+            if (!sums) hipLaunchKernelGGL(gn_bwd_group_kernel<DT>, dim3((unsigned)(a.B * a.G)), dim3(64), 0, st, a);
             hipLaunchKernelGGL((gn_bwd_apply_kernel<DT, VEC, SUB, ACT>), grid, dim3(256), 0, st, a);
         }
     }
-    if (dw || db) {
+    if (!done && (dw || db)) {
         const float *ab = a.ab;
         if (p.fold) {
-            hipLaunchKernelGGL(gn_bwd_join_kernel, dim3((unsigned)(p.fold * blocks)), dim3(1024), 0, st, ab, a.folded, a.C, p.nab, GN_FOLD);
+            hipLaunchKernelGGL(gn_bwd_join_kernel<DT>, dim3((unsigned)(p.fold * blocks)), dim3(1024), 0, st, a, ab, a.folded, p.nab, GN_FOLD, 0);
             ab = a.folded;
         }
-        hipLaunchKernelGGL(gn_dwdb_kernel<DT>, dim3((unsigned)((a.C + 3) / 4)), dim3(256), 0, st, a, ab, p.fold ? p.fold : p.nab, dw, db);
+        hipLaunchKernelGGL(gn_dwdb_kernel<DT>, dim3((unsigned)((a.C + 3) / 4)), dim3(256), 0, st, a, ab, p.fold ? p.fold : p.nab,
+                           dw, db);
     }
     return pngpd_launch_status();
 }
