@@ -309,6 +309,7 @@ __device__ __forceinline__ double lce_block_sum(double v, double *sh) {
 __device__ __forceinline__ void lce_loss(const float *row, const LceArgs &a, int reduction, float *loss, float *kept) {
     __shared__ double sh[16];
     double s = 0.0, n = 0.0;
+#pragma unroll 4
     for (int t = threadIdx.x; t < a.T; t += blockDim.x) {
         if (a.target[t] != a.ignore) n += 1.0;
         s += (double)row[t];
@@ -398,6 +399,7 @@ __device__ __forceinline__ void lce_coef(const LceCoef &a) {
     float top = 1.f;
     if (a.reduction == PNGPD_REDUCE_NONE) {
         top = 0.f;
+#pragma unroll 8
         for (int t = threadIdx.x; t < T; t += 256) {
             const float c = fabsf(a.dloss[t]);
             if (c < INFINITY && a.target[t] != a.ignore) top = fmaxf(top, c);
@@ -408,13 +410,21 @@ __device__ __forceinline__ void lce_coef(const LceCoef &a) {
         top = fmaxf(fmaxf(sh[0], sh[1]), fmaxf(sh[2], sh[3]));
         if (top == 0.f) top = 1.f;
     }
-    for (int t = threadIdx.x; t < T; t += 256) {
-        const long long y = a.target[t];
-        float c = a.reduction == PNGPD_REDUCE_NONE ? a.dloss[t] / top * a.up : a.up;
-        if (y == a.ignore) c = 0.f;
-        else if (y < 0 || y >= a.V) c = NAN;
-        const int k = a.rows.place(t);
-        if (k >= 0) a.coef[k] = c;
+    for (int t0 = threadIdx.x; t0 < T; t0 += 8 * 256) {           // eight rows' loads at a time: one workgroup has all of them
+        long long y[8];
+        float c[8];
+        int k[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int t = min(t0 + 256 * i, T - 1);
+            y[i] = a.target[t]; k[i] = a.rows.place(t);
+            c[i] = a.reduction == PNGPD_REDUCE_NONE ? a.dloss[t] : 1.f;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float v = y[i] == a.ignore ? 0.f : y[i] < 0 || y[i] >= a.V ? NAN : c[i] / top * a.up;
+            if (t0 + 256 * i < T && k[i] >= 0) a.coef[k[i]] = v;
+        }
     }
     if (threadIdx.x == 0) {
         float s = top / a.up;
@@ -612,7 +622,8 @@ struct LceOut {
     int splits;
     void *out;                             // typed: out[n * ldo + m] = scale * sum
     long long ldo;
-    float *part;                           // or fp32 partial sums (splits, T, M), added to what is there
+    float *part;                           // or fp32 partial sums (splits, pn, M), added to what is there
+    int pn;
     int add;
     const float *scale;
     int vec;                               // out's rows are whole 16-byte chunks
@@ -647,7 +658,7 @@ __global__ __launch_bounds__(WGM * WGN * 64, 2) void lce_out_kernel(const LceOut
             f32x16 v = c.acc[i][j];
             const int mb = m0 + wm + 32 * i;
             if (a.part) {
-                float *o = a.part + ((size_t)split * a.rows.T + n) * a.M + mb + 4 * half;
+                float *o = a.part + ((size_t)split * a.pn + n) * a.M + mb + 4 * half;
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
                     if (mb + 8 * q + 4 * half < a.M) {
@@ -683,7 +694,7 @@ __global__ __launch_bounds__(WGM * WGN * 64, 2) void lce_out_kernel(const LceOut
     }
 }
 
-// dx = scale * sum of the splits' partial sums (rows of Dp, a multiple of 4); 0 where a row is not among the kept
+// dx (or dW) = scale * sum of the splits' partial sums (rows of Dp, a multiple of 4); 0 where a row is not among the kept
 template <int DT>
 __global__ __launch_bounds__(256) void lce_dx_kernel(const float *__restrict__ part, int splits, LceRows rows, int D, int Dp,
                                                      const float *__restrict__ scale, void *__restrict__ dx) {
@@ -756,17 +767,17 @@ static const int LCE_BM[4] = {256, 64, 64, 128}, LCE_BN[4] = {256, 64, 32, 128};
 #define LCE_SHAPE2 64, 32, 2, 1, 5
 #define LCE_SHAPE3 128, 128, 2, 2, 2
 static inline int lce_cdiv(long long a, int b) { return (int)((a + b - 1) / b); }
-// 128 x 128 or 64 x 64: the larger one does an operation in 0.75 of the smaller one's time where its tiles fill their rounds of the
-// 256 CUs (forward + backward of 1024 rows, D 2048, 12,000 classes, bf16: 296 us in 128 x 128 tiles and 381 in 64 x 64 ones; of
-// D 1024, 5000 classes, float32, 320 large tiles or 1264 small ones: 536 and 443)
-static int lce_mid(long long M, long long N) {
-    const long long large = (long long)lce_cdiv(M, 128) * lce_cdiv(N, 128), small = (long long)lce_cdiv(M, 64) * lce_cdiv(N, 64);
-    return 3 * ((large + 255) / 256) * 256 <= small ? 3 : 1;
-}
-// The large tile needs a workgroup for every CU; the narrow one is for rows that would leave half of 64 unused.
-static int lce_shape(long long M, long long N) {
+// An operation takes 0.4 of the 64 x 64 tile's time in 256 x 256 tiles and 0.75 in 128 x 128 ones, where they fill their rounds of
+// the 256 CUs and are not mostly padding (forward + backward of 1024 rows, D 2048, 12,000 classes, bf16: 296 us in 128 x 128
+// tiles, 381 in 64 x 64; 1024 rows, D 1024, 5000 classes, float32, 320 tiles of 128 or 1264 of 64: 536 and 443).  least: large
+// tiles at least.  The narrow tile is for rows that would leave half of 64 unused.
+static int lce_shape(long long M, long long N, int least = 256) {
     if (N <= 32) return 2;
-    return (long long)lce_cdiv(M, 256) * lce_cdiv(N, 256) >= 256 ? 0 : lce_mid(M, N);
+    const auto tiles = [&](int n) { return (long long)lce_cdiv(M, n) * lce_cdiv(N, n); };
+    const auto whole = [&](int n) { return (tiles(n) + 255) / 256 * 256; };
+    const long long large = 32 * whole(256), mid = 15 * whole(128), small = 5 * tiles(64);
+    if (tiles(256) >= least && large <= mid && large <= small) return 0;
+    return mid <= small ? 3 : 1;
 }
 
 // Of `n` classes, those that the large tile takes: whole rounds of 256 workgroups (one a CU) of `other` tiles each.  What is
@@ -782,8 +793,9 @@ static int lce_cut(int n, int other) {
 struct LcePlan {
     int Dp, fshape, fmt, fcut, padx, padw;
     int piece, large, ldg, xshape, splits; // classes of a piece, at most of the last one
+    int wsplits;                           // dW: cuts of the rows
     int share, shares;                     // db: rows of a share, shares
-    size_t o_part, o_ps, o_zt, o_row, o_x, o_w, o_coef, o_scale, o_g, o_dx, o_db, bytes;
+    size_t o_part, o_ps, o_zt, o_row, o_x, o_w, o_coef, o_scale, o_g, o_dx, o_dw, o_db, bytes;
 };
 
 static LcePlan lce_plan(const Lce *a, bool bwd) {
@@ -831,6 +843,11 @@ static LcePlan lce_plan(const Lce *a, bool bwd) {
         if (s > p.piece / 256) s = p.piece / 256;
         p.splits = s < 1 ? 1 : (int)s;
         p.o_dx = take((size_t)p.splits * a->T * p.Dp * 4);
+        // dW: few tiles and many rows: cut the rows until there are about 256 workgroups, of at least 512 rows
+        // (forward + backward of 200,000 rows, D 256, 2 classes, float32: 1.1 ms, and 6.1 in four workgroups)
+        const long long vmost = std::min(a->V, p.large), small = (long long)lce_cdiv(p.Dp, 64) * lce_cdiv(vmost, 64);
+        p.wsplits = (int)std::max(1ll, small < 128 ? std::min(256 / small, (long long)a->T / 512) : 1);
+        if (p.wsplits > 1) p.o_dw = take((size_t)p.wsplits * vmost * p.Dp * 4);
         // db: about 1024 workgroups
         const long long across = lce_cdiv(p.piece, es == 4 ? 32 : 64);
         long long n2 = 1024 / across;
@@ -900,6 +917,7 @@ static inline int lce_ldz(int V) { return (V + 255) / 256 * 256; }
 // bytes of 16 bits a class).  (Forward + backward, float32, 1024 x 2048 x 12,000: 1369
 // us, computed again 1752; bf16, 200 x 800 x 40,000: 163 and 169.)
 static bool lce_keeps(int T, int D, int V, int dt) {
+    if (V < 128) return false;                                    // (rows are padded to whole 256 classes)
     const long long bytes = (long long)T * lce_ldz(V) * 4;
     return dt == PNGPD_F32 ? D >= 128 && bytes <= LCE_PIECE_MOST : 4ll * T <= D && bytes <= LCE_PIECE_BYTES && lce_shape(V, T) != 0;
 }
@@ -957,8 +975,7 @@ template <int DT> static int lce_backward(const Lce *a, const LcePlan &p, hipStr
     k.stat = a->stat; k.coef = coef; k.ldg = p.ldg;
     for (int v0 = 0, vc; v0 < a->V; v0 += vc) {
         vc = a->V - v0 <= p.large ? a->V - v0 : p.piece;
-        const int gshape = lce_shape(vc, a->T);
-        const int wshape = (long long)lce_cdiv(p.Dp, 256) * lce_cdiv(vc, 256) >= 192 ? 0 : lce_mid(p.Dp, vc);
+        const int gshape = lce_shape(vc, a->T), wide = lce_shape(p.Dp, vc, 192), wshape = wide == 2 ? 1 : wide;
         const int cols = (vc + 63) / 64 * 64;                      // columns of g that are written (zeros past vc)
         const int gcut = gshape ? vc : lce_cut(vc, lce_cdiv(a->T, 256));
         k.v0 = v0; k.vc = gcut; k.g = ws + p.o_g;
@@ -990,10 +1007,20 @@ template <int DT> static int lce_backward(const Lce *a, const LcePlan &p, hipStr
             o.a = LceOperand{w, k.w.ld}; o.b = LceOperand{g, p.ldg}; o.rows = k.rows;
             o.M = p.Dp; o.N = -1; o.mo = a->D; o.no = a->T; o.K = vc; o.splits = p.splits;
             o.kper = ((long long)vc + 64 * p.splits - 1) / (64 * p.splits) * 64;
-            o.part = part; o.add = v0 > 0; o.scale = scale;
+            o.part = part; o.pn = a->T; o.add = v0 > 0; o.scale = scale;
             if ((rc = lce_out<DT, false>(o, p.xshape, st))) return rc;
         }
-        if (a->dw) {
+        if (a->dw && p.wsplits > 1) {
+            LceOut o = {};
+            o.a = LceOperand{k.x.p, p.Dp}; o.b = LceOperand{g, p.ldg}; o.rows = k.rows;
+            o.M = p.Dp; o.N = cols; o.mo = a->D; o.no = vc; o.K = -1; o.splits = p.wsplits;
+            o.kper = ((long long)a->T + 64 * p.wsplits - 1) / (64 * p.wsplits) * 64;
+            o.part = (float *)(ws + p.o_dw); o.pn = vc; o.scale = scale;
+            if ((rc = lce_out<DT, true>(o, 1, st))) return rc;
+            const long long n = (long long)vc * (p.Dp / 4);
+            hipLaunchKernelGGL(lce_dx_kernel<DT>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, o.part, p.wsplits,
+                               LceRows{nullptr, vc}, a->D, p.Dp, scale, (void *)((E *)a->dw + (long long)v0 * a->D));
+        } else if (a->dw) {
             const int wcut = wshape ? vc : lce_cut(vc, lce_cdiv(p.Dp, 256));
             for (int c0 = 0; c0 < vc; c0 = c0 ? vc : wcut) {       // the large tile's classes, then the rest
                 const int c1 = c0 ? vc : wcut;

@@ -124,6 +124,13 @@ def test_pieces():
     compare(*args, reduction="none", smooth=0.1)
 
 
+@pytest.mark.parametrize("T,D,V,dtype", [(70_001, 64, 2, F32), (30_000, 250, 20, BF16), (9000, 130, 300, F16), (4097, 16, 700, F32)])
+@pytest.mark.parametrize("reduction", ["none", "mean"])
+def test_many_rows_of_few_classes(T, D, V, dtype, reduction):
+    """dW's product is cut along the rows."""
+    compare(*data(T, D, V, dtype, 15), reduction=reduction, smooth=0.1)
+
+
 @pytest.mark.parametrize("T,D,V,dtype", [(8192, 1000, 17300, BF16), (8192, 1000, 22400, F16), (4096, 1024, 40000, F32),
                                          (9000, 300, 70000, BF16)])
 def test_pieces_of_whole_rounds(T, D, V, dtype):

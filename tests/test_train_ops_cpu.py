@@ -162,6 +162,7 @@ def test_loss_entries_check_their_arguments():
     assert lib.pngpd_lce_rows_ints(511) == 0 and lib.pngpd_lce_rows_ints(512) == 1025
     kept = lib.pngpd_lce_z_bytes                                   # float32 of whole 256 classes; 0: not kept
     assert kept(64, 256, 6500, 0) == 64 * 6656 * 4 and kept(64, 127, 6500, 0) == 0 == kept(8192, 1024, 40000, 0)
+    assert kept(64, 256, 127, 0) == 0 and kept(64, 256, 128, 0) == 64 * 256 * 4                  # padding at most doubles them
     assert kept(9, 40, 300, 1) == 9 * 512 * 4 and kept(11, 40, 300, 1) == kept(0, 8, 8, 0) == kept(4, 256, 8, 3) == 0
     assert kept(8192, 1024, 32768, 0) == 1 << 30 and kept(512, 4096, 200000, 2) == 0
     a = args(T=0)
