@@ -34,9 +34,3 @@ template <int DT> __device__ __forceinline__ unsigned pk_half(float a, float b) 
     if constexpr (DT == PNGPD_BF16) return __builtin_bit_cast(unsigned, __builtin_convertvector(v, pk_bf16x2));
     else return __builtin_bit_cast(unsigned, __builtin_convertvector(v, pk_f16x2));
 }
-// c + a.lo b.lo + a.hi b.hi, products exact, float32 sums
-template <int DT> __device__ __forceinline__ float dot_half(unsigned a, unsigned b, float c) {
-    if constexpr (DT == PNGPD_BF16)
-        return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(pk_bf16x2, a), __builtin_bit_cast(pk_bf16x2, b), c, false);
-    else return __builtin_amdgcn_fdot2(__builtin_bit_cast(pk_f16x2, a), __builtin_bit_cast(pk_f16x2, b), c, false);
-}

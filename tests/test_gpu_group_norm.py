@@ -269,3 +269,33 @@ def test_many_samples_of_few_rows(shape, groups, dtype):
         assert torch.equal(bad[name][rest], got[name][rest]), name
     for name in ("dw", "db"):
         assert bad[name][-k:].isnan().all() and torch.equal(bad[name][:-k], got[name][:-k]), name
+
+
+# (B, N, C, groups): one row of groups of eight, four and two; several; a slab; cut along the rows
+CLOSE = [(50, 1, 64, 8), (30, 1, 32, 8), (40, 1, 16, 8), (6, 10, 64, 4), (9, 3, 40, 5), (2, 500, 64, 8), (1, 20000, 64, 8),
+         (9000, 2, 16, 2)]
+
+
+@pytest.mark.parametrize("dtype,base", [(torch.float16, 1500.0), (torch.float16, 30.0), (torch.bfloat16, 200.0)])
+@pytest.mark.parametrize("i", range(len(CLOSE)), ids=[str(s) for s in CLOSE])
+def test_large_mean_of_16_bits(i, dtype, base):
+    """A spread of one or a few units in the last place: the sums of squares have to hold every bit of them."""
+    *shape, groups = CLOSE[i]
+    x, w, b, dy = data(shape, torch.float32, 40 + i, shift=0.0)
+    unit = base * torch.finfo(dtype).eps
+    for spread in (1.0, 4.0):
+        compare((base + spread * unit * x).to(dtype), w.to(dtype), b.to(dtype), groups, "none", dy.to(dtype))
+
+
+@pytest.mark.parametrize("dtype,low,high", [(torch.float16, 2046.0, 2047.0), (torch.float16, 2047.0, 2050.0),
+                                            (torch.bfloat16, 254.0, 255.0), (torch.bfloat16, 255.0, 258.0)])
+@pytest.mark.parametrize("i", range(len(CLOSE)), ids=[str(s) for s in CLOSE])
+def test_two_neighbouring_values(i, dtype, low, high):
+    """Groups of two adjacent values of the type, also of two across a power of two; one odd one among equal ones in each
+    fourth sample."""
+    *shape, groups = CLOSE[i]
+    x, w, b, dy = data(shape, dtype, 60 + i)
+    pick = x > 0
+    pick[::4] = False
+    pick[::4, 0, ::shape[2] // groups] = True
+    compare(torch.where(pick, high, low).to(dtype), w, b, groups, "silu", dy)
