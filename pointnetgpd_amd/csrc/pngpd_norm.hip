@@ -196,20 +196,21 @@ __device__ __forceinline__ float gn_dz(float x, float xh, float dy, float w, flo
         else { float e; const float s = phi_cdf(z, e); return dy * fmaf(z * 0.39894228040143268f, e, s); }
     }
 }
-// dx = rstd (w dz - S1 - xh S2) = dz w r + d k1 + k0
+// dx = rstd (w dz - S1 - xh S2) = r (w dz + d k1 + k0); r outside: r^2 leaves float32's range where spreads pass 1e19 or, with
+// eps = 0, lie below 1e-19
 template <int VEC, int SUB> struct DxPar {
-    float wr[VEC], k0[SUB], k1[SUB];
+    float w[VEC], r[SUB], k0[SUB], k1[SUB];
     // S: (S1, S2) of the column's groups in turn
     __device__ __forceinline__ void set(const ColPar<VEC, SUB> &p, int k, double S1, double S2) {
-        const double r = (double)p.r[k];
-        k1[k] = (float)(-r * r * S2);
-        k0[k] = (float)(-r * (S1 + (double)p.c[k] * S2));
+        r[k] = p.r[k];
+        k1[k] = (float)(-(double)p.r[k] * S2);
+        k0[k] = (float)(-(S1 + (double)p.c[k] * S2));
 #pragma unroll
-        for (int e = k * (VEC / SUB); e < (k + 1) * (VEC / SUB); ++e) wr[e] = p.w[e] * p.r[k];
+        for (int e = k * (VEC / SUB); e < (k + 1) * (VEC / SUB); ++e) w[e] = p.w[e];
     }
     __device__ __forceinline__ float dx(int e, float d, float dz) const {
         const int k = ColPar<VEC, SUB>::sub(e);
-        return fmaf(dz, wr[e], fmaf(d, k1[k], k0[k]));
+        return r[k] * fmaf(dz, w[e], fmaf(d, k1[k], k0[k]));
     }
 };
 

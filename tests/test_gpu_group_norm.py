@@ -299,3 +299,19 @@ def test_two_neighbouring_values(i, dtype, low, high):
     pick[::4] = False
     pick[::4, 0, ::shape[2] // groups] = True
     compare(torch.where(pick, high, low).to(dtype), w, b, groups, "silu", dy)
+
+
+@pytest.mark.parametrize("size", [1e25, 1e-25])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape,groups", [((3, 70, 48), 6), ((1, 20000, 64), 8), ((9000, 2, 16), 2)])
+def test_spreads_whose_squares_leave_float32(shape, groups, dtype, size):
+    """eps = 0: statistics of features of any size, and gradients of the inverse size."""
+    from pointnetgpd_amd.train_ops import group_norm_act
+    x, w, b, dy = data(shape, torch.float32, 80)
+    x, w, b, dy = ((size * x).to(dtype), w.to(dtype), b.to(dtype), dy.to(dtype))
+    leaves = [t.detach().requires_grad_() for t in (x, w, b)]
+    y = group_norm_act(leaves[0], groups, *leaves[1:], eps=0.0, act="silu")
+    got = dict(zip(("y", "dx", "dw", "db"), (y.detach(), *torch.autograd.grad(y, leaves, dy))))
+    want = reference(x, dy, w, b, groups, "silu", eps=0.0)
+    for k, v in got.items():
+        check(v, *want[k], k)
