@@ -33,6 +33,10 @@ def _bytes(dev, n):
     return torch.empty(n, device=dev, dtype=torch.uint8)
 
 
+def _flat(t):
+    return t if t is None or t.is_contiguous() else t.contiguous()
+
+
 def _same_device(ref, name, *others):
     index = ref.get_device()
     for n, t in others:
@@ -50,6 +54,11 @@ def _once(backward):
     """``once_differentiable(backward)`` where the call itself may be differentiated (create_graph), else ``backward``."""
     guarded = once_differentiable(backward)
     return lambda ctx, g: (guarded if torch.is_grad_enabled() else backward)(ctx, g)
+
+
+def _adjacent(x):
+    """(B,N,C) with adjacent channels, as the kernels read it: x itself, or a copy."""
+    return x if x.stride(2) == 1 or x.shape[2] == 1 else x.contiguous()
 
 
 def _gn_call(fn, entry, dev, dims, nbytes, x, w, b, *ptrs):
@@ -87,13 +96,13 @@ def _group_norm_fwd(x, w, b, dims):
 def _group_norm_bwd(ctx, dy):
     x, w, b, stats = ctx.saved_tensors
     dims, nbytes, dev = ctx.call
+    x, w, b, stats = _adjacent(x), _flat(w), _flat(b), _flat(stats)            # (a saved-tensor hook may have moved them)
     need = ctx.needs_input_grad
     dx = torch.empty_like(x, memory_format=torch.contiguous_format) if need[0] else None
     dw = torch.empty_like(w) if need[1] else None
     db = torch.empty_like(b) if need[2] else None
     if nbytes is not None:
-        if not dy.is_contiguous():
-            dy = dy.contiguous()
+        dy = _flat(dy)
         _gn_call(_lib.load().pngpd_group_norm_bwd, "group_norm_bwd", dev, dims, nbytes, x, w, b, stats.data_ptr(), dy.data_ptr(),
                  None if dx is None else dx.data_ptr(), None if dw is None else dw.data_ptr(),
                  None if db is None else db.data_ptr())
@@ -163,9 +172,7 @@ def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, act="none"):
         raise RuntimeError("group_norm_act: weight and bias must be of one type")
     if v.shape[0] >= 2 ** 31 or max(N, C) > 2 ** 30:
         raise RuntimeError("group_norm_act: more than 2^31 - 1 samples, 2^30 positions or 2^30 channels")
-    if v.stride(2) != 1 and C > 1:
-        v = v.contiguous()
-    weight, bias = (t if t is None or t.is_contiguous() else t.contiguous() for t in (weight, bias))
+    v, weight, bias = _adjacent(v), _flat(weight), _flat(bias)
     dims = _gn_dims(v, weight, bias, groups, eps, ACTIVATIONS[act])
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (v, weight, bias)):
         y = GroupNormActFn.apply(v, weight, bias, dims)
@@ -185,6 +192,16 @@ def _lce_call(fn, entry, a, nbytes, dev):
     code = _lib.call_on(dev, fn, ctypes.addressof(a))
     if code:
         _lib.check(code, entry)
+
+
+def _rows(v):
+    """(rows, D) with adjacent channels, as the kernels read it: v itself, or a copy."""
+    return v if (v.shape[1] == 1 or v.stride(1) == 1) and (v.shape[0] == 1 or v.stride(0) >= v.shape[1]) else v.contiguous()
+
+
+def _where(saved):
+    """Where tensors lie and how: a descriptor made for them holds as long as this is the same."""
+    return [0 if t is None else (t.data_ptr(), t.stride()) for t in saved]
 
 
 def _lce_args(scalars, x, w, bias, target, stat, rows, z):
@@ -214,14 +231,15 @@ def _lce_fwd(x, w, bias, target, scalars, train):
 
 
 def _lce_bwd(ctx, dloss):
-    x, w, bias, target, stat, rows, z = saved = ctx.saved_tensors
+    saved = x, w, bias, target, stat, rows, z = ctx.saved_tensors
     made, where, nbytes, dev = ctx.call
     need = ctx.needs_input_grad
-    if not dloss.is_contiguous():
-        dloss = dloss.contiguous()
-    if tuple(0 if t is None else t.data_ptr() for t in saved) == where:
+    dloss = _flat(dloss)
+    if _where(saved) == where:
         a = _lib.LceArgs.from_buffer_copy(made)                                # a copy: two threads may run one node
     else:                                                                      # saved tensors that a hook has moved
+        x, w = _rows(x), _rows(w)
+        bias, target, stat, rows, z = (_flat(t) for t in (bias, target, stat, rows, z))
         a = _lce_args(ctx.scalars, x, w, bias, target, stat, rows, z)
         nbytes = _lib.load().pngpd_lce_workspace_bytes(ctypes.addressof(a), 1)
     dx = torch.empty_like(x, memory_format=torch.contiguous_format) if need[0] else None
@@ -241,8 +259,7 @@ class LinearCrossEntropyFn(torch.autograd.Function):
         loss, made, a = _lce_fwd(x, w, bias, target, scalars, True)
         saved = (x, w, bias, target, *made)
         ctx.scalars = scalars
-        ctx.call = (a, tuple(0 if t is None else t.data_ptr() for t in saved),
-                    _lib.load().pngpd_lce_workspace_bytes(ctypes.addressof(a), 1), x.device)
+        ctx.call = (a, _where(saved), _lib.load().pngpd_lce_workspace_bytes(ctypes.addressof(a), 1), x.device)
         ctx.save_for_backward(*saved)
         return loss
 
@@ -294,10 +311,7 @@ def linear_cross_entropy(x, weight, target, bias=None, reduction="mean", ignore_
         raise RuntimeError(f"linear_cross_entropy: bias must be of x's type ({x.dtype}) or float32, got {bias.dtype}")
     if max(V, target.numel()) >= 2 ** 30 or D > 2 ** 22:
         raise RuntimeError("linear_cross_entropy: more than 2^30 - 1 rows or classes, or 2^22 channels")
-    rows = [v if (v.shape[1] == 1 or v.stride(1) == 1) and (v.shape[0] == 1 or v.stride(0) >= v.shape[1]) else v.contiguous()
-            for v in (x.reshape(-1, D), weight)]
-    if bias is not None and not bias.is_contiguous():
-        bias = bias.contiguous()
+    rows, bias = [_rows(x.reshape(-1, D)), _rows(weight)], _flat(bias)
     target_rows, scalars = target.reshape(-1).contiguous(), (REDUCTIONS[reduction], ignore_index, label_smoothing)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (*rows, bias)):
         loss = LinearCrossEntropyFn.apply(*rows, bias, target_rows, scalars)

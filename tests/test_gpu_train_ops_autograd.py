@@ -78,6 +78,53 @@ def test_saved_tensors_moved_by_hooks(name):
     del hold
 
 
+def _elsewhere(want, place):
+    """Hooks that keep the tensors of shape ``want`` on the host and bring them back as ``place`` lays them out."""
+    return torch.autograd.graph.saved_tensors_hooks(lambda t: (t.cpu(), t),
+                                                    lambda pair: place(pair[0].cuda()) if tuple(pair[0].shape) == want else pair[1])
+
+
+@pytest.mark.parametrize("name", ("loss", "loss_kept"))
+@pytest.mark.parametrize("part", (0, 1))
+def test_saved_rows_come_back_at_their_address_with_other_strides(name, part):
+    """Columns of a wide buffer that a hook brings back dense where the buffer began: the descriptor of the forward pass does
+    not hold for them."""
+    fn, ts, up = cases()[name]
+    want = plain(fn, ts, up)[1]
+    n, d = ts[part].shape
+    buffer = torch.zeros(2 * n * d, device="cuda")
+    wide = buffer.view(n, 2 * d)[:, :d]
+
+    def place(t):
+        buffer.data[:n * d].copy_(t.reshape(-1))
+        buffer.data[n * d:].fill_(float("nan"))
+        return buffer.data[:n * d].view(n, d)
+
+    wide.copy_(ts[part])
+    ls = [wide.detach() if i == part else t.clone() for i, t in enumerate(ts)]
+    assert ls[part].stride(0) == 2 * d
+    ls = [t.requires_grad_() for t in ls]
+    with _elsewhere((n, d), place):
+        out = fn(*ls)
+    same(torch.autograd.grad(out, ls, up), want)
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_saved_tensors_come_back_in_other_layouts(name):
+    """Every saved tensor returned with its last dimension strided, the way a column of a wider buffer is."""
+    fn, ts, up = cases()[name]
+    want = plain(fn, ts, up)[1]
+    ls = leaves(ts)
+
+    def strided(t):
+        out = torch.empty(*t.shape, 2, device=t.device, dtype=t.dtype)[..., 0]
+        return out.copy_(t)
+
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu(), lambda t: strided(t.cuda())):
+        out = fn(*ls)
+    same(torch.autograd.grad(out, ls, up), want)
+
+
 @pytest.mark.parametrize("name", NAMES)
 def test_checkpoint(name):
     from torch.utils.checkpoint import checkpoint
