@@ -8,11 +8,12 @@
                              grasps, one class for each point of a scene.
 
 CUDA tensors run the HIP kernels of libpngpd (a missing library raises), CPU tensors the same formulas in ATen operations.
-The gradients are those of the formulas; they are not differentiable again.
+The gradients are those of the formulas; they are not differentiable again, and forward-mode derivatives raise on CUDA.
 """
 import ctypes
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -51,9 +52,23 @@ def _same_device(ref, name, *others):
 # thread on a far core, 102 -> 93 on a near one; a small group norm 134 -> 125 and 67 -> 65; without the context that
 # call_on spares, 147 and 118 on a far core).
 def _once(backward):
-    """``once_differentiable(backward)`` where the call itself may be differentiated (create_graph), else ``backward``."""
+    """``once_differentiable(backward)`` where the call itself may be differentiated (create_graph), else ``backward``; an
+    upstream gradient with a tangent is refused."""
     guarded = once_differentiable(backward)
-    return lambda ctx, g: (guarded if torch.is_grad_enabled() else backward)(ctx, g)
+
+    def call(ctx, g):
+        if forward_ad._current_level >= 0 and forward_ad.unpack_dual(g).tangent is not None:
+            raise NotImplementedError("the gradients of this operator have no jvp (forward-mode derivatives)")
+        return (guarded if torch.is_grad_enabled() else backward)(ctx, g)
+    return call
+
+
+def _wants_node(*tensors):
+    """Whether the call has to go through its autograd node: an input requires grad, or carries a tangent perhaps (forward-mode
+    derivatives are not implemented, which the node says; past it they would vanish), or a trace is being recorded (of a node it
+    holds the call, otherwise the empty outputs and no kernel)."""
+    return (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+            or forward_ad._current_level >= 0 or torch._C._get_tracing_state() is not None)
 
 
 def _adjacent(x):
@@ -174,7 +189,7 @@ def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, act="none"):
         raise RuntimeError("group_norm_act: more than 2^31 - 1 samples, 2^30 positions or 2^30 channels")
     v, weight, bias = _adjacent(v), _flat(weight), _flat(bias)
     dims = _gn_dims(v, weight, bias, groups, eps, ACTIVATIONS[act])
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (v, weight, bias)):
+    if _wants_node(v, weight, bias):
         y = GroupNormActFn.apply(v, weight, bias, dims)
     else:
         y = _group_norm_fwd(v, weight, bias, dims)[0]
@@ -306,6 +321,8 @@ def linear_cross_entropy(x, weight, target, bias=None, reduction="mean", ignore_
         loss = F.cross_entropy(z.reshape(-1, V), target.reshape(-1), ignore_index=ignore_index, reduction=reduction,
                                label_smoothing=label_smoothing)
         return loss.reshape(target.shape) if reduction == "none" else loss
+    if torch._C._get_tracing_state() is not None:
+        raise RuntimeError("linear_cross_entropy: on CUDA it cannot be recorded by torch.jit.trace")
     _dtype(x, "linear_cross_entropy: x")
     if bias is not None and bias.dtype not in (x.dtype, torch.float32):
         raise RuntimeError(f"linear_cross_entropy: bias must be of x's type ({x.dtype}) or float32, got {bias.dtype}")
@@ -313,7 +330,7 @@ def linear_cross_entropy(x, weight, target, bias=None, reduction="mean", ignore_
         raise RuntimeError("linear_cross_entropy: more than 2^30 - 1 rows or classes, or 2^22 channels")
     rows, bias = [_rows(x.reshape(-1, D)), _rows(weight)], _flat(bias)
     target_rows, scalars = target.reshape(-1).contiguous(), (REDUCTIONS[reduction], ignore_index, label_smoothing)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (*rows, bias)):
+    if _wants_node(*rows, bias):
         loss = LinearCrossEntropyFn.apply(*rows, bias, target_rows, scalars)
     else:
         loss = _lce_fwd(*rows, bias, target_rows, scalars, False)[0]

@@ -229,3 +229,39 @@ def test_captured_and_replayed(name):
         torch.cuda.synchronize()
         assert torch.equal(out.detach(), want[0])
         same(grads, want[1])
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_forward_mode_is_refused(name):
+    """A tangent on any input is an error, under no_grad too, and not a result without one; plain inputs are as ever."""
+    import torch.autograd.forward_ad as fwd
+    fn, ts, up = cases()[name]
+    want = plain(fn, ts, up)[0]
+    with fwd.dual_level():
+        for i, t in enumerate(ts):
+            dual = [fwd.make_dual(u, torch.ones_like(u)) if i == j else u for j, u in enumerate(ts)]
+            with pytest.raises(NotImplementedError, match="jvp"):
+                fn(*dual)
+            with torch.no_grad(), pytest.raises(NotImplementedError, match="jvp"):
+                fn(*dual)
+        assert torch.equal(fn(*ts), want)
+        ls = leaves(ts)
+        out = fn(*ls)
+        with pytest.raises(NotImplementedError, match="jvp"):
+            torch.autograd.grad(out, ls, fwd.make_dual(up, torch.ones_like(up)), retain_graph=True)
+        same(torch.autograd.grad(out, ls, up), plain(fn, ts, up)[1])
+
+
+@pytest.mark.parametrize("name", NAMES)
+@pytest.mark.parametrize("grad", (False, True))
+@pytest.mark.filterwarnings("ignore::torch.jit.TracerWarning")
+def test_traced(name, grad):
+    """A recorded trace of the norm runs the kernels on its new inputs; the loss is not recorded."""
+    fn, ts, up = cases()[name]
+    record = lambda: torch.jit.trace(fn, tuple(leaves(ts) if grad else ts), check_trace=False)
+    if name.startswith("loss"):
+        with pytest.raises(RuntimeError, match="torch.jit.trace"):
+            record()
+        return
+    new = [2 * t + 1 for t in ts]
+    assert torch.equal(record()(*new), fn(*new))
