@@ -317,6 +317,7 @@ def linear_cross_entropy(x, weight, target, bias=None, reduction="mean", ignore_
     if not x.is_cuda or not target.numel():
         F = torch.nn.functional
         f32 = x.dtype in (torch.bfloat16, torch.float16)
+        x = torch.where((target == ignore_index).unsqueeze(-1), torch.zeros_like(x), x)       # an ignored row holds nothing
         z = F.linear(*((t.float() if t is not None and f32 else t) for t in (x, weight, bias)))
         loss = F.cross_entropy(z.reshape(-1, V), target.reshape(-1), ignore_index=ignore_index, reduction=reduction,
                                label_smoothing=label_smoothing)

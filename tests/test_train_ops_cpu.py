@@ -194,3 +194,26 @@ def test_gradients_with_gaps_that_share_memory():
         assert _share_memory([other, buf[:, 6], buf[11]])
         wide = buf.view(20, 24)[:, ::5].t()                 # columns 0, 5, 10 of the even rows, 3 and 8 of the odd ones
     assert _share_memory([wide, buf[::3, 1:4]]) and not _share_memory([wide, buf[::3, 1:3]])
+
+
+@pytest.mark.parametrize("reduction", ["none", "mean", "sum"])
+def test_ignored_rows_hold_nothing_cpu(reduction):
+    """What an ignored row holds reaches neither the loss nor a gradient; all rows ignored: no gradient."""
+    from pointnetgpd_amd.train_ops import linear_cross_entropy
+    g = torch.Generator().manual_seed(3)
+    x, w, b = torch.randn(2, 6, 8, generator=g), torch.randn(9, 8, generator=g), torch.randn(9, generator=g)
+    y = torch.randint(0, 9, (2, 6), generator=g)
+    y[0, 2] = y[1, 3] = y[1, 5] = -100
+
+    def run(x, y):
+        ls = [t.clone().requires_grad_() for t in (x, w, b)]
+        loss = linear_cross_entropy(ls[0], ls[1], y, bias=ls[2], reduction=reduction, label_smoothing=0.1)
+        return loss.detach(), *torch.autograd.grad(loss, ls, torch.ones_like(loss))
+
+    bad = x.clone()
+    bad[0, 2], bad[1, 3] = math.nan, math.inf
+    want, got = run(x, y), run(bad, y)
+    assert all(torch.equal(u, v) for u, v in zip(want, got)) and not got[1][y == -100].any()
+    loss, *grads = run(bad, torch.full_like(y, -100))
+    assert loss.isnan() if reduction == "mean" else not loss.any()
+    assert not any(t.any() for t in grads)
