@@ -241,7 +241,8 @@ class FlatAdam(torch.optim.Optimizer):
     2-norm, as ``clip_grad_norm_`` before the step would; the factor is applied inside the update, the gradient buffer
     keeps the unclipped values (bias corrections from float64: updates differ from the plain step's by up to 1e-4 of
     themselves in the first steps), and ``grad_norm`` holds the norm (a device scalar that no host wait has
-    touched).  The parameters a step leaves alone do not count."""
+    touched: each step's own tensor, but with ``capturable`` one that every step and replay overwrites).  The parameters a
+    step leaves alone do not count."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, capturable=False, max_grad_norm=None):
         if max_grad_norm is not None and not float(max_grad_norm) >= 0.0:
@@ -371,7 +372,9 @@ class FlatAdam(torch.optim.Optimizer):
         with _lib.device_guard(self.device):
             if self.step_dev is not None:
                 _lib.check(lib.pngpd_adam_step_inc(self.step_dev.data_ptr(), stream), "adam_step_inc")
-            if self.max_grad_norm is not None and runs:
+            if self.max_grad_norm is not None:
+                if self.step_dev is None:                         # (a graph's replays write one place)
+                    self.grad_norm = torch.empty((), device=self.device, dtype=torch.float32)
                 k = len(runs)
                 nbytes = lib.pngpd_grad_clip_workspace_bytes(k)
                 ws = torch.empty(nbytes, device=self.device, dtype=torch.uint8)

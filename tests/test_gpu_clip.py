@@ -315,3 +315,23 @@ def test_gradients_with_gaps_that_overlap():
     assert torch.equal(buf[:, keep], want[:, keep])
     scaled = want[:, 4:6].double() * (0.1 / (exact + 1e-6))             # the factor and the product are rounded once each, the norm too
     assert ((buf[:, 4:6].double() - scaled).abs() <= 2.0 ** -22 * scaled.abs()).all()
+
+
+def test_adam_norms_of_several_steps():
+    """What a step leaves in grad_norm stays that step's; with capturable there is one place, as a replay needs."""
+    from pointnetgpd_amd.optim import FlatAdam
+    for capturable in (False, True):
+        g = torch.Generator(device="cuda").manual_seed(5)
+        p = torch.nn.Parameter(torch.randn(300, generator=g, device="cuda"))
+        opt = FlatAdam([p], max_grad_norm=0.5, capturable=capturable)
+        held, want = [], []
+        for k in range(3):
+            p.grad.copy_((k + 1) * torch.randn(300, generator=g, device="cuda"))
+            want.append(norm64([p.grad], 2))
+            opt.step()
+            held.append(opt.grad_norm)
+        if capturable:
+            assert len({t.data_ptr() for t in held}) == 1
+            held, want = held[-1:], want[-1:]
+        for n, v in zip(held, want):
+            assert abs(n.item() - v) <= 1.01 * U * v
