@@ -8,7 +8,8 @@
 // Forward: every tile of z reduces in registers to (max, sum of exponentials, sum) of its rows; a second launch joins the
 // tiles of a row.  Backward: z is computed again, a piece of the vocabulary at a time; the piece's g (rounded once to the
 // inputs' type, as the operand of the matrix instructions has to be) lives in a workspace of bounded size, and two products
-// turn it into the piece's dW and its share of dx.  8 T D V operations for both directions where keeping T V logits takes
+// turn it into the piece's dW and its share of dx.  db sums g in float32, where it is made, before that rounding (and without
+// the second walk over it: 8 in the place of 38 us of a 268 us piece of 8192 rows).  8 T D V operations for both directions where keeping T V logits takes
 // 6: the price of not keeping them, which pays for 16 bits; float32's matrix rate makes keeping them the better way, up to 1 GB.
 // Bound by the matrix cores for T in the hundreds and above, by reading W below.
 // Rows whose target is ignored are left out of the products (from LCE_ROWS rows on): a list of the kept ones is made on
@@ -17,7 +18,7 @@
 // coefficients c_t are scaled to at most 1 the same way; both factors come back in float32 on the way out.
 // Measured (bf16; a large library product reaches 1250 TFLOP/s on this card): 6,550 kept rows of 8192, D 1024, V 100,000: statistics
 // 1.33 ms = 1010 TFLOP/s; of each of 6 pieces g 261 us = 860, dx's product 268 us = 840, dW's 223 us (and 99 for the classes
-// past its rounds) = 930, db 33 us: 5.7 ms in all.  No LDS bank conflict; of the statistics' time the epilogue is 17 %; rows of x
+// past its rounds) = 930, db 5 us: 5.75 ms in all.  No LDS bank conflict; of the statistics' time the epilogue is 17 %; rows of x
 // or W other than a power of two apart change nothing (1480 us at 1024 and at 1088 elements, all rows).  64 rows, D 256, V 6500,
 // float32: eight launches of 3 to 13 us.
 #include <algorithm>
@@ -55,7 +56,8 @@ struct LceArgs {
     float *z;                              // (T, ldz) the logits kept for the backward pass, or NULL
     int ldz;
     void *g;
-    int v0, vc, ldg;                       // the launch's classes (g starts at the first one)
+    float *db;                             // (tiles of rows, ldg): column sums of g's rows, before it is rounded, or NULL
+    int v0, vc, ldg;                       // the launch's classes (g and db start at the first one)
 };                                         // (T above, but for target: by place among the kept rows)
 
 // The kept rows in order: 8 targets a thread and round, the places by a scan over the workgroup.
@@ -434,6 +436,16 @@ __device__ __forceinline__ void lce_coef(const LceCoef &a) {
     }
 }
 
+// one step of a sum over lanes that spreads the values over them: of N values a lane keeps half, and adds its partner's
+template <int N> __device__ __forceinline__ void lce_spread(float (&v)[16], int lane, int k) {
+    const bool up = lane & k;
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+        const float keep = up ? v[N / 2 + i] : v[i], send = up ? v[i] : v[N / 2 + i];
+        v[i] = keep + __shfl_xor(send, k);
+    }
+}
+
 template <int DT, int BM, int BN, int WGM, int WGN, int PIPE>
 __global__ __launch_bounds__(WGM * WGN * 64, 2) void lce_grad_kernel(const LceArgs a) {
     typedef LceCore<DT, false, false, BM, BN, WGM, WGN, PIPE> Core;
@@ -441,6 +453,8 @@ __global__ __launch_bounds__(WGM * WGN * 64, 2) void lce_grad_kernel(const LceAr
     typedef typename elem<DT>::t E;
     extern __shared__ __align__(16) char smem[];
     Side *side = (Side *)(smem + Core::LDS);
+    float *sh = (float *)(side + 2);                              // [WGN][BM]
+    static_assert(WGN * BM * 4 <= WGM * BN * 12, "the room that lce_z_shape allows for");
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
     const int wm = (wave % WGM) * Core::WM, wn = (wave / WGM) * Core::WN;
     const int T = a.rows.count(), nt = (T + BN - 1) / BN, total = a.mt * nt;
@@ -534,81 +548,81 @@ __global__ __launch_bounds__(WGM * WGN * 64, 2) void lce_grad_kernel(const LceAr
                 }
             }
         }
+        // db's share of the tile, in float32 whatever g is stored in: a row's 16 values of 32 lanes end up one a lane pair
+        if (a.db) {
+#pragma unroll
+            for (int i = 0; i < Core::FM; ++i) {
+                float v[16];
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    v[r] = c.acc[i][0][r];
+#pragma unroll
+                    for (int j = 1; j < Core::FN; ++j) v[r] += c.acc[i][j][r];
+                }
+                lce_spread<16>(v, lane, 16); lce_spread<8>(v, lane, 8); lce_spread<4>(v, lane, 4); lce_spread<2>(v, lane, 2);
+                const float u = v[0] + __shfl_xor(v[0], 1);
+                const int r = (lane & 31) >> 1;
+                if (!(lane & 1)) sh[(wave / WGM) * BM + vl + 32 * i + (r & 3) + 8 * (r >> 2)] = u;
+            }
+            lce_lds_barrier();
+            for (int m = threadIdx.x; m < BM; m += Core::THREADS) {
+                float u = sh[m];
+#pragma unroll
+                for (int k = 1; k < WGN; ++k) u += sh[k * BM + m];
+                a.db[(size_t)(n0 / BN) * a.ldg + m0 + m] = u;
+            }
+        }
         if (at >= total) return;
     }
 }
 
-// lce_grad_kernel's epilogue on kept logits: four classes a thread, 1024 of one row a workgroup.
+// lce_grad_kernel's epilogue on kept logits: four classes a thread, 1024 of `share` rows a workgroup.
 template <int DT>
-__global__ __launch_bounds__(256) void lce_kept_grad_kernel(const LceArgs a, int cols) {
+__global__ __launch_bounds__(256) void lce_kept_grad_kernel(const LceArgs a, int cols, int share) {
     typedef typename elem<DT>::t E;
-    const int per = (cols + 1023) / 1024, k = blockIdx.x / per, v = (blockIdx.x - k * per) * 1024 + threadIdx.x * 4;
-    if (k >= a.rows.count() || v >= cols) return;
-    const float m = a.stat[2 * (size_t)k], co = a.coef[k], ks = co / a.stat[2 * (size_t)k + 1], kf = co * (a.smooth / (float)a.V);
-    const long long y = a.target[a.rows.row(k)] - a.v0;           // (an ignored row's co is 0)
-    const f32x4 z = *(const f32x4 *)(a.z + (size_t)k * a.ldz + a.v0 + v);
-    float g[4];
+    const int per = (cols + 1023) / 1024, part = blockIdx.x / per, v = (blockIdx.x - part * per) * 1024 + threadIdx.x * 4;
+    const int k0 = part * share, k1 = min(a.rows.count(), k0 + share);
+    if (k0 >= k1 || v >= cols) return;
+    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 2
+    for (int k = k0; k < k1; ++k) {
+        const float m = a.stat[2 * (size_t)k], co = a.coef[k], ks = co / a.stat[2 * (size_t)k + 1], kf = co * (a.smooth / (float)a.V);
+        const long long y = a.target[a.rows.row(k)] - a.v0;       // (an ignored row's co is 0)
+        const f32x4 z = *(const f32x4 *)(a.z + (size_t)k * a.ldz + a.v0 + v);
+        f32x4 g;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        const float p = __builtin_amdgcn_exp2f(lce_far<DT>(m) ? (z[e] - m) * LOG2E : fmaf(z[e], LOG2E, -(m * LOG2E)));
-        g[e] = fmaf(p, ks, -kf) - (y == v + e ? co * (1.f - a.smooth) : 0.f);
-        if (co == 0.f || v + e >= a.vc) g[e] = 0.f;
+        for (int e = 0; e < 4; ++e) {
+            const float p = __builtin_amdgcn_exp2f(lce_far<DT>(m) ? (z[e] - m) * LOG2E : fmaf(z[e], LOG2E, -(m * LOG2E)));
+            g[e] = fmaf(p, ks, -kf) - (y == v + e ? co * (1.f - a.smooth) : 0.f);
+            if (co == 0.f || v + e >= a.vc) g[e] = 0.f;
+        }
+        E *o = (E *)a.g + (size_t)k * a.ldg + v;
+        if constexpr (DT == PNGPD_F32) *(f32x4 *)o = g;
+        else *(uint2 *)o = lce_half4<DT>(g[0], g[1], g[2], g[3]);
+        sum += g;
     }
-    E *o = (E *)a.g + (size_t)k * a.ldg + v;
-    if constexpr (DT == PNGPD_F32) *(f32x4 *)o = f32x4{g[0], g[1], g[2], g[3]};
-    else *(uint2 *)o = lce_half4<DT>(g[0], g[1], g[2], g[3]);
+    if (a.db) *(f32x4 *)(a.db + (size_t)part * a.ldg + v) = sum;
 }
 
-// db of a piece: column sums of g (as rounded), in two steps.  A thread takes 16 bytes of a row and every 32nd row of the
-// workgroup's share; the shares' sums (S, ldg) in float32, then one thread a class.
+// db of a piece: the sums (S, ldg) joined in fp64, 32 classes by 8 of the S a workgroup.  A sum is of `rows0` kept rows, from
+// class `cut` on of `rows1`.
 template <int DT>
-__global__ __launch_bounds__(256) void lce_db_kernel(const void *__restrict__ gp, LceRows rows, int ldg, int share, int cols,
-                                                     float *__restrict__ out, const float *__restrict__ scale,
-                                                     void *__restrict__ db, int vc, int f32) {
-    constexpr int EPC = DT == PNGPD_F32 ? 4 : 8, X = 8;           // 8 chunks by 32 rows
-    __shared__ float sh[32][X * EPC + 1];
-    const int T = rows.count(), cx = threadIdx.x % X, ry = threadIdx.x / X, v = (blockIdx.x * X + cx) * EPC;
-    const int t0 = blockIdx.y * share, t1 = min(T, t0 + share);
-    const typename elem<DT>::t *g = (const typename elem<DT>::t *)gp + v;
-    float s[EPC];
-#pragma unroll
-    for (int e = 0; e < EPC; ++e) s[e] = 0.f;
-    if (v < cols) {
-#pragma unroll 4
-        for (int t = t0 + ry; t < t1; t += 32) {
-            const uint4 q = *(const uint4 *)(g + (size_t)t * ldg);
-            const unsigned w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-            for (int e = 0; e < EPC; ++e) {
-                if constexpr (DT == PNGPD_F32) s[e] += __uint_as_float(w[e]);
-                else s[e] += half_to_f(DT, (u16)(w[e >> 1] >> (16 * (e & 1))));
-            }
-        }
-    }
-#pragma unroll
-    for (int e = 0; e < EPC; ++e) sh[ry][cx * EPC + e] = s[e];
-    __syncthreads();
-    if (threadIdx.x < X * EPC) {
-        float u = 0.f;
-        for (int k = 0; k < 32; ++k) u += sh[k][threadIdx.x];
-        const int col = blockIdx.x * X * EPC + threadIdx.x;
-        if (gridDim.y > 1) {
-            if (col < cols) out[(size_t)blockIdx.y * ldg + col] = u;
-        } else if (col < vc) {                                     // one share: done
-            u *= *scale;
-            if (f32) ((float *)db)[col] = u;
-            else st_elem<DT>((typename elem<DT>::t *)db + col, u);
-        }
-    }
-}
-template <int DT>
-__global__ __launch_bounds__(256) void lce_db_join_kernel(const float *__restrict__ part, int S, int ldg, int vc,
-                                                          const float *__restrict__ scale, void *__restrict__ db, int f32) {
-    const int v = blockIdx.x * 256 + threadIdx.x;
-    if (v >= vc) return;
+__global__ __launch_bounds__(256) void lce_db_join_kernel(const float *__restrict__ part, LceRows rows, int rows0, int cut, int rows1,
+                                                          int ldg, int vc, const float *__restrict__ scale, void *__restrict__ db,
+                                                          int f32) {
+    __shared__ double sh[8][32];
+    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5, v = blockIdx.x * 32 + tx, per = v < cut ? rows0 : rows1;
+    const int S = (rows.count() + per - 1) / per;
     double s = 0.0;
-    for (int k = 0; k < S; ++k) s += (double)part[(size_t)k * ldg + v];
-    const float o = (float)s * *scale;
+    if (v < vc) {
+#pragma unroll 8
+        for (int k = ty; k < S; k += 8) s += (double)part[(size_t)k * ldg + v];
+    }
+    sh[ty][tx] = s;
+    __syncthreads();
+    if (ty || v >= vc) return;
+    for (int k = 1; k < 8; ++k) s += sh[k][tx];
+    const float o = (float)(s * (double)*scale);
     if (f32) ((float *)db)[v] = o;
     else st_elem<DT>((typename elem<DT>::t *)db + v, o);
 }
@@ -794,7 +808,7 @@ struct LcePlan {
     int Dp, fshape, fmt, fcut, padx, padw;
     int piece, large, ldg, xshape, splits; // classes of a piece, at most of the last one
     int wsplits;                           // dW: cuts of the rows
-    int share, shares;                     // db: rows of a share, shares
+    int share;                             // kept logits: rows of a workgroup (and of a sum of db)
     size_t o_part, o_ps, o_zt, o_row, o_x, o_w, o_coef, o_scale, o_g, o_dx, o_dw, o_db, bytes;
 };
 
@@ -848,13 +862,10 @@ static LcePlan lce_plan(const Lce *a, bool bwd) {
         const long long vmost = std::min(a->V, p.large), small = (long long)lce_cdiv(p.Dp, 64) * lce_cdiv(vmost, 64);
         p.wsplits = (int)std::max(1ll, small < 128 ? std::min(256 / small, (long long)a->T / 512) : 1);
         if (p.wsplits > 1) p.o_dw = take((size_t)p.wsplits * vmost * p.Dp * 4);
-        // db: about 1024 workgroups
-        const long long across = lce_cdiv(p.piece, es == 4 ? 32 : 64);
-        long long n2 = 1024 / across;
-        if (n2 > a->T / 64) n2 = a->T / 64;
-        if (n2 < 1) n2 = 1;
-        p.share = lce_cdiv(a->T, (int)n2); p.shares = lce_cdiv(a->T, p.share);
-        p.o_db = take((size_t)p.shares * p.ldg * 4);
+        // kept logits: about 1024 workgroups;  db: a sum a workgroup there, a tile of rows otherwise (the small tile's: 64 of them,
+        // or all that there are)
+        p.share = (int)std::max(1ll, (long long)a->T * lce_cdiv(p.piece, 1024) / 1024);
+        if (a->bias) p.o_db = take((size_t)lce_cdiv(a->T, a->z ? p.share : 64) * p.ldg * 4);
     }
     p.bytes = at;
     return p;
@@ -978,29 +989,28 @@ template <int DT> static int lce_backward(const Lce *a, const LcePlan &p, hipStr
         const int gshape = lce_shape(vc, a->T), wide = lce_shape(p.Dp, vc, 192), wshape = wide == 2 ? 1 : wide;
         const int cols = (vc + 63) / 64 * 64;                      // columns of g that are written (zeros past vc)
         const int gcut = gshape ? vc : lce_cut(vc, lce_cdiv(a->T, 256));
-        k.v0 = v0; k.vc = gcut; k.g = ws + p.o_g;
+        float *sums = (float *)(ws + p.o_db);
+        k.v0 = v0; k.vc = gcut; k.g = ws + p.o_g; k.db = a->db ? sums : nullptr;
         int rc;
         if (a->z) {
             k.vc = vc;
-            const long long grid = (long long)a->T * ((cols + 1023) / 1024);
+            const long long grid = (long long)lce_cdiv(a->T, p.share) * ((cols + 1023) / 1024);
             if (grid > 0x7fffffffll) return PNGPD_ERR_UNSUPPORTED;
-            hipLaunchKernelGGL(lce_kept_grad_kernel<DT>, dim3((unsigned)grid), dim3(256), 0, st, k, cols);
+            hipLaunchKernelGGL(lce_kept_grad_kernel<DT>, dim3((unsigned)grid), dim3(256), 0, st, k, cols, p.share);
             rc = pngpd_launch_status();
         } else rc = lce_z<DT, true>(k, gshape, st);
         if (rc) return rc;
         if (!a->z && gcut < vc) {
-            k.v0 = v0 + gcut; k.vc = vc - gcut; k.g = (E *)(ws + p.o_g) + gcut;
+            k.v0 = v0 + gcut; k.vc = vc - gcut; k.g = (E *)(ws + p.o_g) + gcut; k.db = a->db ? sums + gcut : nullptr;
             if ((rc = lce_z<DT, true>(k, 1, st))) return rc;
         }
         const E *g = (const E *)(ws + p.o_g);
         const E *w = (const E *)k.w.p + (long long)v0 * k.w.ld;
         if (a->db) {
-            float *sums = (float *)(ws + p.o_db);
             void *db = a->bias_dtype == PNGPD_F32 ? (void *)((float *)a->db + v0) : (void *)((E *)a->db + v0);
-            hipLaunchKernelGGL(lce_db_kernel<DT>, dim3((unsigned)lce_cdiv(cols, DT == PNGPD_F32 ? 32 : 64), p.shares), dim3(256), 0, st,
-                               g, k.rows, p.ldg, p.share, cols, sums, scale, db, vc, a->bias_dtype == PNGPD_F32);
-            if (p.shares > 1) hipLaunchKernelGGL(lce_db_join_kernel<DT>, dim3((unsigned)lce_cdiv(vc, 256)), dim3(256), 0, st, sums, p.shares, p.ldg,
-                               vc, scale, db, a->bias_dtype == PNGPD_F32);
+            hipLaunchKernelGGL(lce_db_join_kernel<DT>, dim3((unsigned)lce_cdiv(vc, 32)), dim3(256), 0, st, sums, k.rows,
+                               a->z ? p.share : LCE_BN[gshape], a->z ? vc : gcut, LCE_BN[1], p.ldg, vc, scale, db,
+                               (int)(a->bias_dtype == PNGPD_F32));
         }
         if (a->dx) {
             LceOut o = {};

@@ -363,3 +363,22 @@ def test_run_together():
         norm = torch.sqrt(sum((r ** 2).sum() for r in grads)).item()
         assert abs(opt.grad_norm.item() - norm) <= 2.0 ** -16 * norm and norm > 0.05
         assert all(0 < (p.detach() - o).abs().max() <= 0.011 for p, o in zip(ps, before))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("T,D,V", [(1, 40, 300), (9, 40, 300), (60, 256, 900), (130, 48, 700), (700, 96, 1500), (1000, 96, 9000),
+                                   (4200, 64, 17_000), (70_001, 16, 2), (200, 3000, 40_000)])
+def test_bias_gradient_is_not_rounded_to_16_bits(T, D, V, dtype):
+    """dx and dW take g rounded to the inputs' type, db sums it as float32: to a float32 bias the error holds no step of 16
+    bits.  The reference's bounds for the same values as float32 inputs, and 20 additions one after the other (a tile's rows:
+    2 in a lane, 32 lanes, 4 waves; with kept logits at most 8 rows here) of |g| <= |c| (p + the target's share)."""
+    x, w, _, y, c = data(T, D, V, dtype, 50, bias=False, ignored=0.2 if T > 4 else 0.0)
+    g = torch.Generator(device="cuda").manual_seed(51)
+    b = torch.randn(V, generator=g, device="cuda")
+    got = run(x, w, b, y, c, "none", 0.1)["db"]
+    assert got.dtype == F32
+    want, bound = reference(x.float(), w.float(), b, y, c, "none", 0.1)["db"]
+    size = torch.softmax(x.double() @ w.double().t() + b.double(), 1) + 0.1 / V
+    size.scatter_add_(1, y.clamp_min(0).unsqueeze(1), torch.full((T, 1), 0.9, device="cuda", dtype=torch.double))
+    size = (torch.where(y != -100, c, torch.zeros_like(c)).double().abs().unsqueeze(1) * size).sum(0)
+    check(got, want, bound + 20 * U32 * size, "db")
