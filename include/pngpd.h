@@ -495,8 +495,10 @@ int pngpd_adam_flat_clip(float *p, const float *g, float *m, float *v, const lon
  * (F.nll_loss(F.log_softmax(F.linear(x, W, bias))), main_1v.py:73-74 with pointnet.py:193-194, for a head of any width).
  * Rows' channels adjacent; ldx, ldw in elements, any (rows at 16-byte addresses of whole 16 bytes are read in place,
  * others are copied into the workspace first).  A target outside [0,V) that is not ignore_index gives a NaN loss and NaN
- * gradients.  Deterministic.  The workspace is bounded in V: a piece's gradient of the logits, 256 MB at most unless 256
- * classes of all rows take more, or up to 1 GB where that lets dW's product fill the CUs.  T and V below 2^30, D up to 2^22.
+ * gradients.  Deterministic.  Workspace: forward 8 bytes (12 with smoothing) for each row and tile of 256 classes, of 128 or 64
+ * where there are few; backward a piece's gradient of the logits (320 MB at most, 1.25 GB where that lets dW's product
+ * fill the CUs, 256 classes of all rows where those take more), a copy of x, and float32 sums of dx (64 MB or the size of x); both a
+ * copy of an operand that cannot be read in place (forward also x of 512 rows or more over 4 GB).  T and V below 2^30, D up to 2^22.
  *   forward   writes stat (T,2), kept (1) and rows (pngpd_lce_rows_ints(T) values, NULL where that is 0: the list of the
  *             rows that are not ignored), which the backward call reads, and loss: (T), or one value; and z, where it is
  *             not NULL (pngpd_lce_z_bytes of room, 0: must be NULL): the logits in float32, only where reading them again

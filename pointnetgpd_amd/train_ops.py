@@ -4,8 +4,9 @@
                              (PointNetGPD/model/pointnet.py:29-31,144-147) needs two samples a rank and keeps statistics of
                              its replica; this one's are of each sample alone.
 * ``linear_cross_entropy`` — the loss of a linear classifier of any width, F.nll_loss(F.log_softmax(F.linear(...)))
-                             (main_1v.py:73-74, pointnet.py:193-194), without rows x classes of logits in memory: codebooks of
-                             grasps, one class for each point of a scene.
+                             (main_1v.py:73-74, pointnet.py:193-194), without all rows x classes of logits in memory (what is
+                             kept of them, and how not to: ``keep_logits``): codebooks of grasps, one class for each point of
+                             a scene.
 
 CUDA tensors run the HIP kernels of libpngpd (a missing library raises), CPU tensors the same formulas in ATen operations.
 The gradients are those of the formulas; they are not differentiable again, and forward-mode derivatives raise on CUDA.
@@ -214,9 +215,11 @@ def _rows(v):
     return v if (v.shape[1] == 1 or v.stride(1) == 1) and (v.shape[0] == 1 or v.stride(0) >= v.shape[1]) else v.contiguous()
 
 
-def _where(saved):
+def _where(x, w, bias, target, stat, rows, z):
     """Where tensors lie and how: a descriptor made for them holds as long as this is the same."""
-    return [0 if t is None else (t.data_ptr(), t.stride()) for t in saved]
+    return (x.data_ptr(), x.stride(), w.data_ptr(), w.stride(), target.data_ptr(), target.stride(), stat.data_ptr(), stat.stride(),
+            bias is None or (bias.data_ptr(), bias.stride()), rows is None or (rows.data_ptr(), rows.stride()),
+            z is None or (z.data_ptr(), z.stride()))
 
 
 def _lce_args(scalars, x, w, bias, target, stat, rows, z):
@@ -230,13 +233,13 @@ def _lce_args(scalars, x, w, bias, target, stat, rows, z):
                         z=None if z is None else z.data_ptr())
 
 
-def _lce_fwd(x, w, bias, target, scalars, train):
-    """-> loss, what the backward pass reads (``train``), the call's arguments."""
+def _lce_fwd(x, w, bias, target, scalars, keep):
+    """-> loss, what the backward pass reads (the logits among it where ``keep`` and they are few), the call's arguments."""
     lib, dev, T = _lib.load(), x.device, x.shape[0]
     stat = torch.empty(2 * T + 1, device=dev, dtype=torch.float32)             # (T,2), then the kept rows' number
     n = lib.pngpd_lce_rows_ints(T)
     rows = torch.empty(n, device=dev, dtype=torch.int32) if n else None
-    n = lib.pngpd_lce_z_bytes(T, x.shape[1], w.shape[0], DTYPES[x.dtype]) if train else 0
+    n = lib.pngpd_lce_z_bytes(T, x.shape[1], w.shape[0], DTYPES[x.dtype]) if keep else 0
     z = torch.empty(n // 4, device=dev, dtype=torch.float32) if n else None
     loss = torch.empty((T,) if scalars[0] == 0 else (), device=dev, dtype=torch.float32)
     a = _lce_args(scalars, x, w, bias, target, stat, rows, z)
@@ -250,7 +253,7 @@ def _lce_bwd(ctx, dloss):
     made, where, nbytes, dev = ctx.call
     need = ctx.needs_input_grad
     dloss = _flat(dloss)
-    if _where(saved) == where:
+    if _where(*saved) == where:
         a = _lib.LceArgs.from_buffer_copy(made)                                # a copy: two threads may run one node
     else:                                                                      # saved tensors that a hook has moved
         x, w = _rows(x), _rows(w)
@@ -263,37 +266,45 @@ def _lce_bwd(ctx, dloss):
     a.dloss = dloss.data_ptr()
     a.dx, a.dw, a.db = (None if t is None else t.data_ptr() for t in (dx, dw, db))
     _lce_call(_lib.load().pngpd_lce_bwd, "pngpd_lce_bwd", a, nbytes, dev)
-    return dx, dw, db, None, None
+    return dx, dw, db, None, None, None
 
 
 class LinearCrossEntropyFn(torch.autograd.Function):
     """x (T,D), w (V,D), target (T) -> loss (T) or (); T, V, D > 0, channels adjacent."""
 
     @staticmethod
-    def forward(ctx, x, w, bias, target, scalars):
-        loss, made, a = _lce_fwd(x, w, bias, target, scalars, True)
+    def forward(ctx, x, w, bias, target, scalars, keep):
+        loss, made, a = _lce_fwd(x, w, bias, target, scalars, keep)
         saved = (x, w, bias, target, *made)
         ctx.scalars = scalars
-        ctx.call = (a, _where(saved), _lib.load().pngpd_lce_workspace_bytes(ctypes.addressof(a), 1), x.device)
+        ctx.call = (a, _where(*saved), _lib.load().pngpd_lce_workspace_bytes(ctypes.addressof(a), 1), x.device)
         ctx.save_for_backward(*saved)
         return loss
 
     backward = staticmethod(_once(_lce_bwd))
 
 
-def linear_cross_entropy(x, weight, target, bias=None, reduction="mean", ignore_index=-100, label_smoothing=0.0):
-    """``F.cross_entropy(F.linear(x, weight, bias), target, ...)`` without the logits: x (..., D), weight (V, D), target
+def linear_cross_entropy(x, weight, target, bias=None, reduction="mean", ignore_index=-100, label_smoothing=0.0,
+                         keep_logits=True):
+    """``F.cross_entropy(F.linear(x, weight, bias), target, ...)`` without all of the logits: x (..., D), weight (V, D), target
     (...) int64, bias (V) or None.  The forward pass reduces the logits tile by tile, the backward pass computes them again
-    a piece of the classes at a time, so memory grows with the rows and not with rows x classes (float32 logits of up to
-    1 GB, and those of a few rows of 16 bits up to 256 MB, are kept for the backward pass: reading them is the faster way).
+    a piece of the classes at a time.  Logits that are few are kept in float32 from the forward to the backward pass, since
+    reading them is the faster way: up to 1 GB of float32 inputs', up to 256 MB of at most D / 4 rows of 16 bits.
+    ``keep_logits=False`` keeps none: then a call holds 16 bytes a row until its backward pass, beside its inputs (or the
+    copies that were needed of them).  Workspaces while a call runs: forward 8 bytes (12 with smoothing) for each row and tile
+    of 256 classes, smaller tiles where there are few; backward the logits' gradient of a piece (320 MB at most, 1.25 GB where
+    less would leave CUs idle, 256 classes where those take more) and copies of x in its type and in float32; both a copy of
+    an operand whose rows are not whole 16-byte pieces at 16-byte addresses, forward also of 512 or more rows over 4 GB.
 
     Returns float32: a scalar for ``reduction`` "mean" (over the rows whose target is not ``ignore_index``; NaN if there is
     none, with zero gradients) or "sum", target's shape for "none".  Ignored rows have loss 0 and no gradient, whatever
     their x holds.  ``label_smoothing`` in [0, 1] as in ``F.cross_entropy``.  A target outside [0, V) gives a NaN loss
-    and NaN gradients (there is no host check: it would wait for the device).  x and weight of one type, float32 (exact
-    fp32 products), bfloat16 or float16 (fp32 accumulation; the logits' gradient is rounded once to that type before its
-    two products); bias of the same type or float32.  A bias of -inf takes a class out.  Rows with adjacent channels are
-    read in place where they start at 16-byte addresses, others through a copy."""
+    and NaN gradients on the GPU (there is no host check: it would wait for the device), an IndexError on the CPU.  x and
+    weight of one type, float32 (exact fp32 products), bfloat16 or float16 (fp32 accumulation; the logits' gradient is
+    rounded once to that type before its two products, and not for the bias's); bias of the same type or float32.  float16
+    holds that gradient over the largest row weight, so a row whose weight is less than 2^-20 of it loses digits of its
+    dx.  A bias of -inf takes a class out.  Rows with adjacent channels are read in place where they start at 16-byte
+    addresses, others through a copy."""
     if not (isinstance(x, torch.Tensor) and isinstance(weight, torch.Tensor)) or x.dim() < 1 or weight.dim() != 2:
         raise RuntimeError("linear_cross_entropy: x must have shape (..., D) and weight (V, D)")
     V, D = weight.shape
@@ -332,7 +343,7 @@ def linear_cross_entropy(x, weight, target, bias=None, reduction="mean", ignore_
     rows, bias = [_rows(x.reshape(-1, D)), _rows(weight)], _flat(bias)
     target_rows, scalars = target.reshape(-1).contiguous(), (REDUCTIONS[reduction], ignore_index, label_smoothing)
     if _wants_node(*rows, bias):
-        loss = LinearCrossEntropyFn.apply(*rows, bias, target_rows, scalars)
+        loss = LinearCrossEntropyFn.apply(*rows, bias, target_rows, scalars, bool(keep_logits))
     else:
         loss = _lce_fwd(*rows, bias, target_rows, scalars, False)[0]
     return loss.reshape(target.shape) if reduction == "none" else loss

@@ -382,3 +382,22 @@ def test_bias_gradient_is_not_rounded_to_16_bits(T, D, V, dtype):
     size.scatter_add_(1, y.clamp_min(0).unsqueeze(1), torch.full((T, 1), 0.9, device="cuda", dtype=torch.double))
     size = (torch.where(y != -100, c, torch.zeros_like(c)).double().abs().unsqueeze(1) * size).sum(0)
     check(got, want, bound + 20 * U32 * size, "db")
+
+
+@pytest.mark.parametrize("dtype,T", [(F32, 600), (F32, 60), (BF16, 60), (F16, 8)])
+def test_logits_are_kept_or_not(dtype, T):
+    """keep_logits=False: what a call holds until its backward pass does not grow with the classes, and the results are the
+    operator's; otherwise few logits are held."""
+    from pointnetgpd_amd.train_ops import linear_cross_entropy
+    x, w, b, y, c = data(T, 256, 20_000, dtype, 60)
+    want = reference(x, w, b, y, c, "mean", 0.1)
+    for keep in (True, False):
+        leaves = [t.detach().requires_grad_() for t in (x, w, b)]
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        loss = linear_cross_entropy(leaves[0], leaves[1], y, bias=leaves[2], label_smoothing=0.1, keep_logits=keep)
+        held = torch.cuda.memory_allocated() - before
+        assert held >= T * 20_000 * 4 if keep else held <= 16 * T + 4 * 1024, held
+        got = dict(zip(("loss", "dx", "dw", "db"), (loss.detach(), *torch.autograd.grad(loss, leaves, c[0]))))
+        for k, v in got.items():
+            check(v, *want[k], k)

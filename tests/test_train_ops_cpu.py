@@ -217,3 +217,31 @@ def test_ignored_rows_hold_nothing_cpu(reduction):
     loss, *grads = run(bad, torch.full_like(y, -100))
     assert loss.isnan() if reduction == "mean" else not loss.any()
     assert not any(t.any() for t in grads)
+
+
+@pytest.mark.parametrize("dtype", [0, 1])
+def test_workspaces_of_the_loss_are_what_the_header_says(dtype):
+    """Forward: 8 bytes a row and tile of classes (12 with smoothing), and the target's logit and the loss of a row, and a copy of
+    many rows that span 4 GB; backward: a
+    piece's gradient of the logits, x in its type and in float32 (64 MB at least), sums for the bias of a 32nd of the piece."""
+    import ctypes
+    from pointnetgpd_amd import _lib
+    lib, es = _lib.load(), 4 if dtype == 0 else 2
+    mb = 1 << 20
+    for T in (1, 30, 64, 500, 1024, 5000, 8192, 40_000, 300_000, 1 << 20):
+        for V in (2, 100, 3000, 33_000, 100_000):
+            for D in (16, 256, 1024, 2048):
+                for bias in (None, 256):
+                    a = _lib.LceArgs(x=256, w=256, bias=bias, target=256, ldx=D, ldw=D, T=T, D=D, V=V, dtype=dtype, bias_dtype=0,
+                                     reduction=1, stat=256, kept=256, rows=256 if T >= 512 else None)
+                    for smoothing, size in ((0.0, 8), (0.1, 12)):
+                        a.smoothing = smoothing
+                        n = lib.pngpd_lce_workspace_bytes(ctypes.addressof(a), 0)
+                        most = size * T * (V / 64 + 1) if T * V < 1 << 25 else size * T * (V / 128 + 1)
+                        copy = T * D * es if T >= 512 and T * D * es >= 4e9 else 0
+                        assert 0 < n <= most + copy + 8 * T + 2048, (T, V, D, n)
+                    n = lib.pngpd_lce_workspace_bytes(ctypes.addressof(a), 1)
+                    piece = max(1.25 * 1024 * mb, T * (256 + 128) * es)
+                    assert n <= (1 + 1 / 16) * piece + T * D * (es + 4) + 4 * T + 72 * mb, (T, V, D, n)
+                    if T * min(V, 256) * es <= 256 * mb and V * T * es <= 256 * mb:       # one piece: no more than its logits
+                        assert n <= (1 + 1 / 16) * T * (V + 256 + 128) * es + T * D * (es + 4) + 4 * T + 72 * mb, (T, V, D, n)
