@@ -270,6 +270,7 @@ class FlatAdam(torch.optim.Optimizer):
         self.capturable = bool(capturable)
         self.max_grad_norm = None if max_grad_norm is None else float(max_grad_norm)
         self.grad_norm = torch.zeros((), device=dev, dtype=torch.float32) if max_grad_norm is not None else None
+        self._clip_ws = None
         # device-resident step count / learning rate for captured graphs (StepLR rewrites group["lr"] in place)
         self.step_dev = torch.zeros((), device=dev, dtype=torch.float32) if capturable else None
         self._step = 0
@@ -376,15 +377,17 @@ class FlatAdam(torch.optim.Optimizer):
                 if self.step_dev is None:                         # (a graph's replays write one place)
                     self.grad_norm = torch.empty((), device=self.device, dtype=torch.float32)
                 k = len(runs)
-                nbytes = lib.pngpd_grad_clip_workspace_bytes(k)
-                ws = torch.empty(nbytes, device=self.device, dtype=torch.uint8)
+                if self._clip_ws is None:                         # kept: two steps at once would race for the parameters too
+                    n = lib.pngpd_grad_clip_workspace_bytes(len(self._params))         # (a run holds a parameter at least)
+                    self._clip_ws = torch.empty(n, device=self.device, dtype=torch.uint8)
+                ws = self._clip_ws
                 _lib.check(lib.pngpd_adam_flat_clip(self.flat_p.data_ptr(), self.flat_g.data_ptr(), self.flat_m.data_ptr(),
                                                     self.flat_v.data_ptr(), (ctypes.c_longlong * k)(*[lo for lo, _ in runs]),
                                                     (ctypes.c_longlong * k)(*[n for _, n in runs]), k, lr_host, lr_dev,
                                                     float(b1), float(b2), float(eps), float(self._step),
                                                     self.step_dev.data_ptr() if self.step_dev is not None else None,
                                                     float(grad_scale), grad_div.data_ptr() if grad_div is not None else None,
-                                                    self.max_grad_norm, self.grad_norm.data_ptr(), ws.data_ptr(), nbytes,
+                                                    self.max_grad_norm, self.grad_norm.data_ptr(), ws.data_ptr(), ws.numel(),
                                                     stream), "adam_flat_clip")
                 runs = []
             for lo, n in runs:
