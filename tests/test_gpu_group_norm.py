@@ -315,3 +315,38 @@ def test_spreads_whose_squares_leave_float32(shape, groups, dtype, size):
     want = reference(x, dy, w, b, groups, "silu", eps=0.0)
     for k, v in got.items():
         check(v, *want[k], k)
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+def test_activations_relative_to_their_tails(act):
+    """w = 0 makes z = b exactly and db = dy slope(z): values and slopes out to |z| = 12 with bounds that follow them.
+    silu: the exponential's argument carries 2 |z| u, the exponential and the reciprocal 2^-23 each, products and sums one u
+    each.  gelu: the published polynomial's own error there, in 64 bits, and of p(t) exp(-z^2/2): 2 z^2 u of the argument,
+    2^-23 of the exponential and of the reciprocal, whose error the polynomial multiplies by its condition (below 8)."""
+    C = 28_001
+    z = torch.linspace(-12, 12, C, device="cuda")
+    x = torch.randn(1, 1, C, generator=torch.Generator(device="cuda").manual_seed(90), device="cuda")
+    dy = torch.linspace(0.5, 2.0, C, device="cuda").flip(0).view(1, 1, C)
+    got = run(x, torch.zeros_like(z), z, 1, act, dy)
+    z, dy = z.double(), dy.double().view(C)
+    if act == "silu":
+        y, slope = value_and_slope(z, act)
+        s = torch.sigmoid(z)
+        ey = U32 * (2 * z.abs() + 16) * y.abs()
+        es = U32 * (2 * z.abs() + 16) * s * (1 + z.abs())
+    else:
+        e, v = torch.exp(-0.5 * z * z), z.abs() * math.sqrt(0.5)
+        phi = 0.5 * torch.erfc(-z * math.sqrt(0.5))
+        y, slope = z * phi, phi + z * e / math.sqrt(2 * math.pi)
+        t = 1 / (1 + 0.3275911 * v)
+        poly = t * (0.254829592 + t * (-0.284496736 + t * (1.421413741 + t * (-1.453152027 + t * 1.061405429))))
+        method = 0.5 * (torch.erfc(v) - poly * e).abs()
+        assert method.max() <= 0.75e-7                                     # the published bound of it
+        k = U32 * (2 * z * z + 64)
+        tail = 0.5 * poly * e                                              # (above zero 1 - tail: one more u)
+        ey = z.abs() * (method + k * tail + U32 * phi) + U32 * y.abs()
+        es = method + k * (tail + z.abs() * e) + 2 * U32 * phi
+    check(got["y"].view(C), y, ey, "y")
+    check(got["db"], dy * slope, dy * es, "db")
+    deep = z < -4                                                          # so a zero or a wrong sign would not pass
+    assert (ey[deep] < 0.2 * y[deep].abs()).all() and (es[deep] < 0.2 * slope[deep].abs()).all()
