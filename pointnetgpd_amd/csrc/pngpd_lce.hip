@@ -8,19 +8,21 @@
 // Forward: every tile of z reduces in registers to (max, sum of exponentials, sum) of its rows; a second launch joins the
 // tiles of a row.  Backward: z is computed again, a piece of the vocabulary at a time; the piece's g (rounded once to the
 // inputs' type, as the operand of the matrix instructions has to be) lives in a workspace of bounded size, and two products
-// turn it into the piece's dW and its share of dx.  db sums g in float32, where it is made, before that rounding (and without
-// the second walk over it: 8 in the place of 38 us of a 268 us piece of 8192 rows).  8 T D V operations for both directions where keeping T V logits takes
-// 6: the price of not keeping them, which pays for 16 bits; float32's matrix rate makes keeping them the better way, up to 1 GB.
+// turn it into the piece's dW and its share of dx.  db sums g in float32, where it is made, before that rounding (a second
+// walk over it took 28 us more of a piece of 6550 rows by 16,384 classes).  8 T D V operations for both directions
+// where keeping T V logits takes 6: the price of not keeping them, which pays for 16 bits; float32's matrix rate makes keeping
+// them the better way, up to 1 GB.
 // Bound by the matrix cores for T in the hundreds and above, by reading W below.
 // Rows whose target is ignored are left out of the products (from LCE_ROWS rows on): a list of the kept ones is made on
 // the device, and the workgroups past them leave.
 // float16 holds g times 2^15 (|g| <= 1: below 65504, and its normal range then reaches down to 2e-9, under 1/V); the
 // coefficients c_t are scaled to at most 1 the same way; both factors come back in float32 on the way out.
-// Measured (bf16; a large library product reaches 1250 TFLOP/s on this card): 6,550 kept rows of 8192, D 1024, V 100,000: statistics
-// 1.33 ms = 1010 TFLOP/s; of each of 6 pieces g 261 us = 860, dx's product 268 us = 840, dW's 223 us (and 99 for the classes
-// past its rounds) = 930, db 5 us: 5.75 ms in all.  No LDS bank conflict; of the statistics' time the epilogue is 17 %; rows of x
-// or W other than a power of two apart change nothing (1480 us at 1024 and at 1088 elements, all rows).  64 rows, D 256, V 6500,
-// float32: eight launches of 3 to 13 us.
+// Measured (bf16; a large library product reaches 1250 TFLOP/s on this card): 6,550 kept rows of 8192, D 1024, V 100,000:
+// statistics 1.33 ms = 1010 TFLOP/s; of each of 6 pieces g 268 us = 840, dx's product 279 us = 805, dW's 221 us (and 98 for
+// the classes past its rounds) = 940, db 5 us: 5.75 - 5.9 ms by card.  float16 takes 4 % longer (1024 rows, D 1024, 50,000
+// classes: 535 and 514 us).  No LDS bank conflict; of the statistics' time the epilogue is 17 %; rows of x or W other than a
+// power of two apart change nothing (1480 us at 1024 and at 1088 elements, all rows).  64 rows, D 256, V 6500, float32: eight
+// launches of 3 to 13 us.
 #include <algorithm>
 
 #include "pngpd_lce_gemm.h"
@@ -924,9 +926,11 @@ static void lce_copy(const Lce *a, const void *src, long long ld, long long R, i
 
 static inline int lce_ldz(int V) { return (V + 255) / 256 * 256; }
 // Whether the logits are kept, in float32, where they are few: written and read they are 8 bytes a logit at the memory's rate
-// (1.6 ps); computed again 2 D operations at the matrix cores' (float32: 0.014 ps D), or W is read again for few rows (2 D
-// bytes of 16 bits a class).  (Forward + backward, float32, 1024 x 2048 x 12,000: 1369
-// us, computed again 1752; bf16, 200 x 800 x 40,000: 163 and 169.)
+// (1.6 ps); computed again 2 D operations at the matrix cores' float32 rate (0.014 ps D), or, for few rows of 16 bits, W read again
+// (2 D bytes a class, against 8 T of the logits).  Forward + backward on the GPU alone, kept and computed again: float32, 64 x 256 x
+// 6500 55 and 61 us, 256 x 128 x 20,000 92 and 102, 1024 x 2048 x 12,000 1375 and 1745; bf16, 1 x 64 x 100,000 77 and 86, 64 x 256 x
+// 40,000 (T = D / 4) 76 and 79, 256 x 1024 x 40,000 174 and 189, 500 x 2048 x 30,000 317 and 349.  More rows of 16 bits are computed
+// again, also of a D past 800 where 2 D operations cost more than 1.6 ps: their large tile does not store them (not measured).
 static bool lce_keeps(int T, int D, int V, int dt) {
     if (V < 128) return false;                                    // (rows are padded to whole 256 classes)
     const long long bytes = (long long)T * lce_ldz(V) * 4;

@@ -17,10 +17,11 @@
 // The sums of x and x^2 are fp64: a cloud's coordinates-like features have means many times their spread, where a
 // float32 E[x^2] - mean^2 loses the variance; memory hides the fp64 rate.  relu's slope is taken from a z in fp64 (its
 // statistics are kept in fp64 for that): it jumps at 0, and a value next to it would otherwise take either side.
-// Measured (a large copy reaches 4.9 TB/s on this card): bf16, 1024 samples of 1024 x 128 in 32 groups, gelu: forward 168 us
-// (537 MB, 3.2 TB/s), backward 285 us (805 MB, 2.8 TB/s; a workgroup's 32-byte pieces of a row reach memory with 23 % more
-// writes); float32, 64 of 750 x 128: 16 and 19 + 4 us; fp16, one sample of 50,000 x 1024: forward 17 + 6 + 37 us, backward
-// 46 + 6 + 59 (102 MB a walk; the second walk finds part of it in the last-level cache).
+// Measured (a large copy reaches 4.9 TB/s on this card): bf16, 1024 samples of 1024 x 128 in 32 groups, gelu: forward 170 us
+// (537 MB, 3.2 TB/s; the vector pipe is busy for 65 % of it, 29 instructions a value, the rest is loads and stores that little else
+// of a workgroup overlaps), backward 286 us (805 MB, 2.8 TB/s; busy for 52 %, 39 a value; a workgroup's 32-byte pieces of a row
+// reach memory with 26 % more writes); float32, 64 of 750 x 128: 16 and 18 + 4 us; fp16, one sample of 50,000 x 1024: forward
+// 18 + 6 + 36 us, backward 46 + 6 + 60 (102 MB a walk; the second walk finds part of it in the last-level cache).
 #include "pngpd_common.h"
 #include "pngpd_types.h"
 
@@ -795,7 +796,7 @@ static GnPlan gn_plan(int B, int N, int C, int G, int dt, int act, int bwd) {
         }
     }
     // more than 16 workgroups a CU, of a few rows each: wider ranges, then several samples side by side, up to 256 columns
-    // (100,000 samples of 1 x 64, bf16, forward: 256 and 24 us; 20,000 of 1 x 1024 in 32 groups, forward + backward: 1311 and 406)
+    // (100,000 samples of 1 x 64, bf16, forward: 256 and 18 us; 20,000 of 1 x 1024 in 32 groups, forward + backward: 1311 and 300)
     while (p.slab && p.ranges > 1 && (long long)B * p.ranges > 4096 && (long long)N << p.lx <= 128) {
         p.gpr = p.gpr * 2 > G ? G : p.gpr * 2;
         p.ranges = (G + p.gpr - 1) / p.gpr;
